@@ -1,0 +1,609 @@
+// Attention over the paged cache for few rows per sequence (one token, drafted
+// tokens, rows with page lists of their own), and the launch that joins split
+// key ranges.
+//
+//   o = softmax(q k^T / 16) v over the positions up to the row's own.
+//
+// Work: an item is a tile of 2 tokens x the 8 query heads of a KV head (16
+// matrix columns; a list has one token) and a chunk of keys, taken by 4 waves
+// that deal its 32-key steps among them.  Bound by the cache's bytes (e4m3: 512
+// a token and KV head), so nothing is staged and nothing passes through LDS in
+// the loop:
+//  * K: A operand of S^T = K Q^T straight from the page: lane l holds 16 bytes
+//    of row l % 16 -- 16 dims of e4m3 (two k-steps; the reduction index may be
+//    ordered freely) or 8 of bf16.
+//  * S^T leaves lane l with column l % 16 and keys 4 (l / 16) + r of both
+//    16-key tiles: the P^T operand of O^T += V^T P^T as it is.
+//  * V: lane l reads 16 dims of exactly those 8 keys (whole rows of 16 lanes);
+//    the operand of dims 16 i + t wants 8 keys of one dim a lane, which is a
+//    byte (or half-word) exchange between registers of the same lane.
+// e4m3 goes to bf16 with the page's power-of-two scale inside the conversion,
+// exactly.  K of the next step is loaded as soon as the scores are formed and V
+// after its products, so loads are always in flight.
+// Scores, maximum, sum and accumulators are fp32; P is rounded to bf16 for the
+// matrix product (its sum too is taken from the fp32 values).
+#include "paged_split.h"
+
+#include <type_traits>
+
+namespace q36 {
+namespace {
+
+constexpr int kCols = 16, kStep = 32, kWaves = 4;
+constexpr int kNoKeys = 0x40000000;
+constexpr float kScoreScale = 0.0625f * kLog2e;
+
+
+template <bool kHi>
+__device__ __forceinline__ unsigned cvt2(unsigned w, float scale) {
+  return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, kHi));
+}
+__device__ __forceinline__ bf16x8 as_bf16x8(unsigned a, unsigned b, unsigned c, unsigned d) {
+  const u32x4 v = {a, b, c, d};
+  return __builtin_bit_cast(bf16x8, v);
+}
+
+struct ListArgs {
+  const int* pages;     // [tokens][KV heads][listed]
+  unsigned listed, chunks, chunk_keys;
+};
+
+template <bool kFp8, bool kList>
+__global__ __launch_bounds__(64 * kWaves, kFp8 ? 2 : 1) void paged_rows_kernel(
+    const bf16* __restrict__ q, PagedCache c, PagedBatch b, PagedOut w, ListArgs list,
+    unsigned target) {
+  constexpr int kElem = kFp8 ? 1 : 2;
+  constexpr int kKLoads = 4 * kElem, kVLoads = kElem;   // 16-byte loads of a K row part, a V row
+  __shared__ unsigned find[40];
+  __shared__ float ol[kWaves][kCols][kD];
+  __shared__ float mll[kWaves][kCols][2];
+
+  const unsigned head = blockIdx.x % c.heads, item = blockIdx.x / c.heads;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, g = lane >> 4;
+  const unsigned hq = c.heads * kGroup;
+
+  // the item: rows t0 .. t0 + n_tok, keys [key0, key1) of the sequence or of the list
+  unsigned seq;
+  int t0, n_tok, key0, key1, pos0;
+  size_t slot;
+  bool single;
+  if constexpr (kList) {
+    t0 = (int)(item / list.chunks);
+    const unsigned chunk = item % list.chunks;
+    seq = __builtin_amdgcn_readfirstlane(paged_find_row(b, t0));
+    if (seq >= b.seqs) return;
+    const PagedSeq s = paged_seq(b, seq);
+    if (t0 < s.a || t0 >= s.z) return;
+    pos0 = s.pos(t0);
+    if (pos0 < 0 && list.chunks > 1) return;   // the joining launch writes its zeros
+    n_tok = 1;
+    key0 = (int)(chunk * list.chunk_keys);
+    key1 = min(key0 + (int)list.chunk_keys, (int)(list.listed << c.shift));
+    slot = item;
+    single = list.chunks == 1;
+  } else {
+    PagedSplit sp;
+    if (!paged_split<2>(b, item, target, blockIdx.x == 0 ? w.head : nullptr, find, sp)) return;
+    seq = sp.seq;
+    const PagedSeq s = paged_seq(b, seq);
+    const unsigned chunks = ((unsigned)s.len + sp.chunk - 1) / sp.chunk;
+    t0 = s.a + 2 * (int)(sp.local / chunks);
+    n_tok = min(2, s.z - t0);
+    pos0 = s.pos(t0);
+    key0 = (int)(sp.local % chunks * sp.chunk);
+    const int end = pos0 + n_tok;
+    if (key0 >= end) return;
+    key1 = min(key0 + (int)sp.chunk, end);
+    slot = item;
+    single = end <= (int)sp.chunk;
+  }
+  const int lim_max = pos0 + n_tok - 1;
+  const int tok = col >> 3;
+  const int lim = tok < n_tok ? pos0 + tok : -1;   // this column's last key
+
+  bf16x8 qf[8];
+  {
+    const bf16* qp = q + ((size_t)(t0 + tok) * hq + head * kGroup + (col & 7)) * kD;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      // the dims of k-step s as the K operand below has them
+      const int d = kFp8 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g;
+      qf[s] = lim >= 0 ? *reinterpret_cast<const bf16x8*>(qp + d) : bf16x8{};
+    }
+  }
+  f32x4 o[16];
+#pragma unroll
+  for (int t = 0; t < 16; ++t) o[t] = f32x4{};
+  float m = -INFINITY, l = 0.f;
+
+  const int n_steps = (key1 - key0 + kStep - 1) / kStep;
+  const int my_steps = n_steps > wave ? (n_steps - wave + kWaves - 1) / kWaves : 0;
+  const int* table = b.table + seq * b.table_stride;
+  const int* mine = kList ? list.pages + ((size_t)t0 * c.heads + head) * list.listed : nullptr;
+  const int page_mask = (1 << c.shift) - 1;
+  const unsigned koff = col * kD * kElem + 16 * g;
+  const unsigned voff = 4 * g * kD * kElem + 16 * kElem * col;
+  const size_t head_off = (size_t)head << (c.shift + 8);   // elements
+
+  // 32 steps (64 tiles of 16 keys) at a time: lane j holds what tile j needs
+  for (int s0 = 0; s0 < my_steps; s0 += 32) {
+    int d_key = kNoKeys, d_row = 0;
+    unsigned d_page = 0, d_ke = 127, d_ve = 127;
+    {
+      const int step = wave + kWaves * (s0 + (lane >> 1));
+      const int at = key0 + step * kStep + (lane & 1) * 16;   // of the sequence, or of the list
+      if (at < key1) {
+        int logical = at >> c.shift;
+        bool any = true;
+        if constexpr (kList) {
+          logical = mine[logical];
+          any = logical >= 0 && logical <= (pos0 >> c.shift);
+        }
+        if (any) {
+          const unsigned pid = (unsigned)table[logical];
+          const int first = (logical << c.shift) + (at & page_mask);
+          if (pid < c.pages && first <= lim_max) {
+            d_page = pid;
+            d_row = at & page_mask;
+            d_key = first;
+            if constexpr (kFp8) {
+              d_ke = c.k_exp[(size_t)pid * c.heads + head];
+              d_ve = c.v_exp[(size_t)pid * c.heads + head];
+            }
+          }
+        }
+      }
+    }
+    const int n = min(32, my_steps - s0);
+    u32x4 kr[2][kKLoads], vr[2][4][kVLoads];
+    const auto load_k = [&](int i) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const unsigned pid = __builtin_amdgcn_readlane(d_page, 2 * i + h);
+        const int row = __builtin_amdgcn_readlane(d_row, 2 * i + h);
+        const char* p = c.k + pid * c.k_stride + (head_off + (size_t)row * kD) * kElem;
+#pragma unroll
+        for (int j = 0; j < kKLoads; ++j)
+          kr[h][j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + koff + 64 * j));
+      }
+    };
+    const auto load_v = [&](int i) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const unsigned pid = __builtin_amdgcn_readlane(d_page, 2 * i + h);
+        const int row = __builtin_amdgcn_readlane(d_row, 2 * i + h);
+        const char* p = c.v + pid * c.v_stride + (head_off + (size_t)row * kD) * kElem;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int j = 0; j < kVLoads; ++j)
+            vr[h][e][j] = __builtin_nontemporal_load(
+                reinterpret_cast<const u32x4*>(p + voff + e * kD * kElem + 16 * j));
+      }
+    };
+    load_k(0);
+    load_v(0);
+    for (int i = 0; i < n; ++i) {
+      const int ka = __builtin_amdgcn_readlane(d_key, 2 * i), kb = __builtin_amdgcn_readlane(d_key, 2 * i + 1);
+      f32x4 s[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        s[h] = f32x4{};
+        if constexpr (kFp8) {
+          const float sc = paged_scale((unsigned)__builtin_amdgcn_readlane(d_ke, 2 * i + h));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const u32x4 x = kr[h][j];
+            s[h] = mfma16x16x32(as_bf16x8(cvt2<false>(x[0], sc), cvt2<true>(x[0], sc), cvt2<false>(x[1], sc),
+                                          cvt2<true>(x[1], sc)), qf[2 * j], s[h]);
+            s[h] = mfma16x16x32(as_bf16x8(cvt2<false>(x[2], sc), cvt2<true>(x[2], sc), cvt2<false>(x[3], sc),
+                                          cvt2<true>(x[3], sc)), qf[2 * j + 1], s[h]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) s[h] = mfma16x16x32(__builtin_bit_cast(bf16x8, kr[h][j]), qf[j], s[h]);
+        }
+      }
+      const int ahead = min(i + 1, n - 1);   // the last step loads its own keys again
+      load_k(ahead);
+      // keys of this lane: ka + 4 g + r, kb + 4 g + r
+      const bool edge = max(ka, kb) + 15 > lim_max - (n_tok - 1);
+      if (edge) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[0][r] = ka + 4 * g + r <= lim ? s[0][r] : -INFINITY;
+          s[1][r] = kb + 4 * g + r <= lim ? s[1][r] : -INFINITY;
+        }
+      }
+      float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                       fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+      mx = wave_max_xor(mx, 16);
+      mx = wave_max_xor(mx, 32);
+      mx *= kScoreScale;
+      if (__any(mx > m)) {
+        const float mn = fmaxf(m, mx);
+        const float a = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= a;
+#pragma unroll
+        for (int t = 0; t < 16; ++t) o[t] *= a;
+      }
+      const float base = m == -INFINITY ? 0.f : m;
+      float p[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r >> 2][r & 3], kScoreScale, -base));
+        l += p[r];
+      }
+      bf16x8 pb;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) pb[r] = f2bf(p[r]);
+
+      // O^T += V^T P^T; `mine`: the columns of whose rows the products are wanted
+      const auto pv = [&](auto all, bool mine) {
+        const auto add = [&](f32x4& acc, const bf16x8& a) {
+          const f32x4 r = mfma16x16x32(a, pb, acc);
+          if constexpr (decltype(all)::value) {
+            acc = r;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] = mine ? r[e] : acc[e];
+          }
+        };
+        if constexpr (kFp8) {
+          const float sa = paged_scale((unsigned)__builtin_amdgcn_readlane(d_ve, 2 * i));
+          const float sb = paged_scale((unsigned)__builtin_amdgcn_readlane(d_ve, 2 * i + 1));
+#pragma unroll
+          for (int d = 0; d < 4; ++d) {
+            // [key 0, key 1] of dims 4d, 4d+1 and 4d+2, 4d+3; [key 2, key 3] likewise
+            unsigned x[2][4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              x[h][0] = __builtin_amdgcn_perm(vr[h][1][0][d], vr[h][0][0][d], 0x05010400);
+              x[h][1] = __builtin_amdgcn_perm(vr[h][3][0][d], vr[h][2][0][d], 0x05010400);
+              x[h][2] = __builtin_amdgcn_perm(vr[h][1][0][d], vr[h][0][0][d], 0x07030602);
+              x[h][3] = __builtin_amdgcn_perm(vr[h][3][0][d], vr[h][2][0][d], 0x07030602);
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              add(o[4 * d + 2 * u],
+                  as_bf16x8(cvt2<false>(x[0][2 * u], sa), cvt2<false>(x[0][2 * u + 1], sa),
+                            cvt2<false>(x[1][2 * u], sb), cvt2<false>(x[1][2 * u + 1], sb)));
+              add(o[4 * d + 2 * u + 1],
+                  as_bf16x8(cvt2<true>(x[0][2 * u], sa), cvt2<true>(x[0][2 * u + 1], sa),
+                            cvt2<true>(x[1][2 * u], sb), cvt2<true>(x[1][2 * u + 1], sb)));
+            }
+          }
+        } else {
+#pragma unroll
+          for (int d = 0; d < 8; ++d) {
+            const auto word = [&](int h, int e) { return vr[h][e][d >> 2][d & 3]; };
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const unsigned sel = u ? 0x07060302 : 0x05040100;
+              add(o[2 * d + u], as_bf16x8(__builtin_amdgcn_perm(word(0, 1), word(0, 0), sel),
+                                          __builtin_amdgcn_perm(word(0, 3), word(0, 2), sel),
+                                          __builtin_amdgcn_perm(word(1, 1), word(1, 0), sel),
+                                          __builtin_amdgcn_perm(word(1, 3), word(1, 2), sel)));
+            }
+          }
+        }
+      };
+      if (!edge) {
+        pv(std::true_type{}, true);
+      } else {
+        // What a row must not see may hold anything, NaN among it, and 0 * NaN is
+        // one: the values past a row's last key are cleared, and each token's
+        // columns take only the products with what it sees.
+        for (int t = n_tok - 1; t >= 0; --t) {   // the last clears least
+          const int vl = pos0 + t;
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const bool out = (h ? kb : ka) + 4 * g + e > vl;
+#pragma unroll
+              for (int j = 0; j < kVLoads; ++j) vr[h][e][j] = out ? u32x4{} : vr[h][e][j];
+            }
+          pv(std::false_type{}, tok == t);
+        }
+      }
+      load_v(ahead);
+    }
+  }
+
+  // the waves' partials of each column, joined in LDS
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  if (g == 0) {
+    mll[wave][col][0] = m;
+    mll[wave][col][1] = l;
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int t = 0; t < 16; t += 4) {
+      const f32x4 v = {o[t][r], o[t + 1][r], o[t + 2][r], o[t + 3][r]};
+      *reinterpret_cast<f32x4*>(&ol[wave][col][64 * g + 16 * r + t]) = v;
+    }
+  __syncthreads();
+  const int oc = tid >> 4, od = (tid & 15) * 4;   // a column, 4 dims of each 64
+  if (oc >= 8 * n_tok) return;
+  float mm = mll[0][oc][0];
+#pragma unroll
+  for (int x = 1; x < kWaves; ++x) mm = fmaxf(mm, mll[x][oc][0]);
+  const float base = mm == -INFINITY ? 0.f : mm;
+  float f[kWaves], lsum = 0.f;
+#pragma unroll
+  for (int x = 0; x < kWaves; ++x) {
+    f[x] = __builtin_amdgcn_exp2f(mll[x][oc][0] - base);
+    lsum += f[x] * mll[x][oc][1];
+  }
+  const size_t row = t0 + (oc >> 3), qh = head * kGroup + (oc & 7);
+  const float inv = lsum == 0.f ? 0.f : 1.0f / lsum;
+  const unsigned rows = kList ? 8 : kCols;
+  const size_t part = (slot * c.heads + head) * rows + oc;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int d = 64 * j + od;
+    f32x4 v = f32x4{};
+#pragma unroll
+    for (int x = 0; x < kWaves; ++x) v += f[x] * *reinterpret_cast<const f32x4*>(&ol[x][oc][d]);
+    if (single) {
+      bf16x4 r;
+      if (w.gate != nullptr) {
+        const bf16x4 gt = *reinterpret_cast<const bf16x4*>(w.gate + row * w.gate_stride + qh * 2 * kD + kD + d);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = f2bf(lsum == 0.f ? 0.f : paged_gate(v[e] * inv, gt[e]));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = f2bf(v[e] * inv);
+      }
+      *reinterpret_cast<bf16x4*>(w.out + (row * hq + qh) * kD + d) = r;
+    } else {
+      *reinterpret_cast<f32x4*>(w.o + part * kD + d) = v;
+    }
+  }
+  if (!single && od == 0) {
+    w.ml[part * 2] = mm;
+    w.ml[part * 2 + 1] = lsum;
+  }
+}
+
+// Joins the chunks of one row, head and 64 dims: 16 groups of 16 lanes take
+// every 16th chunk each, 4 dims a lane.  Rows that see nothing become zeros.
+__global__ __launch_bounds__(256) void paged_combine_kernel(PagedBatch b, unsigned heads, PagedOut w,
+                                                            unsigned tile, unsigned listed_chunks) {
+  __shared__ float acc[4][16][4];
+  __shared__ float stat[4][2];
+  const unsigned hq = heads * kGroup;
+  const unsigned slice = blockIdx.x & 3, qh = (blockIdx.x >> 2) % hq, t = (blockIdx.x >> 2) / hq;
+  const unsigned seq = __builtin_amdgcn_readfirstlane(paged_find_row(b, (int)t));
+  if (seq >= b.seqs) return;
+  const PagedSeq s = paged_seq(b, seq);
+  if ((int)t < s.a || (int)t >= s.z) return;
+  const int pos = s.pos((int)t);
+  unsigned n, rows;
+  size_t first, stride = 1;
+  unsigned r;
+  if (listed_chunks != 0) {
+    n = pos < 0 ? 0 : listed_chunks;
+    first = (size_t)t * listed_chunks;
+    rows = 8;
+    r = qh % kGroup;
+  } else {
+    const unsigned chunk = w.head[0] * kSplitBlock, own = t - s.a;
+    const int end = min((int)(own / tile * tile + tile), s.z - s.a) - (s.z - s.a) + s.len;
+    const unsigned chunks = ((unsigned)s.len + chunk - 1) / chunk;
+    n = end > 0 ? ((unsigned)end + chunk - 1) / chunk : 0;
+    first = w.head[1 + seq] + (size_t)(own / tile) * chunks;
+    rows = 8 * tile;
+    r = own % tile * 8 + qh % kGroup;
+  }
+  if (n == 1) return;
+  const int group = threadIdx.x >> 4, wave = threadIdx.x >> 6;
+  const unsigned d = slice * 64 + (threadIdx.x & 15) * 4;
+  const unsigned head = qh / kGroup;
+  float m = -INFINITY, l = 0.f;
+  f32x4 o = f32x4{};
+  for (unsigned i0 = 0; i0 < n; i0 += 64) {   // 4 chunks a group at once
+    float cm[4], cl[4];
+    f32x4 co[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const unsigned i = i0 + 16 * u + group;
+      cm[u] = -INFINITY;
+      cl[u] = 0.f;
+      co[u] = f32x4{};
+      if (i < n) {
+        const size_t part = ((first + i * stride) * heads + head) * rows + r;
+        cm[u] = w.ml[part * 2];
+        cl[u] = w.ml[part * 2 + 1];
+        co[u] = *reinterpret_cast<const f32x4*>(w.o + part * kD + d);
+      }
+    }
+    float mn = m;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) mn = fmaxf(mn, cm[u]);
+    const float base = mn == -INFINITY ? 0.f : mn;
+    const float a = __builtin_amdgcn_exp2f(m - base);
+    l *= a;
+    o *= a;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float f = __builtin_amdgcn_exp2f(cm[u] - base);
+      l += f * cl[u];
+      o += f * co[u];
+    }
+    m = mn;
+  }
+  // groups of a wave, then the waves
+#pragma unroll
+  for (int x = 16; x < 64; x <<= 1) {
+    const float om = __shfl_xor(m, x, 64), mn = fmaxf(m, om);
+    const float base = mn == -INFINITY ? 0.f : mn;
+    const float f = __builtin_amdgcn_exp2f(m - base), fo = __builtin_amdgcn_exp2f(om - base);
+    l = l * f + __shfl_xor(l, x, 64) * fo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = o[e] * f + __shfl_xor(o[e], x, 64) * fo;
+    m = mn;
+  }
+  if ((threadIdx.x & 63) < 16) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[wave][threadIdx.x & 15][e] = o[e];
+    if ((threadIdx.x & 63) == 0) {
+      stat[wave][0] = m;
+      stat[wave][1] = l;
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x >= 16) return;
+  float mm = stat[0][0];
+  for (int x = 1; x < 4; ++x) mm = fmaxf(mm, stat[x][0]);
+  const float base = mm == -INFINITY ? 0.f : mm;
+  float lsum = 0.f;
+  f32x4 v = f32x4{};
+  for (int x = 0; x < 4; ++x) {
+    const float f = __builtin_amdgcn_exp2f(stat[x][0] - base);
+    lsum += f * stat[x][1];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] += f * acc[x][threadIdx.x][e];
+  }
+  const float inv = lsum == 0.f ? 0.f : 1.0f / lsum;
+  bf16x4 res;
+  if (w.gate != nullptr) {
+    const bf16x4 gt = *reinterpret_cast<const bf16x4*>(w.gate + t * w.gate_stride + qh * 2 * kD + kD + d);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) res[e] = f2bf(lsum == 0.f ? 0.f : paged_gate(v[e] * inv, gt[e]));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) res[e] = f2bf(v[e] * inv);
+  }
+  *reinterpret_cast<bf16x4*>(w.out + ((size_t)t * hq + qh) * kD + d) = res;
+}
+
+bool paged_out_of(const void* q, const PagedCache& c, const void* q_gate, unsigned stride, void* out,
+                  const void* ws, PagedOut& o) {
+  if (q == nullptr || out == nullptr || !aligned16(q) || (reinterpret_cast<uintptr_t>(out) & 7u) ||
+      ws == nullptr || !aligned16(ws))
+    return false;
+  if (q_gate != nullptr && (stride < c.heads * kGroup * 2 * kD || stride % 4 ||
+                            (reinterpret_cast<uintptr_t>(q_gate) & 7u)))
+    return false;
+  o.gate = static_cast<const bf16*>(q_gate);
+  o.gate_stride = stride;
+  o.out = static_cast<bf16*>(out);
+  return true;
+}
+
+// Items per KV head that fill the GPU (two workgroups a CU) some times over, so
+// that unequal chunks even out; one sequence takes at most kMaxChunks.
+unsigned rows_target(const PagedBatch& b, unsigned heads) {
+  const unsigned t = 1024u / heads;
+  return t < 64 ? 64 : t;
+}
+
+
+// Keys of a listed chunk: whole blocks, so that all rows' chunks fill the GPU.
+void list_plan(const PagedBatch& b, const PagedCache& c, unsigned listed, ListArgs& l) {
+  const size_t keys = (size_t)listed << c.shift;
+  const size_t rows = (size_t)b.tokens * c.heads;
+  const size_t blocks = (keys + kSplitBlock - 1) / kSplitBlock;
+  const size_t want = (1024 + rows - 1) / rows;                 // chunks of a row
+  const size_t per = want >= blocks ? 1 : (blocks + want - 1) / want;
+  l.chunk_keys = (unsigned)(per * kSplitBlock);
+  l.chunks = (unsigned)((blocks + per - 1) / per);
+  l.listed = listed;
+}
+
+}  // namespace
+
+int paged_combine(const PagedBatch& b, const PagedCache& c, const PagedOut& o, unsigned tile,
+                  unsigned listed_chunks, void* stream) {
+  const unsigned hq = c.heads * kGroup;
+  hipLaunchKernelGGL(paged_combine_kernel, dim3(b.tokens * hq * 4), dim3(256), 0,
+                     static_cast<hipStream_t>(stream), b, c.heads, o, tile, listed_chunks);
+  return static_cast<int>(hipGetLastError());
+}
+
+}  // namespace q36
+
+using namespace q36;
+
+Q36_EXPORT size_t qwen36_paged_attention_workspace_bytes(const qwen36_paged_cache* cache,
+                                                         const qwen36_paged_batch* batch) {
+  PagedCache c;
+  PagedBatch b;
+  if (!paged_cache_of(cache, c) || !paged_batch_of(batch, cache->page_tokens, b)) return 0;
+  return split_ws_bytes(b.seqs, paged_items<2>(b, rows_target(b, c.heads)), c.heads, kCols);
+}
+
+Q36_EXPORT int qwen36_paged_attention(const void* q, const qwen36_paged_cache* cache,
+                                      const qwen36_paged_batch* batch, const void* q_gate,
+                                      unsigned q_gate_row_stride, void* out, void* workspace,
+                                      size_t workspace_bytes, void* stream) {
+  PagedCache c;
+  PagedBatch b;
+  PagedOut o;
+  if (!paged_cache_of(cache, c) || !paged_batch_of(batch, cache->page_tokens, b) ||
+      !paged_out_of(q, c, q_gate, q_gate_row_stride, out, workspace, o) ||
+      workspace_bytes < qwen36_paged_attention_workspace_bytes(cache, batch))
+    return Q36_EINVAL;
+  const unsigned target = rows_target(b, c.heads), items = paged_items<2>(b, target);
+  split_ws(workspace, b.seqs, items, c.heads, kCols, o);
+  const ListArgs none = {};
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const dim3 grid(items * c.heads), block(64 * kWaves);
+  if (cache->cache_type == QWEN36_PAGED_E4M3)
+    hipLaunchKernelGGL((paged_rows_kernel<true, false>), grid, block, 0, st, static_cast<const bf16*>(q), c, b, o,
+                       none, target);
+  else
+    hipLaunchKernelGGL((paged_rows_kernel<false, false>), grid, block, 0, st, static_cast<const bf16*>(q), c, b, o,
+                       none, target);
+  const int e = static_cast<int>(hipGetLastError());
+  return e != Q36_OK ? e : paged_combine(b, c, o, 2, 0, stream);
+}
+
+Q36_EXPORT size_t qwen36_paged_sparse_attention_workspace_bytes(const qwen36_paged_cache* cache,
+                                                                const qwen36_paged_batch* batch,
+                                                                unsigned listed) {
+  PagedCache c;
+  PagedBatch b;
+  if (!paged_cache_of(cache, c) || !paged_batch_of(batch, cache->page_tokens, b) || listed == 0 ||
+      listed > 1024)
+    return 0;
+  ListArgs l;
+  list_plan(b, c, listed, l);
+  return split_ws_bytes(0, (size_t)b.tokens * l.chunks, c.heads, 8);
+}
+
+Q36_EXPORT int qwen36_paged_sparse_attention(const void* q, const qwen36_paged_cache* cache,
+                                             const qwen36_paged_batch* batch, const void* pages,
+                                             unsigned listed, const void* q_gate,
+                                             unsigned q_gate_row_stride, void* out, void* workspace,
+                                             size_t workspace_bytes, void* stream) {
+  PagedCache c;
+  PagedBatch b;
+  PagedOut o;
+  if (!paged_cache_of(cache, c) || !paged_batch_of(batch, cache->page_tokens, b) || listed == 0 ||
+      listed > 1024 || pages == nullptr ||
+      !paged_out_of(q, c, q_gate, q_gate_row_stride, out, workspace, o) ||
+      workspace_bytes < qwen36_paged_sparse_attention_workspace_bytes(cache, batch, listed))
+    return Q36_EINVAL;
+  ListArgs l;
+  list_plan(b, c, listed, l);
+  l.pages = static_cast<const int*>(pages);
+  split_ws(workspace, 0, (size_t)b.tokens * l.chunks, c.heads, 8, o);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const dim3 grid(b.tokens * l.chunks * c.heads), block(64 * kWaves);
+  if (cache->cache_type == QWEN36_PAGED_E4M3)
+    hipLaunchKernelGGL((paged_rows_kernel<true, true>), grid, block, 0, st, static_cast<const bf16*>(q), c, b, o,
+                       l, 0u);
+  else
+    hipLaunchKernelGGL((paged_rows_kernel<false, true>), grid, block, 0, st, static_cast<const bf16*>(q), c, b, o,
+                       l, 0u);
+  const int e = static_cast<int>(hipGetLastError());
+  return e != Q36_OK || l.chunks == 1 ? e : paged_combine(b, c, o, 1, l.chunks, stream);
+}

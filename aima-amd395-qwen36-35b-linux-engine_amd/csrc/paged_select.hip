@@ -1,0 +1,236 @@
+// Choosing the pages of a sparse attention: a score for each page from its
+// keys' bounds, and the pages of the highest scores.
+//
+//   score(page) = 2^e max_h sum_d max(qi_hd kmax_d, qi_hd kmin_d)
+//
+// an upper estimate of the page's largest q.k, in whole numbers: qi and the
+// bounds are int8, the sums stay below 2^22, and scores of different pages are
+// compared as (integer, exponent), so nothing is rounded, no order of summation
+// shows and ties are ties.
+//
+// max(q a, q b) with a >= b is q+ a + q- b for q's positive and negative parts,
+// so the score of 16 pages for 8 heads is a chain of 8 int8 matrix products of
+// 64 dims.  Bound by the bounds' bytes (512 a page and KV head) and, for few
+// rows, by latency: a launch that scores over the whole GPU and one workgroup
+// per (row, KV head) that selects, its keys in registers, by bisecting the
+// key's 32 bits (a ballot and a scalar bit count per 64 keys and step).
+#include "paged_common.h"
+
+namespace q36 {
+namespace {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+// Orders (score, exponent) as an unsigned number; pages without keys are below
+// all of these (1), pages behind the row's last are 0.
+__device__ __forceinline__ unsigned score_key(int s, unsigned e) {
+  if (s == 0) return 0x80000000u;
+  const unsigned u = __float_as_uint((float)(s < 0 ? -s : s));   // exact: |s| < 2^23
+  const unsigned mag = (((u >> 23) + e) << 22) | ((u & 0x7fffffu) >> 1);
+  return s < 0 ? 0x7fffffffu - mag : 0x80000000u + mag;
+}
+
+// A wave scores 16 pages at a time for one row: pages in the matrix rows, the 8
+// heads in the columns (doubled).
+__global__ __launch_bounds__(256) void paged_score_kernel(const bf16* __restrict__ q, PagedCache c,
+                                                          PagedBatch b, unsigned* __restrict__ keys,
+                                                          unsigned blocks, unsigned per_wave) {
+  const unsigned head = blockIdx.x % c.heads, block = blockIdx.x / c.heads % blocks;
+  const unsigned t = blockIdx.x / c.heads / blocks;
+  const int lane = threadIdx.x & 63, col = lane & 7, row = lane & 15, g = lane >> 4;
+  const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned seq = __builtin_amdgcn_readfirstlane(paged_find_row(b, (int)t));
+  if (seq >= b.seqs) return;
+  const PagedSeq s = paged_seq(b, seq);
+  const int pos = s.pos((int)t);
+  if ((int)t < s.a || (int)t >= s.z || pos < 0) return;
+  const unsigned n = ((unsigned)pos >> c.shift) + 1;
+  const unsigned p0 = (block * 4 + wave) * per_wave * 16;
+  if (p0 >= n) return;
+
+  // this lane's 64 dims of its head: 64 j + 16 g + [0, 16)
+  const bf16* qp = q + ((size_t)t * c.heads * kGroup + head * kGroup + col) * kD + 16 * g;
+  bf16x8 x[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] = *reinterpret_cast<const bf16x8*>(qp + 64 * (j >> 1) + 8 * (j & 1));
+  unsigned amax = 0;   // bits of the largest finite magnitude
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const unsigned u = __float_as_uint(bf2f(x[j][e])) & 0x7fffffffu;
+      if (u < 0x7f800000u) amax = max(amax, u);
+    }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) amax = max(amax, (unsigned)__shfl_xor(amax, o, 64));
+  // q * 2^-f with the largest in [64, 128), in two factors (f may be past one's range)
+  const int f = (int)(amax >> 23) - 127 - 6;
+  const float f1 = ldexpf(1.f, -f / 2), f2 = ldexpf(1.f, -f - (-f / 2));
+  i32x4 qpos[4], qneg[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      unsigned up = 0, un = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float v = bf2f(x[2 * j + (w >> 1)][4 * (w & 1) + e]);
+        const float r = v == v ? fminf(fmaxf(rintf(v * f1 * f2), -127.f), 127.f) : 0.f;
+        const int i = (int)r;
+        up |= (unsigned)max(i, 0) << (8 * e);
+        un |= ((unsigned)min(i, 0) & 0xffu) << (8 * e);
+      }
+      qpos[j][w] = (int)up;
+      qneg[j][w] = (int)un;
+    }
+
+  const int* table = b.table + seq * b.table_stride;
+  unsigned* kp = keys + ((size_t)t * c.heads + head) * b.width;
+  for (unsigned i = 0; i < per_wave; ++i) {
+    const unsigned first = p0 + 16 * i;
+    if (first >= n) break;
+    const unsigned mine = first + row;
+    unsigned pid = mine < n ? (unsigned)table[mine] : ~0u;
+    const bool there = pid < c.pages;
+    if (!there) pid = 0;
+    const int8_t* bp = c.bounds + ((size_t)pid * c.heads + head) * 2 * kD + 16 * g;
+    i32x4 a[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) a[j] = *reinterpret_cast<const i32x4*>(bp + 64 * j);
+    const unsigned e = c.k_exp[(size_t)pid * c.heads + head];
+    i32x4 d = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      d = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[j], qpos[j], d, 0, 0, 0);
+      d = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[4 + j], qneg[j], d, 0, 0, 0);
+    }
+    // lane: pages 4 g + r of its head; the largest over the heads
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      int v = d[r];
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) v = max(v, __shfl_xor(v, o, 64));
+      const int from = 4 * g + r;
+      const unsigned pe = __shfl(e, from, 64);
+      const bool ok = __shfl((int)there, from, 64);
+      if (row == r && first + from < n) kp[first + from] = ok ? score_key(v, pe) : 1u;
+    }
+  }
+}
+
+// One workgroup per (row, KV head); thread i holds the keys of pages
+// [i kPer, + kPer).
+template <int kPer>
+__global__ __launch_bounds__(256) void paged_pick_kernel(PagedCache c, PagedBatch b,
+                                                         const unsigned* __restrict__ keys,
+                                                         unsigned budget, unsigned sinks,
+                                                         unsigned recents, int* __restrict__ pages) {
+  __shared__ unsigned cnt[2][4];
+  __shared__ unsigned scan[4];
+  const unsigned head = blockIdx.x % c.heads, t = blockIdx.x / c.heads, tid = threadIdx.x;
+  const unsigned wave = tid >> 6;
+  const unsigned seq = __builtin_amdgcn_readfirstlane(paged_find_row(b, (int)t));
+  if (seq >= b.seqs) return;
+  const PagedSeq s = paged_seq(b, seq);
+  if ((int)t < s.a || (int)t >= s.z) return;
+  const int pos = s.pos((int)t);
+  const unsigned n = pos < 0 ? 0u : ((unsigned)pos >> c.shift) + 1;
+  int* out = pages + ((size_t)t * c.heads + head) * budget;
+  if (n <= budget) {
+    for (unsigned i = tid; i < budget; i += 256) out[i] = i < n ? (int)i : -1;
+    return;
+  }
+  const unsigned* kp = keys + ((size_t)t * c.heads + head) * b.width;
+  unsigned k[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const unsigned p = tid * kPer + j;
+    k[j] = p >= n ? 0u : p < sinks || p + recents >= n ? ~0u : kp[p];
+  }
+  // largest v with at least `budget` keys >= v, bit by bit
+  unsigned v = 0, equal = 0;
+  for (int bit = 31; bit >= 0; --bit) {
+    const unsigned cand = v | (1u << bit);
+    unsigned m = 0;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) m += __popcll(__ballot(k[j] >= cand));
+    if ((tid & 63) == 0) cnt[bit & 1][wave] = m;
+    __syncthreads();
+    m = cnt[bit & 1][0] + cnt[bit & 1][1] + cnt[bit & 1][2] + cnt[bit & 1][3];
+    if (m >= budget) v = cand;
+    if (m == budget) break;   // exactly the keys >= v
+  }
+  // keys above v, and of those equal to it the lowest pages
+  unsigned gt = 0, eq = 0;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    gt += k[j] > v;
+    eq += k[j] == v;
+  }
+  const unsigned own = (gt << 16) | eq;   // each at most 16384 over the workgroup
+  unsigned in = wave_scan_add(own);
+  if ((tid & 63) == 63) scan[wave] = in;
+  __syncthreads();
+  unsigned total = 0;
+  for (unsigned w = 0; w < 4; ++w) {
+    const unsigned x = scan[w];
+    if (w < wave) in += x;
+    total += x;
+  }
+  in -= own;
+  equal = budget - (total >> 16);   // how many equal ones are taken
+  unsigned eq_before = in & 0xffffu, at = (in >> 16) + min(eq_before, equal);
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const bool tie = k[j] == v;
+    if (k[j] > v || (tie && eq_before < equal)) out[at++] = (int)(tid * kPer + j);
+    eq_before += tie;
+  }
+}
+
+}  // namespace
+}  // namespace q36
+
+using namespace q36;
+
+Q36_EXPORT size_t qwen36_paged_select_workspace_bytes(const qwen36_paged_cache* cache,
+                                                      const qwen36_paged_batch* batch) {
+  PagedCache c;
+  PagedBatch b;
+  if (!paged_cache_of(cache, c) || !paged_batch_of(batch, cache->page_tokens, b)) return 0;
+  return (size_t)b.tokens * c.heads * b.width * 4;
+}
+
+Q36_EXPORT int qwen36_paged_select(const void* q, const qwen36_paged_cache* cache,
+                                   const qwen36_paged_batch* batch, unsigned budget,
+                                   unsigned sink_pages, unsigned recent_pages, void* pages,
+                                   void* workspace, size_t workspace_bytes, void* stream) {
+  PagedCache c;
+  PagedBatch b;
+  if (!paged_cache_of(cache, c) || !paged_batch_of(batch, cache->page_tokens, b) ||
+      c.bounds == nullptr || q == nullptr || !aligned16(q) || pages == nullptr || budget == 0 ||
+      budget > 1024 || recent_pages == 0 || sink_pages > budget || recent_pages > budget - sink_pages ||
+      workspace == nullptr || !aligned16(workspace) ||
+      workspace_bytes < qwen36_paged_select_workspace_bytes(cache, batch))
+    return Q36_EINVAL;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  unsigned* keys = static_cast<unsigned*>(workspace);
+  if (b.width > budget) {   // else every row takes all its pages
+    const size_t rows = (size_t)b.tokens * c.heads, groups = (b.width + 63) / 64;
+    size_t per = rows * groups / 8192;   // 16-page groups a wave takes
+    per = per < 1 ? 1 : per > 16 ? 16 : per;
+    const unsigned blocks = (unsigned)((groups + per - 1) / per);
+    hipLaunchKernelGGL(paged_score_kernel, dim3((unsigned)(rows * blocks)), dim3(256), 0, st,
+                       static_cast<const bf16*>(q), c, b, keys, blocks, (unsigned)per);
+    const int e = static_cast<int>(hipGetLastError());
+    if (e != Q36_OK) return e;
+  }
+  const dim3 grid(b.tokens * c.heads);
+  if (b.width <= 2048)
+    hipLaunchKernelGGL(paged_pick_kernel<8>, grid, dim3(256), 0, st, c, b, keys, budget, sink_pages,
+                       recent_pages, static_cast<int*>(pages));
+  else
+    hipLaunchKernelGGL(paged_pick_kernel<65>, grid, dim3(256), 0, st, c, b, keys, budget, sink_pages,
+                       recent_pages, static_cast<int*>(pages));
+  return static_cast<int>(hipGetLastError());
+}

@@ -1,0 +1,126 @@
+// How attention over the paged cache is split: (tile of rows, chunk of keys)
+// items, their partials in the workspace, and the launch that joins them.
+//
+// The lengths are on the device, so every workgroup works the split out for
+// itself: with w blocks of 128 keys over all tiles of a KV head, chunks of
+//   max(1, w / target, longest / 256)
+// blocks give at most target + tiles items, whatever the mixture of lengths:
+// one sequence of 128K fills the GPU as 32 of 4K do.  The grid is that bound,
+// and workgroups without an item end.  A tile of one chunk is written straight
+// to the output.
+#pragma once
+
+#include "paged_common.h"
+
+namespace q36 {
+
+constexpr unsigned kSplitBlock = 128;    // keys; chunks are whole blocks
+constexpr unsigned kMaxChunks = 256;
+
+struct PagedOut {
+  const bf16* gate;       // NULL, or q_gate's row 0
+  bf16* out;
+  float* ml;              // [slot][KV head][8 * tile tokens][2]: m (log2 domain), l
+  float* o;               // [slot][KV head][8 * tile tokens][256]
+  unsigned* head;         // [0]: chunk blocks, [1 + i]: first slot of sequence i
+  size_t gate_stride;
+};
+
+struct PagedSplit {
+  unsigned chunk;         // keys of a chunk
+  unsigned seq, local;    // the item's sequence and its place there
+};
+
+// The item of this workgroup (all threads call it; lds holds 40 words); false
+// if there is none.  Item 0 also writes the split down for the joining launch.
+template <unsigned kTile>
+__device__ __forceinline__ bool paged_split(const PagedBatch& b, unsigned item, unsigned target,
+                                            unsigned* head, unsigned* lds, PagedSplit& r) {
+  const unsigned tid = threadIdx.x, n = blockDim.x, wave = tid >> 6, waves = n >> 6;
+  const auto tiles = [&](const PagedSeq& s) { return (unsigned)(s.z - s.a + (int)kTile - 1) / kTile; };
+  const auto blocks = [&](const PagedSeq& s) {
+    return ((unsigned)s.len + kSplitBlock - 1) / kSplitBlock;
+  };
+  unsigned cb;
+  if (b.seqs == 1) {
+    const PagedSeq s = paged_seq(b, 0);
+    const unsigned l = blocks(s), w = tiles(s) * l;
+    cb = max(1u, max((w + target - 1) / target, (l + kMaxChunks - 1) / kMaxChunks));
+    r.chunk = cb * kSplitBlock;
+    r.seq = 0;
+    r.local = item;
+    if (head != nullptr && tid == 0) {
+      head[0] = cb;
+      head[1] = 0;
+    }
+    return item < tiles(s) * ((l + cb - 1) / cb);
+  }
+  unsigned w = 0, longest = 0;
+  for (unsigned i = tid; i < b.seqs; i += n) {
+    const PagedSeq s = paged_seq(b, i);
+    const unsigned t = tiles(s), l = t ? blocks(s) : 0u;
+    w += t * l;
+    longest = max(longest, l);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    w += __shfl_xor(w, o, 64);
+    longest = max(longest, (unsigned)__shfl_xor(longest, o, 64));
+  }
+  if ((tid & 63) == 0) {
+    lds[20 + wave] = w;
+    lds[30 + wave] = longest;
+  }
+  __syncthreads();
+  w = 0;
+  for (unsigned i = 0; i < waves; ++i) {
+    w += lds[20 + i];
+    longest = max(longest, lds[30 + i]);
+  }
+  cb = __builtin_amdgcn_readfirstlane(
+      max(1u, max((w + target - 1) / target, (longest + kMaxChunks - 1) / kMaxChunks)));
+  r.chunk = cb * kSplitBlock;
+  if (head != nullptr && tid == 0) head[0] = cb;
+  return paged_find_item(b, item, lds, [&](unsigned i) {
+    const PagedSeq s = paged_seq(b, i);
+    return tiles(s) * ((blocks(s) + cb - 1) / cb);
+  }, r.seq, r.local, head != nullptr ? head + 1 : nullptr);
+}
+
+// Items of a KV head at most, for the grid and the workspace.
+template <unsigned kTile>
+inline unsigned paged_items(const PagedBatch& b, unsigned target) {
+  const unsigned t = b.tokens / kTile + b.seqs;
+  return (t < b.tokens ? t : b.tokens) + target;
+}
+
+__device__ __forceinline__ float paged_gate(float o, bf16 g) {
+  return o * (1.0f / (1.0f + expf(-bf2f(g))));
+}
+
+inline size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
+inline size_t split_ws_bytes(unsigned seqs, size_t slots, unsigned heads, unsigned rows) {
+  return round256(((size_t)seqs + 1) * 4) + round256(slots * heads * rows * 8) +
+         slots * heads * rows * kD * 4;
+}
+inline void split_ws(void* ws, unsigned seqs, size_t slots, unsigned heads, unsigned rows, PagedOut& o) {
+  char* p = static_cast<char*>(ws);
+  o.head = reinterpret_cast<unsigned*>(p);
+  p += round256(((size_t)seqs + 1) * 4);
+  o.ml = reinterpret_cast<float*>(p);
+  p += round256(slots * heads * rows * 8);
+  o.o = reinterpret_cast<float*>(p);
+}
+
+// The target for tiles of kTile tokens.
+unsigned paged_target_rows(const PagedBatch& b, unsigned heads);
+// Joins the partials of tiles of `tile` tokens; listed_chunks != 0: every row
+// has that many slots.  Rows of one chunk are already written.
+int paged_combine(const PagedBatch& b, const PagedCache& c, const PagedOut& o, unsigned tile,
+                  unsigned listed_chunks, void* stream);
+// Tiles of 32 tokens, for prompts (paged_prefill.hip).
+size_t paged_prefill_ws(const PagedBatch& b, const PagedCache& c);
+int paged_prefill(const void* q, const PagedCache& c, bool fp8, const PagedBatch& b, PagedOut o,
+                  void* ws, void* stream);
+
+}  // namespace q36

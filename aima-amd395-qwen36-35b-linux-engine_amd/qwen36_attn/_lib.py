@@ -20,6 +20,24 @@ _u64 = ctypes.c_ulonglong
 _pu32 = ctypes.POINTER(ctypes.c_uint)
 _pu64 = ctypes.POINTER(ctypes.c_ulonglong)
 
+
+class PagedCacheArgs(ctypes.Structure):
+    """qwen36_paged_cache"""
+    _fields_ = [("k_pages", _vp), ("v_pages", _vp), ("k_exp", _vp), ("v_exp", _vp),
+                ("bounds", _vp), ("k_page_stride", _sz), ("v_page_stride", _sz),
+                ("num_pages", _u32), ("page_tokens", _u32), ("kv_heads", _u32),
+                ("cache_type", _u32)]
+
+
+class PagedBatchArgs(ctypes.Structure):
+    """qwen36_paged_batch"""
+    _fields_ = [("page_table", _vp), ("cu_tokens", _vp), ("seq_lens", _vp), ("table_stride", _sz),
+                ("table_width", _u32), ("seqs", _u32), ("tokens", _u32)]
+
+
+_pcache = ctypes.POINTER(PagedCacheArgs)
+_pbatch = ctypes.POINTER(PagedBatchArgs)
+
 # name -> (restype, argtypes).  Mirrors include/qwen36_attn.h.
 SIGNATURES: dict[str, tuple] = {
     # FMHA provider ABI (drop-in for qrt_ck_fmha_*)
@@ -91,6 +109,16 @@ SIGNATURES: dict[str, tuple] = {
     "qwen36_prefix_cache_capture": (_i32, [_vp, _pu32, _u32, _vp, _vp, _pu32, _pu64]),
     "qwen36_prefix_cache_copy_terminal": (_i32, [_vp, _u32, _vp, _vp]),
     "qwen36_prefix_cache_destroy": (_i32, [_vp]),
+    # paged KV cache
+    "qwen36_paged_append": (_i32, [_vp, _u32, _vp, _u32, _vp, _u32, _vp, _vp, _vp, _vp, _u32,
+                                   _pcache, _pbatch, _vp, _vp]),
+    "qwen36_paged_attention_workspace_bytes": (_sz, [_pcache, _pbatch]),
+    "qwen36_paged_attention": (_i32, [_vp, _pcache, _pbatch, _vp, _u32, _vp, _vp, _sz, _vp]),
+    "qwen36_paged_select_workspace_bytes": (_sz, [_pcache, _pbatch]),
+    "qwen36_paged_select": (_i32, [_vp, _pcache, _pbatch, _u32, _u32, _u32, _vp, _vp, _sz, _vp]),
+    "qwen36_paged_sparse_attention_workspace_bytes": (_sz, [_pcache, _pbatch, _u32]),
+    "qwen36_paged_sparse_attention": (_i32, [_vp, _pcache, _pbatch, _vp, _u32, _vp, _u32, _vp,
+                                             _vp, _sz, _vp]),
     "qwen36_gdn_decode_step": (_i32, [_vp, _u32, _vp, _vp, _vp, _vp, _vp, _u32, _vp,
                                       _vp, _vp, _u32, _vp, _vp, _vp, _vp, _u32, _vp]),
 }

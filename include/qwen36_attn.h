@@ -453,6 +453,126 @@ int qwen36_prefix_cache_capture(void* pool, const unsigned* tokens, unsigned n,
 int qwen36_prefix_cache_copy_terminal(void* pool, unsigned index, void* dst, void* stream);
 int qwen36_prefix_cache_destroy(void* pool);
 
+/* ---- paged KV cache --------------------------------------------------------
+ * No counterpart in the reference, whose caches are dense and hold one
+ * sequence.  A pool of pages serves a ragged batch of sequences: a page holds
+ * page_tokens (16, 32, 64 or 128) tokens of every KV head, [kv_heads]
+ * [page_tokens][256]; pages are k_page_stride / v_page_stride elements apart
+ * (multiples of 16 bytes), so K and V may be slices of one allocation.
+ * kv_heads is 1 to 16 (the model's 2, or a tensor-parallel share); query head
+ * h reads KV head h / 8.
+ * cache_type QWEN36_PAGED_BF16, or QWEN36_PAGED_E4M3: OCP e4m3 values times a
+ * scale for each page and KV head, a power of two held as the byte e of
+ * 2^(e - 127) (E8M0) in k_exp, v_exp [num_pages][kv_heads] (bytes of 16 to
+ * 247, as the append writes them).
+ * bounds: NULL, or int8 [num_pages][kv_heads][2][256]: each channel's largest
+ * and smallest key of the page, rounded outwards to steps of
+ * 4 * 2^(k_exp - 127) (a bf16 cache with bounds has k_exp too). */
+#define QWEN36_PAGED_BF16 0
+#define QWEN36_PAGED_E4M3 1
+typedef struct {
+  void* k_pages;
+  void* v_pages;
+  void* k_exp;
+  void* v_exp;
+  void* bounds;
+  size_t k_page_stride;
+  size_t v_page_stride;
+  unsigned num_pages;
+  unsigned page_tokens;
+  unsigned kv_heads;
+  unsigned cache_type;
+} qwen36_paged_cache;
+
+/* The batch of a call.  Rows [cu_tokens[i], cu_tokens[i+1]) of the call's
+ * `tokens` rows are the last tokens of sequence i, whose length with them is
+ * seq_lens[i]: the row j before its end is at position seq_lens[i] - j.
+ * page_table[i * table_stride + p] is the page of its positions
+ * [p * page_tokens, + page_tokens).  All int32 in device memory, read when the
+ * launch runs, so a captured call follows them.  Rows behind the last sequence
+ * are left as they were.  Nothing there can make a launch read or write out of
+ * bounds: a page id outside [0, num_pages) holds no tokens (and takes none), a
+ * sequence longer than its table (or than the rotation tables) has none, rows
+ * of negative position see nothing.  A page that an append writes must belong
+ * to one sequence of the batch. */
+typedef struct {
+  const void* page_table;
+  const void* cu_tokens;
+  const void* seq_lens;
+  size_t table_stride;
+  unsigned table_width;
+  unsigned seqs;
+  unsigned tokens;
+} qwen36_paged_batch;
+
+/* qwen36_paged_append: head norm and rotation of the new rows' queries and
+ * keys, and the keys and raw values into their pages (the paged form of
+ * qwen36_head_norm_rope, with its arithmetic and roundings; the rotation comes
+ * from fp32 tables cosv, sinv [positions, 32], e.g. qwen36_rotary_table's).
+ * q_gate rows [q | gate] of each query head (stride >= kv_heads * 4096), k_raw,
+ * v_raw rows of kv_heads * 256; strides in elements, multiples of 4, 8-byte
+ * aligned; tables 16-byte aligned.  q_out [tokens, 8 * kv_heads, 256] bf16.
+ * e4m3: the page's scale byte becomes the least e with
+ * max |x| <= 448 * 2^(e - 127) over the page's tokens (never less than 16, and
+ * never less than before while the page keeps rows); kept rows are rescaled
+ * when it grows.  Values that are not finite are stored as NaN and take no part
+ * in the scale; in the bounds a NaN counts as 0 and infinities as +-127 steps.
+ * Rows of a page behind the new ones keep their bytes. */
+int qwen36_paged_append(const void* q_gate, unsigned q_row_stride, const void* k_raw,
+                        unsigned k_row_stride, const void* v_raw, unsigned v_row_stride,
+                        const void* q_weight, const void* k_weight, const float* cosv,
+                        const float* sinv, unsigned positions, const qwen36_paged_cache* cache,
+                        const qwen36_paged_batch* batch, void* q_out, void* stream);
+
+/* qwen36_paged_attention: out = softmax(q k^T / 16) v over each row's
+ * positions [0, its own], q [tokens, 8 * kv_heads, 256] bf16 as the append
+ * writes it, out [tokens, kv_heads * 2048] bf16.  q_gate: NULL, or the rows of
+ * the append (its gate halves): then out = bf16(attention * sigmoid(gate)),
+ * rounded once (qwen36_output_gate rounds the attention and the sigmoid first).
+ * A row that sees nothing is zeros.  One token per sequence, drafted tokens and
+ * prompts in any mixture; tokens of the rows' own sequence must have been
+ * appended.  workspace of qwen36_paged_attention_workspace_bytes(...) bytes,
+ * 16-byte aligned; calls that overlap on one workspace race. */
+size_t qwen36_paged_attention_workspace_bytes(const qwen36_paged_cache* cache,
+                                              const qwen36_paged_batch* batch);
+int qwen36_paged_attention(const void* q, const qwen36_paged_cache* cache,
+                           const qwen36_paged_batch* batch, const void* q_gate,
+                           unsigned q_gate_row_stride, void* out, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
+/* qwen36_paged_select: for each row and KV head the pages that a sparse
+ * attention reads, pages [tokens, kv_heads, budget] int32: logical page
+ * indices, ascending, -1 behind the last.  A row at position p has
+ * n = p / page_tokens + 1 pages.  n <= budget: all of them; else the first
+ * sink_pages, the last recent_pages (at least 1) and those of the highest
+ * scores, ties to the lower index, budget in all (sink_pages + recent_pages <=
+ * budget <= 1024).  The score of a page is 2^k_exp times the largest over the
+ * KV head's 8 query heads of sum_d max(qi_d kmax_d, qi_d kmin_d) with the
+ * bounds' integers and qi = q in steps of a power of two that puts the 8 heads'
+ * largest finite magnitude in [64, 128), rounded to nearest even and cut to
+ * +-127 (NaN counts as 0): whole numbers, so the selection is exact.  A page id
+ * outside the pool scores below every other.  Needs bounds; workspace of
+ * qwen36_paged_select_workspace_bytes(...) bytes, 16-byte aligned. */
+size_t qwen36_paged_select_workspace_bytes(const qwen36_paged_cache* cache,
+                                           const qwen36_paged_batch* batch);
+int qwen36_paged_select(const void* q, const qwen36_paged_cache* cache,
+                        const qwen36_paged_batch* batch, unsigned budget, unsigned sink_pages,
+                        unsigned recent_pages, void* pages, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/* qwen36_paged_sparse_attention: qwen36_paged_attention over the positions up
+ * to the row's own in the listed pages only.  pages [tokens, kv_heads, listed]
+ * int32 logical page indices in any order, listed <= 1024; an index outside the
+ * row's pages (such as -1) lists nothing, a page listed twice counts twice. */
+size_t qwen36_paged_sparse_attention_workspace_bytes(const qwen36_paged_cache* cache,
+                                                     const qwen36_paged_batch* batch,
+                                                     unsigned listed);
+int qwen36_paged_sparse_attention(const void* q, const qwen36_paged_cache* cache,
+                                  const qwen36_paged_batch* batch, const void* pages,
+                                  unsigned listed, const void* q_gate,
+                                  unsigned q_gate_row_stride, void* out, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
