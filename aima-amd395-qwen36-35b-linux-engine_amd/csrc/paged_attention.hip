@@ -24,8 +24,6 @@
 // matrix product (its sum too is taken from the fp32 values).
 #include "paged_split.h"
 
-#include <type_traits>
-
 namespace q36 {
 namespace {
 
@@ -34,10 +32,6 @@ constexpr int kNoKeys = 0x40000000;
 constexpr float kScoreScale = 0.0625f * kLog2e;
 
 
-template <bool kHi>
-__device__ __forceinline__ unsigned cvt2(unsigned w, float scale) {
-  return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, kHi));
-}
 __device__ __forceinline__ bf16x8 as_bf16x8(unsigned a, unsigned b, unsigned c, unsigned d) {
   const u32x4 v = {a, b, c, d};
   return __builtin_bit_cast(bf16x8, v);
@@ -48,6 +42,21 @@ struct ListArgs {
   unsigned listed, chunks, chunk_keys;
 };
 
+__device__ __forceinline__ void paged_store(const PagedOut& w, unsigned hq, size_t t, unsigned qh, unsigned d,
+                                            const f32x4& o, float l) {
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  bf16x4 r;
+  if (w.gate != nullptr) {
+    const bf16x4 g = *reinterpret_cast<const bf16x4*>(w.gate + t * w.gate_stride + qh * 2 * kD + kD + d);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] = f2bf(l == 0.f ? 0.f : paged_gate(o[e] * inv, g[e]));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] = f2bf(l == 0.f ? 0.f : o[e] * inv);
+  }
+  *reinterpret_cast<bf16x4*>(w.out + (t * hq + qh) * kD + d) = r;
+}
+
 template <bool kFp8, bool kList>
 __global__ __launch_bounds__(64 * kWaves, kFp8 ? 2 : 1) void paged_rows_kernel(
     const bf16* __restrict__ q, PagedCache c, PagedBatch b, PagedOut w, ListArgs list,
@@ -57,6 +66,7 @@ __global__ __launch_bounds__(64 * kWaves, kFp8 ? 2 : 1) void paged_rows_kernel(
   __shared__ unsigned find[40];
   __shared__ float ol[kWaves][kCols][kD];
   __shared__ float mll[kWaves][kCols][2];
+  __shared__ int odd[kWaves];   // whether a V value that only the second token sees is not finite
 
   const unsigned head = blockIdx.x % c.heads, item = blockIdx.x / c.heads;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -117,6 +127,7 @@ __global__ __launch_bounds__(64 * kWaves, kFp8 ? 2 : 1) void paged_rows_kernel(
 #pragma unroll
   for (int t = 0; t < 16; ++t) o[t] = f32x4{};
   float m = -INFINITY, l = 0.f;
+  bool strange = false;
 
   const int n_steps = (key1 - key0 + kStep - 1) / kStep;
   const int my_steps = n_steps > wave ? (n_steps - wave + kWaves - 1) / kWaves : 0;
@@ -241,73 +252,66 @@ __global__ __launch_bounds__(64 * kWaves, kFp8 ? 2 : 1) void paged_rows_kernel(
 #pragma unroll
       for (int r = 0; r < 8; ++r) pb[r] = f2bf(p[r]);
 
-      // O^T += V^T P^T; `mine`: the columns of whose rows the products are wanted
-      const auto pv = [&](auto all, bool mine) {
-        const auto add = [&](f32x4& acc, const bf16x8& a) {
-          const f32x4 r = mfma16x16x32(a, pb, acc);
-          if constexpr (decltype(all)::value) {
-            acc = r;
-          } else {
+      if (edge) {
+        // Behind a row's position V may hold anything, and 0 * NaN is NaN: rows that
+        // no token sees are cleared, and of the one that only the second token sees
+        // what is not finite (it gets that at the end).
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[e] = mine ? r[e] : acc[e];
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = (h ? kb : ka) + 4 * g + e;
+#pragma unroll
+            for (int j = 0; j < kVLoads; ++j)
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const unsigned u = key > lim_max ? 0u : vr[h][e][j][x];
+                const unsigned bad = key > pos0 ? not_finite<kFp8>(u) : 0u;
+                vr[h][e][j][x] = u & ~bad;
+                strange |= bad != 0;
+              }
           }
-        };
-        if constexpr (kFp8) {
-          const float sa = paged_scale((unsigned)__builtin_amdgcn_readlane(d_ve, 2 * i));
-          const float sb = paged_scale((unsigned)__builtin_amdgcn_readlane(d_ve, 2 * i + 1));
+      }
+      if constexpr (kFp8) {
+        const float sa = paged_scale((unsigned)__builtin_amdgcn_readlane(d_ve, 2 * i));
+        const float sb = paged_scale((unsigned)__builtin_amdgcn_readlane(d_ve, 2 * i + 1));
 #pragma unroll
-          for (int d = 0; d < 4; ++d) {
-            // [key 0, key 1] of dims 4d, 4d+1 and 4d+2, 4d+3; [key 2, key 3] likewise
-            unsigned x[2][4];
+        for (int d = 0; d < 4; ++d) {
+          // [key 0, key 1] of dims 4d, 4d+1 and 4d+2, 4d+3; [key 2, key 3] likewise
+          unsigned x[2][4];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              x[h][0] = __builtin_amdgcn_perm(vr[h][1][0][d], vr[h][0][0][d], 0x05010400);
-              x[h][1] = __builtin_amdgcn_perm(vr[h][3][0][d], vr[h][2][0][d], 0x05010400);
-              x[h][2] = __builtin_amdgcn_perm(vr[h][1][0][d], vr[h][0][0][d], 0x07030602);
-              x[h][3] = __builtin_amdgcn_perm(vr[h][3][0][d], vr[h][2][0][d], 0x07030602);
-            }
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              add(o[4 * d + 2 * u],
-                  as_bf16x8(cvt2<false>(x[0][2 * u], sa), cvt2<false>(x[0][2 * u + 1], sa),
-                            cvt2<false>(x[1][2 * u], sb), cvt2<false>(x[1][2 * u + 1], sb)));
-              add(o[4 * d + 2 * u + 1],
-                  as_bf16x8(cvt2<true>(x[0][2 * u], sa), cvt2<true>(x[0][2 * u + 1], sa),
-                            cvt2<true>(x[1][2 * u], sb), cvt2<true>(x[1][2 * u + 1], sb)));
-            }
+          for (int h = 0; h < 2; ++h) {
+            x[h][0] = __builtin_amdgcn_perm(vr[h][1][0][d], vr[h][0][0][d], 0x05010400);
+            x[h][1] = __builtin_amdgcn_perm(vr[h][3][0][d], vr[h][2][0][d], 0x05010400);
+            x[h][2] = __builtin_amdgcn_perm(vr[h][1][0][d], vr[h][0][0][d], 0x07030602);
+            x[h][3] = __builtin_amdgcn_perm(vr[h][3][0][d], vr[h][2][0][d], 0x07030602);
           }
-        } else {
 #pragma unroll
-          for (int d = 0; d < 8; ++d) {
-            const auto word = [&](int h, int e) { return vr[h][e][d >> 2][d & 3]; };
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const unsigned sel = u ? 0x07060302 : 0x05040100;
-              add(o[2 * d + u], as_bf16x8(__builtin_amdgcn_perm(word(0, 1), word(0, 0), sel),
-                                          __builtin_amdgcn_perm(word(0, 3), word(0, 2), sel),
-                                          __builtin_amdgcn_perm(word(1, 1), word(1, 0), sel),
-                                          __builtin_amdgcn_perm(word(1, 3), word(1, 2), sel)));
-            }
+          for (int u = 0; u < 2; ++u) {
+            o[4 * d + 2 * u] = mfma16x16x32(
+                as_bf16x8(cvt2<false>(x[0][2 * u], sa), cvt2<false>(x[0][2 * u + 1], sa),
+                          cvt2<false>(x[1][2 * u], sb), cvt2<false>(x[1][2 * u + 1], sb)),
+                pb, o[4 * d + 2 * u]);
+            o[4 * d + 2 * u + 1] = mfma16x16x32(
+                as_bf16x8(cvt2<true>(x[0][2 * u], sa), cvt2<true>(x[0][2 * u + 1], sa),
+                          cvt2<true>(x[1][2 * u], sb), cvt2<true>(x[1][2 * u + 1], sb)),
+                pb, o[4 * d + 2 * u + 1]);
           }
         }
-      };
-      if (!edge) {
-        pv(std::true_type{}, true);
       } else {
-        // What a row must not see may hold anything, NaN among it, and 0 * NaN is
-        // one: the values past a row's last key are cleared, and each token's
-        // columns take only the products with what it sees.
-        for (int t = n_tok - 1; t >= 0; --t) {   // the last clears least
-          const int vl = pos0 + t;
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+        for (int d = 0; d < 8; ++d) {
+          const auto word = [&](int h, int e) { return vr[h][e][d >> 2][d & 3]; };
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const bool out = (h ? kb : ka) + 4 * g + e > vl;
-#pragma unroll
-              for (int j = 0; j < kVLoads; ++j) vr[h][e][j] = out ? u32x4{} : vr[h][e][j];
-            }
-          pv(std::false_type{}, tok == t);
+          for (int u = 0; u < 2; ++u) {
+            const unsigned sel = u ? 0x07060302 : 0x05040100;
+            o[2 * d + u] = mfma16x16x32(
+                as_bf16x8(__builtin_amdgcn_perm(word(0, 1), word(0, 0), sel),
+                          __builtin_amdgcn_perm(word(0, 3), word(0, 2), sel),
+                          __builtin_amdgcn_perm(word(1, 1), word(1, 0), sel),
+                          __builtin_amdgcn_perm(word(1, 3), word(1, 2), sel)),
+                pb, o[2 * d + u]);
+          }
         }
       }
       load_v(ahead);
@@ -320,6 +324,10 @@ __global__ __launch_bounds__(64 * kWaves, kFp8 ? 2 : 1) void paged_rows_kernel(
   if (g == 0) {
     mll[wave][col][0] = m;
     mll[wave][col][1] = l;
+  }
+  if (!kList) {
+    const int any = __any(strange);
+    if (lane == 0) odd[wave] = any;
   }
 #pragma unroll
   for (int r = 0; r < 4; ++r)
@@ -342,7 +350,6 @@ __global__ __launch_bounds__(64 * kWaves, kFp8 ? 2 : 1) void paged_rows_kernel(
     lsum += f[x] * mll[x][oc][1];
   }
   const size_t row = t0 + (oc >> 3), qh = head * kGroup + (oc & 7);
-  const float inv = lsum == 0.f ? 0.f : 1.0f / lsum;
   const unsigned rows = kList ? 8 : kCols;
   const size_t part = (slot * c.heads + head) * rows + oc;
 #pragma unroll
@@ -351,17 +358,10 @@ __global__ __launch_bounds__(64 * kWaves, kFp8 ? 2 : 1) void paged_rows_kernel(
     f32x4 v = f32x4{};
 #pragma unroll
     for (int x = 0; x < kWaves; ++x) v += f[x] * *reinterpret_cast<const f32x4*>(&ol[x][oc][d]);
+    if (!kList && oc >= 8 && (odd[0] | odd[1] | odd[2] | odd[3]))
+      add_not_finite<kFp8>(v, c, table, head, lim_max, key1 - 1, key0, d);
     if (single) {
-      bf16x4 r;
-      if (w.gate != nullptr) {
-        const bf16x4 gt = *reinterpret_cast<const bf16x4*>(w.gate + row * w.gate_stride + qh * 2 * kD + kD + d);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) r[e] = f2bf(lsum == 0.f ? 0.f : paged_gate(v[e] * inv, gt[e]));
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) r[e] = f2bf(v[e] * inv);
-      }
-      *reinterpret_cast<bf16x4*>(w.out + (row * hq + qh) * kD + d) = r;
+      paged_store(w, hq, row, qh, d, v, lsum);
     } else {
       *reinterpret_cast<f32x4*>(w.o + part * kD + d) = v;
     }
@@ -372,43 +372,97 @@ __global__ __launch_bounds__(64 * kWaves, kFp8 ? 2 : 1) void paged_rows_kernel(
   }
 }
 
-// Joins the chunks of one row, head and 64 dims: 16 groups of 16 lanes take
-// every 16th chunk each, 4 dims a lane.  Rows that see nothing become zeros.
+// The partials of one row and head.
+struct Parts {
+  size_t first;     // of chunk 0
+  unsigned n;       // chunks (0: the row sees nothing, 1: it is written already)
+  unsigned stride;  // partials between chunks
+};
+__device__ __forceinline__ bool paged_parts(const PagedBatch& b, unsigned heads, const PagedOut& w, unsigned tile,
+                                            unsigned listed_chunks, unsigned t, unsigned qh, Parts& p) {
+  const unsigned seq = __builtin_amdgcn_readfirstlane(paged_find_row(b, (int)t));
+  if (seq >= b.seqs) return false;
+  const PagedSeq s = paged_seq(b, seq);
+  if ((int)t < s.a || (int)t >= s.z) return false;
+  size_t slot;
+  unsigned r;
+  if (listed_chunks != 0) {
+    p.n = s.pos((int)t) < 0 ? 0 : listed_chunks;
+    slot = (size_t)t * listed_chunks;
+    r = qh % kGroup;
+  } else {
+    const unsigned chunk = w.head[0] * kSplitBlock, own = t - s.a, in = own / tile;
+    const int end = s.len - (s.z - s.a) + min((int)((in + 1) * tile), s.z - s.a);
+    p.n = end > 0 ? ((unsigned)end + chunk - 1) / chunk : 0;
+    slot = w.head[1 + seq] + (size_t)in * (((unsigned)s.len + chunk - 1) / chunk);
+    r = own % tile * kGroup + qh % kGroup;
+  }
+  p.stride = heads * kGroup * tile;
+  p.first = (slot * heads + qh / kGroup) * kGroup * tile + r;
+  return true;
+}
+
+// Merges four chunks (absent ones: m = -inf, l = 0, o = 0) into (m, l, o).
+__device__ __forceinline__ void paged_merge4(float& m, float& l, f32x4& o, const float (&cm)[4], const float (&cl)[4],
+                                             const f32x4 (&co)[4]) {
+  const float mn = fmaxf(fmaxf(fmaxf(cm[0], cm[1]), fmaxf(cm[2], cm[3])), m);
+  const float base = mn == -INFINITY ? 0.f : mn;
+  const float a = __builtin_amdgcn_exp2f(m - base);
+  l *= a;
+  o *= a;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const float f = __builtin_amdgcn_exp2f(cm[u] - base);
+    l += f * cl[u];
+    o += f * co[u];
+  }
+  m = mn;
+}
+
+// Many rows of few chunks: a wave per row and head, 4 dims a lane.
+__global__ __launch_bounds__(256) void paged_combine_rows_kernel(PagedBatch b, unsigned heads, PagedOut w,
+                                                                 unsigned tile, unsigned listed_chunks) {
+  const unsigned hq = heads * kGroup;
+  const unsigned i = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned t = i / hq, qh = i % hq;
+  if (t >= b.tokens) return;
+  Parts p;
+  if (!paged_parts(b, heads, w, tile, listed_chunks, t, qh, p) || p.n == 1) return;
+  const unsigned d = (threadIdx.x & 63) * 4;
+  float m = -INFINITY, l = 0.f;
+  f32x4 o = f32x4{};
+  for (unsigned i0 = 0; i0 < p.n; i0 += 4) {
+    float cm[4], cl[4];
+    f32x4 co[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const bool there = i0 + u < p.n;
+      const size_t part = p.first + (size_t)(there ? i0 + u : i0) * p.stride;
+      cm[u] = there ? w.ml[part * 2] : -INFINITY;
+      cl[u] = there ? w.ml[part * 2 + 1] : 0.f;
+      co[u] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(w.o + part * kD + d));
+      if (!there) co[u] = f32x4{};
+    }
+    paged_merge4(m, l, o, cm, cl, co);
+  }
+  paged_store(w, hq, t, qh, d, o, l);
+}
+
+// Few rows of many chunks: a workgroup per row, head and 64 dims; 16 groups of
+// 16 lanes take every 16th chunk each, 4 dims a lane.
 __global__ __launch_bounds__(256) void paged_combine_kernel(PagedBatch b, unsigned heads, PagedOut w,
                                                             unsigned tile, unsigned listed_chunks) {
   __shared__ float acc[4][16][4];
   __shared__ float stat[4][2];
   const unsigned hq = heads * kGroup;
   const unsigned slice = blockIdx.x & 3, qh = (blockIdx.x >> 2) % hq, t = (blockIdx.x >> 2) / hq;
-  const unsigned seq = __builtin_amdgcn_readfirstlane(paged_find_row(b, (int)t));
-  if (seq >= b.seqs) return;
-  const PagedSeq s = paged_seq(b, seq);
-  if ((int)t < s.a || (int)t >= s.z) return;
-  const int pos = s.pos((int)t);
-  unsigned n, rows;
-  size_t first, stride = 1;
-  unsigned r;
-  if (listed_chunks != 0) {
-    n = pos < 0 ? 0 : listed_chunks;
-    first = (size_t)t * listed_chunks;
-    rows = 8;
-    r = qh % kGroup;
-  } else {
-    const unsigned chunk = w.head[0] * kSplitBlock, own = t - s.a;
-    const int end = min((int)(own / tile * tile + tile), s.z - s.a) - (s.z - s.a) + s.len;
-    const unsigned chunks = ((unsigned)s.len + chunk - 1) / chunk;
-    n = end > 0 ? ((unsigned)end + chunk - 1) / chunk : 0;
-    first = w.head[1 + seq] + (size_t)(own / tile) * chunks;
-    rows = 8 * tile;
-    r = own % tile * 8 + qh % kGroup;
-  }
-  if (n == 1) return;
+  Parts p;
+  if (!paged_parts(b, heads, w, tile, listed_chunks, t, qh, p) || p.n == 1) return;
   const int group = threadIdx.x >> 4, wave = threadIdx.x >> 6;
   const unsigned d = slice * 64 + (threadIdx.x & 15) * 4;
-  const unsigned head = qh / kGroup;
   float m = -INFINITY, l = 0.f;
   f32x4 o = f32x4{};
-  for (unsigned i0 = 0; i0 < n; i0 += 64) {   // 4 chunks a group at once
+  for (unsigned i0 = 0; i0 < p.n; i0 += 64) {   // 4 chunks a group at once
     float cm[4], cl[4];
     f32x4 co[4];
 #pragma unroll
@@ -417,27 +471,14 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedBatch b, unsign
       cm[u] = -INFINITY;
       cl[u] = 0.f;
       co[u] = f32x4{};
-      if (i < n) {
-        const size_t part = ((first + i * stride) * heads + head) * rows + r;
+      if (i < p.n) {
+        const size_t part = p.first + (size_t)i * p.stride;
         cm[u] = w.ml[part * 2];
         cl[u] = w.ml[part * 2 + 1];
         co[u] = *reinterpret_cast<const f32x4*>(w.o + part * kD + d);
       }
     }
-    float mn = m;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) mn = fmaxf(mn, cm[u]);
-    const float base = mn == -INFINITY ? 0.f : mn;
-    const float a = __builtin_amdgcn_exp2f(m - base);
-    l *= a;
-    o *= a;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const float f = __builtin_amdgcn_exp2f(cm[u] - base);
-      l += f * cl[u];
-      o += f * co[u];
-    }
-    m = mn;
+    paged_merge4(m, l, o, cm, cl, co);
   }
   // groups of a wave, then the waves
 #pragma unroll
@@ -471,17 +512,7 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedBatch b, unsign
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] += f * acc[x][threadIdx.x][e];
   }
-  const float inv = lsum == 0.f ? 0.f : 1.0f / lsum;
-  bf16x4 res;
-  if (w.gate != nullptr) {
-    const bf16x4 gt = *reinterpret_cast<const bf16x4*>(w.gate + t * w.gate_stride + qh * 2 * kD + kD + d);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) res[e] = f2bf(lsum == 0.f ? 0.f : paged_gate(v[e] * inv, gt[e]));
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) res[e] = f2bf(v[e] * inv);
-  }
-  *reinterpret_cast<bf16x4*>(w.out + ((size_t)t * hq + qh) * kD + d) = res;
+  paged_store(w, hq, t, qh, d, v, lsum);
 }
 
 bool paged_out_of(const void* q, const PagedCache& c, const void* q_gate, unsigned stride, void* out,
@@ -498,13 +529,33 @@ bool paged_out_of(const void* q, const PagedCache& c, const void* q_gate, unsign
   return true;
 }
 
-// Items per KV head that fill the GPU (two workgroups a CU) some times over, so
-// that unequal chunks even out; one sequence takes at most kMaxChunks.
-unsigned rows_target(const PagedBatch& b, unsigned heads) {
-  const unsigned t = 1024u / heads;
-  return t < 64 ? 64 : t;
+// How a call is cut: tokens of a tile, items of a KV head aimed at, items at most.
+struct Plan {
+  unsigned tile, target, items;
+};
+Plan paged_plan(const PagedBatch& b, unsigned heads) {
+  Plan p;
+  const unsigned mean = (b.tokens + b.seqs - 1) / b.seqs;
+  p.tile = mean <= 2 ? 2 : mean <= 8 ? 8 : mean <= 16 ? 16 : 32;
+  if (p.tile == 2) {   // two workgroups a CU, some times over, so that unequal chunks even out
+    p.target = 1024u / heads;
+  } else {
+    // A workgroup of 8 waves a CU, as many of 4, two of 2: the chunks of a tile that
+    // fill whole rounds of the GPU best, each chunk more costing some partials.
+    const unsigned tiles = (b.tokens + p.tile - 1) / p.tile, at_once = p.tile == 32 ? 256 : 512;
+    unsigned best = 1;
+    double least = 1e30;
+    for (unsigned n = 1; n <= 64; ++n) {
+      const double rounds = (double)(((size_t)tiles * heads * n + at_once - 1) / at_once);
+      const double cost = rounds / n * (1.0 + 0.01 * n);
+      if (cost < least) least = cost, best = n;
+    }
+    p.target = tiles * best;
+  }
+  if (p.target < 64) p.target = 64;
+  p.items = paged_items(b, p.tile, p.target);
+  return p;
 }
-
 
 // Keys of a listed chunk: whole blocks, so that all rows' chunks fill the GPU.
 void list_plan(const PagedBatch& b, const PagedCache& c, unsigned listed, ListArgs& l) {
@@ -523,8 +574,15 @@ void list_plan(const PagedBatch& b, const PagedCache& c, unsigned listed, ListAr
 int paged_combine(const PagedBatch& b, const PagedCache& c, const PagedOut& o, unsigned tile,
                   unsigned listed_chunks, void* stream) {
   const unsigned hq = c.heads * kGroup;
-  hipLaunchKernelGGL(paged_combine_kernel, dim3(b.tokens * hq * 4), dim3(256), 0,
-                     static_cast<hipStream_t>(stream), b, c.heads, o, tile, listed_chunks);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  // 2,048 rows of 4 chunks: 217 us with a workgroup per 64 dims, 37 with a wave
+  // per row; one row of 256 chunks: 4 and 12.
+  if (b.tokens >= 256 / c.heads)
+    hipLaunchKernelGGL(paged_combine_rows_kernel, dim3((b.tokens * hq + 3) / 4), dim3(256), 0, st, b, c.heads, o, tile,
+                       listed_chunks);
+  else
+    hipLaunchKernelGGL(paged_combine_kernel, dim3(b.tokens * hq * 4), dim3(256), 0, st, b, c.heads, o, tile,
+                       listed_chunks);
   return static_cast<int>(hipGetLastError());
 }
 
@@ -537,7 +595,8 @@ Q36_EXPORT size_t qwen36_paged_attention_workspace_bytes(const qwen36_paged_cach
   PagedCache c;
   PagedBatch b;
   if (!paged_cache_of(cache, c) || !paged_batch_of(batch, cache->page_tokens, b)) return 0;
-  return split_ws_bytes(b.seqs, paged_items<2>(b, rows_target(b, c.heads)), c.heads, kCols);
+  const Plan p = paged_plan(b, c.heads);
+  return split_ws_bytes(b.seqs, p.items, c.heads, 8 * p.tile);
 }
 
 Q36_EXPORT int qwen36_paged_attention(const void* q, const qwen36_paged_cache* cache,
@@ -551,19 +610,24 @@ Q36_EXPORT int qwen36_paged_attention(const void* q, const qwen36_paged_cache* c
       !paged_out_of(q, c, q_gate, q_gate_row_stride, out, workspace, o) ||
       workspace_bytes < qwen36_paged_attention_workspace_bytes(cache, batch))
     return Q36_EINVAL;
-  const unsigned target = rows_target(b, c.heads), items = paged_items<2>(b, target);
-  split_ws(workspace, b.seqs, items, c.heads, kCols, o);
-  const ListArgs none = {};
-  hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 grid(items * c.heads), block(64 * kWaves);
-  if (cache->cache_type == QWEN36_PAGED_E4M3)
-    hipLaunchKernelGGL((paged_rows_kernel<true, false>), grid, block, 0, st, static_cast<const bf16*>(q), c, b, o,
-                       none, target);
-  else
-    hipLaunchKernelGGL((paged_rows_kernel<false, false>), grid, block, 0, st, static_cast<const bf16*>(q), c, b, o,
-                       none, target);
-  const int e = static_cast<int>(hipGetLastError());
-  return e != Q36_OK ? e : paged_combine(b, c, o, 2, 0, stream);
+  const Plan p = paged_plan(b, c.heads);
+  const bool fp8 = cache->cache_type == QWEN36_PAGED_E4M3;
+  split_ws(workspace, b.seqs, p.items, c.heads, 8 * p.tile, o);
+  int e;
+  if (p.tile == 2) {
+    const ListArgs none = {};
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const dim3 grid(p.items * c.heads), block(64 * kWaves);
+    const bf16* x = static_cast<const bf16*>(q);
+    if (fp8)
+      hipLaunchKernelGGL((paged_rows_kernel<true, false>), grid, block, 0, st, x, c, b, o, none, p.target);
+    else
+      hipLaunchKernelGGL((paged_rows_kernel<false, false>), grid, block, 0, st, x, c, b, o, none, p.target);
+    e = static_cast<int>(hipGetLastError());
+  } else {
+    e = paged_prefill(q, c, fp8, b, o, p.tile, p.items, p.target, stream);
+  }
+  return e != Q36_OK ? e : paged_combine(b, c, o, p.tile, 0, stream);
 }
 
 Q36_EXPORT size_t qwen36_paged_sparse_attention_workspace_bytes(const qwen36_paged_cache* cache,

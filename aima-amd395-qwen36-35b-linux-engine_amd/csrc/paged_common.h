@@ -136,6 +136,50 @@ __device__ __forceinline__ unsigned paged_scale_byte(float amax) {
 }
 __device__ __forceinline__ float paged_scale(unsigned e) { return __uint_as_float(e << 23); }
 
+// Two e4m3 values (one half of w) as bf16, times a power of two: exact.
+template <bool kHi>
+__device__ __forceinline__ unsigned cvt2(unsigned w, float scale) {
+  return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, kHi));
+}
+
+// Ones over the bytes (e4m3) or halves (bf16) of u that are not finite.
+template <bool kFp8>
+__device__ __forceinline__ unsigned not_finite(unsigned u) {
+  if constexpr (kFp8)
+    return ((((u & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu;
+  else
+    return ((((u & 0x7f807f80u) + 0x00800080u) & 0x80008000u) >> 15) * 0xffffu;
+}
+
+// Adds to four dims what is not finite in the V rows of keys [lo, hi] from key
+// `from` on: a weight above zero times it is itself.
+template <bool kFp8>
+__device__ __noinline__ f32x4 sum_not_finite(const char* v, size_t stride, const int* table, unsigned pages,
+                                             unsigned shift, unsigned head, int lo, int hi, int d) {
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  for (int key = lo; key <= hi; ++key) {
+    const unsigned pid = (unsigned)table[key >> shift];
+    if (pid >= pages) continue;
+    const size_t at = ((size_t)head << (shift + 8)) + (size_t)(key & ((1 << shift) - 1)) * kD + d;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (kFp8) {
+        const unsigned x = *reinterpret_cast<const uint8_t*>(v + pid * stride + at + e);
+        if ((x & 0x7fu) == 0x7fu) s[e] += NAN;
+      } else {
+        const float x = bf2f(*reinterpret_cast<const bf16*>(v + pid * stride + 2 * (at + e)));
+        if (!(fabsf(x) < INFINITY)) s[e] += x;
+      }
+    }
+  }
+  return s;
+}
+template <bool kFp8>
+__device__ __forceinline__ void add_not_finite(f32x4& o, const PagedCache& c, const int* table, unsigned head,
+                                               int lo, int hi, int from, int d) {
+  o += sum_not_finite<kFp8>(c.v, c.v_stride, table, c.pages, c.shift, head, max(lo, from), hi, d);
+}
+
 // Host side: the entry points' structures, checked.
 inline bool paged_cache_of(const qwen36_paged_cache* c, PagedCache& o) {
   if (c == nullptr || c->k_pages == nullptr || c->v_pages == nullptr || c->num_pages == 0 ||

@@ -118,15 +118,15 @@ __global__ __launch_bounds__(256) void paged_score_kernel(const bf16* __restrict
   }
 }
 
-// One workgroup per (row, KV head); thread i holds the keys of pages
-// [i kPer, + kPer).
-template <int kPer>
-__global__ __launch_bounds__(256) void paged_pick_kernel(PagedCache c, PagedBatch b,
+// One workgroup of kWaves waves per (row, KV head); thread i holds the keys of
+// pages [i kPer, + kPer).
+template <int kPer, int kWaves>
+__global__ __launch_bounds__(64 * kWaves) void paged_pick_kernel(PagedCache c, PagedBatch b,
                                                          const unsigned* __restrict__ keys,
                                                          unsigned budget, unsigned sinks,
                                                          unsigned recents, int* __restrict__ pages) {
-  __shared__ unsigned cnt[2][4];
-  __shared__ unsigned scan[4];
+  __shared__ unsigned cnt[2][kWaves];
+  __shared__ unsigned scan[kWaves];
   const unsigned head = blockIdx.x % c.heads, t = blockIdx.x / c.heads, tid = threadIdx.x;
   const unsigned wave = tid >> 6;
   const unsigned seq = __builtin_amdgcn_readfirstlane(paged_find_row(b, (int)t));
@@ -137,7 +137,7 @@ __global__ __launch_bounds__(256) void paged_pick_kernel(PagedCache c, PagedBatc
   const unsigned n = pos < 0 ? 0u : ((unsigned)pos >> c.shift) + 1;
   int* out = pages + ((size_t)t * c.heads + head) * budget;
   if (n <= budget) {
-    for (unsigned i = tid; i < budget; i += 256) out[i] = i < n ? (int)i : -1;
+    for (unsigned i = tid; i < budget; i += 64 * kWaves) out[i] = i < n ? (int)i : -1;
     return;
   }
   const unsigned* kp = keys + ((size_t)t * c.heads + head) * b.width;
@@ -156,7 +156,9 @@ __global__ __launch_bounds__(256) void paged_pick_kernel(PagedCache c, PagedBatc
     for (int j = 0; j < kPer; ++j) m += __popcll(__ballot(k[j] >= cand));
     if ((tid & 63) == 0) cnt[bit & 1][wave] = m;
     __syncthreads();
-    m = cnt[bit & 1][0] + cnt[bit & 1][1] + cnt[bit & 1][2] + cnt[bit & 1][3];
+    m = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) m += cnt[bit & 1][w];
     if (m >= budget) v = cand;
     if (m == budget) break;   // exactly the keys >= v
   }
@@ -172,7 +174,7 @@ __global__ __launch_bounds__(256) void paged_pick_kernel(PagedCache c, PagedBatc
   if ((tid & 63) == 63) scan[wave] = in;
   __syncthreads();
   unsigned total = 0;
-  for (unsigned w = 0; w < 4; ++w) {
+  for (unsigned w = 0; w < kWaves; ++w) {
     const unsigned x = scan[w];
     if (w < wave) in += x;
     total += x;
@@ -226,11 +228,13 @@ Q36_EXPORT int qwen36_paged_select(const void* q, const qwen36_paged_cache* cach
     if (e != Q36_OK) return e;
   }
   const dim3 grid(b.tokens * c.heads);
+  // up to 2,048 pages in 4 waves of 8 a lane, up to the longest sequence's 16,391
+  // in 16 waves of 17
   if (b.width <= 2048)
-    hipLaunchKernelGGL(paged_pick_kernel<8>, grid, dim3(256), 0, st, c, b, keys, budget, sink_pages,
+    hipLaunchKernelGGL((paged_pick_kernel<8, 4>), grid, dim3(256), 0, st, c, b, keys, budget, sink_pages,
                        recent_pages, static_cast<int*>(pages));
   else
-    hipLaunchKernelGGL(paged_pick_kernel<65>, grid, dim3(256), 0, st, c, b, keys, budget, sink_pages,
+    hipLaunchKernelGGL((paged_pick_kernel<17, 16>), grid, dim3(1024), 0, st, c, b, keys, budget, sink_pages,
                        recent_pages, static_cast<int*>(pages));
   return static_cast<int>(hipGetLastError());
 }

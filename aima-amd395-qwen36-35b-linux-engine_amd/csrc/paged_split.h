@@ -88,9 +88,8 @@ __device__ __forceinline__ bool paged_split(const PagedBatch& b, unsigned item, 
 }
 
 // Items of a KV head at most, for the grid and the workspace.
-template <unsigned kTile>
-inline unsigned paged_items(const PagedBatch& b, unsigned target) {
-  const unsigned t = b.tokens / kTile + b.seqs;
+inline unsigned paged_items(const PagedBatch& b, unsigned tile, unsigned target) {
+  const unsigned t = b.tokens / tile + b.seqs;
   return (t < b.tokens ? t : b.tokens) + target;
 }
 
@@ -112,15 +111,12 @@ inline void split_ws(void* ws, unsigned seqs, size_t slots, unsigned heads, unsi
   o.o = reinterpret_cast<float*>(p);
 }
 
-// The target for tiles of kTile tokens.
-unsigned paged_target_rows(const PagedBatch& b, unsigned heads);
 // Joins the partials of tiles of `tile` tokens; listed_chunks != 0: every row
 // has that many slots.  Rows of one chunk are already written.
 int paged_combine(const PagedBatch& b, const PagedCache& c, const PagedOut& o, unsigned tile,
                   unsigned listed_chunks, void* stream);
-// Tiles of 32 tokens, for prompts (paged_prefill.hip).
-size_t paged_prefill_ws(const PagedBatch& b, const PagedCache& c);
-int paged_prefill(const void* q, const PagedCache& c, bool fp8, const PagedBatch& b, PagedOut o,
-                  void* ws, void* stream);
+// Tiles of 8, 16 or 32 tokens (paged_prefill.hip).
+int paged_prefill(const void* q, const PagedCache& c, bool fp8, const PagedBatch& b, const PagedOut& o,
+                  unsigned tile, unsigned items, unsigned target, void* stream);
 
 }  // namespace q36
