@@ -32,6 +32,14 @@ constexpr int kNoKeys = 0x40000000;
 constexpr float kScoreScale = 0.0625f * kLog2e;
 
 
+// A cache streams through once (nontemporal: 127 us against 128 for 32 sequences),
+// listed pages are shared by rows (plain: 132 against 204 for a turn of 300).
+template <bool kOnce>
+__device__ __forceinline__ u32x4 load16(const char* p) {
+  const u32x4* x = reinterpret_cast<const u32x4*>(p);
+  return kOnce ? __builtin_nontemporal_load(x) : *x;
+}
+
 __device__ __forceinline__ bf16x8 as_bf16x8(unsigned a, unsigned b, unsigned c, unsigned d) {
   const u32x4 v = {a, b, c, d};
   return __builtin_bit_cast(bf16x8, v);
@@ -82,10 +90,8 @@ __global__ __launch_bounds__(64 * kWaves, kFp8 ? 2 : 1) void paged_rows_kernel(
   if constexpr (kList) {
     t0 = (int)(item / list.chunks);
     const unsigned chunk = item % list.chunks;
-    seq = __builtin_amdgcn_readfirstlane(paged_find_row(b, t0));
-    if (seq >= b.seqs) return;
-    const PagedSeq s = paged_seq(b, seq);
-    if (t0 < s.a || t0 >= s.z) return;
+    PagedSeq s;
+    if (!paged_find_row(b, t0, seq, s)) return;
     pos0 = s.pos(t0);
     if (pos0 < 0 && list.chunks > 1) return;   // the joining launch writes its zeros
     n_tok = 1;
@@ -177,7 +183,7 @@ __global__ __launch_bounds__(64 * kWaves, kFp8 ? 2 : 1) void paged_rows_kernel(
         const char* p = c.k + pid * c.k_stride + (head_off + (size_t)row * kD) * kElem;
 #pragma unroll
         for (int j = 0; j < kKLoads; ++j)
-          kr[h][j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + koff + 64 * j));
+          kr[h][j] = load16<!kList>(p + koff + 64 * j);
       }
     };
     const auto load_v = [&](int i) {
@@ -190,8 +196,7 @@ __global__ __launch_bounds__(64 * kWaves, kFp8 ? 2 : 1) void paged_rows_kernel(
         for (int e = 0; e < 4; ++e)
 #pragma unroll
           for (int j = 0; j < kVLoads; ++j)
-            vr[h][e][j] = __builtin_nontemporal_load(
-                reinterpret_cast<const u32x4*>(p + voff + e * kD * kElem + 16 * j));
+            vr[h][e][j] = load16<!kList>(p + voff + e * kD * kElem + 16 * j);
       }
     };
     load_k(0);
@@ -380,10 +385,9 @@ struct Parts {
 };
 __device__ __forceinline__ bool paged_parts(const PagedBatch& b, unsigned heads, const PagedOut& w, unsigned tile,
                                             unsigned listed_chunks, unsigned t, unsigned qh, Parts& p) {
-  const unsigned seq = __builtin_amdgcn_readfirstlane(paged_find_row(b, (int)t));
-  if (seq >= b.seqs) return false;
-  const PagedSeq s = paged_seq(b, seq);
-  if ((int)t < s.a || (int)t >= s.z) return false;
+  unsigned seq;
+  PagedSeq s;
+  if (!paged_find_row(b, (int)t, seq, s)) return false;
   size_t slot;
   unsigned r;
   if (listed_chunks != 0) {
@@ -562,7 +566,7 @@ void list_plan(const PagedBatch& b, const PagedCache& c, unsigned listed, ListAr
   const size_t keys = (size_t)listed << c.shift;
   const size_t rows = (size_t)b.tokens * c.heads;
   const size_t blocks = (keys + kSplitBlock - 1) / kSplitBlock;
-  const size_t want = (1024 + rows - 1) / rows;                 // chunks of a row
+  const size_t want = rows >= 512 ? 1 : 512 / rows;   // chunks of a row: two workgroups a CU at once
   const size_t per = want >= blocks ? 1 : (blocks + want - 1) / want;
   l.chunk_keys = (unsigned)(per * kSplitBlock);
   l.chunks = (unsigned)((blocks + per - 1) / per);
@@ -575,8 +579,8 @@ int paged_combine(const PagedBatch& b, const PagedCache& c, const PagedOut& o, u
                   unsigned listed_chunks, void* stream) {
   const unsigned hq = c.heads * kGroup;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  // 2,048 rows of 4 chunks: 217 us with a workgroup per 64 dims, 37 with a wave
-  // per row; one row of 256 chunks: 4 and 12.
+  // 2,048 tokens: 217 us with a workgroup per 64 dims (4 chunks), 24 with a wave per
+  // row (2 chunks).
   if (b.tokens >= 256 / c.heads)
     hipLaunchKernelGGL(paged_combine_rows_kernel, dim3((b.tokens * hq + 3) / 4), dim3(256), 0, st, b, c.heads, o, tile,
                        listed_chunks);

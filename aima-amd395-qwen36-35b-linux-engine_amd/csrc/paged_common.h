@@ -55,9 +55,26 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedBatch& b, unsigned i) {
   return s;
 }
 
-// The sequence that holds row t, by one wave with one load per 64 sequences;
-// seqs where none does.
-__device__ __forceinline__ unsigned paged_find_row(const PagedBatch& b, int t) {
+// The sequence that holds row t, and where it stands; false where none does.
+// By one wave: up to 64 sequences are looked at in one round of loads, more by a
+// search with a load per 64 and a second round.
+__device__ __forceinline__ bool paged_find_row(const PagedBatch& b, int t, unsigned& seq, PagedSeq& s) {
+  if (b.seqs == 1) {
+    seq = 0;
+    s = paged_seq(b, 0);
+    return t >= s.a && t < s.z;
+  }
+  if (b.seqs <= 64) {
+    const unsigned i = min(threadIdx.x & 63, b.seqs - 1);
+    const PagedSeq mine = paged_seq(b, i);
+    const unsigned long long in = __ballot(t >= mine.a && t < mine.z);
+    if (in == 0) return false;
+    seq = __ffsll(in) - 1;
+    s.a = __builtin_amdgcn_readlane(mine.a, seq);
+    s.z = __builtin_amdgcn_readlane(mine.z, seq);
+    s.len = __builtin_amdgcn_readlane(mine.len, seq);
+    return true;
+  }
   const unsigned lane = threadIdx.x & 63;
   unsigned n = 0;
   for (unsigned i0 = 0; i0 < b.seqs; i0 += 64) {
@@ -66,7 +83,10 @@ __device__ __forceinline__ unsigned paged_find_row(const PagedBatch& b, int t) {
     n += __popcll(done);
     if (done != ~0ull) break;
   }
-  return n;
+  seq = __builtin_amdgcn_readfirstlane(n);
+  if (seq >= b.seqs) return false;
+  s = paged_seq(b, seq);
+  return t >= s.a && t < s.z;
 }
 
 __device__ __forceinline__ unsigned wave_scan_add(unsigned v) {

@@ -12,8 +12,8 @@
 // so the score of 16 pages for 8 heads is a chain of 8 int8 matrix products of
 // 64 dims.  Bound by the bounds' bytes (512 a page and KV head) and, for few
 // rows, by latency: a launch that scores over the whole GPU and one workgroup
-// per (row, KV head) that selects, its keys in registers, by bisecting the
-// key's 32 bits (a ballot and a scalar bit count per 64 keys and step).
+// per (row, KV head) that selects, its keys in registers, by halving their
+// range.
 #include "paged_common.h"
 
 namespace q36 {
@@ -39,14 +39,31 @@ __global__ __launch_bounds__(256) void paged_score_kernel(const bf16* __restrict
   const unsigned t = blockIdx.x / c.heads / blocks;
   const int lane = threadIdx.x & 63, col = lane & 7, row = lane & 15, g = lane >> 4;
   const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const unsigned seq = __builtin_amdgcn_readfirstlane(paged_find_row(b, (int)t));
-  if (seq >= b.seqs) return;
-  const PagedSeq s = paged_seq(b, seq);
+  unsigned seq;
+  PagedSeq s;
+  if (!paged_find_row(b, (int)t, seq, s)) return;
   const int pos = s.pos((int)t);
-  if ((int)t < s.a || (int)t >= s.z || pos < 0) return;
+  if (pos < 0) return;
   const unsigned n = ((unsigned)pos >> c.shift) + 1;
   const unsigned p0 = (block * 4 + wave) * per_wave * 16;
   if (p0 >= n) return;
+
+  const int* table = b.table + seq * b.table_stride;
+  unsigned* kp = keys + ((size_t)t * c.heads + head) * b.width;
+  i32x4 a[8];
+  unsigned e;
+  bool there;
+  const auto load = [&](unsigned first) {   // 16 pages' bounds and scales; pages of none read page 0
+    const unsigned mine = first + row;
+    unsigned pid = mine < n ? (unsigned)table[mine] : ~0u;
+    there = pid < c.pages;
+    if (!there) pid = 0;
+    const int8_t* bp = c.bounds + ((size_t)pid * c.heads + head) * 2 * kD + 16 * g;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) a[j] = *reinterpret_cast<const i32x4*>(bp + 64 * j);
+    e = c.k_exp[(size_t)pid * c.heads + head];
+  };
+  load(p0);   // on the way while the queries are quantised
 
   // this lane's 64 dims of its head: 64 j + 16 g + [0, 16)
   const bf16* qp = q + ((size_t)t * c.heads * kGroup + head * kGroup + col) * kD + 16 * g;
@@ -63,47 +80,37 @@ __global__ __launch_bounds__(256) void paged_score_kernel(const bf16* __restrict
     }
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) amax = max(amax, (unsigned)__shfl_xor(amax, o, 64));
-  // q * 2^-f with the largest in [64, 128), in two factors (f may be past one's range)
-  const int f = (int)(amax >> 23) - 127 - 6;
-  const float f1 = ldexpf(1.f, -f / 2), f2 = ldexpf(1.f, -f - (-f / 2));
+  // in steps that put the largest in [64, 128) (and are 2^-127 at least)
+  const float f = ldexpf(1.f, min(127 + 6 - (int)(amax >> 23), 127));
   i32x4 qpos[4], qneg[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j)
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      unsigned up = 0, un = 0;
+      unsigned i[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float v = bf2f(x[2 * j + (w >> 1)][4 * (w & 1) + e]);
-        const float r = v == v ? fminf(fmaxf(rintf(v * f1 * f2), -127.f), 127.f) : 0.f;
-        const int i = (int)r;
-        up |= (unsigned)max(i, 0) << (8 * e);
-        un |= ((unsigned)min(i, 0) & 0xffu) << (8 * e);
+        i[e] = (unsigned)(int)(v == v ? __builtin_amdgcn_fmed3f(rintf(v * f), -127.f, 127.f) : 0.f);
       }
-      qpos[j][w] = (int)up;
-      qneg[j][w] = (int)un;
+      const unsigned lo = __builtin_amdgcn_perm(i[1], i[0], 0x0c0c0400), hi = __builtin_amdgcn_perm(i[3], i[2], 0x04000c0c);
+      const unsigned all = lo | hi, sign = ((all >> 7) & 0x01010101u) * 0xffu;
+      qpos[j][w] = (int)(all & ~sign);
+      qneg[j][w] = (int)(all & sign);
     }
 
-  const int* table = b.table + seq * b.table_stride;
-  unsigned* kp = keys + ((size_t)t * c.heads + head) * b.width;
   for (unsigned i = 0; i < per_wave; ++i) {
     const unsigned first = p0 + 16 * i;
     if (first >= n) break;
-    const unsigned mine = first + row;
-    unsigned pid = mine < n ? (unsigned)table[mine] : ~0u;
-    const bool there = pid < c.pages;
-    if (!there) pid = 0;
-    const int8_t* bp = c.bounds + ((size_t)pid * c.heads + head) * 2 * kD + 16 * g;
-    i32x4 a[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) a[j] = *reinterpret_cast<const i32x4*>(bp + 64 * j);
-    const unsigned e = c.k_exp[(size_t)pid * c.heads + head];
     i32x4 d = {0, 0, 0, 0};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       d = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[j], qpos[j], d, 0, 0, 0);
       d = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[4 + j], qneg[j], d, 0, 0, 0);
     }
+    const unsigned e_now = e;
+    const bool there_now = there;
+    if (i + 1 < per_wave && first + 16 < n) load(first + 16);
     // lane: pages 4 g + r of its head; the largest over the heads
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -111,8 +118,8 @@ __global__ __launch_bounds__(256) void paged_score_kernel(const bf16* __restrict
 #pragma unroll
       for (int o = 1; o < 8; o <<= 1) v = max(v, __shfl_xor(v, o, 64));
       const int from = 4 * g + r;
-      const unsigned pe = __shfl(e, from, 64);
-      const bool ok = __shfl((int)there, from, 64);
+      const unsigned pe = __shfl(e_now, from, 64);
+      const bool ok = __shfl((int)there_now, from, 64);
       if (row == r && first + from < n) kp[first + from] = ok ? score_key(v, pe) : 1u;
     }
   }
@@ -129,10 +136,13 @@ __global__ __launch_bounds__(64 * kWaves) void paged_pick_kernel(PagedCache c, P
   __shared__ unsigned scan[kWaves];
   const unsigned head = blockIdx.x % c.heads, t = blockIdx.x / c.heads, tid = threadIdx.x;
   const unsigned wave = tid >> 6;
-  const unsigned seq = __builtin_amdgcn_readfirstlane(paged_find_row(b, (int)t));
-  if (seq >= b.seqs) return;
-  const PagedSeq s = paged_seq(b, seq);
-  if ((int)t < s.a || (int)t >= s.z) return;
+  const unsigned* kp = keys + ((size_t)t * c.heads + head) * b.width;
+  unsigned k[kPer];   // asked for before the row's length is known: what lies behind it is dropped below
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) k[j] = kp[min(tid * kPer + j, b.width - 1)];
+  unsigned seq;
+  PagedSeq s;
+  if (!paged_find_row(b, (int)t, seq, s)) return;
   const int pos = s.pos((int)t);
   const unsigned n = pos < 0 ? 0u : ((unsigned)pos >> c.shift) + 1;
   int* out = pages + ((size_t)t * c.heads + head) * budget;
@@ -140,16 +150,36 @@ __global__ __launch_bounds__(64 * kWaves) void paged_pick_kernel(PagedCache c, P
     for (unsigned i = tid; i < budget; i += 64 * kWaves) out[i] = i < n ? (int)i : -1;
     return;
   }
-  const unsigned* kp = keys + ((size_t)t * c.heads + head) * b.width;
-  unsigned k[kPer];
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
     const unsigned p = tid * kPer + j;
-    k[j] = p >= n ? 0u : p < sinks || p + recents >= n ? ~0u : kp[p];
+    k[j] = p >= n ? 0u : p < sinks || p + recents >= n ? ~0u : k[j];
   }
-  // largest v with at least `budget` keys >= v, bit by bit
-  unsigned v = 0, equal = 0;
-  for (int bit = 31; bit >= 0; --bit) {
+  // Largest v with at least `budget` keys >= v, bit by bit below the bits that all
+  // scores share: a ballot and a scalar bit count per 64 keys, one exchange between
+  // the waves.
+  unsigned hi = 0, lo = ~0u;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j)
+    if (k[j] != 0 && k[j] != ~0u) hi = max(hi, k[j]), lo = min(lo, k[j]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    hi = max(hi, (unsigned)__shfl_xor(hi, o, 64));
+    lo = min(lo, (unsigned)__shfl_xor(lo, o, 64));
+  }
+  if ((tid & 63) == 0) {
+    cnt[0][wave] = hi;
+    cnt[1][wave] = lo;
+  }
+  __syncthreads();
+  for (int w = 0; w < kWaves; ++w) {
+    hi = max(hi, cnt[0][w]);
+    lo = min(lo, cnt[1][w]);
+  }
+  __syncthreads();
+  const int top = hi == lo ? -1 : 31 - __clz(hi ^ lo);   // the highest bit that differs
+  unsigned v = top < 0 ? hi : hi >> top >> 1 << top << 1, equal = 0;
+  for (int bit = top; bit >= 0; --bit) {
     const unsigned cand = v | (1u << bit);
     unsigned m = 0;
 #pragma unroll
@@ -219,7 +249,7 @@ Q36_EXPORT int qwen36_paged_select(const void* q, const qwen36_paged_cache* cach
   unsigned* keys = static_cast<unsigned*>(workspace);
   if (b.width > budget) {   // else every row takes all its pages
     const size_t rows = (size_t)b.tokens * c.heads, groups = (b.width + 63) / 64;
-    size_t per = rows * groups / 8192;   // 16-page groups a wave takes
+    size_t per = rows * groups / 512;   // 16-page groups a wave takes: the queries are quantised once
     per = per < 1 ? 1 : per > 16 ? 16 : per;
     const unsigned blocks = (unsigned)((groups + per - 1) / per);
     hipLaunchKernelGGL(paged_score_kernel, dim3((unsigned)(rows * blocks)), dim3(256), 0, st,
@@ -228,13 +258,15 @@ Q36_EXPORT int qwen36_paged_select(const void* q, const qwen36_paged_cache* cach
     if (e != Q36_OK) return e;
   }
   const dim3 grid(b.tokens * c.heads);
-  // up to 2,048 pages in 4 waves of 8 a lane, up to the longest sequence's 16,391
-  // in 16 waves of 17
+  const auto pick = [&](auto kernel, unsigned threads) {
+    hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, st, c, b, keys, budget, sink_pages, recent_pages,
+                       static_cast<int*>(pages));
+  };
   if (b.width <= 2048)
-    hipLaunchKernelGGL((paged_pick_kernel<8, 4>), grid, dim3(256), 0, st, c, b, keys, budget, sink_pages,
-                       recent_pages, static_cast<int*>(pages));
-  else
-    hipLaunchKernelGGL((paged_pick_kernel<17, 16>), grid, dim3(1024), 0, st, c, b, keys, budget, sink_pages,
-                       recent_pages, static_cast<int*>(pages));
+    pick(paged_pick_kernel<8, 4>, 256);
+  else if (b.width <= 4352)   // 2,049 pages: 16 waves 20 us, 4 waves 9
+    pick(paged_pick_kernel<17, 4>, 256);
+  else                        // up to the longest sequence's 16,391
+    pick(paged_pick_kernel<17, 16>, 1024);
   return static_cast<int>(hipGetLastError());
 }

@@ -14,17 +14,17 @@ are left as they were.  All arithmetic runs in ``libqwen36_attn.so``.
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
-from ._tensors import ptr, require, stream_handle
+from ._tensors import ptr, require
 from .full_attention import HEAD_DIM, HKV, HQ, MAX_TOKENS
 
 GROUP = HQ // HKV
 PAGE_TOKENS = (16, 32, 64, 128)
 MAX_LISTED = 1024
+# torch.cuda.current_stream(device).cuda_stream without the Stream object (1.9 us a call)
+_stream = torch._C._cuda_getCurrentRawStream
 _TYPES = {torch.bfloat16: 0, torch.float8_e4m3fn: 1}
 
 
@@ -94,6 +94,7 @@ class PagedKVCache:
         self.heads = heads * GROUP
         self.device = k_pages.device
         stride = [t.stride(0) if n > 1 else heads * page * HEAD_DIM for t in (k_pages, v_pages)]
+        self._index = k_pages.get_device()
         self._args = _lib.PagedCacheArgs(ptr(k_pages), ptr(v_pages), ptr(k_exp),
                                          ptr(v_exp) if fp8 else None, ptr(bounds), stride[0],
                                          stride[1], n, page, heads, _TYPES[k_pages.dtype])
@@ -108,48 +109,43 @@ class PagedKVCache:
 
 
 def _batch(cache: PagedKVCache, tokens: int, page_table, cu_tokens, seq_lens) -> _lib.PagedBatchArgs:
-    for name, t in (("page_table", page_table), ("cu_tokens", cu_tokens), ("seq_lens", seq_lens)):
-        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != cache.device:
+    index = cache._index
+    for name, t, dims in (("page_table", page_table, 2), ("cu_tokens", cu_tokens, 1), ("seq_lens", seq_lens, 1)):
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.get_device() != index:
             raise ValueError(f"{name} must be an int32 tensor on the cache's device")
-    seqs = seq_lens.shape[0] if seq_lens.dim() == 1 else 0
-    if seqs < 1 or cu_tokens.shape != (seqs + 1,) or page_table.dim() != 2 or page_table.shape[0] != seqs:
+        if t.dim() != dims or (dims == 1 and not t.is_contiguous()):
+            raise ValueError("a batch is page_table [seqs, width], contiguous cu_tokens [seqs + 1] and seq_lens [seqs]")
+    seqs, (rows, width) = seq_lens.shape[0], page_table.shape
+    if seqs < 1 or cu_tokens.shape[0] != seqs + 1 or rows != seqs or width < 1:
         raise ValueError("a batch is page_table [seqs, width], cu_tokens [seqs + 1] and seq_lens [seqs]")
-    width = page_table.shape[1]
-    if (width < 1 or (width > 1 and page_table.stride(1) != 1) or not cu_tokens.is_contiguous()
-            or not seq_lens.is_contiguous()):
-        raise ValueError("page_table must have contiguous rows, cu_tokens and seq_lens be contiguous")
+    stride, inner = page_table.stride()
+    if width > 1 and inner != 1 or seqs > 1 and stride < width:
+        raise ValueError("page_table must have contiguous rows that do not overlap")
     if width * cache.page_tokens > MAX_TOKENS + 127:
         raise ValueError(f"a sequence has at most {MAX_TOKENS} tokens")
-    stride = page_table.stride(0) if seqs > 1 else width
-    if stride < width:
-        raise ValueError("page_table's rows must not overlap")
-    if not 0 < tokens <= MAX_TOKENS:
-        raise ValueError(f"a call has 1 to {MAX_TOKENS} rows")
-    if seqs > 65536:
-        raise ValueError("a batch has at most 65536 sequences")
+    if not 0 < tokens <= MAX_TOKENS or seqs > 65536:
+        raise ValueError(f"a call has 1 to {MAX_TOKENS} rows of at most 65536 sequences")
     return _lib.PagedBatchArgs(page_table.data_ptr(), cu_tokens.data_ptr(), seq_lens.data_ptr(),
-                               stride, width, seqs, tokens)
+                               stride if seqs > 1 else width, width, seqs, tokens)
 
 
-def _rows(t, name: str, rows: int, width: int, device) -> int:
+def _rows(t, name: str, rows: int, width: int, index: int) -> int:
     """Row stride of a bf16 [rows, width] tensor with unit inner stride."""
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16 or t.device != device:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16 or t.get_device() != index:
         raise ValueError(f"{name} must be a bf16 tensor on the cache's device")
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != width or (width > 1 and t.stride(1) != 1):
+    if t.shape != (rows, width) or t.stride(1) != 1:
         raise ValueError(f"{name} must be [{rows}, {width}] with unit inner stride")
     stride = t.stride(0) if rows > 1 else width
     if stride < width or stride % 4 or t.data_ptr() % 8:
-        raise ValueError(f"{name}'s rows must be 8-byte aligned")
+        raise ValueError(f"{name}'s rows must be 8-byte aligned and not overlap")
     return stride
 
 
 def _queries(q, cache: PagedKVCache) -> int:
-    if not isinstance(q, torch.Tensor) or q.dtype != torch.bfloat16 or q.device != cache.device:
+    if not isinstance(q, torch.Tensor) or q.dtype != torch.bfloat16 or q.get_device() != cache._index:
         raise ValueError("q must be a bf16 tensor on the cache's device")
-    if q.dim() != 3 or q.shape[1] != cache.heads or q.shape[2] != HEAD_DIM or not q.is_contiguous():
-        raise ValueError(f"q must be contiguous [T, {cache.heads}, 256]")
-    if q.data_ptr() % 16:
-        raise ValueError("q must be 16-byte aligned")
+    if q.dim() != 3 or q.shape[1:] != (cache.heads, HEAD_DIM) or not q.is_contiguous() or q.data_ptr() % 16:
+        raise ValueError(f"q must be contiguous [T, {cache.heads}, 256], 16-byte aligned")
     return q.shape[0]
 
 
@@ -160,6 +156,18 @@ def _out(out, shape, dtype, device) -> torch.Tensor:
             or tuple(out.shape) != shape or not out.is_contiguous() or out.data_ptr() % 8:
         raise ValueError(f"out must be contiguous {dtype} {list(shape)} on the cache's device")
     return out
+
+
+def _call(cache: PagedKVCache, name: str, *args) -> None:
+    """The entry point on the cache's device and its current stream."""
+    fn = getattr(_lib.load(), name)
+    if torch.cuda.current_device() == cache._index:
+        status = fn(*args, _stream(cache._index))
+    else:
+        with torch.cuda.device(cache._index):
+            status = fn(*args, _stream(cache._index))
+    if status != 0:
+        raise _lib.KernelError(f"{name} failed: hip_status={status}")
 
 
 # The workspaces below are allocated per call: calls on several streams, and
@@ -177,34 +185,35 @@ def paged_append(q_gate: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm:
     device)``.  An e4m3 page's scale fits its largest value and grows with it;
     a page that gets rows must belong to one sequence.  Returns q [T, heads,
     256] bf16."""
-    dev = cache.device
+    dev, index = cache.device, cache._index
     t = q_gate.shape[0] if isinstance(q_gate, torch.Tensor) and q_gate.dim() == 2 else 0
     batch = _batch(cache, t, page_table, cu_tokens, seq_lens)
-    qs = _rows(q_gate, "q_gate", t, 2 * cache.heads * HEAD_DIM, dev)
-    ks = _rows(k, "k", t, cache.kv_heads * HEAD_DIM, dev)
-    vs = _rows(v, "v", t, cache.kv_heads * HEAD_DIM, dev)
-    for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
-        require(w, name, torch.bfloat16, shape=(HEAD_DIM,))
+    qs = _rows(q_gate, "q_gate", t, 2 * cache.heads * HEAD_DIM, index)
+    ks = _rows(k, "k", t, cache.kv_heads * HEAD_DIM, index)
+    vs = _rows(v, "v", t, cache.kv_heads * HEAD_DIM, index)
     cos, sin = rope
-    for name, w in (("cos", cos), ("sin", sin)):
-        require(w, name, torch.float32, shape=(cos.shape[0], 32))
-        if w.data_ptr() % 16 or w.shape[0] < 1:
-            raise ValueError(f"{name} must be 16-byte aligned [positions, 32]")
-    for name, w in (("q_norm", q_norm), ("k_norm", k_norm), ("cos", cos), ("sin", sin)):
-        if w.device != dev:
-            raise ValueError(f"{name} must be on the cache's device")
+    if not (isinstance(q_norm, torch.Tensor) and isinstance(k_norm, torch.Tensor)
+            and q_norm.dtype == k_norm.dtype == torch.bfloat16 and q_norm.get_device() == index
+            and k_norm.get_device() == index and q_norm.shape == k_norm.shape == (HEAD_DIM,)
+            and q_norm.is_contiguous() and k_norm.is_contiguous()):
+        raise ValueError("q_norm and k_norm must be contiguous bf16 [256] on the cache's device")
+    if not (isinstance(cos, torch.Tensor) and isinstance(sin, torch.Tensor)
+            and cos.dtype == sin.dtype == torch.float32 and cos.get_device() == index
+            and sin.get_device() == index and cos.dim() == 2 and cos.shape[1] == 32
+            and cos.shape == sin.shape and cos.shape[0] > 0 and cos.is_contiguous()
+            and sin.is_contiguous() and not (cos.data_ptr() | sin.data_ptr()) % 16):
+        raise ValueError("rope must be two 16-byte aligned fp32 [positions, 32] on the cache's device")
     q_out = _out(q_out, (t, cache.heads, HEAD_DIM), torch.bfloat16, dev)
-    with torch.cuda.device(dev):
-        _lib.call("qwen36_paged_append", ptr(q_gate), qs, ptr(k), ks, ptr(v), vs, ptr(q_norm),
-                  ptr(k_norm), ptr(cos), ptr(sin), cos.shape[0], ctypes.byref(cache._args),
-                  ctypes.byref(batch), ptr(q_out), stream_handle(dev))
+    _call(cache, "qwen36_paged_append", q_gate.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
+          q_norm.data_ptr(), k_norm.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
+          cache._args, batch, q_out.data_ptr())
     return q_out
 
 
 def _gate(q_gate, t: int, cache: PagedKVCache) -> tuple[int | None, int]:
     if q_gate is None:
         return None, 0
-    return q_gate.data_ptr(), _rows(q_gate, "q_gate", t, 2 * cache.heads * HEAD_DIM, cache.device)
+    return q_gate.data_ptr(), _rows(q_gate, "q_gate", t, 2 * cache.heads * HEAD_DIM, cache._index)
 
 
 def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tensor,
@@ -221,12 +230,10 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
     batch = _batch(cache, t, page_table, cu_tokens, seq_lens)
     gate, gs = _gate(q_gate, t, cache)
     out = _out(out, (t, cache.heads * HEAD_DIM), torch.bfloat16, dev)
-    lib = _lib.load(("qwen36_paged_attention",))
-    nb = lib.qwen36_paged_attention_workspace_bytes(ctypes.byref(cache._args), ctypes.byref(batch))
+    nb = _lib.load().qwen36_paged_attention_workspace_bytes(cache._args, batch)
     ws = torch.empty(nb, dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        _lib.call("qwen36_paged_attention", ptr(q), ctypes.byref(cache._args), ctypes.byref(batch),
-                  gate, gs, ptr(out), ptr(ws), nb, stream_handle(dev))
+    _call(cache, "qwen36_paged_attention", q.data_ptr(), cache._args, batch, gate, gs, out.data_ptr(),
+          ws.data_ptr(), nb)
     return out
 
 
@@ -248,12 +255,10 @@ def select_pages(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tensor,
     if not (sink_pages >= 0 and recent_pages >= 1 and sink_pages + recent_pages <= budget <= MAX_LISTED):
         raise ValueError(f"sink_pages + recent_pages (>= 1) <= budget <= {MAX_LISTED}")
     out = _out(out, (t, cache.kv_heads, budget), torch.int32, dev)
-    lib = _lib.load(("qwen36_paged_select",))
-    nb = lib.qwen36_paged_select_workspace_bytes(ctypes.byref(cache._args), ctypes.byref(batch))
+    nb = _lib.load().qwen36_paged_select_workspace_bytes(cache._args, batch)
     ws = torch.empty(nb, dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        _lib.call("qwen36_paged_select", ptr(q), ctypes.byref(cache._args), ctypes.byref(batch),
-                  budget, sink_pages, recent_pages, ptr(out), ptr(ws), nb, stream_handle(dev))
+    _call(cache, "qwen36_paged_select", q.data_ptr(), cache._args, batch, budget, sink_pages,
+          recent_pages, out.data_ptr(), ws.data_ptr(), nb)
     return out
 
 
@@ -268,22 +273,18 @@ def sparse_paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: tor
     dev = cache.device
     t = _queries(q, cache)
     batch = _batch(cache, t, page_table, cu_tokens, seq_lens)
-    if not isinstance(pages, torch.Tensor) or pages.dtype != torch.int32 or pages.device != dev:
+    if not isinstance(pages, torch.Tensor) or pages.dtype != torch.int32 or pages.get_device() != cache._index:
         raise ValueError("pages must be an int32 tensor on the cache's device")
     if (pages.dim() != 3 or pages.shape[:2] != (t, cache.kv_heads) or not pages.is_contiguous()
             or not 1 <= pages.shape[2] <= MAX_LISTED):
         raise ValueError(f"pages must be contiguous [T, {cache.kv_heads}, 1..{MAX_LISTED}]")
     gate, gs = _gate(q_gate, t, cache)
     out = _out(out, (t, cache.heads * HEAD_DIM), torch.bfloat16, dev)
-    lib = _lib.load(("qwen36_paged_sparse_attention",))
     listed = pages.shape[2]
-    nb = lib.qwen36_paged_sparse_attention_workspace_bytes(ctypes.byref(cache._args),
-                                                           ctypes.byref(batch), listed)
+    nb = _lib.load().qwen36_paged_sparse_attention_workspace_bytes(cache._args, batch, listed)
     ws = torch.empty(nb, dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        _lib.call("qwen36_paged_sparse_attention", ptr(q), ctypes.byref(cache._args),
-                  ctypes.byref(batch), ptr(pages), listed, gate, gs, ptr(out), ptr(ws), nb,
-                  stream_handle(dev))
+    _call(cache, "qwen36_paged_sparse_attention", q.data_ptr(), cache._args, batch, pages.data_ptr(),
+          listed, gate, gs, out.data_ptr(), ws.data_ptr(), nb)
     return out
 
 

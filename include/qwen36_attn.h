@@ -548,9 +548,9 @@ int qwen36_paged_attention(const void* q, const qwen36_paged_cache* cache,
  * scores, ties to the lower index, budget in all (sink_pages + recent_pages <=
  * budget <= 1024).  The score of a page is 2^k_exp times the largest over the
  * KV head's 8 query heads of sum_d max(qi_d kmax_d, qi_d kmin_d) with the
- * bounds' integers and qi = q in steps of a power of two that puts the 8 heads'
- * largest finite magnitude in [64, 128), rounded to nearest even and cut to
- * +-127 (NaN counts as 0): whole numbers, so the selection is exact.  A page id
+ * bounds' integers and qi = q in steps of a power of two (2^-127 at least) that
+ * puts the 8 heads' largest finite magnitude in [64, 128), rounded to nearest
+ * even and cut to +-127 (NaN counts as 0): whole numbers, so the selection is exact.  A page id
  * outside the pool scores below every other.  Needs bounds; workspace of
  * qwen36_paged_select_workspace_bytes(...) bytes, 16-byte aligned. */
 size_t qwen36_paged_select_workspace_bytes(const qwen36_paged_cache* cache,
