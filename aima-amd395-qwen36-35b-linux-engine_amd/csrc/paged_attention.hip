@@ -18,8 +18,9 @@
 //    the operand of dims 16 i + t wants 8 keys of one dim a lane, which is a
 //    byte (or half-word) exchange between registers of the same lane.
 // e4m3 goes to bf16 with the page's power-of-two scale inside the conversion,
-// exactly.  K of the next step is loaded as soon as the scores are formed and V
-// after its products, so loads are always in flight.
+// exactly.  A step's V and the next step's K are asked for while its scores are
+// formed (the compiler's order; V one step ahead as well, held there by fences,
+// took 39.9 us against 38.1 for 128K and 118.7 against 116.2 for 32 sequences).
 // Scores, maximum, sum and accumulators are fp32; P is rounded to bf16 for the
 // matrix product (its sum too is taken from the fp32 values).
 #include "paged_split.h"
@@ -65,56 +66,38 @@ __device__ __forceinline__ void paged_store(const PagedOut& w, unsigned hq, size
   *reinterpret_cast<bf16x4*>(w.out + (t * hq + qh) * kD + d) = r;
 }
 
+// What a workgroup takes at once: rows t0 .. t0 + n_tok and keys [key0, key1) of
+// the sequence, or of the row's list.
+struct Piece {
+  unsigned seq, head;
+  int t0, n_tok, pos0, key0, key1;
+  size_t slot;
+  bool single;
+};
+
+// The waves' accumulators, a column's 64-dim quarters 68 words apart: the four
+// quarters and four neighbouring columns of a store then cover all banks.
+constexpr int kQuarter = 68;
+struct __attribute__((aligned(16))) Shared {
+  float o[kWaves][kCols][4 * kQuarter];
+  float ml[kWaves][kCols][2];
+  int odd[kWaves];   // whether a V value that only the second token sees is not finite
+};
+
 template <bool kFp8, bool kList>
-__global__ __launch_bounds__(64 * kWaves, kFp8 ? 2 : 1) void paged_rows_kernel(
-    const bf16* __restrict__ q, PagedCache c, PagedBatch b, PagedOut w, ListArgs list,
-    unsigned target) {
+__device__ __forceinline__ void paged_piece(const bf16* __restrict__ q, const PagedCache& c, const PagedBatch& b,
+                                            const PagedOut& w, const ListArgs& list, const Piece& pc, Shared& sh) {
   constexpr int kElem = kFp8 ? 1 : 2;
   constexpr int kKLoads = 4 * kElem, kVLoads = kElem;   // 16-byte loads of a K row part, a V row
-  __shared__ unsigned find[40];
-  __shared__ float ol[kWaves][kCols][kD];
-  __shared__ float mll[kWaves][kCols][2];
-  __shared__ int odd[kWaves];   // whether a V value that only the second token sees is not finite
-
-  const unsigned head = blockIdx.x % c.heads, item = blockIdx.x / c.heads;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, g = lane >> 4;
-  const unsigned hq = c.heads * kGroup;
-
-  // the item: rows t0 .. t0 + n_tok, keys [key0, key1) of the sequence or of the list
-  unsigned seq;
-  int t0, n_tok, key0, key1, pos0;
-  size_t slot;
-  bool single;
-  if constexpr (kList) {
-    t0 = (int)(item / list.chunks);
-    const unsigned chunk = item % list.chunks;
-    PagedSeq s;
-    if (!paged_find_row(b, t0, seq, s)) return;
-    pos0 = s.pos(t0);
-    if (pos0 < 0 && list.chunks > 1) return;   // the joining launch writes its zeros
-    n_tok = 1;
-    key0 = (int)(chunk * list.chunk_keys);
-    key1 = min(key0 + (int)list.chunk_keys, (int)(list.listed << c.shift));
-    slot = item;
-    single = list.chunks == 1;
-  } else {
-    PagedSplit sp;
-    if (!paged_split<2>(b, item, target, blockIdx.x == 0 ? w.head : nullptr, find, sp)) return;
-    seq = sp.seq;
-    const PagedSeq s = paged_seq(b, seq);
-    const unsigned chunks = ((unsigned)s.len + sp.chunk - 1) / sp.chunk;
-    t0 = s.a + 2 * (int)(sp.local / chunks);
-    n_tok = min(2, s.z - t0);
-    pos0 = s.pos(t0);
-    key0 = (int)(sp.local % chunks * sp.chunk);
-    const int end = pos0 + n_tok;
-    if (key0 >= end) return;
-    key1 = min(key0 + (int)sp.chunk, end);
-    slot = item;
-    single = end <= (int)sp.chunk;
-  }
+  const unsigned hq = c.heads * kGroup, head = pc.head;
+  // one piece for all lanes: scalar registers, so that loops and addresses are too
+  const unsigned seq = __builtin_amdgcn_readfirstlane(pc.seq);
+  const int t0 = __builtin_amdgcn_readfirstlane(pc.t0), n_tok = __builtin_amdgcn_readfirstlane(pc.n_tok);
+  const int pos0 = __builtin_amdgcn_readfirstlane(pc.pos0);
+  const int key0 = __builtin_amdgcn_readfirstlane(pc.key0), key1 = __builtin_amdgcn_readfirstlane(pc.key1);
   const int lim_max = pos0 + n_tok - 1;
   const int tok = col >> 3;
   const int lim = tok < n_tok ? pos0 + tok : -1;   // this column's last key
@@ -327,53 +310,127 @@ __global__ __launch_bounds__(64 * kWaves, kFp8 ? 2 : 1) void paged_rows_kernel(
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
   if (g == 0) {
-    mll[wave][col][0] = m;
-    mll[wave][col][1] = l;
+    sh.ml[wave][col][0] = m;
+    sh.ml[wave][col][1] = l;
   }
   if (!kList) {
     const int any = __any(strange);
-    if (lane == 0) odd[wave] = any;
+    if (lane == 0) sh.odd[wave] = any;
   }
+  if (col < 8 * n_tok) {
 #pragma unroll
-  for (int r = 0; r < 4; ++r)
+    for (int r = 0; r < 4; ++r)
 #pragma unroll
-    for (int t = 0; t < 16; t += 4) {
-      const f32x4 v = {o[t][r], o[t + 1][r], o[t + 2][r], o[t + 3][r]};
-      *reinterpret_cast<f32x4*>(&ol[wave][col][64 * g + 16 * r + t]) = v;
-    }
+      for (int t = 0; t < 16; t += 4) {
+        const f32x4 v = {o[t][r], o[t + 1][r], o[t + 2][r], o[t + 3][r]};
+        *reinterpret_cast<f32x4*>(&sh.o[wave][col][kQuarter * g + 16 * r + t]) = v;
+      }
+  }
   __syncthreads();
   const int oc = tid >> 4, od = (tid & 15) * 4;   // a column, 4 dims of each 64
   if (oc >= 8 * n_tok) return;
-  float mm = mll[0][oc][0];
+  float mm = sh.ml[0][oc][0];
 #pragma unroll
-  for (int x = 1; x < kWaves; ++x) mm = fmaxf(mm, mll[x][oc][0]);
+  for (int x = 1; x < kWaves; ++x) mm = fmaxf(mm, sh.ml[x][oc][0]);
   const float base = mm == -INFINITY ? 0.f : mm;
   float f[kWaves], lsum = 0.f;
 #pragma unroll
   for (int x = 0; x < kWaves; ++x) {
-    f[x] = __builtin_amdgcn_exp2f(mll[x][oc][0] - base);
-    lsum += f[x] * mll[x][oc][1];
+    f[x] = __builtin_amdgcn_exp2f(sh.ml[x][oc][0] - base);
+    lsum += f[x] * sh.ml[x][oc][1];
   }
   const size_t row = t0 + (oc >> 3), qh = head * kGroup + (oc & 7);
   const unsigned rows = kList ? 8 : kCols;
-  const size_t part = (slot * c.heads + head) * rows + oc;
+  const size_t part = (pc.slot * c.heads + head) * rows + oc;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int d = 64 * j + od;
     f32x4 v = f32x4{};
 #pragma unroll
-    for (int x = 0; x < kWaves; ++x) v += f[x] * *reinterpret_cast<const f32x4*>(&ol[x][oc][d]);
-    if (!kList && oc >= 8 && (odd[0] | odd[1] | odd[2] | odd[3]))
+    for (int x = 0; x < kWaves; ++x) v += f[x] * *reinterpret_cast<const f32x4*>(&sh.o[x][oc][kQuarter * j + od]);
+    if (!kList && oc >= 8 && (sh.odd[0] | sh.odd[1] | sh.odd[2] | sh.odd[3]))
       add_not_finite<kFp8>(v, c, table, head, lim_max, key1 - 1, key0, d);
-    if (single) {
+    if (pc.single) {
       paged_store(w, hq, row, qh, d, v, lsum);
     } else {
       *reinterpret_cast<f32x4*>(w.o + part * kD + d) = v;
     }
   }
-  if (!single && od == 0) {
+  if (!pc.single && od == 0) {
     w.ml[part * 2] = mm;
     w.ml[part * 2 + 1] = lsum;
+  }
+}
+
+// Rows with lists of their own: a workgroup per (row, KV head, chunk of the list).
+template <bool kFp8>
+__global__ __launch_bounds__(64 * kWaves, kFp8 ? 2 : 1) void paged_list_kernel(
+    const bf16* __restrict__ q, PagedCache c, PagedBatch b, PagedOut w, ListArgs list) {
+  __shared__ Shared sh;
+  const unsigned item = blockIdx.x / c.heads, chunk = item % list.chunks;
+  Piece p;
+  PagedSeq s;
+  p.t0 = (int)(item / list.chunks);
+  if (!paged_find_row(b, p.t0, p.seq, s)) return;
+  p.head = blockIdx.x % c.heads;
+  p.pos0 = s.pos(p.t0);
+  p.single = list.chunks == 1;
+  if (p.pos0 < 0 && !p.single) return;   // the joining launch writes its zeros
+  p.n_tok = 1;
+  p.key0 = (int)(chunk * list.chunk_keys);
+  p.key1 = min(p.key0 + (int)list.chunk_keys, (int)(list.listed << c.shift));
+  p.slot = item;
+  paged_piece<kFp8, true>(q, c, b, w, list, p, sh);
+}
+
+// Tiles of two tokens over their sequences: workgroup i of a KV head takes blocks
+// [i per, (i + 1) per) of all its tiles' in a row.
+template <bool kFp8>
+__global__ __launch_bounds__(64 * kWaves, kFp8 ? 2 : 1) void paged_rows_kernel(
+    const bf16* __restrict__ q, PagedCache c, PagedBatch b, PagedOut w, unsigned shares) {
+  __shared__ Shared sh;
+  __shared__ unsigned find[40];
+  const unsigned i = blockIdx.x / c.heads;
+  unsigned total, longest, seq, local;
+  paged_total<2>(b, find, total, longest);
+  const unsigned per = max(1u, (total + shares - 1) / shares);
+  unsigned* put = blockIdx.x == 0 ? w.head : nullptr;
+  if (put != nullptr && threadIdx.x == 0) {
+    put[0] = per;
+    if (b.seqs == 1) put[1] = 0;
+  }
+  if (!paged_find_item(b, i * per, find, [&](unsigned j) {
+        const PagedSeq s = paged_seq(b, j);
+        return paged_tiles<2>(s) * paged_blocks(s);
+      }, seq, local, put != nullptr ? put + 1 : nullptr))
+    return;
+  unsigned left = per;
+  const ListArgs none = {};
+  for (;; ++seq, local = 0) {
+    if (seq >= b.seqs) return;
+    const PagedSeq s = paged_seq(b, seq);
+    const unsigned blocks = paged_blocks(s), n = paged_tiles<2>(s) * blocks;
+    while (local < n) {
+      const unsigned tile = local / blocks, at = local % blocks, take = min(left, blocks - at);
+      Piece p;
+      p.seq = seq;
+      p.head = blockIdx.x % c.heads;
+      p.t0 = s.a + 2 * (int)tile;
+      p.n_tok = min(2, s.z - p.t0);
+      p.pos0 = s.pos(p.t0);
+      const int end = p.pos0 + p.n_tok;
+      p.key0 = (int)(at * kSplitBlock);
+      p.key1 = min((int)((at + take) * kSplitBlock), end);
+      p.slot = (size_t)i + p.t0;   // grows with every step of a share or a tile
+      p.single = p.key0 == 0 && p.key1 == end;
+      if (p.key0 < p.key1) {
+        paged_piece<kFp8, false>(q, c, b, w, none, p, sh);
+        __syncthreads();
+      }
+      left -= take;
+      local += take;
+      if (left == 0) return;
+    }
   }
 }
 
@@ -395,10 +452,17 @@ __device__ __forceinline__ bool paged_parts(const PagedBatch& b, unsigned heads,
     slot = (size_t)t * listed_chunks;
     r = qh % kGroup;
   } else {
-    const unsigned chunk = w.head[0] * kSplitBlock, own = t - s.a, in = own / tile;
+    const unsigned per = w.head[0], own = t - s.a, in = own / tile, blocks = paged_blocks(s);
     const int end = s.len - (s.z - s.a) + min((int)((in + 1) * tile), s.z - s.a);
-    p.n = end > 0 ? ((unsigned)end + chunk - 1) / chunk : 0;
-    slot = w.head[1 + seq] + (size_t)in * (((unsigned)s.len + chunk - 1) / chunk);
+    const unsigned seen = end > 0 ? ((unsigned)end + kSplitBlock - 1) / kSplitBlock : 0;
+    if (tile == 2) {   // shares of the tiles' blocks in a row
+      const unsigned start = w.head[1 + seq] + in * blocks;
+      p.n = seen ? (start + seen - 1) / per - start / per + 1 : 0;
+      slot = (size_t)(start / per) + (s.a + in * tile);
+    } else {
+      p.n = (seen + per - 1) / per;
+      slot = w.head[1 + seq] + (size_t)in * ((blocks + per - 1) / per);
+    }
     r = own % tile * kGroup + qh % kGroup;
   }
   p.stride = heads * kGroup * tile;
@@ -541,8 +605,10 @@ Plan paged_plan(const PagedBatch& b, unsigned heads) {
   Plan p;
   const unsigned mean = (b.tokens + b.seqs - 1) / b.seqs;
   p.tile = mean <= 2 ? 2 : mean <= 8 ? 8 : mean <= 16 ? 16 : 32;
-  if (p.tile == 2) {   // two workgroups a CU, some times over, so that unequal chunks even out
-    p.target = 1024u / heads;
+  if (p.tile == 2) {   // one share for each of two workgroups a CU
+    p.target = 512u / heads;
+    p.items = p.target + b.tokens;
+    return p;
   } else {
     // A workgroup of 8 waves a CU, as many of 4, two of 2: the chunks of a tile that
     // fill whole rounds of the GPU best, each chunk more costing some partials.
@@ -619,14 +685,11 @@ Q36_EXPORT int qwen36_paged_attention(const void* q, const qwen36_paged_cache* c
   split_ws(workspace, b.seqs, p.items, c.heads, 8 * p.tile, o);
   int e;
   if (p.tile == 2) {
-    const ListArgs none = {};
-    hipStream_t st = static_cast<hipStream_t>(stream);
-    const dim3 grid(p.items * c.heads), block(64 * kWaves);
-    const bf16* x = static_cast<const bf16*>(q);
-    if (fp8)
-      hipLaunchKernelGGL((paged_rows_kernel<true, false>), grid, block, 0, st, x, c, b, o, none, p.target);
-    else
-      hipLaunchKernelGGL((paged_rows_kernel<false, false>), grid, block, 0, st, x, c, b, o, none, p.target);
+    const auto launch = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3(p.target * c.heads), dim3(64 * kWaves), 0, static_cast<hipStream_t>(stream),
+                         static_cast<const bf16*>(q), c, b, o, p.target);
+    };
+    fp8 ? launch(paged_rows_kernel<true>) : launch(paged_rows_kernel<false>);
     e = static_cast<int>(hipGetLastError());
   } else {
     e = paged_prefill(q, c, fp8, b, o, p.tile, p.items, p.target, stream);
@@ -664,14 +727,11 @@ Q36_EXPORT int qwen36_paged_sparse_attention(const void* q, const qwen36_paged_c
   list_plan(b, c, listed, l);
   l.pages = static_cast<const int*>(pages);
   split_ws(workspace, 0, (size_t)b.tokens * l.chunks, c.heads, 8, o);
-  hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 grid(b.tokens * l.chunks * c.heads), block(64 * kWaves);
-  if (cache->cache_type == QWEN36_PAGED_E4M3)
-    hipLaunchKernelGGL((paged_rows_kernel<true, true>), grid, block, 0, st, static_cast<const bf16*>(q), c, b, o,
-                       l, 0u);
-  else
-    hipLaunchKernelGGL((paged_rows_kernel<false, true>), grid, block, 0, st, static_cast<const bf16*>(q), c, b, o,
-                       l, 0u);
+  const auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(b.tokens * l.chunks * c.heads), dim3(64 * kWaves), 0,
+                       static_cast<hipStream_t>(stream), static_cast<const bf16*>(q), c, b, o, l);
+  };
+  cache->cache_type == QWEN36_PAGED_E4M3 ? launch(paged_list_kernel<true>) : launch(paged_list_kernel<false>);
   const int e = static_cast<int>(hipGetLastError());
   return e != Q36_OK || l.chunks == 1 ? e : paged_combine(b, c, o, 1, l.chunks, stream);
 }

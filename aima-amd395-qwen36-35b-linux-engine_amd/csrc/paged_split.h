@@ -1,13 +1,16 @@
-// How attention over the paged cache is split: (tile of rows, chunk of keys)
-// items, their partials in the workspace, and the launch that joins them.
+// How attention over the paged cache is split, its partials in the workspace and
+// the launch that joins them.
 //
 // The lengths are on the device, so every workgroup works the split out for
-// itself: with w blocks of 128 keys over all tiles of a KV head, chunks of
-//   max(1, w / target, longest / 256)
-// blocks give at most target + tiles items, whatever the mixture of lengths:
-// one sequence of 128K fills the GPU as 32 of 4K do.  The grid is that bound,
-// and workgroups without an item end.  A tile of one chunk is written straight
-// to the output.
+// itself; w is the number of 128-key blocks over all tiles of rows of a KV head.
+//  * Prompts (tiles of 8 to 32 tokens): (tile, chunk of keys) items, chunks of
+//    max(1, w / target, longest / 256) blocks: at most target + tiles items,
+//    whatever the mixture of lengths.  The grid is that bound, and workgroups
+//    without an item end.
+//  * Single and few tokens (tiles of 2): the tiles' blocks in a row are cut into
+//    one equal share for each workgroup that the GPU holds, so that all end
+//    together; a share may end one tile and begin the next.
+// A tile that one workgroup takes whole is written straight to the output.
 #pragma once
 
 #include "paged_common.h"
@@ -22,7 +25,7 @@ struct PagedOut {
   bf16* out;
   float* ml;              // [slot][KV head][8 * tile tokens][2]: m (log2 domain), l
   float* o;               // [slot][KV head][8 * tile tokens][256]
-  unsigned* head;         // [0]: chunk blocks, [1 + i]: first slot of sequence i
+  unsigned* head;         // [0]: blocks of a chunk or share, [1 + i]: first item or block of sequence i
   size_t gate_stride;
 };
 
@@ -31,34 +34,29 @@ struct PagedSplit {
   unsigned seq, local;    // the item's sequence and its place there
 };
 
-// The item of this workgroup (all threads call it; lds holds 40 words); false
-// if there is none.  Item 0 also writes the split down for the joining launch.
 template <unsigned kTile>
-__device__ __forceinline__ bool paged_split(const PagedBatch& b, unsigned item, unsigned target,
-                                            unsigned* head, unsigned* lds, PagedSplit& r) {
-  const unsigned tid = threadIdx.x, n = blockDim.x, wave = tid >> 6, waves = n >> 6;
-  const auto tiles = [&](const PagedSeq& s) { return (unsigned)(s.z - s.a + (int)kTile - 1) / kTile; };
-  const auto blocks = [&](const PagedSeq& s) {
-    return ((unsigned)s.len + kSplitBlock - 1) / kSplitBlock;
-  };
-  unsigned cb;
+__device__ __forceinline__ unsigned paged_tiles(const PagedSeq& s) {
+  return (unsigned)(s.z - s.a + (int)kTile - 1) / kTile;
+}
+__device__ __forceinline__ unsigned paged_blocks(const PagedSeq& s) {
+  return ((unsigned)s.len + kSplitBlock - 1) / kSplitBlock;
+}
+
+// Blocks of all tiles of a KV head, and of the longest sequence with a tile (all
+// threads call it; lds holds 40 words).
+template <unsigned kTile>
+__device__ __forceinline__ void paged_total(const PagedBatch& b, unsigned* lds, unsigned& w, unsigned& longest) {
   if (b.seqs == 1) {
     const PagedSeq s = paged_seq(b, 0);
-    const unsigned l = blocks(s), w = tiles(s) * l;
-    cb = max(1u, max((w + target - 1) / target, (l + kMaxChunks - 1) / kMaxChunks));
-    r.chunk = cb * kSplitBlock;
-    r.seq = 0;
-    r.local = item;
-    if (head != nullptr && tid == 0) {
-      head[0] = cb;
-      head[1] = 0;
-    }
-    return item < tiles(s) * ((l + cb - 1) / cb);
+    longest = paged_blocks(s);
+    w = paged_tiles<kTile>(s) * longest;
+    return;
   }
-  unsigned w = 0, longest = 0;
+  const unsigned tid = threadIdx.x, n = blockDim.x, wave = tid >> 6, waves = n >> 6;
+  w = longest = 0;
   for (unsigned i = tid; i < b.seqs; i += n) {
     const PagedSeq s = paged_seq(b, i);
-    const unsigned t = tiles(s), l = t ? blocks(s) : 0u;
+    const unsigned t = paged_tiles<kTile>(s), l = t ? paged_blocks(s) : 0u;
     w += t * l;
     longest = max(longest, l);
   }
@@ -77,13 +75,26 @@ __device__ __forceinline__ bool paged_split(const PagedBatch& b, unsigned item, 
     w += lds[20 + i];
     longest = max(longest, lds[30 + i]);
   }
-  cb = __builtin_amdgcn_readfirstlane(
-      max(1u, max((w + target - 1) / target, (longest + kMaxChunks - 1) / kMaxChunks)));
+  w = __builtin_amdgcn_readfirstlane(w);
+  longest = __builtin_amdgcn_readfirstlane(longest);
+}
+
+// The item of this workgroup (all threads call it; lds holds 40 words); false
+// if there is none.  Item 0 also writes the split down for the joining launch.
+template <unsigned kTile>
+__device__ __forceinline__ bool paged_split(const PagedBatch& b, unsigned item, unsigned target,
+                                            unsigned* head, unsigned* lds, PagedSplit& r) {
+  unsigned w, longest;
+  paged_total<kTile>(b, lds, w, longest);
+  const unsigned cb = max(1u, max((w + target - 1) / target, (longest + kMaxChunks - 1) / kMaxChunks));
   r.chunk = cb * kSplitBlock;
-  if (head != nullptr && tid == 0) head[0] = cb;
+  if (head != nullptr && threadIdx.x == 0) {
+    head[0] = cb;
+    if (b.seqs == 1) head[1] = 0;
+  }
   return paged_find_item(b, item, lds, [&](unsigned i) {
     const PagedSeq s = paged_seq(b, i);
-    return tiles(s) * ((blocks(s) + cb - 1) / cb);
+    return paged_tiles<kTile>(s) * ((paged_blocks(s) + cb - 1) / cb);
   }, r.seq, r.local, head != nullptr ? head + 1 : nullptr);
 }
 
