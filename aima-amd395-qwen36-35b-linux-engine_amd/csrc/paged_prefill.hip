@@ -5,15 +5,17 @@
 //
 // Work: an item is a tile of 4 kWaves tokens x the 8 query heads of a KV head
 // (32 matrix columns a wave) and a chunk of keys; bound by the matrix products
-// (16,384 operations a (row's token, key) pair and KV head).  Per 32-key tile:
-//  * K and V of the next tile leave their pages for registers, 16 bytes a lane,
-//    become bf16 there (e4m3 with the page's scale inside the conversion, once
-//    for all 8 heads and 4 kWaves tokens) and go to the other half of an LDS
-//    double buffer, so that conversion costs 1/16 of what it would behind LDS;
-//  * S^T = K Q^T, online softmax in fp32, O^T += V^T P^T on 32x32x16 products:
-//    A = K rows from LDS, B = Q^T in registers; A = V^T by transposed LDS reads,
-//    B = P^T, the S^T accumulator as it is.  LDS operands are read 4 products
-//    ahead (the order is pinned by scheduling barriers).
+// (16,384 operations a (row's token, key) pair and KV head) and by LDS, which
+// every wave reads whole.  Stages of 32 KB (64 keys of e4m3, 32 of bf16):
+//  * K and V rows go from their pages straight to LDS in the pages' type (no
+//    registers), a stage ahead of their use.  The 16-byte chunks of a row are
+//    exchanged by its number (chunk ^ (row & 15)) on the way, which leaves the
+//    row-wise K reads and the transposed V reads free of bank conflicts.
+//  * per 32 keys: S^T = K Q^T, online softmax in fp32, O^T += V^T P^T on 32x32x16
+//    products.  A = K rows; B = Q^T in registers; A = V^T by transposed LDS reads;
+//    B = P^T, the S^T accumulator as it is.  e4m3 becomes bf16 behind LDS, with
+//    the page's scale inside the conversion: half the LDS bytes, which pays for
+//    the 128 conversions a wave has besides its 32 products.
 // The reference maximum is the first visible tile's and is raised (with a
 // rescale) only when a tile's probabilities sum past 2^20.
 #include "paged_split.h"
@@ -22,13 +24,14 @@ namespace q36 {
 namespace {
 
 constexpr int kKeys = 32;
-constexpr int kRowB = kD * 2;                      // a bf16 row in LDS
-// LDS tile: block b (0..15) holds rows b and b + 16; 1040 (K) and 1088 (V) bytes
-// apart, which keeps the 16-byte K reads and the transposed V reads free of bank
-// conflicts.
-constexpr int kKBlk = 1040, kVBlk = 1088;
-constexpr int kKTile = 16 * kKBlk, kStage = kKTile + 16 * kVBlk;
-constexpr int kLds = 2 * kStage;                   // 68,096 bytes
+constexpr int kHalf = 16384, kStage = 2 * kHalf;   // K, V of a stage
+constexpr int kLds = 2 * kStage;
+
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(1))) void global_void;
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
+
 constexpr float kScoreScale = 0.0625f * kLog2e;
 
 template <bool kFp8, int kWaves>
@@ -38,7 +41,11 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
   __shared__ unsigned find[40];
   __shared__ int odd;   // whether a V value that some rows must not see is not finite
   constexpr int kElem = kFp8 ? 1 : 2;
-  constexpr int kTile = 4 * kWaves, kPass = 8 / kWaves;   // 4 kWaves rows a pass
+  constexpr int kTile = 4 * kWaves;
+  constexpr int kRowB = kD * kElem, kStageKeys = kHalf / kRowB;   // bytes of a row, keys of a stage
+  constexpr int kSubs = kStageKeys / kKeys, kGroups = kStageKeys / 16;
+  constexpr int kLoads = 16 / kWaves;                // 1 KB loads of K (and of V) a wave and stage
+  constexpr int kBlockStages = 1024 / kStageKeys;    // stages of a 1,024-key block
 
   const unsigned head = blockIdx.x % c.heads, item = blockIdx.x / c.heads;
   const unsigned hq = c.heads * kGroup;
@@ -71,10 +78,12 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
 
   bf16x8 qf[16];
   {
-    const bf16* qp = q + ((size_t)(t0 + tok) * hq + head * kGroup + (lj & 7)) * kD + 8 * lg;
+    const bf16* qp = q + ((size_t)(t0 + tok) * hq + head * kGroup + (lj & 7)) * kD + (kFp8 ? 16 : 8) * lg;
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-      qf[i] = lim >= 0 ? *reinterpret_cast<const bf16x8*>(qp + 16 * i) : bf16x8{};
+      // the dims of k-step i as the K operand has them: an e4m3 chunk holds two steps
+      qf[i] = lim >= 0 ? *reinterpret_cast<const bf16x8*>(qp + (kFp8 ? 32 * (i >> 1) + 8 * (i & 1) : 16 * i))
+                       : bf16x8{};
   }
   f32x16 o[8];
 #pragma unroll
@@ -101,15 +110,12 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
     }
   };
 
-  // ---- raw rows of the tile to come
-  u32x4 rk[kPass][kElem], rv[kPass][kElem];
-  unsigned rexp[kPass];
-  unsigned r_ok = 0, ok = 0;     // bit h: the 16 keys h of the tile have a page
-  int r_tile = 0;
+  // ---- a stage's rows, 4 (e4m3) or 2 (bf16) a load: one page each
+  unsigned ok = 0, ok_next = 0;            // bit g: the 16 keys g of the stage have a page
+  unsigned e0 = 0, e1 = 0, e2 = 0, e3 = 0;  // scale bytes of the loaded stage's 16-key groups (K, V << 8)
   const size_t head_off = ((size_t)head << (c.shift + 8)) * kElem;
-  const unsigned in_row = (lane & 15) * 16;
-  const auto load_tile = [&](int i) {
-    const int at = i & 31;
+  const auto load_stage = [&](int i) {
+    const int at = i % kBlockStages;
     if (at == 0) {
       if (i == 0) {
         fetch_pages(kv_first);
@@ -118,123 +124,129 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
       d_page = n_page;
       d_exp = n_exp;
       d_ok = __ballot(n_ok);
-    } else if (at == 8) {
-      fetch_pages(kv_first + (i + 24) * kKeys);
-    } else if (at == 20) {
+    } else if (at == kBlockStages / 4) {
+      fetch_pages(kv_first + (i - at + kBlockStages) * kStageKeys);
+    } else if (at == kBlockStages * 5 / 8) {
       fetch_scales();
     }
-    r_ok = (unsigned)(d_ok >> (2 * at)) & 3u;
-    r_tile = i;
+    ok_next = (unsigned)(d_ok >> (kGroups * at)) & ((1u << kGroups) - 1);
+    if constexpr (kFp8) {
+      e0 = __builtin_amdgcn_readlane(d_exp, 4 * at);
+      e1 = __builtin_amdgcn_readlane(d_exp, 4 * at + 1);
+      e2 = __builtin_amdgcn_readlane(d_exp, 4 * at + 2);
+      e3 = __builtin_amdgcn_readlane(d_exp, 4 * at + 3);
+    }
+    char* to = lds + (i & 1) * kStage;
 #pragma unroll
-    for (int p = 0; p < kPass; ++p) {
-      const int row = p * 4 * kWaves + 4 * wave;       // first of this wave's 4
-      const int from = 2 * at + (row >> 4);
-      const unsigned pid = __builtin_amdgcn_readlane(d_page, from);
-      const int prow = (kv_first + i * kKeys + row) & page_mask;
-      rexp[p] = __builtin_amdgcn_readlane(d_exp, from);
-      const unsigned voff = (lane >> 4) * kD * kElem + in_row;
-      const char* kp = c.k + pid * c.k_stride + head_off + (size_t)prow * kD * kElem;
-      const char* vp = c.v + pid * c.v_stride + head_off + (size_t)prow * kD * kElem;
-#pragma unroll
-      for (int e = 0; e < kElem; ++e) {
-        rk[p][e] = *reinterpret_cast<const u32x4*>(kp + voff + 256 * e);
-        rv[p][e] = *reinterpret_cast<const u32x4*>(vp + voff + 256 * e);
-      }
+    for (int j = 0; j < kLoads; ++j) {
+      const int row0 = (j * kWaves + wave) * (1024 / kRowB);            // uniform
+      const int row = row0 + lane / (kRowB / 16);
+      const unsigned pid = __builtin_amdgcn_readlane(d_page, kGroups * at + (row0 >> 4));
+      const int prow = (kv_first + i * kStageKeys + row0) & page_mask;
+      const unsigned off = (row - row0) * kRowB + (((lane & (kRowB / 16 - 1)) ^ (row & 15)) << 4);
+      const char* kp = c.k + pid * c.k_stride + head_off + (size_t)prow * kRowB;
+      const char* vp = c.v + pid * c.v_stride + head_off + (size_t)prow * kRowB;
+      __builtin_amdgcn_global_load_lds((global_void*)(kp + off), (lds_void*)(to + row0 * kRowB), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((global_void*)(vp + off), (lds_void*)(to + kHalf + row0 * kRowB), 16, 0, 0);
     }
   };
-  const auto store_tile = [&](int stage) {
-    const int key0 = kv_first + r_tile * kKeys;
-    const bool edge = key0 + kKeys - 1 > pos0 || r_ok != 3u;
+  // Behind the tile's first position V may hold anything, and 0 * NaN is NaN: rows
+  // that no token sees are cleared, and of the others what is not finite (the
+  // tokens that do see it get it at the end).
+  const auto clean_stage = [&](int i) {
     bool strange = false;
+    for (int x = tid; x < kHalf / 16; x += 64 * kWaves) {
+      const int row = x / (kRowB / 16), key = kv_first + i * kStageKeys + row;
+      u32x4* p = reinterpret_cast<u32x4*>(lds + (i & 1) * kStage + kHalf) + x;
+      const bool out = key >= kv_stop || !((ok >> (row >> 4)) & 1u), some = key > pos0;
+      if (!out && !some) continue;
+      u32x4 v = *p;
 #pragma unroll
-    for (int p = 0; p < kPass; ++p) {
-      const int row = p * 4 * kWaves + 4 * wave + (lane >> 4);
-      if (edge) {
-        // Behind the tile's first position V may hold anything, and 0 * NaN is NaN:
-        // rows that no token sees are cleared, and of the others what is not finite
-        // (the tokens that do see it get it at the end).
-        const bool out = key0 + row >= kv_stop || !((r_ok >> (row >> 4)) & 1u);
-        const bool some = key0 + row > pos0;
-#pragma unroll
-        for (int e = 0; e < kElem; ++e)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const unsigned u = out ? 0u : rv[p][e][x], bad = some ? not_finite<kFp8>(u) : 0u;
-            rv[p][e][x] = u & ~bad;
-            strange |= bad != 0;
-          }
+      for (int e = 0; e < 4; ++e) {
+        const unsigned u = out ? 0u : v[e], bad = some ? not_finite<kFp8>(u) : 0u;
+        v[e] = u & ~bad;
+        strange |= bad != 0;
       }
-      char* kb = lds + stage * kStage + (row & 15) * kKBlk + (row >> 4) * kRowB;
-      char* vb = lds + stage * kStage + kKTile + (row & 15) * kVBlk + (row >> 4) * kRowB;
-      if constexpr (kFp8) {
-        const float ks = paged_scale(rexp[p] & 0xffu), vs = paged_scale(rexp[p] >> 8);
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const unsigned k0 = rk[p][0][2 * x], k1 = rk[p][0][2 * x + 1];
-          const unsigned v0 = rv[p][0][2 * x], v1 = rv[p][0][2 * x + 1];
-          *reinterpret_cast<u32x4*>(kb + 2 * in_row + 16 * x) =
-              u32x4{cvt2<false>(k0, ks), cvt2<true>(k0, ks), cvt2<false>(k1, ks), cvt2<true>(k1, ks)};
-          *reinterpret_cast<u32x4*>(vb + 2 * in_row + 16 * x) =
-              u32x4{cvt2<false>(v0, vs), cvt2<true>(v0, vs), cvt2<false>(v1, vs), cvt2<true>(v1, vs)};
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < kElem; ++e) {
-          *reinterpret_cast<u32x4*>(kb + in_row + 256 * e) = rk[p][e];
-          *reinterpret_cast<u32x4*>(vb + in_row + 256 * e) = rv[p][e];
-        }
-      }
+      *p = v;
     }
     if (strange) odd = 1;
   };
 
-  const int kbase = (lj & 15) * kKBlk + (lj >> 4) * kRowB + lg * 16;
+  // per-lane LDS addresses; k-steps and dim tiles flip bits of the chunk number
+  const int kbase = lj * kRowB + ((lg ^ (lj & 15)) << 4);
   const int grp = lane >> 4, m16 = lane & 15;
-  const int vbase = (4 * lg + (m16 >> 2)) * kVBlk + 32 * (grp & 1) + 8 * (m16 & 3);
+  const int vrow = kFp8 ? 8 * (m16 >> 3) + 4 * lg + ((m16 >> 1) & 3) : 4 * lg + (m16 >> 2);
+  const int vchunk = kFp8 ? grp & 1 : 2 * (grp & 1) + ((m16 >> 1) & 1);
+  const int vbase = vrow * kRowB + ((vchunk ^ vrow) << 4) + 8 * (m16 & 1);
 
-  const int n_tiles = (kv_stop - kv_first + kKeys - 1) / kKeys;
+  const int n_stages = (kv_stop - kv_first + kStageKeys - 1) / kStageKeys;
   if (tid == 0) odd = 0;
-  __syncthreads();
-  load_tile(0);
-  store_tile(0);
-  unsigned ok_next = r_ok;
-  if (n_tiles > 1) load_tile(1);
-  for (int t = 0; t < n_tiles; ++t) {
-    const int kv0 = kv_first + t * kKeys, stage = t & 1;
+  load_stage(0);
+  for (int st = 0; st < n_stages; ++st) {
     ok = ok_next;
-    __syncthreads();   // tile t is in LDS, tile t - 1 is used up
-    if (t + 1 < n_tiles) {
-      store_tile(stage ^ 1);
-      ok_next = r_ok;
-      if (t + 2 < n_tiles) load_tile(t + 2);
+    const unsigned f0 = e0, f1 = e1, f2 = e2, f3 = e3;
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();   // stage st is in LDS, stage st - 1 is used up
+    const int key_st = kv_first + st * kStageKeys;
+    if (key_st + kStageKeys - 1 > pos0 || ok != (1u << kGroups) - 1) {
+      clean_stage(st);
+      __syncthreads();
     }
+    if (st + 1 < n_stages) load_stage(st + 1);
+#pragma unroll 1
+    for (int sub = 0; sub < kSubs; ++sub) {
+    const int kv0 = key_st + sub * kKeys;
     if (kv0 > wave_lim) continue;
-    const char* kp = lds + stage * kStage + kbase;
-    const char* vp = lds + stage * kStage + kKTile + vbase;
-
-    bf16x8 kr[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) kr[i] = *reinterpret_cast<const bf16x8*>(kp + i * 32);
+    const char* kp = lds + (st & 1) * kStage + sub * kKeys * kRowB;
+    const char* vp = kp + kHalf;
+    const unsigned okh = ok >> (2 * sub), ea = sub ? f2 : f0, eb = sub ? f3 : f1;
     f32x16 x = f32x16{};
+    // the wave with products to issue goes before the one in its softmax (2,048
+    // tokens over 30K: 970 us without, 944 with)
+    __builtin_amdgcn_s_setprio(1);
+    if constexpr (kFp8) {
+      const float ks = paged_scale((lj < 16 ? ea : eb) & 0xffu);
+      u32x4 kr[4];
+      const auto kread = [&](int i) { return *reinterpret_cast<const u32x4*>(kp + (kbase ^ (i << 5))); };
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      x = mfma32x32x16(kr[i & 3], qf[i], x);
-      if (i + 4 < 16) kr[i & 3] = *reinterpret_cast<const bf16x8*>(kp + (i + 4) * 32);
-    }
-    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+      for (int i = 0; i < 4; ++i) kr[i] = kread(i);
 #pragma unroll
-    for (int i = 0; i < 12; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      for (int i = 0; i < 8; ++i) {
+        const u32x4 r = kr[i & 3];
+        if (i + 4 < 8) kr[i & 3] = kread(i + 4);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const u32x4 a = {cvt2<false>(r[2 * h], ks), cvt2<true>(r[2 * h], ks), cvt2<false>(r[2 * h + 1], ks),
+                           cvt2<true>(r[2 * h + 1], ks)};
+          x = mfma32x32x16(__builtin_bit_cast(bf16x8, a), qf[2 * i + h], x);
+        }
+      }
+    } else {
+      bf16x8 kr[4];
+      const auto kread = [&](int i) { return *reinterpret_cast<const bf16x8*>(kp + (kbase ^ (i << 5))); };
+#pragma unroll
+      for (int i = 0; i < 4; ++i) kr[i] = kread(i);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        x = mfma32x32x16(kr[i & 3], qf[i], x);
+        if (i + 4 < 16) kr[i & 3] = kread(i + 4);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+      for (int i = 0; i < 12; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
     }
-    __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+    __builtin_amdgcn_s_setprio(0);
     // lane: keys kv0 + 8 (r / 4) + 4 lg + r % 4 of its column
     const bool diag = kv0 + kKeys - 1 > wave_first;
-    if (diag || ok != 3u) {
+    if (diag || (okh & 3u) != 3u) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int key = kv0 + 8 * (r >> 2) + 4 * lg + (r & 3);
-        x[r] = key <= lim && ((ok >> (r >> 3)) & 1u) ? x[r] : -INFINITY;
+        x[r] = key <= lim && ((okh >> (r >> 3)) & 1u) ? x[r] : -INFINITY;
       }
     }
     const auto col_max = [&]() {
@@ -273,27 +285,50 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
       }
     }
     l += psum;
+    __builtin_amdgcn_s_setprio(1);
 
-    i16x4 va[4][2];
-    const auto vread = [&](int i, int to) {
-      const char* p = vp + (i >> 3) * kRowB + (i & 7) * 64;
-      va[to][0] = lds_read_tr16(p);
-      va[to][1] = lds_read_tr16(p + 8 * kVBlk);
-    };
+    if constexpr (kFp8) {
+      i32x2 va[4];
+      const auto vread = [&](int i) {   // keys 16 (i / 8) .. + 16, dims 32 (i % 8) .. + 32
+        return __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+            (lds_i32x2*)(vp + (i >> 3) * 16 * kRowB + (vbase ^ ((i & 7) << 5))));
+      };
 #pragma unroll
-    for (int i = 0; i < 4; ++i) vread(i, i);
+      for (int i = 0; i < 4; ++i) va[i] = vread(i);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      o[i & 7] = mfma32x32x16(cat_bf16x8(va[i & 3][0], va[i & 3][1]), pb[i >> 3], o[i & 7]);
-      if (i + 4 < 16) vread(i + 4, i & 3);
+      for (int i = 0; i < 16; ++i) {
+        const float vs = paged_scale((i < 8 ? ea : eb) >> 8);
+        const i32x2 r = va[i & 3];
+        if (i + 4 < 16) va[i & 3] = vread(i + 4);
+        const u32x4 a = {cvt2<false>((unsigned)r[0], vs), cvt2<true>((unsigned)r[0], vs),
+                         cvt2<false>((unsigned)r[1], vs), cvt2<true>((unsigned)r[1], vs)};
+        o[i & 7] = mfma32x32x16(__builtin_bit_cast(bf16x8, a), pb[i >> 3], o[i & 7]);
+      }
+    } else {
+      i16x4 va[4][2];
+      const auto vread = [&](int i, int to) {
+        const char* p = vp + (i >> 3) * 16 * kRowB;
+        const int at = vbase ^ ((i & 7) << 6);
+        va[to][0] = lds_read_tr16(p + at);
+        va[to][1] = lds_read_tr16(p + 8 * kRowB + (at ^ 128));   // keys + 8
+      };
+#pragma unroll
+      for (int i = 0; i < 4; ++i) vread(i, i);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        o[i & 7] = mfma32x32x16(cat_bf16x8(va[i & 3][0], va[i & 3][1]), pb[i >> 3], o[i & 7]);
+        if (i + 4 < 16) vread(i + 4, i & 3);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x100, 8, 1);
+#pragma unroll
+      for (int i = 0; i < 12; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, 4, 1);
     }
-    __builtin_amdgcn_sched_group_barrier(0x100, 8, 1);
-#pragma unroll
-    for (int i = 0; i < 12; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
-      __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+    __builtin_amdgcn_s_setprio(0);
     }
-    __builtin_amdgcn_sched_group_barrier(0x008, 4, 1);
   }
 
   // ---- out through LDS in four rounds of 64 dims, so that stores are whole

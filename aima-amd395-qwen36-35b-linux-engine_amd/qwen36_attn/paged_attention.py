@@ -25,6 +25,8 @@ PAGE_TOKENS = (16, 32, 64, 128)
 MAX_LISTED = 1024
 # torch.cuda.current_stream(device).cuda_stream without the Stream object (1.9 us a call)
 _stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch.cuda.current_device
+_WEIGHT = (HEAD_DIM,)
 _TYPES = {torch.bfloat16: 0, torch.float8_e4m3fn: 1}
 
 
@@ -95,6 +97,7 @@ class PagedKVCache:
         self.device = k_pages.device
         stride = [t.stride(0) if n > 1 else heads * page * HEAD_DIM for t in (k_pages, v_pages)]
         self._index = k_pages.get_device()
+        self._max_width = (MAX_TOKENS + 127) // page
         self._args = _lib.PagedCacheArgs(ptr(k_pages), ptr(v_pages), ptr(k_exp),
                                          ptr(v_exp) if fp8 else None, ptr(bounds), stride[0],
                                          stride[1], n, page, heads, _TYPES[k_pages.dtype])
@@ -108,45 +111,55 @@ class PagedKVCache:
                      for p, e in ((self.k_pages, self.k_exp), (self.v_pages, self.v_exp)))
 
 
+_BATCH = "a batch is page_table [seqs, width], contiguous cu_tokens [seqs + 1] and seq_lens [seqs]"
+
+
 def _batch(cache: PagedKVCache, tokens: int, page_table, cu_tokens, seq_lens) -> _lib.PagedBatchArgs:
-    index = cache._index
-    for name, t, dims in (("page_table", page_table, 2), ("cu_tokens", cu_tokens, 1), ("seq_lens", seq_lens, 1)):
-        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.get_device() != index:
-            raise ValueError(f"{name} must be an int32 tensor on the cache's device")
-        if t.dim() != dims or (dims == 1 and not t.is_contiguous()):
-            raise ValueError("a batch is page_table [seqs, width], contiguous cu_tokens [seqs + 1] and seq_lens [seqs]")
-    seqs, (rows, width) = seq_lens.shape[0], page_table.shape
-    if seqs < 1 or cu_tokens.shape[0] != seqs + 1 or rows != seqs or width < 1:
-        raise ValueError("a batch is page_table [seqs, width], cu_tokens [seqs + 1] and seq_lens [seqs]")
+    index, kind = cache._index, torch.int32
+    if not (isinstance(page_table, torch.Tensor) and isinstance(cu_tokens, torch.Tensor)
+            and isinstance(seq_lens, torch.Tensor) and page_table.dtype is kind
+            and cu_tokens.dtype is kind and seq_lens.dtype is kind
+            and page_table.get_device() == index and cu_tokens.get_device() == index
+            and seq_lens.get_device() == index):
+        raise ValueError("page_table, cu_tokens and seq_lens must be int32 tensors on the cache's device")
+    if page_table.dim() != 2 or not cu_tokens.is_contiguous() or not seq_lens.is_contiguous():
+        raise ValueError(_BATCH)
+    rows, width = page_table.shape
+    if seq_lens.shape != (rows,) or cu_tokens.shape != (rows + 1,) or rows < 1 or width < 1:
+        raise ValueError(_BATCH)
     stride, inner = page_table.stride()
-    if width > 1 and inner != 1 or seqs > 1 and stride < width:
+    if width > 1 and inner != 1 or rows > 1 and stride < width:
         raise ValueError("page_table must have contiguous rows that do not overlap")
-    if width * cache.page_tokens > MAX_TOKENS + 127:
+    if width > cache._max_width:
         raise ValueError(f"a sequence has at most {MAX_TOKENS} tokens")
-    if not 0 < tokens <= MAX_TOKENS or seqs > 65536:
+    if not 0 < tokens <= MAX_TOKENS or rows > 65536:
         raise ValueError(f"a call has 1 to {MAX_TOKENS} rows of at most 65536 sequences")
     return _lib.PagedBatchArgs(page_table.data_ptr(), cu_tokens.data_ptr(), seq_lens.data_ptr(),
-                               stride if seqs > 1 else width, width, seqs, tokens)
+                               stride if rows > 1 else width, width, rows, tokens)
 
 
-def _rows(t, name: str, rows: int, width: int, index: int) -> int:
-    """Row stride of a bf16 [rows, width] tensor with unit inner stride."""
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16 or t.get_device() != index:
+def _rows(t, name: str, rows: int, width: int, index: int) -> tuple[int, int]:
+    """Address and row stride of a bf16 [rows, width] tensor with unit inner stride."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.bfloat16 or t.get_device() != index:
         raise ValueError(f"{name} must be a bf16 tensor on the cache's device")
-    if t.shape != (rows, width) or t.stride(1) != 1:
-        raise ValueError(f"{name} must be [{rows}, {width}] with unit inner stride")
-    stride = t.stride(0) if rows > 1 else width
-    if stride < width or stride % 4 or t.data_ptr() % 8:
-        raise ValueError(f"{name}'s rows must be 8-byte aligned and not overlap")
-    return stride
+    if t.shape != (rows, width):
+        raise ValueError(f"{name} must be [{rows}, {width}]")
+    stride, inner = t.stride()
+    if rows == 1:
+        stride = width
+    at = t.data_ptr()
+    if inner != 1 or stride < width or (at | 2 * stride) & 7:
+        raise ValueError(f"{name} must have unit inner stride and 8-byte aligned rows that do not overlap")
+    return at, stride
 
 
 def _queries(q, cache: PagedKVCache) -> int:
-    if not isinstance(q, torch.Tensor) or q.dtype != torch.bfloat16 or q.get_device() != cache._index:
+    if not isinstance(q, torch.Tensor) or q.dtype is not torch.bfloat16 or q.get_device() != cache._index:
         raise ValueError("q must be a bf16 tensor on the cache's device")
-    if q.dim() != 3 or q.shape[1:] != (cache.heads, HEAD_DIM) or not q.is_contiguous() or q.data_ptr() % 16:
+    t = q.shape[0] if q.dim() == 3 else 0
+    if q.shape != (t, cache.heads, HEAD_DIM) or not q.is_contiguous() or q.data_ptr() & 15:
         raise ValueError(f"q must be contiguous [T, {cache.heads}, 256], 16-byte aligned")
-    return q.shape[0]
+    return t
 
 
 def _out(out, shape, dtype, device) -> torch.Tensor:
@@ -160,12 +173,13 @@ def _out(out, shape, dtype, device) -> torch.Tensor:
 
 def _call(cache: PagedKVCache, name: str, *args) -> None:
     """The entry point on the cache's device and its current stream."""
-    fn = getattr(_lib.load(), name)
-    if torch.cuda.current_device() == cache._index:
-        status = fn(*args, _stream(cache._index))
+    fn = getattr(_lib._LIB or _lib.load(), name)
+    index = cache._index
+    if _current_device() == index:
+        status = fn(*args, _stream(index))
     else:
-        with torch.cuda.device(cache._index):
-            status = fn(*args, _stream(cache._index))
+        with torch.cuda.device(index):
+            status = fn(*args, _stream(index))
     if status != 0:
         raise _lib.KernelError(f"{name} failed: hip_status={status}")
 
@@ -188,32 +202,34 @@ def paged_append(q_gate: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm:
     dev, index = cache.device, cache._index
     t = q_gate.shape[0] if isinstance(q_gate, torch.Tensor) and q_gate.dim() == 2 else 0
     batch = _batch(cache, t, page_table, cu_tokens, seq_lens)
-    qs = _rows(q_gate, "q_gate", t, 2 * cache.heads * HEAD_DIM, index)
-    ks = _rows(k, "k", t, cache.kv_heads * HEAD_DIM, index)
-    vs = _rows(v, "v", t, cache.kv_heads * HEAD_DIM, index)
+    qp, qs = _rows(q_gate, "q_gate", t, 2 * cache.heads * HEAD_DIM, index)
+    kp, ks = _rows(k, "k", t, cache.kv_heads * HEAD_DIM, index)
+    vp, vs = _rows(v, "v", t, cache.kv_heads * HEAD_DIM, index)
     cos, sin = rope
     if not (isinstance(q_norm, torch.Tensor) and isinstance(k_norm, torch.Tensor)
-            and q_norm.dtype == k_norm.dtype == torch.bfloat16 and q_norm.get_device() == index
-            and k_norm.get_device() == index and q_norm.shape == k_norm.shape == (HEAD_DIM,)
+            and q_norm.dtype is k_norm.dtype is torch.bfloat16 and q_norm.get_device() == index
+            and k_norm.get_device() == index and q_norm.shape == k_norm.shape == _WEIGHT
             and q_norm.is_contiguous() and k_norm.is_contiguous()):
         raise ValueError("q_norm and k_norm must be contiguous bf16 [256] on the cache's device")
     if not (isinstance(cos, torch.Tensor) and isinstance(sin, torch.Tensor)
-            and cos.dtype == sin.dtype == torch.float32 and cos.get_device() == index
-            and sin.get_device() == index and cos.dim() == 2 and cos.shape[1] == 32
-            and cos.shape == sin.shape and cos.shape[0] > 0 and cos.is_contiguous()
-            and sin.is_contiguous() and not (cos.data_ptr() | sin.data_ptr()) % 16):
-        raise ValueError("rope must be two 16-byte aligned fp32 [positions, 32] on the cache's device")
+            and cos.dtype is sin.dtype is torch.float32 and cos.get_device() == index
+            and sin.get_device() == index and cos.dim() == 2 and cos.is_contiguous()
+            and sin.is_contiguous()):
+        raise ValueError("rope must be two contiguous fp32 tensors on the cache's device")
+    positions, pairs = cos.shape
+    cp, sp = cos.data_ptr(), sin.data_ptr()
+    if pairs != 32 or positions < 1 or sin.shape != (positions, 32) or (cp | sp) & 15:
+        raise ValueError("rope must be two 16-byte aligned [positions, 32]")
     q_out = _out(q_out, (t, cache.heads, HEAD_DIM), torch.bfloat16, dev)
-    _call(cache, "qwen36_paged_append", q_gate.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
-          q_norm.data_ptr(), k_norm.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
-          cache._args, batch, q_out.data_ptr())
+    _call(cache, "qwen36_paged_append", qp, qs, kp, ks, vp, vs, q_norm.data_ptr(), k_norm.data_ptr(),
+          cp, sp, positions, cache._args, batch, q_out.data_ptr())
     return q_out
 
 
 def _gate(q_gate, t: int, cache: PagedKVCache) -> tuple[int | None, int]:
     if q_gate is None:
         return None, 0
-    return q_gate.data_ptr(), _rows(q_gate, "q_gate", t, 2 * cache.heads * HEAD_DIM, cache._index)
+    return _rows(q_gate, "q_gate", t, 2 * cache.heads * HEAD_DIM, cache._index)
 
 
 def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tensor,
