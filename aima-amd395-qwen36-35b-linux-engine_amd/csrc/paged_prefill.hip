@@ -9,7 +9,7 @@
 // every wave reads whole.  Stages of 32 KB (64 keys of e4m3, 32 of bf16):
 //  * K and V rows go from their pages straight to LDS in the pages' type (no
 //    registers), a stage ahead of their use.  The 16-byte chunks of a row are
-//    exchanged by its number (chunk ^ (row & 15)) on the way, which leaves the
+//    exchanged by its number on the way, which leaves the
 //    row-wise K reads and the transposed V reads free of bank conflicts.
 //  * per 32 keys: S^T = K Q^T, online softmax in fp32, O^T += V^T P^T on 32x32x16
 //    products.  A = K rows; B = Q^T in registers; A = V^T by transposed LDS reads;
@@ -19,6 +19,8 @@
 // The reference maximum is the first visible tile's and is raised (with a
 // rescale) only when a tile's probabilities sum past 2^20.
 #include "paged_split.h"
+
+#include <atomic>
 
 namespace q36 {
 namespace {
@@ -31,14 +33,24 @@ typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(1))) void global_void;
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
+typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+
+// The exchange of a row's 16-byte chunks: chunk c of row r lies at c ^ swap(r).
+// Rows 0-15 take 16 different places for one chunk (K reads, V of e4m3), rows
+// r .. r + 3 disjoint ones for four chunks (V of bf16).
+__device__ __forceinline__ int swap(int row) { return (row & 3) << 2 | ((row >> 2) & 3); }
 
 constexpr float kScoreScale = 0.0625f * kLog2e;
 
+__device__ __forceinline__ i16x4 tr16(unsigned at) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(uintptr_t)at);
+}
+
 template <bool kFp8, int kWaves>
 __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefill_kernel(
-    const bf16* __restrict__ q, PagedCache c, PagedBatch b, PagedOut w, unsigned target) {
+    const bf16* __restrict__ q, PagedCache c, PagedBatch b, PagedOut w, unsigned slots, unsigned target) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
-  __shared__ unsigned find[40];
+  __shared__ unsigned find[52];
   __shared__ int odd;   // whether a V value that some rows must not see is not finite
   constexpr int kElem = kFp8 ? 1 : 2;
   constexpr int kTile = 4 * kWaves;
@@ -50,7 +62,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
   const unsigned head = blockIdx.x % c.heads, item = blockIdx.x / c.heads;
   const unsigned hq = c.heads * kGroup;
   PagedSplit sp;
-  if (!paged_split<kTile>(b, item, target, blockIdx.x == 0 ? w.head : nullptr, find, sp)) return;
+  if (!paged_split<kTile>(b, item, slots, target, blockIdx.x == 0 ? w.head : nullptr, find, sp)) return;
   const PagedSeq s = paged_seq(b, sp.seq);
   const unsigned chunks = ((unsigned)s.len + sp.chunk - 1) / sp.chunk;
   const int n_rows = s.z - s.a;
@@ -76,15 +88,6 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
   const int wave_first = pos0 + wave * 4;
   const int wave_lim = wave * 4 < n_tok ? min(wave_first + 3, end - 1) : -1;
 
-  bf16x8 qf[16];
-  {
-    const bf16* qp = q + ((size_t)(t0 + tok) * hq + head * kGroup + (lj & 7)) * kD + (kFp8 ? 16 : 8) * lg;
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      // the dims of k-step i as the K operand has them: an e4m3 chunk holds two steps
-      qf[i] = lim >= 0 ? *reinterpret_cast<const bf16x8*>(qp + (kFp8 ? 32 * (i >> 1) + 8 * (i & 1) : 16 * i))
-                       : bf16x8{};
-  }
   f32x16 o[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) o[i] = f32x16{};
@@ -110,6 +113,18 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
     }
   };
 
+  // the first block's before the queries: loads return in order
+  fetch_pages(kv_first);
+  fetch_scales();
+  bf16x8 qf[16];
+  {
+    const bf16* qp = q + ((size_t)(t0 + tok) * hq + head * kGroup + (lj & 7)) * kD + (kFp8 ? 16 : 8) * lg;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      // the dims of k-step i as the K operand has them: an e4m3 chunk holds two steps
+      qf[i] = lim >= 0 ? *reinterpret_cast<const bf16x8*>(qp + (kFp8 ? 32 * (i >> 1) + 8 * (i & 1) : 16 * i))
+                       : bf16x8{};
+  }
   // ---- a stage's rows, 4 (e4m3) or 2 (bf16) a load: one page each
   unsigned ok = 0, ok_next = 0;            // bit g: the 16 keys g of the stage have a page
   unsigned e0 = 0, e1 = 0, e2 = 0, e3 = 0;  // scale bytes of the loaded stage's 16-key groups (K, V << 8)
@@ -117,10 +132,6 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
   const auto load_stage = [&](int i) {
     const int at = i % kBlockStages;
     if (at == 0) {
-      if (i == 0) {
-        fetch_pages(kv_first);
-        fetch_scales();
-      }
       d_page = n_page;
       d_exp = n_exp;
       d_ok = __ballot(n_ok);
@@ -143,7 +154,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
       const int row = row0 + lane / (kRowB / 16);
       const unsigned pid = __builtin_amdgcn_readlane(d_page, kGroups * at + (row0 >> 4));
       const int prow = (kv_first + i * kStageKeys + row0) & page_mask;
-      const unsigned off = (row - row0) * kRowB + (((lane & (kRowB / 16 - 1)) ^ (row & 15)) << 4);
+      const unsigned off = (row - row0) * kRowB + (((lane & (kRowB / 16 - 1)) ^ swap(row)) << 4);
       const char* kp = c.k + pid * c.k_stride + head_off + (size_t)prow * kRowB;
       const char* vp = c.v + pid * c.v_stride + head_off + (size_t)prow * kRowB;
       __builtin_amdgcn_global_load_lds((global_void*)(kp + off), (lds_void*)(to + row0 * kRowB), 16, 0, 0);
@@ -173,11 +184,12 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
   };
 
   // per-lane LDS addresses; k-steps and dim tiles flip bits of the chunk number
-  const int kbase = lj * kRowB + ((lg ^ (lj & 15)) << 4);
+  const unsigned lds0 = (unsigned)(uintptr_t)(lds_void*)lds;
+  const unsigned kbase = lds0 + lj * kRowB + ((lg ^ swap(lj)) << 4);
   const int grp = lane >> 4, m16 = lane & 15;
   const int vrow = kFp8 ? 8 * (m16 >> 3) + 4 * lg + ((m16 >> 1) & 3) : 4 * lg + (m16 >> 2);
   const int vchunk = kFp8 ? grp & 1 : 2 * (grp & 1) + ((m16 >> 1) & 1);
-  const int vbase = vrow * kRowB + ((vchunk ^ vrow) << 4) + 8 * (m16 & 1);
+  const unsigned vbase = lds0 + kHalf + vrow * kRowB + ((vchunk ^ swap(vrow)) << 4) + 8 * (m16 & 1);
 
   const int n_stages = (kv_stop - kv_first + kStageKeys - 1) / kStageKeys;
   if (tid == 0) odd = 0;
@@ -197,8 +209,9 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
     for (int sub = 0; sub < kSubs; ++sub) {
     const int kv0 = key_st + sub * kKeys;
     if (kv0 > wave_lim) continue;
-    const char* kp = lds + (st & 1) * kStage + sub * kKeys * kRowB;
-    const char* vp = kp + kHalf;
+    // (whole rows away: the exchanged bits stay as they are)
+    const unsigned kp = kbase + (st & 1) * kStage + sub * kKeys * kRowB;
+    const unsigned vp = vbase + (st & 1) * kStage + sub * kKeys * kRowB;
     const unsigned okh = ok >> (2 * sub), ea = sub ? f2 : f0, eb = sub ? f3 : f1;
     f32x16 x = f32x16{};
     // the wave with products to issue goes before the one in its softmax (2,048
@@ -207,7 +220,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
     if constexpr (kFp8) {
       const float ks = paged_scale((lj < 16 ? ea : eb) & 0xffu);
       u32x4 kr[4];
-      const auto kread = [&](int i) { return *reinterpret_cast<const u32x4*>(kp + (kbase ^ (i << 5))); };
+      const auto kread = [&](int i) { return *(const lds_u32x4*)(uintptr_t)(kp ^ (i << 5)); };
 #pragma unroll
       for (int i = 0; i < 4; ++i) kr[i] = kread(i);
 #pragma unroll
@@ -223,7 +236,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
       }
     } else {
       bf16x8 kr[4];
-      const auto kread = [&](int i) { return *reinterpret_cast<const bf16x8*>(kp + (kbase ^ (i << 5))); };
+      const auto kread = [&](int i) { return __builtin_bit_cast(bf16x8, *(const lds_u32x4*)(uintptr_t)(kp ^ (i << 5))); };
 #pragma unroll
       for (int i = 0; i < 4; ++i) kr[i] = kread(i);
 #pragma unroll
@@ -291,7 +304,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
       i32x2 va[4];
       const auto vread = [&](int i) {   // keys 16 (i / 8) .. + 16, dims 32 (i % 8) .. + 32
         return __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-            (lds_i32x2*)(vp + (i >> 3) * 16 * kRowB + (vbase ^ ((i & 7) << 5))));
+            (lds_i32x2*)(uintptr_t)((vp ^ ((i & 7) << 5)) + (i >> 3) * 16 * kRowB));
       };
 #pragma unroll
       for (int i = 0; i < 4; ++i) va[i] = vread(i);
@@ -307,10 +320,9 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
     } else {
       i16x4 va[4][2];
       const auto vread = [&](int i, int to) {
-        const char* p = vp + (i >> 3) * 16 * kRowB;
-        const int at = vbase ^ ((i & 7) << 6);
-        va[to][0] = lds_read_tr16(p + at);
-        va[to][1] = lds_read_tr16(p + 8 * kRowB + (at ^ 128));   // keys + 8
+        const unsigned at = vp ^ ((i & 7) << 6);
+        va[to][0] = tr16(at + (i >> 3) * 16 * kRowB);
+        va[to][1] = tr16((at ^ 32) + ((i >> 3) * 16 + 8) * kRowB);   // keys + 8: swap(8) is 2
       };
 #pragma unroll
       for (int i = 0; i < 4; ++i) vread(i, i);
@@ -342,6 +354,20 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
     w.ml[part * 2 + 1] = l;
   }
   const bool zero = l == 0.f;
+  // the gates of this wave's rows, all asked for at once (rows past the end read the
+  // last row's)
+  bf16x4 gt[4][8];
+  if (single && w.gate != nullptr) {
+#pragma unroll
+    for (int rd = 0; rd < 4; ++rd)
+#pragma unroll
+      for (int it = 0; it < 8; ++it) {
+        const int r = it * 4 + (lane >> 4);
+        const size_t row = t0 + min(wave * 4 + (r >> 3), n_tok - 1);
+        gt[rd][it] = *reinterpret_cast<const bf16x4*>(w.gate + row * w.gate_stride + (head * kGroup + (r & 7)) * 2 * kD +
+                                                      kD + rd * 64 + (lane & 15) * 4);
+      }
+  }
   __syncthreads();
   const bool strange_v = odd != 0;
   char* stg = lds + wave * 8192;
@@ -375,9 +401,8 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
       const size_t row = t0 + rt, qh = head * kGroup + (r & 7);
       bf16x4 res;
       if (w.gate != nullptr) {
-        const bf16x4 gt = *reinterpret_cast<const bf16x4*>(w.gate + row * w.gate_stride + qh * 2 * kD + kD + d);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) res[e] = f2bf(v[e] == 0.f ? 0.f : paged_gate(v[e], gt[e]));
+        for (int e = 0; e < 4; ++e) res[e] = f2bf(v[e] == 0.f ? 0.f : paged_gate(v[e], gt[rd][it][e]));
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e) res[e] = f2bf(v[e]);
@@ -388,33 +413,42 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
   }
 }
 
+// More than 64 KB of LDS has to be asked for once on each device.
+int allow_lds(const void* kernel, std::atomic<bool> (&ready)[64]) {
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return Q36_EINVAL;
+  if (ready[dev].load(std::memory_order_acquire)) return Q36_OK;
+  const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+  if (e == hipSuccess) ready[dev].store(true, std::memory_order_release);
+  return static_cast<int>(e);
+}
+
 template <bool kFp8, int kWaves>
 int launch(const bf16* q, const PagedCache& c, const PagedBatch& b, const PagedOut& o, unsigned items,
-           unsigned target, void* stream) {
-  // hipFuncSetAttribute is per device and idempotent
-  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_prefill_kernel<kFp8, kWaves>),
-                                           hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
-  if (e != hipSuccess) return static_cast<int>(e);
+           unsigned slots, unsigned target, void* stream) {
+  static std::atomic<bool> ready[64];
+  const int e = allow_lds(reinterpret_cast<const void*>(&paged_prefill_kernel<kFp8, kWaves>), ready);
+  if (e != Q36_OK) return e;
   hipLaunchKernelGGL((paged_prefill_kernel<kFp8, kWaves>), dim3(items * c.heads), dim3(64 * kWaves), kLds,
-                     static_cast<hipStream_t>(stream), q, c, b, o, target);
+                     static_cast<hipStream_t>(stream), q, c, b, o, slots, target);
   return static_cast<int>(hipGetLastError());
 }
 
 }  // namespace
 
 int paged_prefill(const void* q, const PagedCache& c, bool fp8, const PagedBatch& b, const PagedOut& o,
-                  unsigned tile, unsigned items, unsigned target, void* stream) {
+                  unsigned tile, unsigned items, unsigned slots, unsigned target, void* stream) {
   const bf16* p = static_cast<const bf16*>(q);
   switch (tile) {
     case 8:
-      return fp8 ? launch<true, 2>(p, c, b, o, items, target, stream)
-                 : launch<false, 2>(p, c, b, o, items, target, stream);
+      return fp8 ? launch<true, 2>(p, c, b, o, items, slots, target, stream)
+                 : launch<false, 2>(p, c, b, o, items, slots, target, stream);
     case 16:
-      return fp8 ? launch<true, 4>(p, c, b, o, items, target, stream)
-                 : launch<false, 4>(p, c, b, o, items, target, stream);
+      return fp8 ? launch<true, 4>(p, c, b, o, items, slots, target, stream)
+                 : launch<false, 4>(p, c, b, o, items, slots, target, stream);
     default:
-      return fp8 ? launch<true, 8>(p, c, b, o, items, target, stream)
-                 : launch<false, 8>(p, c, b, o, items, target, stream);
+      return fp8 ? launch<true, 8>(p, c, b, o, items, slots, target, stream)
+                 : launch<false, 8>(p, c, b, o, items, slots, target, stream);
   }
 }
 
