@@ -472,6 +472,7 @@ __device__ __forceinline__ bool paged_parts(const PagedBatch& b, unsigned heads,
     }
     r = own % tile * kGroup + qh % kGroup;
   }
+  if (p.n > w.slots || slot > w.slots - p.n) return false;   // only where sequences overlap
   p.stride = heads * kGroup * tile;
   p.first = (slot * heads + qh / kGroup) * kGroup * tile + r;
   return true;
@@ -494,33 +495,37 @@ __device__ __forceinline__ void paged_merge4(float& m, float& l, f32x4& o, const
   m = mn;
 }
 
-// Many rows of few chunks: a wave per row and head, 4 dims a lane.
+// Many rows of few chunks: a wave per kHeads query heads of a token, 4 dims a lane.
+template <unsigned kHeads>
 __global__ __launch_bounds__(256) void paged_combine_rows_kernel(PagedBatch b, unsigned heads, PagedOut w,
                                                                  unsigned tile, unsigned listed_chunks) {
   const unsigned hq = heads * kGroup;
   const unsigned i = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const unsigned t = i / hq, qh = i % hq;
+  const unsigned t = i * kHeads / hq, h0 = i * kHeads % hq;
   if (t >= b.tokens) return;
   Parts p;
-  if (!paged_parts(b, heads, w, tile, listed_chunks, t, qh, p) || p.n == 1) return;
+  if (!paged_parts(b, heads, w, tile, listed_chunks, t, h0, p) || p.n == 1) return;
   const unsigned d = (threadIdx.x & 63) * 4;
-  float m = -INFINITY, l = 0.f;
-  f32x4 o = f32x4{};
-  for (unsigned i0 = 0; i0 < p.n; i0 += 4) {
-    float cm[4], cl[4];
-    f32x4 co[4];
+#pragma unroll 4
+  for (unsigned h = 0; h < kHeads; ++h) {   // a head's partials are the next rows of its KV head's
+    float m = -INFINITY, l = 0.f;
+    f32x4 o = f32x4{};
+    for (unsigned i0 = 0; i0 < p.n; i0 += 4) {
+      float cm[4], cl[4];
+      f32x4 co[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const bool there = i0 + u < p.n;
-      const size_t part = p.first + (size_t)(there ? i0 + u : i0) * p.stride;
-      cm[u] = there ? w.ml[part * 2] : -INFINITY;
-      cl[u] = there ? w.ml[part * 2 + 1] : 0.f;
-      co[u] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(w.o + part * kD + d));
-      if (!there) co[u] = f32x4{};
+      for (int u = 0; u < 4; ++u) {
+        const bool there = i0 + u < p.n;
+        const size_t part = p.first + h + (size_t)(there ? i0 + u : i0) * p.stride;
+        cm[u] = there ? w.ml[part * 2] : -INFINITY;
+        cl[u] = there ? w.ml[part * 2 + 1] : 0.f;
+        co[u] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(w.o + part * kD + d));
+        if (!there) co[u] = f32x4{};
+      }
+      paged_merge4(m, l, o, cm, cl, co);
     }
-    paged_merge4(m, l, o, cm, cl, co);
+    paged_store(w, hq, t, h0 + h, d, o, l);
   }
-  paged_store(w, hq, t, qh, d, o, l);
 }
 
 // Few rows of many chunks: a workgroup per row, head and 64 dims; 16 groups of
@@ -643,11 +648,18 @@ int paged_combine(const PagedBatch& b, const PagedCache& c, const PagedOut& o, u
                   unsigned listed_chunks, void* stream) {
   const unsigned hq = c.heads * kGroup;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  // 2,048 tokens: 217 us with a workgroup per 64 dims (4 chunks), 24 with a wave per
-  // row (2 chunks).
-  if (b.tokens >= 256 / c.heads)
-    hipLaunchKernelGGL(paged_combine_rows_kernel, dim3((b.tokens * hq + 3) / 4), dim3(256), 0, st, b, c.heads, o, tile,
+  // 2,048 tokens of 2 chunks: 24 us with a wave per head (217 with a workgroup per 64
+  // dims and 4 chunks).  Where thousands of tokens have one chunk a wave per 8 heads
+  // ends sooner (4,020 tokens: 16 us and 5); 200 tokens of 18 chunks take 18 more so.
+  const unsigned pairs = b.tokens * c.heads;
+  const auto rows = [&](auto kernel, unsigned per) {
+    hipLaunchKernelGGL(kernel, dim3((b.tokens * (hq / per) + 3) / 4), dim3(256), 0, st, b, c.heads, o, tile,
                        listed_chunks);
+  };
+  if (pairs >= 2048)
+    rows(paged_combine_rows_kernel<kGroup>, kGroup);
+  else if (pairs >= 256)
+    rows(paged_combine_rows_kernel<1>, 1);
   else
     hipLaunchKernelGGL(paged_combine_kernel, dim3(b.tokens * hq * 4), dim3(256), 0, st, b, c.heads, o, tile,
                        listed_chunks);

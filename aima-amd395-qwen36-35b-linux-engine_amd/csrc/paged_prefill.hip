@@ -78,6 +78,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
   const int kv_stop = min(kv_first + (int)sp.chunk, end);
   const size_t slot = item - sp.local + (size_t)qt * chunks + chunk;
   const bool single = end <= (int)sp.chunk;
+  if (slot >= w.slots) return;   // overlapping sequences: more tiles than rows
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);

@@ -27,6 +27,7 @@ struct PagedOut {
   float* o;               // [slot][KV head][8 * tile tokens][256]
   unsigned* head;         // [0]: blocks of a chunk or share, [1 + i]: first item or block of sequence i
   size_t gate_stride;
+  unsigned slots;         // that the workspace holds; offsets that make more have none for the rest
 };
 
 struct PagedSplit {
@@ -151,6 +152,7 @@ inline size_t split_ws_bytes(unsigned seqs, size_t slots, unsigned heads, unsign
 }
 inline void split_ws(void* ws, unsigned seqs, size_t slots, unsigned heads, unsigned rows, PagedOut& o) {
   char* p = static_cast<char*>(ws);
+  o.slots = (unsigned)slots;
   o.head = reinterpret_cast<unsigned*>(p);
   p += round256(((size_t)seqs + 1) * 4);
   o.ml = reinterpret_cast<float*>(p);

@@ -493,8 +493,9 @@ typedef struct {
  * are left as they were.  Nothing there can make a launch read or write out of
  * bounds: a page id outside [0, num_pages) holds no tokens (and takes none), a
  * sequence longer than its table (or than the rotation tables) has none, rows
- * of negative position see nothing.  A page that an append writes must belong
- * to one sequence of the batch. */
+ * of negative position see nothing, and the rows of sequences that overlap are
+ * any of theirs or left as they were.  A page that an append writes must belong
+ * to one sequence of the batch; read, pages may be shared. */
 typedef struct {
   const void* page_table;
   const void* cu_tokens;

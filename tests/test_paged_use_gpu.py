@@ -212,6 +212,47 @@ def test_many_sequences(gpu, seqs, new):
     check(got, want, tol, rows)
 
 
+@pytest.mark.parametrize("cu,tokens", [([0, 100] * 6 + [0], 100), ([0, 2] * 20 + [0], 30), ([50, 0, 99, 7, 200, 3, 3, -5, 60], 60),
+                                       ([0, 2 ** 31 - 1, -2 ** 31, 90], 90), ([0, 17] * 5 + [0], 40)])
+def test_offsets_of_no_batch_stay_in_bounds(gpu, cu, tokens):
+    """Offsets that overlap, fall or leave the call: whatever the rows then hold,
+    nothing is written outside the outputs, the workspaces and the table's pages."""
+    import ctypes
+    from qwen36_attn import _lib
+    seqs, page, width = len(cu) - 1, 16, 60
+    b = R.Batch([900], [1], page, seed=3)
+    c, _ = filled_cache(gpu, b, 2, FP8, True, seed=3)
+    table = b.table.repeat(seqs, 1)[:, :width].contiguous().to(gpu)
+    where = (table, torch.tensor(cu, dtype=torch.int64).clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32).to(gpu),
+             torch.tensor([900 - i for i in range(seqs)], dtype=torch.int32, device=gpu))
+    batch = pa._batch(c, tokens, *where)
+    q = syn.randn((tokens, 16, 256), syn.gen(1)).to(gpu)
+    lib, edge = _lib.load(), 1 << 20
+
+    def guarded(n):
+        return torch.full((n + edge,), 0x5A, dtype=torch.uint8, device=gpu)
+    n = lib.qwen36_paged_attention_workspace_bytes(c._args, batch)
+    ws, out = guarded(n), guarded(tokens * 4096 * 2)
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.qwen36_paged_attention(q.data_ptr(), c._args, batch, None, 0, out.data_ptr(), ws.data_ptr(), n, stream) == 0
+    m = lib.qwen36_paged_select_workspace_bytes(c._args, batch)
+    ws2, pages = guarded(m), guarded(tokens * 2 * 8 * 4)
+    assert lib.qwen36_paged_select(q.data_ptr(), c._args, batch, 8, 1, 1, pages.data_ptr(), ws2.data_ptr(), m, stream) == 0
+    k = lib.qwen36_paged_sparse_attention_workspace_bytes(c._args, batch, 8)
+    ws3, out3 = guarded(k), guarded(tokens * 4096 * 2)
+    assert lib.qwen36_paged_sparse_attention(q.data_ptr(), c._args, batch, pages.data_ptr(), 8, None, 0, out3.data_ptr(),
+                                             ws3.data_ptr(), k, stream) == 0
+    x = layer_rows(gpu, tokens, 2, 2)
+    before = R.CacheState(c)
+    pa.paged_append(*x, fa.rotary_table(1024, 0, gpu), c, *where)
+    torch.cuda.synchronize()
+    for t in (ws, out, ws2, pages, ws3, out3):
+        assert (t[-edge:] == 0x5A).all()
+    after = R.CacheState(c)
+    spare = [p for p in range(b.pool) if p not in b.table[0].tolist()]
+    assert torch.equal(after.k[spare], before.k[spare]) and torch.equal(after.v[spare], before.v[spare])
+
+
 def test_results_do_not_depend_on_what_memory_held(gpu):
     b = R.Batch([600, 70], [2, 40], 16, seed=11)
     c, _ = filled_cache(gpu, b, 2, BF16, True, seed=11)
