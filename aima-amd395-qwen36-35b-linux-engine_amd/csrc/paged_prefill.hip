@@ -11,11 +11,14 @@
 //    registers), a stage ahead of their use.  The 16-byte chunks of a row are
 //    exchanged by its number on the way, which leaves the
 //    row-wise K reads and the transposed V reads free of bank conflicts.
-//  * per 32 keys: S^T = K Q^T, online softmax in fp32, O^T += V^T P^T on 32x32x16
-//    products.  A = K rows; B = Q^T in registers; A = V^T by transposed LDS reads;
-//    B = P^T, the S^T accumulator as it is.  e4m3 becomes bf16 behind LDS, with
-//    the page's scale inside the conversion: half the LDS bytes, which pays for
-//    the 128 conversions a wave has besides its 32 products.
+//  * per 32 keys: S^T = K Q^T, online softmax in fp32, O^T += V^T P^T.  A = K rows;
+//    B = Q^T in registers; A = V^T by transposed LDS reads; B = P^T, the S^T
+//    accumulator as it is.  bf16: 32x32x16 products throughout.  e4m3: K is taken as
+//    it lies, by 32x32x64 products with the page's scale byte in the instruction,
+//    against Q as the sum of two e4m3 values (as much matrix time as bf16, no
+//    conversions); V becomes bf16 behind LDS, the scale inside the conversion.
+//    Converting K too took 922 us for 2,048 tokens over 30K, so 863; a tile's
+//    prologue is 1 us longer (93 tokens over 2K: 37.4 and 39.1).
 // The reference maximum is the first visible tile's and is raised (with a
 // rescale) only when a tile's probabilities sum past 2^20.
 #include "paged_split.h"
@@ -32,6 +35,7 @@ constexpr int kLds = 2 * kStage;
 typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(1))) void global_void;
 typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
 
@@ -44,6 +48,63 @@ constexpr float kScoreScale = 0.0625f * kLog2e;
 
 __device__ __forceinline__ i16x4 tr16(unsigned at) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(uintptr_t)at);
+}
+
+// 32 bf16 values (and the 32 of lane ^ 32: one scale) as e4m3 sums
+// v = 2^(e - 127) (a + 2^-kSplitDown b): a to nearest, b the rest, which has at most the
+// 4 bits that a leaves of 8 and is at most half a step of a's, 16 of 448 (so 2^4 times
+// it is in range).  What is not finite is a NaN.  Returns e.  The conversions divide by
+// the scale that they are given.
+constexpr unsigned kSplitDown = 4;
+__device__ __forceinline__ unsigned split_e4m3(const u32x4 (&v)[4], i32x8& a, i32x8& b) {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  u16x2 top = {0, 0};   // magnitudes as bits; those past 0x7f7f are not finite
+#pragma unroll
+  for (int j = 0; j < 16; ++j)
+    top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, v[j >> 2][j & 3] & 0x7fff7fffu));
+  unsigned amax = max((unsigned)top[0], (unsigned)top[1]);
+  amax = max(amax, (unsigned)__shfl_xor(amax, 32, 64));
+  const bool strange = amax >= 0x7f80u;
+  if (__any(strange)) {   // the largest finite one, the slow way
+    amax = 0;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      const unsigned m = (v[j >> 3][(j >> 1) & 3] >> (16 * (j & 1))) & 0x7fffu;
+      amax = max(amax, m < 0x7f80u ? m : 0u);
+    }
+    amax = max(amax, (unsigned)__shfl_xor(amax, 32, 64));
+  }
+  const unsigned e = paged_scale_byte(__uint_as_float(amax << 16));
+  const float s1 = paged_scale(e), s2 = paged_scale(e - kSplitDown);
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    const unsigned lo = v[w >> 1][2 * (w & 1)], hi = v[w >> 1][2 * (w & 1) + 1];
+    const float x0 = __uint_as_float(lo << 16), x1 = __uint_as_float(lo & 0xffff0000u);
+    const float x2 = __uint_as_float(hi << 16), x3 = __uint_as_float(hi & 0xffff0000u);
+    s16x2 p = {0, 0}, r = {0, 0};
+    p = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(p, x0, x1, s1, false);
+    p = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(p, x2, x3, s1, true);
+    const unsigned pw = __builtin_bit_cast(unsigned, p);
+    const f32x2 a0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(pw, s1, false);
+    const f32x2 a1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(pw, s1, true);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, x0 - a0[0], x1 - a0[1], s2, false);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, x2 - a1[0], x3 - a1[1], s2, true);
+    a[w] = (int)pw;
+    b[w] = __builtin_bit_cast(int, r);
+  }
+  if (__any(strange)) {
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const unsigned m = (v[w >> 1][2 * (w & 1) + (j >> 1)] >> (16 * (j & 1))) & 0x7fffu;
+        if (m >= 0x7f80u) a[w] |= 0x7f << (8 * j);
+      }
+    }
+  }
+  return e;
 }
 
 template <bool kFp8, int kWaves>
@@ -117,14 +178,31 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
   // the first block's before the queries: loads return in order
   fetch_pages(kv_first);
   fetch_scales();
-  bf16x8 qf[16];
+  // Q^T operand.  bf16: k-step i has dims 16 i + 8 lg.  e4m3: the sum of two e4m3
+  // values with a scale for each 64 dims (step i: this lane has dims 64 i + 32 lg),
+  // which holds a bf16 value exactly unless it is 2^-14 of the 64's largest or less
+  // (then to 2^-22 of that).
+  bf16x8 qf[kFp8 ? 1 : 16];
+  i32x8 q1[kFp8 ? 4 : 1], q2[kFp8 ? 4 : 1];
+  unsigned qs1 = 0, qs2 = 0;   // scale bytes of the 4 steps
   {
-    const bf16* qp = q + ((size_t)(t0 + tok) * hq + head * kGroup + (lj & 7)) * kD + (kFp8 ? 16 : 8) * lg;
+    const bf16* qp = q + ((size_t)(t0 + tok) * hq + head * kGroup + (lj & 7)) * kD + (kFp8 ? 32 : 8) * lg;
+    if constexpr (kFp8) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      // the dims of k-step i as the K operand has them: an e4m3 chunk holds two steps
-      qf[i] = lim >= 0 ? *reinterpret_cast<const bf16x8*>(qp + (kFp8 ? 32 * (i >> 1) + 8 * (i & 1) : 16 * i))
-                       : bf16x8{};
+      for (int i = 0; i < 4; ++i) {
+        u32x4 v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          v[j] = lim >= 0 ? *reinterpret_cast<const u32x4*>(qp + 64 * i + 8 * j) : u32x4{};
+        const unsigned e = split_e4m3(v, q1[i], q2[i]);
+        qs1 |= e << (8 * i);
+        qs2 |= (e - kSplitDown) << (8 * i);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        qf[i] = lim >= 0 ? *reinterpret_cast<const bf16x8*>(qp + 16 * i) : bf16x8{};
+    }
   }
   // ---- a stage's rows, 4 (e4m3) or 2 (bf16) a load: one page each
   unsigned ok = 0, ok_next = 0;            // bit g: the 16 keys g of the stage have a page
@@ -186,7 +264,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
 
   // per-lane LDS addresses; k-steps and dim tiles flip bits of the chunk number
   const unsigned lds0 = (unsigned)(uintptr_t)(lds_void*)lds;
-  const unsigned kbase = lds0 + lj * kRowB + ((lg ^ swap(lj)) << 4);
+  const unsigned kbase = lds0 + lj * kRowB + (((kFp8 ? 2 * lg : lg) ^ swap(lj)) << 4);
   const int grp = lane >> 4, m16 = lane & 15;
   const int vrow = kFp8 ? 8 * (m16 >> 3) + 4 * lg + ((m16 >> 1) & 3) : 4 * lg + (m16 >> 2);
   const int vchunk = kFp8 ? grp & 1 : 2 * (grp & 1) + ((m16 >> 1) & 1);
@@ -219,22 +297,25 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
     // tokens over 30K: 970 us without, 944 with)
     __builtin_amdgcn_s_setprio(1);
     if constexpr (kFp8) {
-      const float ks = paged_scale((lj < 16 ? ea : eb) & 0xffu);
-      u32x4 kr[4];
-      const auto kread = [&](int i) { return *(const lds_u32x4*)(uintptr_t)(kp ^ (i << 5)); };
-#pragma unroll
-      for (int i = 0; i < 4; ++i) kr[i] = kread(i);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const u32x4 r = kr[i & 3];
-        if (i + 4 < 8) kr[i & 3] = kread(i + 4);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const u32x4 a = {cvt2<false>(r[2 * h], ks), cvt2<true>(r[2 * h], ks), cvt2<false>(r[2 * h + 1], ks),
-                           cvt2<true>(r[2 * h + 1], ks)};
-          x = mfma32x32x16(__builtin_bit_cast(bf16x8, a), qf[2 * i + h], x);
-        }
-      }
+      // the page's scale byte of this lane's key goes into the product as it is
+      const int ks = (int)((lj < 16 ? ea : eb) & 0xffu);
+      i32x8 kr[2];
+      const auto kread = [&](int i) {   // dims 64 i + 32 lg .. + 32
+        const u32x4 lo = *(const lds_u32x4*)(uintptr_t)(kp ^ (i << 6)), hi = *(const lds_u32x4*)(uintptr_t)(kp ^ (i << 6) ^ 16);
+        return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+      };
+      kr[0] = kread(0);
+      kr[1] = kread(1);
+      x = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kr[0], q1[0], x, 0, 0, 0, ks, 0, (int)qs1);
+      x = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kr[0], q2[0], x, 0, 0, 0, ks, 0, (int)qs2);
+      kr[0] = kread(2);
+      x = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kr[1], q1[1], x, 0, 0, 0, ks, 1, (int)qs1);
+      x = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kr[1], q2[1], x, 0, 0, 0, ks, 1, (int)qs2);
+      kr[1] = kread(3);
+      x = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kr[0], q1[2], x, 0, 0, 0, ks, 2, (int)qs1);
+      x = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kr[0], q2[2], x, 0, 0, 0, ks, 2, (int)qs2);
+      x = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kr[1], q1[3], x, 0, 0, 0, ks, 3, (int)qs1);
+      x = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kr[1], q2[3], x, 0, 0, 0, ks, 3, (int)qs2);
     } else {
       bf16x8 kr[4];
       const auto kread = [&](int i) { return __builtin_bit_cast(bf16x8, *(const lds_u32x4*)(uintptr_t)(kp ^ (i << 5))); };

@@ -249,7 +249,7 @@ Q36_EXPORT int qwen36_paged_select(const void* q, const qwen36_paged_cache* cach
   unsigned* keys = static_cast<unsigned*>(workspace);
   if (b.width > budget) {   // else every row takes all its pages
     const size_t rows = (size_t)b.tokens * c.heads, groups = (b.width + 63) / 64;
-    size_t per = rows * groups / 512;   // 16-page groups a wave takes: the queries are quantised once
+    size_t per = rows * groups / 1024;   // 16-page groups a wave takes: the queries are quantised once
     per = per < 1 ? 1 : per > groups ? groups : per;
     const unsigned blocks = (unsigned)((groups + per - 1) / per);
     hipLaunchKernelGGL(paged_score_kernel, dim3((unsigned)(rows * blocks)), dim3(256), 0, st,

@@ -163,6 +163,8 @@ def attend_row(state, b, q, i, h, pos, pages):
     # fp32 scores: 256 products and sums of 2^-24 each, once in p and once in its sum;
     # exp2, its argument and the fp32 sums of n keys; P rounded to bf16 (2^-8)
     score = (q.abs() @ k.abs().t()).amax(-1, keepdim=True) / 16 * 258 * 2.0 ** -24
+    # a query as the sum of two e4m3 values: to 2^-22 of the largest of its 64 dims
+    score = score + q.abs().amax(-1, keepdim=True) * k.abs().sum(-1).amax() / 16 * 2.0 ** -22
     rel = 2.0 ** -8 + 2 * score + (2 * k.shape[0] + 64) * 2.0 ** -24
     return o, rel * (p @ v.abs()) + 2.0 ** -8 * o.abs() + 1e-30
 

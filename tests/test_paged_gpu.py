@@ -254,6 +254,37 @@ def test_later_rows_of_nan_do_not_reach_earlier_ones(gpu, dtype, lens, new):
         assert torch.isnan(got[last]).all()
 
 
+@pytest.mark.parametrize("new", [1, 2, 5, 12, 40])
+@pytest.mark.parametrize("dtype", [FP8, BF16])
+def test_queries_of_unequal_sizes_and_not_finite_ones(gpu, dtype, new):
+    """Channels from 2^-30 to 2^3 in one query; a query with a NaN, one with an
+    infinity: their rows are not finite, their neighbours as ever."""
+    b = R.Batch([190, 77], [new, new], 32, seed=new)
+    c, state = filled_cache(gpu, b, 2, dtype, seed=new)
+    g = syn.gen(new)
+    q = torch.randn(b.tokens, 16, 256, generator=g) * torch.exp2(torch.randint(-30, 4, (1, 1, 256), generator=g).float())
+    q = q.to(BF16)
+    q[new - 1, 3, 17], q[b.tokens - 1, 9, 200] = float("nan"), float("inf")
+    q2 = q.clone()
+    q2[new - 1, 3], q2[b.tokens - 1, 9] = 0, 0
+    want, tol, rows = R.attend(state, b, q2)
+    got = pa.paged_attention(q.to(gpu), c, *b.where(gpu)).view(b.tokens, 16, 256)
+    assert not torch.isfinite(got[new - 1, 3]).any() and not torch.isfinite(got[b.tokens - 1, 9]).any()
+    got[new - 1, 3] = want.view(b.tokens, 16, 256)[new - 1, 3].to(got)
+    got[b.tokens - 1, 9] = want.view(b.tokens, 16, 256)[b.tokens - 1, 9].to(got)
+    tol = tol + 2.0 ** -8 * want.abs()      # of the two rows put in above
+    check(got.flatten(1), want, tol, rows)
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -100, 2.0 ** -20, 2.0 ** 6])
+def test_queries_of_all_sizes(gpu, scale):
+    b = R.Batch([130], [50], 16, seed=1)
+    c, state = filled_cache(gpu, b, 1, FP8, seed=1)
+    q = (syn.randn((50, 8, 256), syn.gen(3)).float() * scale).to(BF16)
+    want, tol, rows = R.attend(state, b, q)
+    check(pa.paged_attention(q.to(gpu), c, *b.where(gpu)), want, tol, rows)
+
+
 def test_attention_with_pages_that_hold_nothing(gpu):
     """Page ids outside the pool hold no tokens; a row whose pages are all such,
     a sequence longer than its table and rows of negative position are zeros."""
