@@ -17,8 +17,9 @@
 //    it lies, by 32x32x64 products with the page's scale byte in the instruction,
 //    against Q as the sum of two e4m3 values (as much matrix time as bf16, no
 //    conversions); V becomes bf16 behind LDS, the scale inside the conversion.
-//    Converting K too took 922 us for 2,048 tokens over 30K, so 863; a tile's
-//    prologue is 1 us longer (93 tokens over 2K: 37.4 and 39.1).
+//    Converting K too took 922 us for 2,048 tokens over 30K, so 869, with the reads
+//    and products of e4m3 in a stated order (sched_group_barrier) 846; a tile's
+//    prologue is 1 us longer (93 tokens over 2K: 37.4 and 39.0).
 // The reference maximum is the first visible tile's and is raised (with a
 // rescale) only when a tile's probabilities sum past 2^20.
 #include "paged_split.h"
@@ -316,6 +317,14 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
       x = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kr[0], q2[2], x, 0, 0, 0, ks, 2, (int)qs2);
       x = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kr[1], q1[3], x, 0, 0, 0, ks, 3, (int)qs1);
       x = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kr[1], q2[3], x, 0, 0, 0, ks, 3, (int)qs2);
+      // two steps of K ahead: left alone, each step's reads are issued and waited for
+      // right before its products
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
     } else {
       bf16x8 kr[4];
       const auto kread = [&](int i) { return __builtin_bit_cast(bf16x8, *(const lds_u32x4*)(uintptr_t)(kp ^ (i << 5))); };
@@ -383,21 +392,35 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
     __builtin_amdgcn_s_setprio(1);
 
     if constexpr (kFp8) {
-      i32x2 va[4];
+      // six V operands on their way (chunk of 2,048: 4 take 1% more, 8 spill)
+      constexpr int kRing = 6;
+      i32x2 va[kRing];
       const auto vread = [&](int i) {   // keys 16 (i / 8) .. + 16, dims 32 (i % 8) .. + 32
         return __builtin_amdgcn_ds_read_tr8_b64_v2i32(
             (lds_i32x2*)(uintptr_t)((vp ^ ((i & 7) << 5)) + (i >> 3) * 16 * kRowB));
       };
 #pragma unroll
-      for (int i = 0; i < 4; ++i) va[i] = vread(i);
+      for (int i = 0; i < kRing; ++i) va[i] = vread(i);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float vs = paged_scale((i < 8 ? ea : eb) >> 8);
-        const i32x2 r = va[i & 3];
-        if (i + 4 < 16) va[i & 3] = vread(i + 4);
+        const i32x2 r = va[i % kRing];
         const u32x4 a = {cvt2<false>((unsigned)r[0], vs), cvt2<true>((unsigned)r[0], vs),
                          cvt2<false>((unsigned)r[1], vs), cvt2<true>((unsigned)r[1], vs)};
         o[i & 7] = mfma32x32x16(__builtin_bit_cast(bf16x8, a), pb[i >> 3], o[i & 7]);
+        if (i + kRing < 16) va[i % kRing] = vread(i + kRing);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x100, kRing, 1);
+#pragma unroll
+      for (int i = 0; i < 16 - kRing; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x002, 5, 1);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
+      }
+#pragma unroll
+      for (int i = 0; i < kRing; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x002, 5, 1);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
       }
     } else {
       i16x4 va[4][2];
