@@ -17,9 +17,9 @@
 //    it lies, by 32x32x64 products with the page's scale byte in the instruction,
 //    against Q as the sum of two e4m3 values (as much matrix time as bf16, no
 //    conversions); V becomes bf16 behind LDS, the scale inside the conversion.
-//    Converting K too took 922 us for 2,048 tokens over 30K, so 869, with the reads
-//    and products of e4m3 in a stated order (sched_group_barrier) 846; a tile's
-//    prologue is 1 us longer (93 tokens over 2K: 37.4 and 39.0).
+//    2,048 tokens over 30K: with K converted too 6% more than with the parts, and
+//    those 884 us, with the reads and products of e4m3 in a stated order 855; the
+//    parts make a tile's prologue 1 us longer (93 tokens over 2K: 37.4 and 38.7).
 // The reference maximum is the first visible tile's and is raised (with a
 // rescale) only when a tile's probabilities sum past 2^20.
 #include "paged_split.h"
@@ -392,8 +392,9 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
     __builtin_amdgcn_s_setprio(1);
 
     if constexpr (kFp8) {
-      // six V operands on their way (chunk of 2,048: 4 take 1% more, 8 spill)
-      constexpr int kRing = 6;
+      // four V operands on their way, in this order (chunk of 2,048: 855 us; left to the
+      // compiler 884, six in groups of sched_group_barrier 861)
+      constexpr int kRing = 4;
       i32x2 va[kRing];
       const auto vread = [&](int i) {   // keys 16 (i / 8) .. + 16, dims 32 (i % 8) .. + 32
         return __builtin_amdgcn_ds_read_tr8_b64_v2i32(
@@ -401,6 +402,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
       };
 #pragma unroll
       for (int i = 0; i < kRing; ++i) va[i] = vread(i);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float vs = paged_scale((i < 8 ? ea : eb) >> 8);
@@ -409,18 +411,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
                          cvt2<false>((unsigned)r[1], vs), cvt2<true>((unsigned)r[1], vs)};
         o[i & 7] = mfma32x32x16(__builtin_bit_cast(bf16x8, a), pb[i >> 3], o[i & 7]);
         if (i + kRing < 16) va[i % kRing] = vread(i + kRing);
-      }
-      __builtin_amdgcn_sched_group_barrier(0x100, kRing, 1);
-#pragma unroll
-      for (int i = 0; i < 16 - kRing; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x002, 5, 1);
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
-      }
-#pragma unroll
-      for (int i = 0; i < kRing; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x002, 5, 1);
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
+        __builtin_amdgcn_sched_barrier(0);
       }
     } else {
       i16x4 va[4][2];
