@@ -3,10 +3,12 @@
 //
 //   o = softmax(q k^T / 16) v over the positions up to the row's own.
 //
-// Work: an item is a tile of 4 kWaves tokens x the 8 query heads of a KV head
+// Work: an item is a tile of 8, 16 or 32 tokens x the 8 query heads of a KV head
 // (32 matrix columns a wave) and a chunk of keys; bound by the matrix products
 // (16,384 operations a (row's token, key) pair and KV head) and by LDS, which
-// every wave reads whole.  Stages of 32 KB (64 keys of e4m3, 32 of bf16):
+// every wave reads whole.  8 tokens over e4m3 take four waves, two for each half of
+// a stage's keys, joined at the end: 5 tokens of each of 16 sequences over 12K, two
+// KV heads, 72 us with two waves, 65 with four.  Stages of 32 KB (64 keys of e4m3, 32 of bf16):
 //  * K and V rows go from their pages straight to LDS in the pages' type (no
 //    registers), a stage ahead of their use.  The 16-byte chunks of a row are
 //    exchanged by its number on the way, which leaves the
@@ -108,16 +110,18 @@ __device__ __forceinline__ unsigned split_e4m3(const u32x4 (&v)[4], i32x8& a, i3
   return e;
 }
 
-template <bool kFp8, int kWaves>
+template <bool kFp8, int kWaves, int kParts>
 __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefill_kernel(
     const bf16* __restrict__ q, PagedCache c, PagedBatch b, PagedOut w, unsigned slots, unsigned target) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   __shared__ unsigned find[52];
+  __shared__ float ml[kParts == 2 ? 64 : 1][2];   // maxima and sums of the second half
   __shared__ int odd;   // whether a V value that some rows must not see is not finite
   constexpr int kElem = kFp8 ? 1 : 2;
-  constexpr int kTile = 4 * kWaves;
+  constexpr int kTile = 4 * kWaves / kParts;
   constexpr int kRowB = kD * kElem, kStageKeys = kHalf / kRowB;   // bytes of a row, keys of a stage
   constexpr int kSubs = kStageKeys / kKeys, kGroups = kStageKeys / 16;
+  static_assert(kParts == 1 || (kParts == 2 && kSubs == 2 && kWaves == 4));
   constexpr int kLoads = 16 / kWaves;                // 1 KB loads of K (and of V) a wave and stage
   constexpr int kBlockStages = 1024 / kStageKeys;    // stages of a 1,024-key block
 
@@ -145,11 +149,14 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lj = lane & 31, lg = lane >> 5;
-  const int tok = wave * 4 + (lj >> 3);            // of the tile
+  // wave w has rows w % kRowWaves of the tile and the part w / kRowWaves of each stage
+  constexpr int kRowWaves = kWaves / kParts;
+  const int part = wave / kRowWaves, first = wave % kRowWaves * 4;   // of its four tokens
+  const int tok = first + (lj >> 3);               // of the tile
   const bool live = tok < n_tok;
   const int lim = live ? pos0 + tok : -1;          // this column's last key
-  const int wave_first = pos0 + wave * 4;
-  const int wave_lim = wave * 4 < n_tok ? min(wave_first + 3, end - 1) : -1;
+  const int wave_first = pos0 + first;
+  const int wave_lim = first < n_tok ? min(wave_first + 3, end - 1) : -1;
 
   f32x16 o[8];
 #pragma unroll
@@ -286,7 +293,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
     }
     if (st + 1 < n_stages) load_stage(st + 1);
 #pragma unroll 1
-    for (int sub = 0; sub < kSubs; ++sub) {
+    for (int sub = part; sub < kSubs; sub += kParts) {
     const int kv0 = key_st + sub * kKeys;
     if (kv0 > wave_lim) continue;
     // (whole rows away: the exchanged bits stay as they are)
@@ -439,32 +446,66 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
     }
   }
 
+  l += __shfl_xor(l, 32, 64);
+  if constexpr (kParts == 2) {   // join the two halves of the keys
+    __syncthreads();
+    f32x4* ex = reinterpret_cast<f32x4*>(lds + wave % kRowWaves * 32768) + lane;
+    if (part == 1) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        ex[i * 64] = f32x4{o[i >> 2][4 * (i & 3)], o[i >> 2][4 * (i & 3) + 1], o[i >> 2][4 * (i & 3) + 2],
+                           o[i >> 2][4 * (i & 3) + 3]};
+      if (lg == 0) {
+        ml[wave % kRowWaves * 32 + lj][0] = l == 0.f ? -INFINITY : m;
+        ml[wave % kRowWaves * 32 + lj][1] = l;
+      }
+    }
+    __syncthreads();
+    if (part == 0) {
+      const float m1 = ml[wave * 32 + lj][0], l1 = ml[wave * 32 + lj][1];
+      const float mx = fmaxf(l == 0.f ? -INFINITY : m, m1);
+      const float a0 = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(m - mx);
+      const float a1 = l1 == 0.f ? 0.f : __builtin_amdgcn_exp2f(m1 - mx);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const f32x4 v = ex[i * 64];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float u = o[i >> 2][4 * (i & 3) + e];
+          o[i >> 2][4 * (i & 3) + e] = (l == 0.f ? 0.f : u * a0) + (l1 == 0.f ? 0.f : v[e] * a1);
+        }
+      }
+      m = mx;
+      l = l * a0 + l1 * a1;
+    }
+  }
+
   // ---- out through LDS in four rounds of 64 dims, so that stores are whole
   // 256-byte (fp32 partials) or 128-byte row segments
-  l += __shfl_xor(l, 32, 64);
   const float inv = single ? (l == 0.f ? 0.f : 1.0f / l) : 1.0f;
   const size_t part0 = (slot * c.heads + head) * (8 * kTile);
-  if (!single && lg == 0 && live) {
-    const size_t part = part0 + wave * 32 + lj;
-    w.ml[part * 2] = l == 0.f ? -INFINITY : m;   // what saw nothing weighs nothing
-    w.ml[part * 2 + 1] = l;
+  if (!single && lg == 0 && live && part == 0) {
+    const size_t at = part0 + first * 8 + lj;
+    w.ml[at * 2] = l == 0.f ? -INFINITY : m;   // what saw nothing weighs nothing
+    w.ml[at * 2 + 1] = l;
   }
   const bool zero = l == 0.f;
   // the gates of this wave's rows, all asked for at once (rows past the end read the
   // last row's)
   bf16x4 gt[4][8];
-  if (single && w.gate != nullptr) {
+  if (single && w.gate != nullptr && part == 0) {
 #pragma unroll
     for (int rd = 0; rd < 4; ++rd)
 #pragma unroll
       for (int it = 0; it < 8; ++it) {
         const int r = it * 4 + (lane >> 4);
-        const size_t row = t0 + min(wave * 4 + (r >> 3), n_tok - 1);
+        const size_t row = t0 + min(first + (r >> 3), n_tok - 1);
         gt[rd][it] = *reinterpret_cast<const bf16x4*>(w.gate + row * w.gate_stride + (head * kGroup + (r & 7)) * 2 * kD +
                                                       kD + rd * 64 + (lane & 15) * 4);
       }
   }
   __syncthreads();
+  if (part != 0) return;
   const bool strange_v = odd != 0;
   char* stg = lds + wave * 8192;
 #pragma unroll
@@ -487,11 +528,11 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
     for (int it = 0; it < 8; ++it) {
       const int r = it * 4 + (lane >> 4), ch = lane & 15;
       f32x4 v = *reinterpret_cast<const f32x4*>(stg + r * 256 + ((ch ^ (r & 15)) * 16));
-      const int rt = wave * 4 + (r >> 3), d = rd * 64 + ch * 4;
+      const int rt = first + (r >> 3), d = rd * 64 + ch * 4;
       if (rt >= n_tok) continue;
       if (strange_v) add_not_finite<kFp8>(v, c, table, head, pos0 + 1, min(pos0 + rt, kv_stop - 1), kv_first, d);
       if (!single) {
-        *reinterpret_cast<f32x4*>(w.o + (part0 + wave * 32 + r) * kD + d) = v;
+        *reinterpret_cast<f32x4*>(w.o + (part0 + first * 8 + r) * kD + d) = v;
         continue;
       }
       const size_t row = t0 + rt, qh = head * kGroup + (r & 7);
@@ -519,13 +560,13 @@ int allow_lds(const void* kernel, std::atomic<bool> (&ready)[64]) {
   return static_cast<int>(e);
 }
 
-template <bool kFp8, int kWaves>
+template <bool kFp8, int kWaves, int kParts = 1>
 int launch(const bf16* q, const PagedCache& c, const PagedBatch& b, const PagedOut& o, unsigned items,
            unsigned slots, unsigned target, void* stream) {
   static std::atomic<bool> ready[64];
-  const int e = allow_lds(reinterpret_cast<const void*>(&paged_prefill_kernel<kFp8, kWaves>), ready);
+  const int e = allow_lds(reinterpret_cast<const void*>(&paged_prefill_kernel<kFp8, kWaves, kParts>), ready);
   if (e != Q36_OK) return e;
-  hipLaunchKernelGGL((paged_prefill_kernel<kFp8, kWaves>), dim3(items * c.heads), dim3(64 * kWaves), kLds,
+  hipLaunchKernelGGL((paged_prefill_kernel<kFp8, kWaves, kParts>), dim3(items * c.heads), dim3(64 * kWaves), kLds,
                      static_cast<hipStream_t>(stream), q, c, b, o, slots, target);
   return static_cast<int>(hipGetLastError());
 }
@@ -537,7 +578,7 @@ int paged_prefill(const void* q, const PagedCache& c, bool fp8, const PagedBatch
   const bf16* p = static_cast<const bf16*>(q);
   switch (tile) {
     case 8:
-      return fp8 ? launch<true, 2>(p, c, b, o, items, slots, target, stream)
+      return fp8 ? launch<true, 4, 2>(p, c, b, o, items, slots, target, stream)
                  : launch<false, 2>(p, c, b, o, items, slots, target, stream);
     case 16:
       return fp8 ? launch<true, 4>(p, c, b, o, items, slots, target, stream)

@@ -285,6 +285,22 @@ def test_queries_of_all_sizes(gpu, scale):
     check(pa.paged_attention(q.to(gpu), c, *b.where(gpu)), want, tol, rows)
 
 
+@pytest.mark.parametrize("scale", [1.5, 2.0 ** 6])
+@pytest.mark.parametrize("dtype", [FP8, BF16])
+@pytest.mark.parametrize("lens,new", [([3, 8, 32, 33], [3, 8, 8, 3]), ([64, 65, 96, 97, 128, 129], [4, 5, 8, 8, 1, 8]),
+                                      ([1100, 2081, 40], [5, 8, 7]), ([5000], [8]), ([31, 0, 0, 2050], [6, 0, 0, 6])])
+def test_drafts_over_parts_of_a_stage(gpu, lens, new, dtype, scale):
+    """Three to eight rows a sequence, whose keys end in either half of 64, or leave the
+    second half empty; large queries put the two halves' maxima far apart."""
+    b = R.Batch(lens, new, 16, seed=sum(lens), rows_behind=1)
+    c, state = filled_cache(gpu, b, 2, dtype, seed=sum(new))
+    g = syn.gen(len(lens))
+    q = (syn.randn((b.tokens, 16, 256), g).float() * scale).to(BF16)
+    gate = torch.randn(b.tokens, 16 * 512, generator=g).to(BF16)
+    want, tol, rows = R.attend(state, b, q, gate)
+    check(pa.paged_attention(q.to(gpu), c, *b.where(gpu), q_gate=gate.to(gpu)), want, tol, rows)
+
+
 def test_attention_with_pages_that_hold_nothing(gpu):
     """Page ids outside the pool hold no tokens; a row whose pages are all such,
     a sequence longer than its table and rows of negative position are zeros."""
