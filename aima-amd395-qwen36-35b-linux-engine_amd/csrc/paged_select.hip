@@ -30,98 +30,115 @@ __device__ __forceinline__ unsigned score_key(int s, unsigned e) {
   return s < 0 ? 0x7fffffffu - mag : 0x80000000u + mag;
 }
 
-// A wave scores 16 pages at a time for one row: pages in the matrix rows, the 8
-// heads in the columns (doubled).
+// A wave scores 16 pages at a time: pages in the matrix rows, in the columns the 8
+// heads of one row (twice) or, with kPair, of rows 2 i and 2 i + 1 where one sequence
+// has both; else it takes the two in turn.
+template <bool kPair>
 __global__ __launch_bounds__(256) void paged_score_kernel(const bf16* __restrict__ q, PagedCache c,
                                                           PagedBatch b, unsigned* __restrict__ keys,
                                                           unsigned blocks, unsigned per_wave) {
   const unsigned head = blockIdx.x % c.heads, block = blockIdx.x / c.heads % blocks;
-  const unsigned t = blockIdx.x / c.heads / blocks;
+  const unsigned item = blockIdx.x / c.heads / blocks;
   const int lane = threadIdx.x & 63, col = lane & 7, row = lane & 15, g = lane >> 4;
   const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  unsigned seq;
-  PagedSeq s;
-  if (!paged_find_row(b, (int)t, seq, s)) return;
-  const int pos = s.pos((int)t);
-  if (pos < 0) return;
-  const unsigned n = ((unsigned)pos >> c.shift) + 1;
   const unsigned p0 = (block * 4 + wave) * per_wave * 16;
-  if (p0 >= n) return;
+  const auto score = [&](unsigned t) {   // returns how many rows it took
+    unsigned seq;
+    PagedSeq s;
+    if (!paged_find_row(b, (int)t, seq, s)) return 1u;
+    const bool both = kPair && t % 2 == 0 && (int)t + 1 < s.z;
+    const unsigned took = both ? 2 : 1;
+    const int pos = s.pos((int)t) + (both ? 1 : 0);   // the last row's
+    if (pos < 0) return took;
+    const unsigned n = ((unsigned)pos >> c.shift) + 1;
+    if (p0 >= n) return took;
+    // this lane's column: its row of the call, the pages that it sees
+    const unsigned second = both ? lane >> 3 & 1 : 0;
+    const int my_pos = pos - (both ? 1 : 0) + (int)second;
+    const unsigned my_t = t + second, my_n = my_pos < 0 ? 0 : ((unsigned)my_pos >> c.shift) + 1;
 
-  const int* table = b.table + seq * b.table_stride;
-  unsigned* kp = keys + ((size_t)t * c.heads + head) * b.width;
-  i32x4 a[8];
-  unsigned e;
-  bool there;
-  const auto load = [&](unsigned first) {   // 16 pages' bounds and scales; pages of none read page 0
-    const unsigned mine = first + row;
-    unsigned pid = mine < n ? (unsigned)table[mine] : ~0u;
-    there = pid < c.pages;
-    if (!there) pid = 0;
-    const int8_t* bp = c.bounds + ((size_t)pid * c.heads + head) * 2 * kD + 16 * g;
+    const int* table = b.table + seq * b.table_stride;
+    unsigned* kp = keys + ((size_t)my_t * c.heads + head) * b.width;
+    i32x4 a[8];
+    unsigned e;
+    bool there;
+    const auto load = [&](unsigned first) {   // 16 pages' bounds and scales; pages of none read page 0
+      const unsigned mine = first + row;
+      unsigned pid = mine < n ? (unsigned)table[mine] : ~0u;
+      there = pid < c.pages;
+      if (!there) pid = 0;
+      const int8_t* bp = c.bounds + ((size_t)pid * c.heads + head) * 2 * kD + 16 * g;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) a[j] = *reinterpret_cast<const i32x4*>(bp + 64 * j);
-    e = c.k_exp[(size_t)pid * c.heads + head];
-  };
-  load(p0);   // on the way while the queries are quantised
+      for (int j = 0; j < 8; ++j) a[j] = *reinterpret_cast<const i32x4*>(bp + 64 * j);
+      e = c.k_exp[(size_t)pid * c.heads + head];
+    };
+    load(p0);   // on the way while the queries are quantised
 
-  // this lane's 64 dims of its head: 64 j + 16 g + [0, 16)
-  const bf16* qp = q + ((size_t)t * c.heads * kGroup + head * kGroup + col) * kD + 16 * g;
-  bf16x8 x[8];
+    // this lane's 64 dims of its head: 64 j + 16 g + [0, 16)
+    const bf16* qp = q + ((size_t)my_t * c.heads * kGroup + head * kGroup + col) * kD + 16 * g;
+    bf16x8 x[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) x[j] = *reinterpret_cast<const bf16x8*>(qp + 64 * (j >> 1) + 8 * (j & 1));
-  unsigned amax = 0;   // bits of the largest finite magnitude
+    for (int j = 0; j < 8; ++j) x[j] = *reinterpret_cast<const bf16x8*>(qp + 64 * (j >> 1) + 8 * (j & 1));
+    unsigned amax = 0;   // bits of the largest finite magnitude
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
+    for (int j = 0; j < 8; ++j)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const unsigned u = __float_as_uint(bf2f(x[j][e])) & 0x7fffffffu;
-      if (u < 0x7f800000u) amax = max(amax, u);
-    }
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) amax = max(amax, (unsigned)__shfl_xor(amax, o, 64));
-  // in steps that put the largest in [64, 128) (and are 2^-127 at least)
-  const float f = ldexpf(1.f, min(127 + 6 - (int)(amax >> 23), 127));
-  i32x4 qpos[4], qneg[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      unsigned i[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float v = bf2f(x[2 * j + (w >> 1)][4 * (w & 1) + e]);
-        i[e] = (unsigned)(int)(v == v ? __builtin_amdgcn_fmed3f(rintf(v * f), -127.f, 127.f) : 0.f);
+      for (int e = 0; e < 8; ++e) {
+        const unsigned u = __float_as_uint(bf2f(x[j][e])) & 0x7fffffffu;
+        if (u < 0x7f800000u) amax = max(amax, u);
       }
-      const unsigned lo = __builtin_amdgcn_perm(i[1], i[0], 0x0c0c0400), hi = __builtin_amdgcn_perm(i[3], i[2], 0x04000c0c);
-      const unsigned all = lo | hi, sign = ((all >> 7) & 0x01010101u) * 0xffu;
-      qpos[j][w] = (int)(all & ~sign);
-      qneg[j][w] = (int)(all & sign);
-    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1)   // (the columns of 8 .. 15 are another row's, or the same)
+      if (o != 8) amax = max(amax, (unsigned)__shfl_xor(amax, o, 64));
+    // in steps that put the largest in [64, 128) (and are 2^-127 at least)
+    const float f = ldexpf(1.f, min(127 + 6 - (int)(amax >> 23), 127));
+    i32x4 qpos[4], qneg[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        unsigned i[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float v = bf2f(x[2 * j + (w >> 1)][4 * (w & 1) + e]);
+          i[e] = (unsigned)(int)(v == v ? __builtin_amdgcn_fmed3f(rintf(v * f), -127.f, 127.f) : 0.f);
+        }
+        const unsigned lo = __builtin_amdgcn_perm(i[1], i[0], 0x0c0c0400), hi = __builtin_amdgcn_perm(i[3], i[2], 0x04000c0c);
+        const unsigned all = lo | hi, sign = ((all >> 7) & 0x01010101u) * 0xffu;
+        qpos[j][w] = (int)(all & ~sign);
+        qneg[j][w] = (int)(all & sign);
+      }
 
-  for (unsigned i = 0; i < per_wave; ++i) {
-    const unsigned first = p0 + 16 * i;
-    if (first >= n) break;
-    i32x4 d = {0, 0, 0, 0};
+    for (unsigned i = 0; i < per_wave; ++i) {
+      const unsigned first = p0 + 16 * i;
+      if (first >= n) break;
+      i32x4 d = {0, 0, 0, 0};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      d = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[j], qpos[j], d, 0, 0, 0);
-      d = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[4 + j], qneg[j], d, 0, 0, 0);
+      for (int j = 0; j < 4; ++j) {
+        d = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[j], qpos[j], d, 0, 0, 0);
+        d = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[4 + j], qneg[j], d, 0, 0, 0);
+      }
+      const unsigned e_now = e;
+      const bool there_now = there;
+      if (i + 1 < per_wave && first + 16 < n) load(first + 16);
+      // lane: pages 4 g + r of its head; the largest over the heads
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        int v = d[r];
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) v = max(v, __shfl_xor(v, o, 64));
+        const int from = 4 * g + r;
+        const unsigned pe = __shfl(e_now, from, 64);
+        const bool ok = __shfl((int)there_now, from, 64);
+        if (col == r && (both || row == r) && first + from < my_n) kp[first + from] = ok ? score_key(v, pe) : 1u;
+      }
     }
-    const unsigned e_now = e;
-    const bool there_now = there;
-    if (i + 1 < per_wave && first + 16 < n) load(first + 16);
-    // lane: pages 4 g + r of its head; the largest over the heads
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      int v = d[r];
-#pragma unroll
-      for (int o = 1; o < 8; o <<= 1) v = max(v, __shfl_xor(v, o, 64));
-      const int from = 4 * g + r;
-      const unsigned pe = __shfl(e_now, from, 64);
-      const bool ok = __shfl((int)there_now, from, 64);
-      if (row == r && first + from < n) kp[first + from] = ok ? score_key(v, pe) : 1u;
-    }
+    return took;
+  };
+  if constexpr (kPair) {
+    if (score(2 * item) == 1 && 2 * item + 1 < b.tokens) score(2 * item + 1);
+  } else {
+    score(item);
   }
 }
 
@@ -248,12 +265,18 @@ Q36_EXPORT int qwen36_paged_select(const void* q, const qwen36_paged_cache* cach
   hipStream_t st = static_cast<hipStream_t>(stream);
   unsigned* keys = static_cast<unsigned*>(workspace);
   if (b.width > budget) {   // else every row takes all its pages
-    const size_t rows = (size_t)b.tokens * c.heads, groups = (b.width + 63) / 64;
+    // two rows at a time where sequences have two rows or more on average (300 rows of
+    // one sequence over 512 pages: 13.9 us, one at a time 18.4)
+    const bool pair = b.tokens >= 2 * b.seqs;
+    const size_t rows = (size_t)(pair ? (b.tokens + 1) / 2 : b.tokens) * c.heads, groups = (b.width + 63) / 64;
     size_t per = rows * groups / 1024;   // 16-page groups a wave takes: the queries are quantised once
     per = per < 1 ? 1 : per > groups ? groups : per;
     const unsigned blocks = (unsigned)((groups + per - 1) / per);
-    hipLaunchKernelGGL(paged_score_kernel, dim3((unsigned)(rows * blocks)), dim3(256), 0, st,
-                       static_cast<const bf16*>(q), c, b, keys, blocks, (unsigned)per);
+    const auto score = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(rows * blocks)), dim3(256), 0, st, static_cast<const bf16*>(q), c,
+                         b, keys, blocks, (unsigned)per);
+    };
+    pair ? score(paged_score_kernel<true>) : score(paged_score_kernel<false>);
     const int e = static_cast<int>(hipGetLastError());
     if (e != Q36_OK) return e;
   }

@@ -391,6 +391,22 @@ def test_selection_ties_and_odd_queries(gpu):
         assert got[row, h].tolist() == mine, (row, h)
 
 
+@pytest.mark.parametrize("lens,new,page", [
+    ([330, 290, 50, 401], [3, 5, 0, 7], 16), ([257, 258, 259], [2, 2, 3], 16), ([1, 600, 0, 1, 700], [1, 1, 0, 1, 33], 32),
+    ([2100], [131], 64), ([3, 640], [9, 6], 16)])
+def test_selection_for_rows_by_twos(gpu, lens, new, page):
+    """Sequences of odd numbers of rows, rows on both sides of a page's end, rows of
+    negative position, and neighbours whose queries are of quite different sizes."""
+    b = R.Batch(lens, new, page, seed=len(lens))
+    c, state = filled_cache(gpu, b, 2, FP8, True, seed=sum(new))
+    g = syn.gen(sum(lens))
+    q = torch.randn(b.tokens, 16, 256, generator=g) * torch.exp2(torch.randint(-9, 9, (b.tokens, 1, 1), generator=g).float())
+    q = q.to(BF16)
+    got = pa.select_pages(q.to(gpu), c, *b.where(gpu), 6, 1, 2).cpu()
+    for (row, h), mine in R.select(state, b, q, 6, 1, 2).items():
+        assert got[row, h].tolist() == mine + [-1] * (6 - len(mine)), (row, h)
+
+
 def test_selection_over_many_pages(gpu):
     """More pages than one register block: 5,000 pages of 16 tokens."""
     n = 80000
