@@ -266,7 +266,7 @@ Q36_EXPORT int qwen36_paged_select(const void* q, const qwen36_paged_cache* cach
   unsigned* keys = static_cast<unsigned*>(workspace);
   if (b.width > budget) {   // else every row takes all its pages
     // two rows at a time where sequences have two rows or more on average (300 rows of
-    // one sequence over 512 pages: 13.9 us, one at a time 18.4)
+    // one sequence over 512 pages: 14.2 us, one at a time 18.4)
     const bool pair = b.tokens >= 2 * b.seqs;
     const size_t rows = (size_t)(pair ? (b.tokens + 1) / 2 : b.tokens) * c.heads, groups = (b.width + 63) / 64;
     size_t per = rows * groups / 1024;   // 16-page groups a wave takes: the queries are quantised once
