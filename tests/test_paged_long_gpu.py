@@ -209,3 +209,44 @@ def test_selection_over_thousands_of_pages(gpu, width, seqs, new, heads):
             for h in range(heads):
                 want = picked(state, b, q[row, 8 * h:8 * h + 8], i, h, pos, budget, sinks, recents)
                 assert got[row, h].tolist() == want, (row, h, budget)
+
+
+# ------------------------------------------------------------------- memory
+
+@pytest.mark.parametrize("dtype", [FP8, BF16])
+@pytest.mark.parametrize("lens,new", [([1500, 70, 3], [1, 1, 1]), ([900, 300], [2, 2]), ([2000, 70, 4], [5, 8, 6]),
+                                      ([1000, 41, 9], [16, 12, 12]), ([1600, 70, 20], [90, 40, 33]), ([7000], [1])])
+def test_results_do_not_depend_on_what_workspaces_and_outputs_held(gpu, dtype, lens, new):
+    """Workspaces and outputs of the test's own, filled with bytes of one pattern right
+    before each call: the same results whatever they held, and rows behind the last
+    sequence as they were.  Every size of tile, split rows, lists in several chunks."""
+    b = R.Batch(lens, new, 16, seed=sum(new), rows_behind=2)
+    c, _ = filled_cache(gpu, b, 2, dtype, True, seed=sum(lens))
+    q, gate = (x.to(gpu) for x in queries(b, 2, 9))
+    where, lib, t = b.where(gpu), _lib.load(), b.tokens
+    batch, stream = pa._batch(c, t, *where), torch.cuda.current_stream().cuda_stream
+    listed, live = 12, t - 2
+    sizes = (lib.qwen36_paged_attention_workspace_bytes(c._args, batch), lib.qwen36_paged_select_workspace_bytes(c._args, batch),
+             lib.qwen36_paged_sparse_attention_workspace_bytes(c._args, batch, listed))
+    want = None
+    for fill in (0x00, 0xFF, 0x7F, 0x5A):
+        def own(n, fill=fill):
+            return torch.full((n,), fill, dtype=torch.uint8, device=gpu)
+        ws, out, pages, sparse = [own(n) for n in sizes], own(t * 8192), own(t * 2 * listed * 4), own(t * 8192)
+        assert lib.qwen36_paged_attention(q.data_ptr(), c._args, batch, gate.data_ptr(), gate.stride(0), out.data_ptr(),
+                                          ws[0].data_ptr(), sizes[0], stream) == 0
+        assert lib.qwen36_paged_select(q.data_ptr(), c._args, batch, listed, 1, 1, pages.data_ptr(), ws[1].data_ptr(),
+                                       sizes[1], stream) == 0
+        assert lib.qwen36_paged_sparse_attention(q.data_ptr(), c._args, batch, pages.data_ptr(), listed, gate.data_ptr(),
+                                                 gate.stride(0), sparse.data_ptr(), ws[2].data_ptr(), sizes[2], stream) == 0
+        got = [x.view(t, -1) for x in (out, pages, sparse)]
+        for x in got:
+            assert (x[live:] == fill).all()
+        got = [x[:live] for x in got]
+        if want is None:
+            want = got
+        for x, y in zip(got, want):
+            assert torch.equal(x, y), fill
+    ref = pa.select_pages(q, c, *where, listed)[:live]
+    assert torch.equal(want[1].reshape(-1).view(torch.int32), ref.reshape(-1))
+    assert torch.equal(want[0].reshape(-1).view(BF16), pa.paged_attention(q, c, *where, q_gate=gate)[:live].reshape(-1))
