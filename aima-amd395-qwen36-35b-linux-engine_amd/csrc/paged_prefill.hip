@@ -502,6 +502,9 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
     w.ml[at * 2 + 1] = l;
   }
   const bool zero = l == 0.f;
+  // bit j: column j saw nothing and is zeros whatever its gate (an attention of exactly
+  // zero is not: its product with a NaN gate is a NaN)
+  const unsigned none = (unsigned)__ballot(zero);
   // the gates of this wave's rows, all asked for at once (rows past the end read the
   // last row's)
   bf16x4 gt[4][8];
@@ -550,8 +553,9 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 4 ? 2 : 1) void paged_prefil
       const size_t row = t0 + rt, qh = head * kGroup + (r & 7);
       bf16x4 res;
       if (w.gate != nullptr) {
+        const bool nothing = (none >> r) & 1u;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) res[e] = f2bf(v[e] == 0.f ? 0.f : paged_gate(v[e], gt[rd][it][e]));
+        for (int e = 0; e < 4; ++e) res[e] = f2bf(nothing ? 0.f : paged_gate(v[e], gt[rd][it][e]));
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e) res[e] = f2bf(v[e]);
