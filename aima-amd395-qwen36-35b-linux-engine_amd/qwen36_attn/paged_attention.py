@@ -198,7 +198,10 @@ def paged_append(q_gate: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm:
     sin) [positions, 32], e.g. ``full_attention.rotary_table(capacity, 0,
     device)``.  An e4m3 page's scale fits its largest value and grows with it;
     a page that gets rows must belong to one sequence.  Returns q [T, heads,
-    256] bf16."""
+    256] bf16.  A sequence longer than ``rope`` or than the page table has no tokens:
+    neither its pages nor its q are written (as rows of negative position and rows
+    behind the last sequence).  The calls that attend do not know ``rope``; give them
+    such a sequence with a length of 0."""
     dev, index = cache.device, cache._index
     t = q_gate.shape[0] if isinstance(q_gate, torch.Tensor) and q_gate.dim() == 2 else 0
     batch = _batch(cache, t, page_table, cu_tokens, seq_lens)
@@ -308,7 +311,9 @@ class PagedFullAttentionLayer:
     """One gated GQA layer over a paged cache, ``full_attention.FullAttentionLayer``
     for a ragged batch: the projections, the append, the attention (over selected
     pages if ``budget`` is given) with the output gate, and o_proj.  ``weights`` as
-    there; ``rope``: fp32 (cos, sin) tables that reach the longest sequence."""
+    there, for all of the model's heads; ``rope``: fp32 (cos, sin) tables that reach the
+    longest sequence.  A sequence longer than they or the page table has no tokens: its
+    rows are zeros and its pages stay as they are."""
 
     def __init__(self, weights: dict, cache: PagedKVCache,
                  rope: tuple[torch.Tensor, torch.Tensor], budget: int | None = None,
@@ -331,6 +336,10 @@ class PagedFullAttentionLayer:
         q_gate, k, v = self._qkv(inp) if one else self._qkv.split_rows(linear(inp, self._qkv.w))
         where = (page_table, cu_tokens, seq_lens)
         q = paged_append(q_gate, k, v, w["q_norm"], w["k_norm"], self.rope, self.cache, *where)
+        positions = self.rope[0].shape[0]
+        if min(page_table.shape[1] * self.cache.page_tokens, MAX_TOKENS) > positions:
+            # a longer sequence has no tokens for the append, so neither for the attention
+            where = (page_table, cu_tokens, seq_lens.masked_fill(seq_lens > positions, 0))
         if self.budget is None:
             attn = paged_attention(q, self.cache, *where, q_gate=q_gate)
         else:

@@ -1,12 +1,15 @@
 """The paged-cache operators where a row's answer hangs on something rare: gates
-that are NaN over an attention of exactly zero."""
+that are NaN over an attention of exactly zero, sequences that outgrow the
+rotation tables of a layer."""
 import pytest
 import torch
 
+from qwen36_attn import full_attention as fa
 from qwen36_attn import paged_attention as pa
 from qwen36_attn import synthetic as syn
 from tests import paged_reference as R
 from tests.test_paged_gpu import filled_cache, upload
+from tests.test_paged_use_gpu import layer_weights
 
 pytestmark = pytest.mark.gpu
 FP8, BF16 = torch.float8_e4m3fn, torch.bfloat16
@@ -32,3 +35,23 @@ def test_nan_gate_over_an_attention_of_zero(gpu, dtype, new):
         want = bad[row] if pos >= 0 else torch.zeros_like(bad[row])
         assert torch.equal(torch.isnan(got[row]), want), (row, pos)
         assert (got[row][~want] == 0).all(), (row, pos)
+
+
+@pytest.mark.parametrize("budget", [None, 2])
+def test_layer_over_a_sequence_longer_than_its_rotation_tables(gpu, budget):
+    """Tables of 70 positions under a page table of 96: nothing of the sequence of 71
+    tokens is appended, so nothing of it is attended; the others are as ever."""
+    page, w = 32, layer_weights(gpu, 5)
+    b = R.Batch([70, 71, 40], [3, 2, 1], page, seed=5)
+    outs, caches = [], []
+    for lens in ([70, 71, 40], [70, 0, 40]):
+        b.lens = lens
+        cache, _ = filled_cache(gpu, R.Batch([70, 71, 40], [3, 2, 1], page, seed=5), 2, FP8, True, seed=6)
+        layer = pa.PagedFullAttentionLayer(w, cache, fa.rotary_table(70, 0, gpu), budget)
+        inp = syn.randn((6, 2048), syn.gen(7)).to(gpu)
+        outs.append(layer.forward(inp, *b.where(gpu)))
+        caches.append(R.CacheState(cache))
+    assert (outs[0][3:5] == 0).all()
+    assert torch.equal(outs[0], outs[1]) and (outs[0][:3] != 0).any() and (outs[0][5] != 0).any()
+    for name in ("k", "v", "ke", "ve", "bounds"):
+        assert torch.equal(getattr(caches[0], name), getattr(caches[1], name)), name
