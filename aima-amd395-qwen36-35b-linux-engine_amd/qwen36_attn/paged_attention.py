@@ -28,6 +28,8 @@ _stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch.cuda.current_device
 _WEIGHT = (HEAD_DIM,)
 _TYPES = {torch.bfloat16: 0, torch.float8_e4m3fn: 1}
+_FIXED = frozenset(("k_pages", "v_pages", "k_exp", "v_exp", "bounds", "num_pages", "kv_heads",
+                    "page_tokens", "heads", "device", "_index", "_max_width", "_args"))
 
 
 class PagedKVCache:
@@ -36,7 +38,8 @@ class PagedKVCache:
     [num_pages, kv_heads] uint8, the scale of a page and head being
     2^(byte - 127); ``bounds`` [num_pages, kv_heads, 2, 256] int8 where pages are
     to be selected: each channel's largest and smallest key in steps of
-    4 * 2^(k_exp - 127).  ``kv_heads`` is 2, or a tensor-parallel share."""
+    4 * 2^(k_exp - 127).  ``kv_heads`` is 2, or a tensor-parallel share.  The
+    attributes are fixed; the tensors' contents are the caller's to change."""
 
     def __init__(self, num_pages: int, page_tokens: int, device, dtype=torch.float8_e4m3fn,
                  kv_heads: int = HKV, bounds: bool = False) -> None:
@@ -90,17 +93,27 @@ class PagedKVCache:
         for t in (v_pages, k_exp, v_exp, bounds):
             if t is not None and t.device != k_pages.device:
                 raise ValueError("the cache's tensors must be on one device")
-        self.k_pages, self.v_pages = k_pages, v_pages
-        self.k_exp, self.v_exp, self.bounds = k_exp, v_exp, bounds
-        self.num_pages, self.kv_heads, self.page_tokens = n, heads, page
-        self.heads = heads * GROUP
-        self.device = k_pages.device
         stride = [t.stride(0) if n > 1 else heads * page * HEAD_DIM for t in (k_pages, v_pages)]
-        self._index = k_pages.get_device()
-        self._max_width = (MAX_TOKENS + 127) // page
-        self._args = _lib.PagedCacheArgs(ptr(k_pages), ptr(v_pages), ptr(k_exp),
-                                         ptr(v_exp) if fp8 else None, ptr(bounds), stride[0],
-                                         stride[1], n, page, heads, _TYPES[k_pages.dtype])
+        self.__dict__.update(
+            k_pages=k_pages, v_pages=v_pages, k_exp=k_exp, v_exp=v_exp, bounds=bounds,
+            num_pages=n, kv_heads=heads, page_tokens=page, heads=heads * GROUP,
+            device=k_pages.device, _index=k_pages.get_device(), _max_width=(MAX_TOKENS + 127) // page,
+            _args=_lib.PagedCacheArgs(ptr(k_pages), ptr(v_pages), ptr(k_exp),
+                                      ptr(v_exp) if fp8 else None, ptr(bounds), stride[0],
+                                      stride[1], n, page, heads, _TYPES[k_pages.dtype]))
+
+    # The calls use the addresses and sizes of ``_args``: another tensor in an
+    # attribute's place would go unseen, and the old one's memory would be reused.
+    def __setattr__(self, name: str, value) -> None:
+        if name in _FIXED:
+            raise AttributeError(f"{name}: a cache's tensors and sizes are fixed (PagedKVCache.of makes one "
+                                 "over other tensors)")
+        object.__setattr__(self, name, value)
+
+    def __delattr__(self, name: str) -> None:
+        if name in _FIXED:
+            raise AttributeError(f"{name}: a cache's tensors and sizes are fixed")
+        object.__delattr__(self, name)
 
     def values(self) -> tuple[torch.Tensor, torch.Tensor]:
         """K and V pages as the bf16 values that they hold (e4m3 values times a
