@@ -148,10 +148,11 @@ template <int kPer, int kWaves>
 __global__ __launch_bounds__(64 * kWaves) void paged_pick_kernel(PagedCache c, PagedBatch b,
                                                          const unsigned* __restrict__ keys,
                                                          unsigned budget, unsigned sinks,
-                                                         unsigned recents, int* __restrict__ pages) {
+                                                         unsigned recents, int* __restrict__ pages,
+                                                         unsigned first) {
   __shared__ unsigned cnt[2][kWaves];
   __shared__ unsigned scan[kWaves];
-  const unsigned head = blockIdx.x % c.heads, t = blockIdx.x / c.heads, tid = threadIdx.x;
+  const unsigned item = first + blockIdx.x, head = item % c.heads, t = item / c.heads, tid = threadIdx.x;
   const unsigned wave = tid >> 6;
   const unsigned* kp = keys + ((size_t)t * c.heads + head) * b.width;
   unsigned k[kPer];   // asked for before the row's length is known: what lies behind it is dropped below
@@ -280,10 +281,12 @@ Q36_EXPORT int qwen36_paged_select(const void* q, const qwen36_paged_cache* cach
     const int e = static_cast<int>(hipGetLastError());
     if (e != Q36_OK) return e;
   }
-  const dim3 grid(b.tokens * c.heads);
+  const unsigned items = b.tokens * c.heads;
   const auto pick = [&](auto kernel, unsigned threads) {
-    hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, st, c, b, keys, budget, sink_pages, recent_pages,
-                       static_cast<int*>(pages));
+    const unsigned most = 0x80000000u / threads;   // a launch has less than 2^32 threads
+    for (unsigned at = 0; at < items; at += most)
+      hipLaunchKernelGGL(kernel, dim3(items - at < most ? items - at : most), dim3(threads), 0, st, c, b, keys,
+                         budget, sink_pages, recent_pages, static_cast<int*>(pages), at);
   };
   if (b.width <= 2048)
     pick(paged_pick_kernel<8, 4>, 256);

@@ -1,6 +1,6 @@
 """The paged-cache operators where a row's answer hangs on something rare: gates
 that are NaN over an attention of exactly zero, sequences that outgrow the
-rotation tables of a layer."""
+rotation tables of a layer, more rows than one launch holds."""
 import pytest
 import torch
 
@@ -55,3 +55,31 @@ def test_layer_over_a_sequence_longer_than_its_rotation_tables(gpu, budget):
     assert torch.equal(outs[0], outs[1]) and (outs[0][:3] != 0).any() and (outs[0][5] != 0).any()
     for name in ("k", "v", "ke", "ve", "bounds"):
         assert torch.equal(getattr(caches[0], name), getattr(caches[1], name)), name
+
+
+def test_selection_of_more_rows_than_one_launch_holds(gpu):
+    """262,144 rows of 16 KV heads over a table of 4,353 pages: 2^32 threads.  The
+    last 80 rows see something."""
+    heads, page, width, rows, budget = 16, 16, 4353, 262144, 2
+    need = rows * heads * (8 * 256 * 2 + width * 4 + budget * 4)
+    if torch.cuda.mem_get_info()[0] < need + (4 << 30):
+        pytest.skip("needs 90 GB of free GPU memory")
+    g = syn.gen(1)
+    c = pa.PagedKVCache(5, page, gpu, FP8, heads, True)
+    c.bounds.copy_(torch.randint(-100, 101, c.bounds.shape, generator=g, dtype=torch.int8).sort(2, descending=True)[0])
+    c.k_exp.copy_(torch.randint(118, 121, c.k_exp.shape, generator=g, dtype=torch.uint8))
+    state = R.CacheState(c)
+    b = R.Batch([80], [80], page, spare=0)
+    q = torch.empty(rows, heads * 8, 256, dtype=BF16, device=gpu)
+    mine = syn.randn((80, heads * 8, 256), g)
+    q[-80:] = mine.to(gpu)
+    table = torch.zeros(1, width, dtype=torch.int32, device=gpu)
+    table[:, :5] = b.table.to(gpu)
+    got = pa.select_pages(q, c, table, torch.tensor([0, rows], dtype=torch.int32, device=gpu),
+                          torch.tensor([80], dtype=torch.int32, device=gpu), budget)
+    assert bool((got[:-80] == -1).all())
+    got = got[-80:].cpu()
+    for (row, h), want in R.select(state, b, mine, budget, 1, 1).items():
+        assert got[row, h].tolist() == want + [-1] * (budget - len(want)), (row, h)
+    del q, got, table
+    torch.cuda.empty_cache()
