@@ -127,10 +127,13 @@ __device__ __forceinline__ bool paged_split(const PagedBatch& b, unsigned item, 
   }, r.seq, r.local, head != nullptr ? head + 1 : nullptr);
 }
 
-// Items of a KV head at most, for the grid and the workspace.
+// Items of a KV head at most, for the grid and the workspace: the tiles and `target`
+// more, and no more chunks of a tile than the page table has blocks of keys (17 rows
+// over a page of 128: 0.5 MB of partials, not 136).
 inline unsigned paged_items(const PagedBatch& b, unsigned tile, unsigned target) {
-  const unsigned t = b.tokens / tile + b.seqs;
-  return (t < b.tokens ? t : b.tokens) + target;
+  const unsigned t = b.tokens / tile + b.seqs, tiles = t < b.tokens ? t : b.tokens;
+  const size_t whole = (size_t)tiles * ((b.max_len + kSplitBlock - 1) / kSplitBlock);
+  return whole < tiles + target ? (unsigned)whole : tiles + target;
 }
 
 // o * sigmoid(g) within a few fp32 ulps (rounded to bf16 by the caller): e^-g from
