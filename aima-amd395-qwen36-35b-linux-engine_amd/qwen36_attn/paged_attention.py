@@ -161,7 +161,7 @@ def _rows(t, name: str, rows: int, width: int, index: int) -> tuple[int, int]:
     if rows == 1:
         stride = width
     at = t.data_ptr()
-    if inner != 1 or stride < width or (at | 2 * stride) & 7:
+    if inner != 1 or not width <= stride < 1 << 32 or (at | 2 * stride) & 7:
         raise ValueError(f"{name} must have unit inner stride and 8-byte aligned rows that do not overlap")
     return at, stride
 

@@ -3,6 +3,7 @@ change, and how the workspaces grow."""
 import ctypes
 
 import pytest
+import torch
 
 from tests.test_paged_abi import batch, cache, lib  # noqa: F401
 
@@ -45,3 +46,17 @@ def test_attention_workspace_of_short_tables(lib):  # noqa: F811
     # and no more than before for long tables: tiles and twice the workgroups that the GPU holds
     long = bytes_of(seqs=1, tokens=2048, table_width=2048, table_stride=2048)
     assert long <= (64 + 1 + 256) * 32 * partial + 4096
+
+
+@pytest.mark.parametrize("stride,ok", [(4096, True), ((1 << 32) - 4, True), (4095, False), (1 << 32, False),
+                                       ((1 << 32) + 4096, False)])
+def test_row_strides_of_the_c_interface(stride, ok):
+    """The C calls take row strides of 32 bits: a longer one would lose its upper bits
+    on the way and other rows be read.  (Tensors without memory.)"""
+    from qwen36_attn import paged_attention as pa
+    t = torch.empty_strided((2, 4096), (stride, 1), dtype=torch.bfloat16, device="meta")
+    if ok:
+        assert pa._rows(t, "q_gate", 2, 4096, t.get_device())[1] == stride
+    else:
+        with pytest.raises(ValueError):
+            pa._rows(t, "q_gate", 2, 4096, t.get_device())
