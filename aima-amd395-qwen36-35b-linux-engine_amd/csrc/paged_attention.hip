@@ -20,7 +20,7 @@
 // e4m3 goes to bf16 with the page's power-of-two scale inside the conversion,
 // exactly.  A step's V and the next step's K are asked for while its scores are
 // formed (the compiler's order; V one step ahead as well, held there by fences,
-// took 39.9 us against 38.1 for 128K and 118.7 against 116.2 for 32 sequences).
+// was 5% slower over 128K and 2% over 32 sequences).
 // Scores, maximum, sum and accumulators are fp32; P is rounded to bf16 for the
 // matrix product (its sum too is taken from the fp32 values).
 #include "paged_split.h"
@@ -33,8 +33,9 @@ constexpr int kNoKeys = 0x40000000;
 constexpr float kScoreScale = 0.0625f * kLog2e;
 
 
-// A cache streams through once (nontemporal: 127 us against 128 for 32 sequences),
-// listed pages are shared by rows (plain: 132 against 204 for a turn of 300).
+// A cache streams through once: nontemporal 32.8 us over 128K of e4m3, plain 36.3 (32
+// sequences 112 and 122; bf16 alike in both).  Listed pages are shared by rows: plain
+// 113.5 us for a turn of 300 over bf16, nontemporal 208 (e4m3 70 and 94).
 template <bool kOnce>
 __device__ __forceinline__ u32x4 load16(const char* p) {
   const u32x4* x = reinterpret_cast<const u32x4*>(p);
@@ -612,6 +613,20 @@ bool paged_out_of(const void* q, const PagedCache& c, const void* q_gate, unsign
 
 // How a call is cut: tokens of a tile, workgroups of a KV head that the GPU holds
 // at once, items of a KV head aimed at, items (or slots of partials) at most.
+// One tile for the whole call, by the mean rows of a sequence; graph us with tiles of
+// 2 / 8 / 16 / 32 over two KV heads, first 16 sequences over 12,000, then 128 over 1,000:
+//   rows    e4m3                            bf16
+//    2   49  57  57  76   35  47  46  63    88  89  88  91   61  67  67  72
+//    3   77  60  60  78   61  49  48  66   155  92  91  94  114  70  69  75
+//    8  115  65  68  80  118  66  66  70   263  98  99  95  226  84  85  80
+//    9  164  77  73  80  146  70  70  71   353 117 102  96  281 108  90  81
+//   16  219  86  87  88  226  74  84  75   486 125 115 104  434 108 102  87
+//   17  280 110 103 102  254 116  86  85   602 193 130 115  492 177 108  93
+// The border of 2 is clear, those of 8 and 16 are e4m3's over long caches; bf16 would
+// gain up to 15% by tiles of 32 from 8 rows on.  Sequences far from the mean pay for
+// the one tile: 255 single tokens over 16,000 and one turn of 256 rows over 30,000
+// together 1,184 us, alone 663 and 132; 63 single tokens and a prompt of 2,048 rows
+// together 1,429, alone 175 and 836.
 struct Plan {
   unsigned tile, slots, target, items;
 };

@@ -3,10 +3,11 @@
 //
 //   score(page) = 2^e max_h sum_d max(qi_hd kmax_d, qi_hd kmin_d)
 //
-// an upper estimate of the page's largest q.k, in whole numbers: qi and the
-// bounds are int8, the sums stay below 2^22, and scores of different pages are
-// compared as (integer, exponent), so nothing is rounded, no order of summation
-// shows and ties are ties.
+// an estimate of the page's largest q.k, in whole numbers: qi and the bounds are
+// int8, the sums stay below 2^22, and scores of different pages are compared as
+// (integer, exponent), so no sum is rounded, no order of summation shows and ties
+// are ties.  (No upper bound: q is rounded to qi, and the bounds are of the keys as
+// appended, which e4m3 moves by up to half a step, 16 scales or 4 steps of a bound.)
 //
 // max(q a, q b) with a >= b is q+ a + q- b for q's positive and negative parts,
 // so the score of 16 pages for 8 heads is a chain of 8 int8 matrix products of
@@ -288,9 +289,13 @@ Q36_EXPORT int qwen36_paged_select(const void* q, const qwen36_paged_cache* cach
       hipLaunchKernelGGL(kernel, dim3(items - at < most ? items - at : most), dim3(threads), 0, st, c, b, keys,
                          budget, sink_pages, recent_pages, static_cast<int*>(pages), at);
   };
+  // The whole call with its attention, graph us, one row and 16: up to 2,048 pages
+  // 20.3 to 22.0 and 26.8 to 32.2, with 17 keys a thread 21.9 to 23.6 and 28.5 to
+  // 33.6; 3,000 and 4,352 pages 22.2 and 23.5, 39.5 and 44.2, with 16 waves 27.0 and
+  // 29.6, 46.0 and 50.6.
   if (b.width <= 2048)
     pick(paged_pick_kernel<8, 4>, 256);
-  else if (b.width <= 4352)   // 2,049 pages: 16 waves 20 us, 4 waves 9
+  else if (b.width <= 4352)
     pick(paged_pick_kernel<17, 4>, 256);
   else                        // up to the longest sequence's 16,391
     pick(paged_pick_kernel<17, 16>, 1024);

@@ -137,9 +137,11 @@ inline unsigned paged_items(const PagedBatch& b, unsigned tile, unsigned target)
 }
 
 // o * sigmoid(g) within a few fp32 ulps (rounded to bf16 by the caller): e^-g from
-// the hardware exp2 with log2(e) split, as gate4_bf16_fast has it; gates past 60
-// count as 60, where the sigmoid is 1.  With expf and a division the epilogue of a
-// 32-token tile took 13 us.
+// the hardware exp2 with log2(e) split, as gate4_bf16_fast has it, but without its
+// exact form next to a rounding border: the product is rounded once, so there is no
+// sigmoid in bf16 to agree on.  Gates past 60 count as 60, where the sigmoid is 1; one
+// below 2^-126 (gates under -87) may count as 0.  With expf and a division the epilogue
+// of a 32-token tile took 13 us.
 __device__ __forceinline__ float paged_gate(float o, bf16 gate) {
   float g = bf2f(gate);
   g = g > 60.f ? 60.f : g;

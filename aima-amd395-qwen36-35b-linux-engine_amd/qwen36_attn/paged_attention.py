@@ -256,7 +256,8 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
     own, scale 1/16; the rows' own keys must have been appended.  q [T, heads,
     256] bf16 as ``paged_append`` returns it.  ``q_gate`` (its input rows): the
     output is ``attention * sigmoid(gate)``, rounded once.  Rows that see
-    nothing are zeros.  Returns bf16 [T, heads * 256]."""
+    nothing are zeros.  The workspace of a call grows with its rows (two KV heads:
+    259 MiB for 8,192, 4.2 GiB for 262,144).  Returns bf16 [T, heads * 256]."""
     dev = cache.device
     t = _queries(q, cache)
     batch = _batch(cache, t, page_table, cu_tokens, seq_lens)
@@ -276,9 +277,9 @@ def select_pages(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tensor,
     """For each row and KV head the pages that a sparse attention reads: int32
     [T, kv_heads, budget] logical page indices, ascending, -1 behind the last.
     Rows of at most ``budget`` pages take all; others the first
-    ``sink_pages``, the last ``recent_pages`` and those whose bounds allow the
-    largest q.k (in whole numbers, so exactly; ties to the lower page).  The
-    cache needs ``bounds``."""
+    ``sink_pages``, the last ``recent_pages`` and those of the highest scores,
+    estimates of the page's largest q.k from its bounds in whole numbers (so the
+    choice is exact; ties to the lower page).  The cache needs ``bounds``."""
     dev = cache.device
     t = _queries(q, cache)
     batch = _batch(cache, t, page_table, cu_tokens, seq_lens)

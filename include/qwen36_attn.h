@@ -466,8 +466,10 @@ int qwen36_prefix_cache_destroy(void* pool);
  * 2^(e - 127) (E8M0) in k_exp, v_exp [num_pages][kv_heads] (bytes of 16 to
  * 247, as the append writes them).
  * bounds: NULL, or int8 [num_pages][kv_heads][2][256]: each channel's largest
- * and smallest key of the page, rounded outwards to steps of
- * 4 * 2^(k_exp - 127) (a bf16 cache with bounds has k_exp too). */
+ * and smallest key of the page as appended (before e4m3 rounds it), rounded
+ * outwards to steps of 4 * 2^(k_exp - 127) (a bf16 cache with bounds has k_exp
+ * too).  Scale and bounds cover every row that the page got since it last got
+ * its first: rows that are taken back and written again stay in them. */
 #define QWEN36_PAGED_BF16 0
 #define QWEN36_PAGED_E4M3 1
 typedef struct {
@@ -532,8 +534,18 @@ int qwen36_paged_append(const void* q_gate, unsigned q_row_stride, const void* k
  * rounded once (qwen36_output_gate rounds the attention and the sigmoid first).
  * A row that sees nothing is zeros.  One token per sequence, drafted tokens and
  * prompts in any mixture; tokens of the rows' own sequence must have been
- * appended.  workspace of qwen36_paged_attention_workspace_bytes(...) bytes,
- * 16-byte aligned; calls that overlap on one workspace race. */
+ * appended.
+ * Precision: scores, maxima, sums and accumulators are fp32; the softmax's
+ * numerators are rounded to bf16 for the product with V (their sum is not);
+ * over e4m3 pages, calls of more than two rows a sequence on average take q as
+ * the sum of two e4m3 values with a scale for each 64 channels, which is q
+ * unless it is 2^-14 of the 64's largest or less (then to 2^-22 of that); the
+ * gate's sigmoid is within a few fp32 ulps (0 where it is below 2^-126).
+ * workspace of qwen36_paged_attention_workspace_bytes(...) bytes, 16-byte
+ * aligned; calls that overlap on one workspace race.  It grows with the call's
+ * rows, as the lengths are not known to the host: two KV heads and long tables
+ * 259 MiB for 8,192 rows, 4.2 GiB for 262,144; shorter chunks of a prompt need
+ * less. */
 size_t qwen36_paged_attention_workspace_bytes(const qwen36_paged_cache* cache,
                                               const qwen36_paged_batch* batch);
 int qwen36_paged_attention(const void* q, const qwen36_paged_cache* cache,
@@ -553,7 +565,9 @@ int qwen36_paged_attention(const void* q, const qwen36_paged_cache* cache,
  * puts the 8 heads' largest finite magnitude in [64, 128), rounded to nearest
  * even and cut to +-127 (NaN counts as 0): whole numbers, so the selection is exact.  A page id
  * outside the pool scores below every other.  Needs bounds; workspace of
- * qwen36_paged_select_workspace_bytes(...) bytes, 16-byte aligned. */
+ * qwen36_paged_select_workspace_bytes(...) bytes, 16-byte aligned: 4 for each
+ * row, KV head and page of the table's width (2 GiB for 32,768 rows of two KV
+ * heads over 8,192 pages). */
 size_t qwen36_paged_select_workspace_bytes(const qwen36_paged_cache* cache,
                                            const qwen36_paged_batch* batch);
 int qwen36_paged_select(const void* q, const qwen36_paged_cache* cache,
