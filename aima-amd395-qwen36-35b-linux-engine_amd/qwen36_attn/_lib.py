@@ -35,6 +35,13 @@ class PagedBatchArgs(ctypes.Structure):
                 ("table_width", _u32), ("seqs", _u32), ("tokens", _u32)]
 
 
+class StateBatchArgs(ctypes.Structure):
+    """qwen36_state_batch"""
+    _fields_ = [("cu_tokens", _vp), ("slots", _vp), ("has_state", _vp), ("seqs", _u32),
+                ("tokens", _u32), ("num_slots", _u32)]
+
+
+_psbatch = ctypes.POINTER(StateBatchArgs)
 _pcache = ctypes.POINTER(PagedCacheArgs)
 _pbatch = ctypes.POINTER(PagedBatchArgs)
 
@@ -119,6 +126,11 @@ SIGNATURES: dict[str, tuple] = {
     "qwen36_paged_sparse_attention_workspace_bytes": (_sz, [_pcache, _pbatch, _u32]),
     "qwen36_paged_sparse_attention": (_i32, [_vp, _pcache, _pbatch, _vp, _u32, _vp, _u32, _vp,
                                              _vp, _sz, _vp]),
+    # Gated DeltaNet over ragged batches
+    "qwen36_gdn_ragged_conv1d": (_i32, [_vp, _u32, _vp, _vp, _sz, _psbatch, _vp, _vp]),
+    "qwen36_gdn_ragged_delta_workspace_bytes": (_sz, [_psbatch, _u32]),
+    "qwen36_gdn_ragged_delta": (_i32, [_vp, _vp, _vp, _u32, _u32, _u32, _vp, _vp, _vp, _sz,
+                                       _psbatch, _u32, _vp, _vp, _sz, _vp]),
     "qwen36_gdn_decode_step": (_i32, [_vp, _u32, _vp, _vp, _vp, _vp, _vp, _u32, _vp,
                                       _vp, _vp, _u32, _vp, _vp, _vp, _vp, _u32, _vp]),
 }

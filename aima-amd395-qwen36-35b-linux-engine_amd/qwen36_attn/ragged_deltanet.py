@@ -1,0 +1,178 @@
+"""Gated DeltaNet over ragged batches, states in slots.
+
+No counterpart in the reference, which runs one sequence
+(``linear_attention``, four_layer_mini_engine.py:6378-6544).  Prompts, drafted
+tokens and single tokens of any number of sequences go through the same calls,
+next to ``paged_attention`` for the full-attention layers.
+
+The batch of a call is ``cu_tokens`` int32 [seqs + 1] (row offsets of the call),
+``slots`` int32 [seqs] (where each sequence's states are) and ``has_state`` bool
+[seqs] or None (all True): where False the sequence begins with zeros, whatever
+its slot holds.  They are GPU tensors, read when the launch runs.  A sequence
+without rows, or with a slot outside the pool, is padding: its rows and slot stay
+as they are, as do rows behind the last sequence.  A slot must belong to one
+sequence of the batch.  All arithmetic runs in ``libqwen36_attn.so``.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from ._tensors import launch
+from .full_attention import MAX_TOKENS
+from .gated_deltanet import CONV_DIM, DK, DV, HK, HV, KEY_DIM, VALUE_DIM
+
+_STATE = (HV, DK, DV)
+
+
+def _pool(t, name: str, dtype, shape: tuple) -> tuple[int, int, int, int]:
+    """Device index, slots, address and slot stride in elements of a [slots, ...] pool."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or not t.is_cuda:
+        raise ValueError(f"{name} must be a {dtype} GPU tensor")
+    if t.dim() != len(shape) + 1 or t.shape[1:] != shape or t.shape[0] < 1:
+        raise ValueError(f"{name} must be [slots, {', '.join(map(str, shape))}]")
+    n, least = t.shape[0], shape[0]
+    for m in shape[1:]:
+        least *= m
+    stride = t.stride(0) if n > 1 else least
+    if not t[0].is_contiguous() or stride < least or stride * t.element_size() % 16 or t.data_ptr() % 16:
+        raise ValueError(f"{name}: a slot must be contiguous, 16-byte aligned and apart from the others")
+    return t.get_device(), n, t.data_ptr(), stride
+
+
+def _batch(index: int, tokens: int, n_slots: int, cu_tokens, slots, has_state) -> _lib.StateBatchArgs:
+    for t in (cu_tokens, slots):
+        if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.get_device() != index \
+                or t.dim() != 1 or not t.is_contiguous():
+            raise ValueError("cu_tokens [seqs + 1] and slots [seqs] must be contiguous int32 tensors "
+                             "on the pool's device")
+    seqs = slots.shape[0]
+    if cu_tokens.shape[0] != seqs + 1 or not 1 <= seqs <= 65536:
+        raise ValueError("a batch is cu_tokens [seqs + 1] and slots [seqs] of 1 to 65536 sequences")
+    if has_state is not None and (not isinstance(has_state, torch.Tensor) or has_state.dtype is not torch.bool
+                                  or has_state.get_device() != index or has_state.shape != (seqs,)
+                                  or not has_state.is_contiguous()):
+        raise ValueError("has_state must be a contiguous bool tensor [seqs] on the pool's device")
+    if not 0 < tokens <= MAX_TOKENS:
+        raise ValueError(f"a call has 1 to {MAX_TOKENS} rows")
+    return _lib.StateBatchArgs(cu_tokens.data_ptr(), slots.data_ptr(),
+                               None if has_state is None else has_state.data_ptr(), seqs, tokens, n_slots)
+
+
+def _heads(t, name: str, tokens: int, heads: tuple, index: int) -> int:
+    """Token stride of a bf16 [tokens, heads, 128] tensor with contiguous rows."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.bfloat16 or t.get_device() != index:
+        raise ValueError(f"{name} must be a bf16 tensor on the pool's device")
+    if t.dim() != 3 or t.shape[0] != tokens or t.shape[1] not in heads or t.shape[2] != DK:
+        raise ValueError(f"{name} must be [{tokens}, {' or '.join(map(str, heads))}, 128]")
+    width = t.shape[1] * DK
+    stride = t.stride(0) if tokens > 1 else width
+    if t.stride(2) != 1 or t.stride(1) != DK or not width <= stride < 1 << 32 or stride % 8 or t.data_ptr() % 16:
+        raise ValueError(f"{name} must have contiguous, 16-byte aligned rows that do not overlap")
+    return stride
+
+
+def _scalars(t, name: str, tokens: int, index: int) -> int:
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.float32 or t.get_device() != index \
+            or t.shape != (tokens, HV) or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous fp32 [{tokens}, 32] on the pool's device")
+    return t.data_ptr()
+
+
+def _out(out, shape: tuple, device) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=torch.bfloat16, device=device)
+    if not isinstance(out, torch.Tensor) or out.dtype is not torch.bfloat16 or out.device != device \
+            or tuple(out.shape) != shape or not out.is_contiguous() or out.data_ptr() % 16:
+        raise ValueError(f"out must be contiguous bf16 {list(shape)} on the pool's device")
+    return out
+
+
+def ragged_conv1d(mixed_qkv: torch.Tensor, weight: torch.Tensor, states: torch.Tensor,
+                  cu_tokens: torch.Tensor, slots: torch.Tensor, has_state: torch.Tensor | None = None,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """``gated_deltanet.causal_conv1d`` for a batch, with its arithmetic: mixed_qkv
+    [T, 8192] bf16 (unit inner stride), weight [8192, 4] bf16, states [slots, 8192, 3]
+    bf16, replaced in place by each sequence's last three inputs.  Returns SiLU(conv)
+    [T, 8192] bf16."""
+    index, n, sp, ss = _pool(states, "states", torch.bfloat16, (CONV_DIM, 3))
+    t = mixed_qkv.shape[0] if isinstance(mixed_qkv, torch.Tensor) and mixed_qkv.dim() == 2 else 0
+    if t == 0 or mixed_qkv.dtype is not torch.bfloat16 or mixed_qkv.get_device() != index \
+            or mixed_qkv.shape[1] != CONV_DIM:
+        raise ValueError("mixed_qkv must be bf16 [T, 8192] on the pool's device")
+    stride = mixed_qkv.stride(0) if t > 1 else CONV_DIM
+    if mixed_qkv.stride(1) != 1 or not CONV_DIM <= stride < 1 << 32 or stride % 8 or mixed_qkv.data_ptr() % 16:
+        raise ValueError("mixed_qkv must have unit inner stride and 16-byte aligned rows that do not overlap")
+    if not isinstance(weight, torch.Tensor) or weight.dtype is not torch.bfloat16 or weight.get_device() != index \
+            or weight.shape != (CONV_DIM, 4) or not weight.is_contiguous() or weight.data_ptr() % 16:
+        raise ValueError("weight must be contiguous bf16 [8192, 4] on the pool's device")
+    batch = _batch(index, t, n, cu_tokens, slots, has_state)
+    out = _out(out, (t, CONV_DIM), states.device)
+    launch(index, "qwen36_gdn_ragged_conv1d", mixed_qkv.data_ptr(), stride, weight.data_ptr(), sp, ss, batch,
+           out.data_ptr())
+    return out
+
+
+def ragged_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
+                      states: torch.Tensor, cu_tokens: torch.Tensor, slots: torch.Tensor,
+                      has_state: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                      longest: int | None = None) -> torch.Tensor:
+    """The gated delta rule for a batch: q, k [T, 16 (or 32 repeated), 128], v [T, 32,
+    128] bf16 (q and k are l2-normalised in the kernel), g (log decay), beta [T, 32]
+    fp32, states [slots, 32, 128 (k), 128 (v)] fp32, replaced in place by the sequences'
+    last states.  ``longest``: the most rows that a sequence of the call has, where the
+    caller knows it; it only chooses between the forms for few and for many tokens (a
+    sequence may have more).  Returns [T, 32, 128] bf16."""
+    index, n, sp, ss = _pool(states, "states", torch.float32, _STATE)
+    t = v.shape[0] if isinstance(v, torch.Tensor) and v.dim() == 3 else 0
+    qs, ks = _heads(q, "q", t, (HK, HV), index), _heads(k, "k", t, (HK, HV), index)
+    if q.shape != k.shape or qs != ks:
+        raise ValueError("q and k must share shape and token stride")
+    vs = _heads(v, "v", t, (HV,), index)
+    gp, bp = _scalars(g, "g", t, index), _scalars(beta, "beta", t, index)
+    if longest is not None and longest < 1:
+        raise ValueError("longest must be positive")
+    batch = _batch(index, t, n, cu_tokens, slots, has_state)
+    out = _out(out, (t, HV, DV), states.device)
+    most = min(longest or 0, MAX_TOKENS)
+    nb = (_lib._LIB or _lib.load()).qwen36_gdn_ragged_delta_workspace_bytes(batch, most)
+    # allocated per call: calls on several streams, and graphs captured apart, never share one
+    ws = torch.empty(nb, dtype=torch.uint8, device=states.device) if nb else None
+    launch(index, "qwen36_gdn_ragged_delta", q.data_ptr(), k.data_ptr(), v.data_ptr(), q.shape[1], qs, vs, gp, bp,
+           sp, ss, batch, most, out.data_ptr(), None if ws is None else ws.data_ptr(), nb)
+    return out
+
+
+class RaggedLinearAttentionLayer:
+    """One Gated-DeltaNet layer over ragged batches, ``gated_deltanet.
+    LinearAttentionLayer`` for many sequences: the projections, the convolution and the
+    delta rule with their states in ``conv_states`` [slots, 8192, 3] bf16 and
+    ``ssm_states`` [slots, 32, 128, 128] fp32, the gated norm and out_proj.
+    ``weights`` as there."""
+
+    def __init__(self, weights: dict, conv_states: torch.Tensor, ssm_states: torch.Tensor) -> None:
+        if _pool(conv_states, "conv_states", torch.bfloat16, (CONV_DIM, 3))[:2] \
+                != _pool(ssm_states, "ssm_states", torch.float32, _STATE)[:2]:
+            raise ValueError("conv_states and ssm_states must have the same slots on one device")
+        from .projections import FusedProjection
+        self.w, self.conv_states, self.ssm_states = weights, conv_states, ssm_states
+        self._in_proj = FusedProjection(weights["in_proj_qkv"], weights["in_proj_z"], weights["in_proj_b"],
+                                        weights["in_proj_a"])
+
+    def forward(self, inp: torch.Tensor, cu_tokens: torch.Tensor, slots: torch.Tensor,
+                has_state: torch.Tensor | None = None, longest: int | None = None) -> torch.Tensor:
+        """inp [T, 2048]: the new rows of the batch's sequences.  Returns [T, 2048]; rows
+        of padding hold nothing of use."""
+        from .gated_deltanet import gated_rmsnorm, gating
+        from .prefill_gemm import linear
+        from .projections import gemv
+        w, t = self.w, inp.shape[0]
+        mixed, z, b, a = self._in_proj(inp) if t == 1 else self._in_proj.split_rows(linear(inp, self._in_proj.w))
+        conv = ragged_conv1d(mixed, w["conv1d"], self.conv_states, cu_tokens, slots, has_state)
+        q = conv[:, :KEY_DIM].view(t, HK, DK)
+        k = conv[:, KEY_DIM:2 * KEY_DIM].view(t, HK, DK)
+        v = conv[:, 2 * KEY_DIM:].view(t, HV, DV)
+        g, beta = gating(a, b, w["A_log"], w["dt_bias"])
+        core = ragged_delta_rule(q, k, v, g, beta, self.ssm_states, cu_tokens, slots, has_state, longest=longest)
+        gated = gated_rmsnorm(core, z, w["norm"])
+        return gemv(w["out_proj"], gated.view(1, VALUE_DIM)) if t == 1 else linear(gated, w["out_proj"])

@@ -588,6 +588,50 @@ int qwen36_paged_sparse_attention(const void* q, const qwen36_paged_cache* cache
                                   unsigned q_gate_row_stride, void* out, void* workspace,
                                   size_t workspace_bytes, void* stream);
 
+/* ---- Gated DeltaNet over ragged batches --------------------------------------
+ * No counterpart in the reference, which runs one sequence.  Rows
+ * [cu_tokens[i], cu_tokens[i+1]) of the call's `tokens` rows are sequence i, whose
+ * states are in slot slots[i] of the pools.  has_state: NULL (every sequence goes on
+ * from its slot), or bytes: where 0 the sequence begins with zeros, whatever the slot
+ * holds.  All in device memory (int32, int32, bytes), read when the launch runs, so a
+ * captured call follows them.  Nothing there can make a launch read or write out of
+ * bounds: offsets are cut to the call's rows; a sequence without rows, or with a slot
+ * outside [0, num_slots), is padding: its rows and slot stay as they are, as do rows
+ * behind the last sequence.  A slot must belong to one sequence of the batch.
+ * At most 65536 sequences and 262144 rows. */
+typedef struct {
+  const void* cu_tokens;
+  const void* slots;
+  const void* has_state;
+  unsigned seqs;
+  unsigned tokens;
+  unsigned num_slots;
+} qwen36_state_batch;
+
+/* qwen36_gdn_ragged_conv1d: qwen36_gdn_conv1d for a batch, with its arithmetic:
+ * x [tokens, >= 8192 stride], weight [8192, 4], out [tokens, 8192] bf16; states
+ * bf16 [num_slots][8192][3], slots slot_stride elements apart, each replaced by its
+ * sequence's last three inputs.  Strides multiples of 8, pointers 16-byte aligned. */
+int qwen36_gdn_ragged_conv1d(const void* x, unsigned x_row_stride, const void* weight, void* states,
+                             size_t slot_stride, const qwen36_state_batch* batch, void* out,
+                             void* stream);
+
+/* qwen36_gdn_ragged_delta: the gated delta rule for a batch (qwen36_gdn_recurrent's
+ * and qwen36_gdn_chunk_prefill's tensors): q, k [tokens, qk_heads (16 | 32), 128],
+ * v [tokens, 32, 128] bf16 with token strides (multiples of 8), g, beta fp32
+ * [tokens, 32], out bf16 [tokens, 32, 128]; states fp32 [num_slots][32][128 k][128 v],
+ * slots slot_stride elements (a multiple of 4) apart, replaced by the sequences' last
+ * states.  longest: 0, or the most rows that a sequence has as the host knows it; it
+ * only chooses the launches, a sequence may have more.  Pointers 16-byte aligned (g and
+ * beta 4); workspace of qwen36_gdn_ragged_delta_workspace_bytes(...) bytes (0: none);
+ * calls that overlap on one workspace race. */
+size_t qwen36_gdn_ragged_delta_workspace_bytes(const qwen36_state_batch* batch, unsigned longest);
+int qwen36_gdn_ragged_delta(const void* q, const void* k, const void* v, unsigned qk_heads,
+                            unsigned qk_token_stride, unsigned v_token_stride, const void* g,
+                            const void* beta, void* states, size_t slot_stride,
+                            const qwen36_state_batch* batch, unsigned longest, void* out,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,218 @@
+"""The Gated-DeltaNet convolution and delta rule over ragged batches against plain
+forms in 64 bits: lengths from one token to many chunks, slots in any order,
+sequences without a state, padding, strides, captured calls, the layer."""
+import pytest
+import torch
+
+from qwen36_attn import gated_deltanet as gd
+from qwen36_attn import ragged_deltanet as rd
+from qwen36_attn import synthetic as syn
+from tests import ragged_reference as R
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+
+
+def batch(lens, slots, has, gpu):
+    return (torch.tensor(R.cu_of(lens), dtype=torch.int32, device=gpu),
+            torch.tensor(slots, dtype=torch.int32, device=gpu), torch.tensor(has, device=gpu))
+
+
+CONV = [([1], [2], [True], 0), ([1], [0], [False], 1), ([2, 1, 3], [3, 0, 1], [True, False, True], 0),
+        ([4, 5, 0, 17, 1, 66], [5, 2, 3, 0, 6, 1], [True, False, True, True, False, True], 3),
+        ([3, 2, 7], [-1, 4, 9], [True, True, True], 2), ([1] * 70, list(range(69, -1, -1)), [i % 3 > 0 for i in range(70)], 0),
+        ([9, 200, 1], [1, 0, 2], [False, False, True], 5)]
+
+
+@pytest.mark.parametrize("lens,slots,has,behind", CONV)
+def test_conv(gpu, lens, slots, has, behind):
+    """Against 64 bits, and bit for bit against the operator of one sequence.  The sum is
+    rounded to bf16 (off by a step of 2^-8 of it where 32 and 64 bits fall on two sides:
+    SiLU's slope is below 1.1), the result once more."""
+    g = torch.Generator(device=gpu).manual_seed(len(lens))
+    t, n = sum(lens) + behind, max(7, len(lens))
+    x = torch.randn(t, 8192 + 24, generator=g, device=gpu).to(BF16)[:, :8192]
+    w = torch.randn(8192, 4, generator=g, device=gpu).to(BF16)
+    pool = torch.randn(n, 2, 8192, 3, generator=g, device=gpu).to(BF16)
+    states, before = pool[:, 0], pool.clone()
+    out = torch.full((t, 8192), 7.0, dtype=BF16, device=gpu)
+    cu, sl, h = batch(lens, slots, has, gpu)
+    rd.ragged_conv1d(x, w, states, cu, sl, h, out=out)
+    want, after = R.conv(x, w, before[:, 0], R.cu_of(lens), slots, has)
+    there = ~want.isnan()
+    assert torch.equal(out[~there], torch.full_like(out[~there], 7.0))
+    y = out[there].double()
+    assert ((y - want[there]).abs() <= 2.0 ** -8 * want[there].abs() + 1.1 * 2.0 ** -7 * want[there].abs() + 1e-4).all()
+    assert ((y - want[there]).norm() / want[there].norm()).item() <= 2.0 ** -8
+    assert torch.equal(states.double(), after)
+    assert torch.equal(pool[:, 1], before[:, 1])
+    a = 0
+    for m, slot, hs in zip(lens, slots, has):
+        if m and 0 <= slot < n:
+            old = before[slot, 0].contiguous() if hs else torch.zeros(8192, 3, dtype=BF16, device=gpu)
+            one, last = gd.causal_conv1d(x[a:a + m], old, w)
+            assert torch.equal(out[a:a + m], one) and torch.equal(states[slot], last)
+        a += m
+
+
+def core(gpu, t, seed, a_max=2.0, qk_heads=16, pad=0):
+    g = torch.Generator(device=gpu).manual_seed(seed)
+    x = torch.nn.functional.silu(torch.randn(t, 2 * qk_heads * 128 + 4096 + pad, generator=g, device=gpu)).to(BF16)
+    q = x[:, :qk_heads * 128].view(t, qk_heads, 128)
+    k = x[:, qk_heads * 128:2 * qk_heads * 128].view(t, qk_heads, 128)
+    v = x[:, 2 * qk_heads * 128:2 * qk_heads * 128 + 4096].view(t, 32, 128)
+    gg = -torch.nn.functional.softplus(torch.randn(t, 32, generator=g, device=gpu)) \
+        * torch.rand(32, generator=g, device=gpu) * a_max
+    return q, k, v, gg, torch.sigmoid(torch.randn(t, 32, generator=g, device=gpu)), g
+
+
+def check_delta(out, states, want, after, untouched):
+    """fp32 dot products of 128 keys or 64 tokens, a few roundings each: 256 units of 2^-24
+    of the 2-norm (earlier errors decay with the state that holds them), which is at most
+    2^-12 of a row's largest value for an element; the output is rounded to bf16."""
+    there = ~want.isnan()
+    assert torch.equal(out[~there], torch.full_like(out[~there], 7.0))
+    err = (out.double() - want).abs()
+    tol = 2.0 ** -8 * want.abs() + 2.0 ** -12 * want.abs().amax(-1, keepdim=True)
+    bad = there & ~(err <= tol)
+    assert not bad.any(), (bad.nonzero()[:4].tolist(), (err / tol)[there].max().item())
+    rel = (states.double() - after).flatten(1).norm(dim=1) / after.flatten(1).norm(dim=1).clamp(min=1e-30)
+    print("state errors", rel.max().item(), flush=True)
+    assert rel.max().item() <= 256 * 2.0 ** -24
+    assert torch.equal(states[untouched].double(), after[untouched])
+
+
+DELTA = [([1], [2], [True], 0, None), ([1], [0], [False], 2, 1), ([2, 1, 8], [3, 0, 1], [True, False, True], 0, 8),
+         ([9, 16, 17, 1], [3, 0, 1, 4], [True, False, True, True], 1, None),
+         ([64, 63, 65, 0, 1, 128], [5, 2, 3, 0, 6, 1], [True, False, True, True, False, True], 3, 128),
+         ([64, 63, 65, 0, 1, 128], [5, 2, 3, 0, 6, 1], [False, True, True, True, False, False], 0, None),
+         ([70, 30, 3], [-1, 4, 9], [True, True, True], 2, 70), ([1] * 70, list(range(69, -1, -1)), [i % 3 > 0 for i in range(70)], 0, 1),
+         ([1] * 66 + [130] + [1] * 3 + [77], list(range(71)), [i % 5 > 0 for i in range(71)], 0, None),
+         ([1, 513, 2, 40], [3, 2, 1, 0], [True, True, False, False], 0, 1),       # more rows than `longest` says
+         ([1000], [1], [True], 0, 1000)]
+
+
+@pytest.mark.parametrize("lens,slots,has,behind,longest", DELTA)
+def test_delta(gpu, lens, slots, has, behind, longest):
+    t, n = sum(lens) + behind, max(7, len(lens))
+    q, k, v, g, beta, gen = core(gpu, t, 3 * len(lens) + max(lens))
+    states = torch.randn(n, 32, 128, 128, generator=gen, device=gpu) * 0.2
+    before = states.clone()
+    out = torch.full((t, 32, 128), 7.0, dtype=BF16, device=gpu)
+    cu, sl, h = batch(lens, slots, has, gpu)
+    print("delta", lens[:8], longest, flush=True)
+    rd.ragged_delta_rule(q, k, v, g, beta, states, cu, sl, h, out=out, longest=longest)
+    want, after = R.delta(q, k, v, g, beta, before, R.cu_of(lens), slots, has)
+    used = {s for s, m in zip(slots, lens) if m}
+    check_delta(out, states, want, after, [i for i in range(n) if i not in used])
+
+
+@pytest.mark.parametrize("a_max", [16.0, 0.02])
+@pytest.mark.parametrize("qk_heads,pad", [(16, 40), (32, 8)])
+def test_delta_decays_heads_and_strides(gpu, a_max, qk_heads, pad):
+    """Fast and slow decays, 32 repeated key heads, padded rows, slots apart."""
+    lens, slots, has = [150, 1, 12, 300], [2, 0, 3, 1], [True, True, False, True]
+    q, k, v, g, beta, gen = core(gpu, sum(lens), 11, a_max, qk_heads, pad)
+    pool = torch.randn(5, 2, 32, 128, 128, generator=gen, device=gpu) * 0.2
+    before = pool.clone()
+    out = torch.full((sum(lens), 32, 128), 7.0, dtype=BF16, device=gpu)
+    cu, sl, h = batch(lens, slots, has, gpu)
+    rd.ragged_delta_rule(q, k, v, g, beta, pool[:, 1], cu, sl, h, out=out)
+    want, after = R.delta(q, k, v, g, beta, before[:, 1], R.cu_of(lens), slots, has)
+    check_delta(out, pool[:, 1], want, after, [4])
+    assert torch.equal(pool[:, 0], before[:, 0])
+
+
+def test_delta_of_rows_without_keys(gpu):
+    """Rows of zeros (a norm of nothing), gates of zero and decays to nothing."""
+    lens, slots, has = [100, 3], [0, 1], [True, True]
+    q, k, v, g, beta, gen = core(gpu, 103, 5)
+    q, k, beta, g = q.clone(), k.clone(), beta.clone(), g.clone()
+    k[10:20] = 0
+    q[30:40] = 0
+    beta[50:60] = 0
+    g[70] = -200.0
+    g[101] = -1000.0
+    states = torch.randn(3, 32, 128, 128, generator=gen, device=gpu)
+    before = states.clone()
+    out = torch.full((103, 32, 128), 7.0, dtype=BF16, device=gpu)
+    rd.ragged_delta_rule(q, k, v, g, beta, states, *batch(lens, slots, has, gpu), out=out)
+    want, after = R.delta(q, k, v, g, beta, before, R.cu_of(lens), slots, has)
+    check_delta(out, states, want, after, [2])
+
+
+def test_captured_calls_follow_the_batch(gpu):
+    """One capture, replayed over other lengths, slots and states, with eager work
+    between; each replay against the eager call."""
+    t, n = 160, 6
+    q, k, v, g, beta, gen = core(gpu, t, 9)
+    w = torch.randn(8192, 4, generator=gen, device=gpu).to(BF16)
+    x = torch.randn(t, 8192, generator=gen, device=gpu).to(BF16)
+    conv = torch.randn(n, 8192, 3, generator=gen, device=gpu).to(BF16)
+    ssm = torch.randn(n, 32, 128, 128, generator=gen, device=gpu) * 0.2
+    cu, sl, h = batch([100, 1, 59], [0, 1, 2], [True] * 3, gpu)
+    first = conv.clone(), ssm.clone()
+
+    def step():
+        return rd.ragged_conv1d(x, w, conv, cu, sl, h), rd.ragged_delta_rule(q, k, v, g, beta, ssm, cu, sl, h)
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for lens, slots, has in (([100, 1, 59], [0, 1, 2], [True] * 3), ([1, 1, 1], [5, 3, 4], [True, False, True]),
+                             ([0, 130, 30], [1, 0, 5], [False, True, True]), ([1, 2, 157], [2, -1, 3], [True] * 3)):
+        for p, q0 in zip((conv, ssm), first):
+            p.copy_(q0)
+        for p, q0 in zip((cu, sl, h), batch(lens, slots, has, gpu)):
+            p.copy_(q0)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [o.clone() for o in outs] + [conv.clone(), ssm.clone()]
+        for p, q0 in zip((conv, ssm), first):
+            p.copy_(q0)
+        rows = torch.zeros(t, dtype=torch.bool, device=gpu)
+        for a, z, s in zip(R.cu_of(lens), R.cu_of(lens)[1:], slots):
+            rows[a:z] = s >= 0
+        want = list(step()) + [conv, ssm]
+        for i, (a, b) in enumerate(zip(got, want)):
+            assert torch.equal(a[rows] if i < 2 else a, b[rows] if i < 2 else b), (lens, i)
+
+
+def test_layer_over_prompts_and_decode_steps(gpu):
+    """The layer over a batch against the layer of one sequence, turn by turn."""
+    w = {k: v.to(gpu) for k, v in syn.linear_attention_weights(syn.gen(4), a_max=2.0).items()}
+    n, slots = 3, [4, 0, 2]
+    conv = torch.full((5, 8192, 3), 3.0, dtype=BF16, device=gpu)
+    ssm = torch.full((5, 32, 128, 128), 3.0, device=gpu)
+    layer = rd.RaggedLinearAttentionLayer(w, conv, ssm)
+    singles = [gd.LinearAttentionLayer(w, gpu) for _ in range(n)]
+    for step, lens in enumerate(([70, 5, 130], [1, 33, 1], [1, 1, 1], [0, 1, 0])):
+        inp = syn.randn((sum(lens), 2048), syn.gen(50 + step)).to(gpu)
+        cu, sl, h = batch(lens, slots, [step > 0] * n, gpu)
+        got = layer.forward(inp, cu, sl, h, longest=max(lens))
+        for i, (a, m) in enumerate(zip(R.cu_of(lens), lens)):
+            if m:
+                one = singles[i].forward(inp[a:a + m], "prefill" if m > 1 else "decode")
+                # bf16 roundings of the projections (each of another product order), the conv,
+                # the norm's two and the output, carried through the delta rule: 8 of 2^-8 at most
+                rel = ((got[a:a + m].double() - one.double()).norm() / one.double().norm()).item()
+                assert rel <= 8 * 2.0 ** -8, (step, i, rel)
+                s = (ssm[slots[i]].double() - singles[i].ssm_state.double()).norm() / singles[i].ssm_state.double().norm()
+                assert s.item() <= 8 * 2.0 ** -8
+    assert (ssm[1] == 3.0).all() and (conv[3] == 3.0).all()
+
+
+def test_on_another_stream(gpu):
+    lens, slots, has = [5, 90], [1, 0], [True, True]
+    q, k, v, g, beta, gen = core(gpu, 95, 21)
+    states = torch.randn(2, 32, 128, 128, generator=gen, device=gpu)
+    other = states.clone()
+    want = rd.ragged_delta_rule(q, k, v, g, beta, states, *batch(lens, slots, has, gpu))
+    where = batch(lens, slots, has, gpu)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = rd.ragged_delta_rule(q, k, v, g, beta, other, *where)
+    s.synchronize()
+    assert torch.equal(got, want) and torch.equal(other, states)
