@@ -41,6 +41,19 @@ class StateBatchArgs(ctypes.Structure):
                 ("tokens", _u32), ("num_slots", _u32)]
 
 
+class SlotPoolArgs(ctypes.Structure):
+    """qwen36_slot_pool"""
+    _fields_ = [("data", _vp), ("slot_bytes", _sz), ("slot_stride_bytes", _sz)]
+
+
+class PageTablesArgs(ctypes.Structure):
+    """qwen36_page_tables"""
+    _fields_ = [("refs", _vp), ("page_table", _vp), ("seq_lens", _vp), ("table_stride", _sz),
+                ("num_pages", _u32), ("page_tokens", _u32), ("table_width", _u32), ("rows", _u32)]
+
+
+_ptables = ctypes.POINTER(PageTablesArgs)
+_pslots = ctypes.POINTER(SlotPoolArgs)
 _psbatch = ctypes.POINTER(StateBatchArgs)
 _pcache = ctypes.POINTER(PagedCacheArgs)
 _pbatch = ctypes.POINTER(PagedBatchArgs)
@@ -131,6 +144,14 @@ SIGNATURES: dict[str, tuple] = {
     "qwen36_gdn_ragged_delta_workspace_bytes": (_sz, [_psbatch, _u32]),
     "qwen36_gdn_ragged_delta": (_i32, [_vp, _vp, _vp, _u32, _u32, _u32, _vp, _vp, _vp, _sz,
                                        _psbatch, _u32, _vp, _vp, _sz, _vp]),
+    "qwen36_slots_fork": (_i32, [_pslots, _u32, _u32, _vp, _vp]),
+    # page tables
+    "qwen36_pages_trim": (_i32, [_ptables, _vp, _vp]),
+    "qwen36_pages_fork": (_i32, [_ptables, _vp, _vp]),
+    "qwen36_pages_extend_workspace_bytes": (_sz, [_ptables]),
+    "qwen36_pages_extend": (_i32, [_ptables, _vp, _vp, _pcache, _u32, _vp, _sz, _vp]),
+    "qwen36_pages_compact_workspace_bytes": (_sz, [_ptables]),
+    "qwen36_pages_compact": (_i32, [_ptables, _vp, _vp, _sz, _pcache, _u32, _vp, _sz, _vp]),
     "qwen36_gdn_decode_step": (_i32, [_vp, _u32, _vp, _vp, _vp, _vp, _vp, _u32, _vp,
                                       _vp, _vp, _u32, _vp, _vp, _vp, _vp, _u32, _vp]),
 }

@@ -143,6 +143,31 @@ def ragged_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torc
     return out
 
 
+def fork_states(pools, parents: torch.Tensor) -> None:
+    """Slot i of every pool (the layers' [slots, ...] conv and recurrent states) becomes a
+    copy of its slot ``parents[i]`` (int32 [slots], -1: it stays; a child of a slot that
+    is a child of the same call stays too): what ``page_tables.fork`` is for pages."""
+    pools = list(pools)
+    if not pools or not isinstance(parents, torch.Tensor) or parents.dtype is not torch.int32 \
+            or parents.dim() != 1 or not parents.is_cuda or not parents.is_contiguous() \
+            or not 1 <= parents.shape[0] <= 65536:
+        raise ValueError("pools must be one or more tensors and parents a contiguous int32 GPU tensor [slots]")
+    n, args = parents.shape[0], []
+    for t in pools:
+        if not isinstance(t, torch.Tensor) or t.device != parents.device or t.dim() < 2 or t.shape[0] != n \
+                or not t[0].is_contiguous():
+            raise ValueError("a pool must be [slots, ...] with contiguous slots on the device of parents")
+        size = t[0].numel() * t.element_size()
+        stride = t.stride(0) * t.element_size() if n > 1 else size
+        if size < 1 or size % 16 or stride % 16 or stride < size or t.data_ptr() % 16:
+            raise ValueError("a pool's slots must be 16-byte aligned, multiples of 16 bytes and apart")
+        args.append(_lib.SlotPoolArgs(t.data_ptr(), size, stride))
+    if len({a.data for a in args}) < len(args):
+        raise ValueError("a pool is listed twice")
+    launch(parents.get_device(), "qwen36_slots_fork", (_lib.SlotPoolArgs * len(args))(*args), len(args), n,
+           parents.data_ptr())
+
+
 class RaggedLinearAttentionLayer:
     """One Gated-DeltaNet layer over ragged batches, ``gated_deltanet.
     LinearAttentionLayer`` for many sequences: the projections, the convolution and the

@@ -632,6 +632,71 @@ int qwen36_gdn_ragged_delta(const void* q, const void* k, const void* v, unsigne
                             const qwen36_state_batch* batch, unsigned longest, void* out,
                             void* workspace, size_t workspace_bytes, void* stream);
 
+/* qwen36_slots_fork: slot i of every pool becomes a copy of its slot parent[i] (int32
+ * [slots] in device memory; -1: it stays; a child of a slot that is a child of the same
+ * call stays too).  Slots are slot_bytes (a multiple of 16, at most 2^30) at multiples
+ * of slot_stride_bytes (one of 16); data 16-byte aligned; at most 1024 pools. */
+typedef struct {
+  void* data;
+  size_t slot_bytes;
+  size_t slot_stride_bytes;
+} qwen36_slot_pool;
+int qwen36_slots_fork(const qwen36_slot_pool* pools, unsigned n_pools, unsigned slots,
+                      const void* parent, void* stream);
+
+/* ---- page tables -------------------------------------------------------------
+ * No counterpart in the reference, whose caches are dense.  page_table int32
+ * [rows][table_stride], seq_lens int32 [rows] (0: an empty row) and refs int32
+ * [num_pages], how many entries of the table name each page (0: free), in device
+ * memory, read and written when the launches run; one set for the caches of all layers.
+ * Calls take a number for every row.  Nothing there can make a launch read or write out
+ * of bounds: a row whose length is negative or above what the table holds is left as it
+ * is, a page id outside the pool holds nothing.  Calls on the same tables must be
+ * ordered (one stream).  All numbers are whole and nothing depends on timing. */
+typedef struct {
+  void* refs;
+  void* page_table;
+  void* seq_lens;
+  size_t table_stride;
+  unsigned num_pages;
+  unsigned page_tokens;
+  unsigned table_width;
+  unsigned rows;
+} qwen36_page_tables;
+
+/* qwen36_pages_trim: row i keeps its first keep[i] tokens (int32; 0 gives it up); pages
+ * without tokens leave it (-1) and lose a count. */
+int qwen36_pages_trim(const qwen36_page_tables* tables, const void* keep, void* stream);
+
+/* qwen36_pages_fork: the empty row i becomes a fork of row parent[i] (int32, -1: it
+ * stays), whose pages gain a count.  A child of a row that is a child of the same call
+ * stays. */
+int qwen36_pages_fork(const qwen36_page_tables* tables, const void* parent, void* stream);
+
+/* qwen36_pages_extend: row i grows by add[i] tokens (int32; none if not positive): the
+ * lowest free pages go to the rows in their order, to each all that it needs or nothing
+ * (once the pool cannot serve a row, it serves no later one that needs pages; a row that
+ * asks for more than its table holds needs none and gets nothing).  A row whose last page
+ * is not full and has other holders gets a copy of it in every cache (pages, scales,
+ * bounds).  granted int32 [rows]: 0 where the row could not grow, else 1.  The caches
+ * have num_pages pages of page_tokens; at most 1024; workspace of
+ * qwen36_pages_extend_workspace_bytes(...) bytes, 16-byte aligned. */
+size_t qwen36_pages_extend_workspace_bytes(const qwen36_page_tables* tables);
+int qwen36_pages_extend(const qwen36_page_tables* tables, const void* add, void* granted,
+                        const qwen36_paged_cache* caches, unsigned n_caches, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/* qwen36_pages_compact: with n pages held, those at n or behind go, in every cache, to
+ * the free pages before n, in ascending order; refs_out [num_pages] and table_out (rows
+ * table_out_stride apart) are the counts and the table after it, entries behind a row's
+ * length -1; they may be refs and the table themselves.  Workspace of
+ * qwen36_pages_compact_workspace_bytes(...) bytes, 16-byte aligned. */
+size_t qwen36_pages_compact_workspace_bytes(const qwen36_page_tables* tables);
+int qwen36_pages_compact(const qwen36_page_tables* tables, void* refs_out, void* table_out,
+                         size_t table_out_stride, const qwen36_paged_cache* caches,
+                         unsigned n_caches, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
 #ifdef __cplusplus
 }
 #endif
