@@ -52,6 +52,13 @@ class PageTablesArgs(ctypes.Structure):
                 ("num_pages", _u32), ("page_tokens", _u32), ("table_width", _u32), ("rows", _u32)]
 
 
+class AdaptersArgs(ctypes.Structure):
+    """qwen36_adapters"""
+    _fields_ = [("a", _vp), ("b", _vp), ("ranks", _vp), ("scales", _vp), ("adapters", _u32),
+                ("rank", _u32), ("k", _u32), ("slices", _u32), ("widths", _u32 * 4)]
+
+
+_padapters = ctypes.POINTER(AdaptersArgs)
 _ptables = ctypes.POINTER(PageTablesArgs)
 _pslots = ctypes.POINTER(SlotPoolArgs)
 _psbatch = ctypes.POINTER(StateBatchArgs)
@@ -152,6 +159,11 @@ SIGNATURES: dict[str, tuple] = {
     "qwen36_pages_extend": (_i32, [_ptables, _vp, _vp, _pcache, _u32, _vp, _sz, _vp]),
     "qwen36_pages_compact_workspace_bytes": (_sz, [_ptables]),
     "qwen36_pages_compact": (_i32, [_ptables, _vp, _vp, _sz, _pcache, _u32, _vp, _sz, _vp]),
+    # adapters
+    "qwen36_adapter_plan_bytes": (_sz, [_u32, _u32, _u32]),
+    "qwen36_adapter_plan": (_i32, [_vp, _vp, _u32, _u32, _u32, _vp, _sz, _vp]),
+    "qwen36_adapter_workspace_bytes": (_sz, [_padapters, _u32, _u32]),
+    "qwen36_adapter_apply": (_i32, [_vp, _sz, _vp, _sz, _padapters, _vp, _sz, _u32, _u32, _vp, _sz, _vp]),
     "qwen36_gdn_decode_step": (_i32, [_vp, _u32, _vp, _vp, _vp, _vp, _vp, _u32, _vp,
                                       _vp, _vp, _u32, _vp, _vp, _vp, _vp, _u32, _vp]),
 }

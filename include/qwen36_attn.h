@@ -697,6 +697,48 @@ int qwen36_pages_compact(const qwen36_page_tables* tables, void* refs_out, void*
                          unsigned n_caches, void* workspace, size_t workspace_bytes,
                          void* stream);
 
+/* ---- adapters ------------------------------------------------------------------
+ * No counterpart in the reference.  Low-rank adapters of many requests beside a shared
+ * projection whose stacked weights are `slices` (1 to 4) slices of widths[s] rows
+ * (multiples of 8, 65536 together at most) over k inputs (a multiple of 128, 16384 at
+ * most): a bf16 [adapters][slices][rank][k], b bf16 [adapters][sum of widths][rank],
+ * rank a multiple of 8, 128 at most; ranks NULL, or int32 [adapters], each adapter's own
+ * rank (cut to [0, rank]; what stands behind it is not used); scales NULL (1), or fp32
+ * [adapters].  1 to 4096 adapters; a and b 16-byte aligned. */
+typedef struct {
+  const void* a;
+  const void* b;
+  const void* ranks;
+  const void* scales;
+  unsigned adapters;
+  unsigned rank;
+  unsigned k;
+  unsigned slices;
+  unsigned widths[4];
+} qwen36_adapters;
+
+/* qwen36_adapter_plan: the rows of a batch by adapter, for any number of
+ * qwen36_adapter_apply calls with the same seqs, tokens and adapters: sequence i, rows
+ * [cu_tokens[i], cu_tokens[i+1]) cut to the call's rows, has adapter adapter_ids[i]
+ * (int32; one outside [0, adapters): none).  plan: qwen36_adapter_plan_bytes(...) bytes,
+ * 16-byte aligned.  Nothing in device memory can make a launch read or write out of
+ * bounds; rows of sequences that overlap are any of theirs or left as they were. */
+size_t qwen36_adapter_plan_bytes(unsigned seqs, unsigned tokens, unsigned adapters);
+int qwen36_adapter_plan(const void* cu_tokens, const void* adapter_ids, unsigned seqs, unsigned tokens,
+                        unsigned adapters, void* plan, size_t plan_bytes, void* stream);
+
+/* qwen36_adapter_apply: for every row with an adapter and every slice
+ * y = bf16(y + scale (x a^T) b^T), x [tokens, k], y [tokens, sum of widths] bf16 in
+ * place, row strides multiples of 8, 16-byte aligned.  Sums are fp32; x a^T, times the
+ * scale, enters the second product as the sum of two bf16 values (2^-17 of it).
+ * workspace of qwen36_adapter_workspace_bytes(...) bytes, 16-byte aligned; calls that
+ * overlap on one workspace race. */
+size_t qwen36_adapter_workspace_bytes(const qwen36_adapters* adapters, unsigned seqs, unsigned tokens);
+int qwen36_adapter_apply(const void* x, size_t x_row_stride, void* y, size_t y_row_stride,
+                         const qwen36_adapters* adapters, const void* plan, size_t plan_bytes,
+                         unsigned seqs, unsigned tokens, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
 #ifdef __cplusplus
 }
 #endif
