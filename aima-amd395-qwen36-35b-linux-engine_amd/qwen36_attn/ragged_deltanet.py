@@ -67,8 +67,8 @@ def _heads(t, name: str, tokens: int, heads: tuple, index: int) -> int:
         raise ValueError(f"{name} must be [{tokens}, {' or '.join(map(str, heads))}, 128]")
     width = t.shape[1] * DK
     stride = t.stride(0) if tokens > 1 else width
-    if t.stride(2) != 1 or t.stride(1) != DK or not width <= stride < 1 << 32 or stride % 8 or t.data_ptr() % 16:
-        raise ValueError(f"{name} must have contiguous, 16-byte aligned rows that do not overlap")
+    if t.stride(2) != 1 or t.stride(1) != DK or not width <= stride <= 1 << 24 or stride % 8 or t.data_ptr() % 16:
+        raise ValueError(f"{name} must have contiguous, 16-byte aligned rows, apart by 2^24 elements at most")
     return stride
 
 

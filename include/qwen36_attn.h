@@ -618,8 +618,8 @@ int qwen36_gdn_ragged_conv1d(const void* x, unsigned x_row_stride, const void* w
 
 /* qwen36_gdn_ragged_delta: the gated delta rule for a batch (qwen36_gdn_recurrent's
  * and qwen36_gdn_chunk_prefill's tensors): q, k [tokens, qk_heads (16 | 32), 128],
- * v [tokens, 32, 128] bf16 with token strides (multiples of 8), g, beta fp32
- * [tokens, 32], out bf16 [tokens, 32, 128]; states fp32 [num_slots][32][128 k][128 v],
+ * v [tokens, 32, 128] bf16 with token strides (multiples of 8, at most 2^24), g, beta
+ * fp32 [tokens, 32], out bf16 [tokens, 32, 128]; states fp32 [num_slots][32][128 k][128 v],
  * slots slot_stride elements (a multiple of 4) apart, replaced by the sequences' last
  * states.  longest: 0, or the most rows that a sequence has as the host knows it; it
  * only chooses the launches, a sequence may have more.  Pointers 16-byte aligned (g and

@@ -34,6 +34,13 @@ def test_bad_batches(lib, bad):  # noqa: F811
     assert lib.qwen36_gdn_ragged_delta_workspace_bytes(batch(**bad), 0) == 0
 
 
+def test_delta_workspace(lib):  # noqa: F811
+    """None where no sequence can be long, or is said to be."""
+    of = lib.qwen36_gdn_ragged_delta_workspace_bytes
+    assert of(batch(seqs=64, tokens=12), 0) == 0 and of(batch(seqs=64, tokens=500), 1) == 0
+    assert of(batch(seqs=64, tokens=500), 0) == of(batch(seqs=64, tokens=500), 200) > 0
+
+
 @pytest.mark.parametrize("change", [{0: None}, {0: 24}, {1: 8184}, {1: 8196}, {2: None}, {2: 8}, {3: None}, {3: 8},
                                     {4: 24568}, {4: 24580}, {5: None}, {6: None}, {6: 8}])
 def test_conv_refuses(lib, change):  # noqa: F811
@@ -44,10 +51,11 @@ def test_conv_refuses(lib, change):  # noqa: F811
 
 
 @pytest.mark.parametrize("change", [{0: None}, {1: None}, {2: None}, {0: 8}, {1: 8}, {2: 8}, {3: 8}, {3: 17}, {3: 32},
-                                    {4: 2040}, {4: 2052}, {5: 4088}, {5: 4100}, {6: None}, {7: None}, {8: None}, {8: 8},
-                                    {9: 32 * 128 * 128 - 4}, {9: 32 * 128 * 128 + 2}, {10: None}, {12: None}, {12: 8}])
+                                    {4: 2040}, {4: 2052}, {4: (1 << 24) + 8}, {5: 4088}, {5: 4100}, {5: (1 << 24) + 8}, {6: None}, {7: None}, {8: None}, {8: 8},
+                                    {9: 32 * 128 * 128 - 4}, {9: 32 * 128 * 128 + 2}, {10: None}, {12: None}, {12: 8},
+                                    {13: None}, {13: 8}, {14: 1000}])
 def test_delta_refuses(lib, change):  # noqa: F811
-    args = delta_args(batch())
+    args = delta_args(batch(tokens=90))
     for i, x in change.items():
         args[i] = x
     assert lib.qwen36_gdn_ragged_delta(*args) == 1
