@@ -12,11 +12,13 @@
 //  * down: h = x A^T in fp32, split over K between the waves of a workgroup and, for few
 //    tiles, between workgroups, whose partial sums the second launch adds in order.
 //  * up: y + (scale h) B^T, rounded to bf16 once.  h enters the bf16 products as the sum
-//    of two bf16 values (2^-17 of it), both in one product: the reduction index runs over
-//    [high rank | low rank] against B twice, so that rank 16 fills one 16x16x32.
+//    of two bf16 values (2^-17 of it).
 // Results depend neither on the order of the requests nor on the tile: a row of a
 // product is computed the same in whatever row of a tile it stands.
+#include "gemm_tile.h"
 #include "paged_common.h"
+
+#include <mutex>
 
 namespace q36 {
 namespace {
@@ -126,22 +128,26 @@ __device__ __forceinline__ bool plan_tile(const Plan& p, unsigned i, unsigned to
 
 // ---- down: h = x A^T ----------------------------------------------------------
 
+constexpr int kDownPitch = 68;
+
 // Workgroup: (tile, slice, 64 of the rank's rows, part of K); its waves a quarter of the
-// part each.  h: [part][place][slice][rank] fp32.
-template <int kTiles>     // of 16 rows
-__global__ __launch_bounds__(256) void adapter_down_kernel(const bf16* __restrict__ x, size_t ldx, Adapters w, Plan p,
+// part each.  h: [part][place][slice][rank] fp32, or, where K is in one part, what the
+// second launch reads as operands: [tile][slice][16 rows][32 of the rank][high, low][lane].
+template <int kTiles, bool kFinal>     // tiles of 16 rows
+__global__ __launch_bounds__(256, 2) void adapter_down_kernel(const bf16* __restrict__ x, size_t ldx, Adapters w, Plan p,
                                                            unsigned tokens, unsigned parts, float* __restrict__ h) {
-  constexpr int kPitch = 68;
-  __shared__ float red[3][16 * kTiles][kPitch];
+  constexpr int kPitch = kDownPitch;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  auto red = reinterpret_cast<float(*)[16 * kTiles][kPitch]>(smem);
   const unsigned groups = (w.rank + 63) / 64;
-  unsigned b = blockIdx.x;
+  // what reads the same rows of x is on one XCD
+  const unsigned each = parts * groups * w.slices, tile = (blockIdx.x >> 3) / each * 8 + (blockIdx.x & 7);
+  unsigned b = (blockIdx.x >> 3) % each;
   const unsigned part = b % parts;
   b /= parts;
-  const unsigned group = b % groups;
-  b /= groups;
-  const unsigned slice = b % w.slices;
+  const unsigned group = b % groups, slice = b / groups;
   unsigned first, count, id;
-  if (!plan_tile(p, b / w.slices, tokens, w.n, first, count, id)) return;
+  if (!plan_tile(p, tile, tokens, w.n, first, count, id)) return;
   const unsigned rank = adapter_rank(w, (int)id);
   if (64 * group >= rank) return;
   const int nt = (int)min((rank - 64 * group + 15) / 16, 4u);      // 16 rows of A each
@@ -164,62 +170,179 @@ __global__ __launch_bounds__(256) void adapter_down_kernel(const bf16* __restric
   for (int m = 0; m < kTiles; ++m)
 #pragma unroll
     for (int c = 0; c < 4; ++c) acc[m][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (unsigned k = 0; k < len; k += 32) {
-    bf16x8 xv[kTiles], av[4];
+  const unsigned steps = len / 32;
+  // operands are asked for three steps ahead
+  bf16x8 xv[4][kTiles], av[4][4];
+  auto load = [&](int s, unsigned k) {
 #pragma unroll
-    for (int m = 0; m < kTiles; ++m) xv[m] = *reinterpret_cast<const bf16x8*>(xp[m] + k);
+    for (int m = 0; m < kTiles; ++m) xv[s][m] = *reinterpret_cast<const bf16x8*>(xp[m] + k);
 #pragma unroll
     for (int c = 0; c < 4; ++c)
-      if (c < nt) av[c] = *reinterpret_cast<const bf16x8*>(ap[c] + k);
+      if (c < nt) av[s][c] = *reinterpret_cast<const bf16x8*>(ap[c] + k);
+  };
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (c < nt) {
+  for (int s = 0; s < 3; ++s)
+    if ((unsigned)s < steps) load(s, 32 * s);
+#pragma unroll 1
+  for (unsigned n = 0; n < steps; n += 4) {
 #pragma unroll
-        for (int m = 0; m < kTiles; ++m) acc[m][c] = mfma16x16x32(av[c], xv[m], acc[m][c]);
-      }
-  }
-  // lane: h of row li, rank rows 16 c + 4 lg + r
-  if (wave > 0) {
-#pragma unroll
-    for (int m = 0; m < kTiles; ++m)
+    for (int s = 0; s < 4; ++s) {
+      if (n + s >= steps) break;
+      if (n + s + 3 < steps) load((s + 3) & 3, 32 * (n + s + 3));
 #pragma unroll
       for (int c = 0; c < 4; ++c)
-        if (c < nt) *reinterpret_cast<f32x4*>(&red[wave - 1][16 * m + li][16 * c + 4 * lg]) = acc[m][c];
-  }
-  __syncthreads();
-  if (wave > 0) return;
+        if (c < nt) {
 #pragma unroll
-  for (int m = 0; m < kTiles; ++m) {
-    const unsigned row = 16 * m + li;
-    if (row >= count) continue;
-    float* o = h + (((size_t)part * tokens + first + row) * w.slices + slice) * w.rank + 64 * group + 4 * lg;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      if (c >= nt) continue;
-      f32x4 s = acc[m][c];
-#pragma unroll
-      for (int u = 0; u < 3; ++u) s += *reinterpret_cast<const f32x4*>(&red[u][row][16 * c + 4 * lg]);
-      if (64 * group + 16 * c + 4 * lg < w.rank) *reinterpret_cast<f32x4*>(o + 16 * c) = s;
+          for (int m = 0; m < kTiles; ++m) acc[m][c] = mfma16x16x32(av[s][c], xv[s][m], acc[m][c]);
+        }
     }
+  }
+  // lane: h of row li, rank rows 16 c + 4 lg + r
+#pragma unroll
+  for (int m = 0; m < kTiles; ++m)
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (c < nt) *reinterpret_cast<f32x4*>(&red[wave][16 * m + li][16 * c + 4 * lg]) = acc[m][c];
+  __syncthreads();
+  if (kFinal) {
+    // the second launch's operands: 16 rows by 32 of the rank, high and low parts
+    const float scale = w.scales != nullptr ? w.scales[id] : 1.0f;
+    const unsigned nk = (w.rank + 31) / 32;
+    bf16x8* o = reinterpret_cast<bf16x8*>(h) + ((size_t)tile * w.slices + slice) * kTiles * nk * 128;
+    for (int it = wave; it < 2 * kTiles; it += 4) {
+      const int m = it >> 1, kb = it & 1;
+      if (64 * group + 32 * kb >= rank) continue;
+      f32x4 s[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        s[e] = *reinterpret_cast<const f32x4*>(&red[0][16 * m + li][32 * kb + 8 * lg + 4 * e]);
+#pragma unroll
+        for (int u = 1; u < 4; ++u) s[e] += *reinterpret_cast<const f32x4*>(&red[u][16 * m + li][32 * kb + 8 * lg + 4 * e]);
+      }
+      bf16x8 hi, lo;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float v = 64 * group + 32 * kb + 8 * lg + e < rank ? scale * s[e >> 2][e & 3] : 0.f;
+        hi[e] = f2bf(v);
+        lo[e] = f2bf(v - bf2f(hi[e]));
+      }
+      bf16x8* at = o + ((m * nk + 2 * group + kb) * 2) * 64 + lane;
+      at[0] = hi;
+      at[64] = lo;
+    }
+    return;
+  }
+  for (int it = tid; it < 16 * kTiles * 16; it += 256) {
+    const unsigned row = it >> 4, c = 4 * (it & 15);
+    if (row >= count || 64 * group + c >= rank) continue;
+    f32x4 s = *reinterpret_cast<const f32x4*>(&red[0][row][c]);
+#pragma unroll
+    for (int u = 1; u < 4; ++u) s += *reinterpret_cast<const f32x4*>(&red[u][row][c]);
+    *reinterpret_cast<f32x4*>(h + (((size_t)part * tokens + first + row) * w.slices + slice) * w.rank + 64 * group + c) = s;
+  }
+}
+
+// The same for tiles of 64 rows by a ring of four stages in LDS, filled straight from
+// memory, 128 bytes of a row at a time.  8,190 rows of K = 2048 beside three slices of rank
+// 64: 23.6 us; 36 with operands from memory (adapter_down_kernel<4>, whatever its depth of
+// prefetch and number of workgroups: a load of 16 rows 4 KB apart takes a CU some 80
+// cycles), which is left for rows of x that reach behind 2^31 bytes.  Waves 2 x 2: 32 of
+// the rank's rows by 32 rows of x.
+using DownCfg = GemmCfg<1, 1, 2, 2, 2, 64, 4>;
+
+template <bool kFinal>
+__global__ __launch_bounds__(256, 2) void adapter_down_ring_kernel(const bf16* __restrict__ x, size_t ldx, Adapters w,
+                                                                   Plan p, unsigned tokens, unsigned parts,
+                                                                   float* __restrict__ h) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const unsigned groups = (w.rank + 63) / 64;
+  const unsigned each = parts * groups * w.slices, tile = (blockIdx.x >> 3) / each * 8 + (blockIdx.x & 7);
+  unsigned b = (blockIdx.x >> 3) % each;
+  const unsigned part = b % parts;
+  b /= parts;
+  const unsigned group = b % groups, slice = b / groups;
+  unsigned first, count, id;
+  if (!plan_tile(p, tile, tokens, w.n, first, count, id)) return;
+  const unsigned rank = adapter_rank(w, (int)id);
+  if (64 * group >= rank) return;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wm = wave & 1, wn = wave >> 1, li = lane & 31;
+  const unsigned len = w.k / parts;
+  const u32x4 xr = g_rsrc(x + part * len, (unsigned)((((size_t)tokens - 1) * ldx + len) * 2));
+  const u32x4 ar = g_rsrc(w.a + ((size_t)id * w.slices + slice) * w.rank * w.k + part * len,
+                          ((rank - 1) * w.k + len) * 2);
+  FetchPlan<DownCfg> fp;
+#pragma unroll
+  for (int j = 0; j < DownCfg::Instr; ++j) {
+    const int srow = fetch_stage_row<DownCfg>(wave, j, lane);
+    const unsigned at = fetch_chunk_off<DownCfg>(srow, lane);
+    unsigned off = kGOob;
+    if (srow < 64) {
+      const unsigned r = 64 * group + srow;
+      if (r < rank) off = r * w.k * 2 + at;
+    } else if ((unsigned)(srow - 64) < count) {
+      const unsigned r = (unsigned)p.rows[first + srow - 64];
+      if (r < tokens) off = (unsigned)(r * ldx * 2) + at;
+    }
+    fp.off[j] = off;
+    const bool mine = __builtin_amdgcn_readfirstlane(srow) < 64;     // a wave's rows are of one kind
+    fp.rs[j] = mine ? ar : xr;
+  }
+  f32x16 acc[1][1];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) acc[0][0][e] = 0.f;
+  const int brow[1] = {64 + 32 * wn + li};
+  gemm_mainloop<DownCfg>(smem, fp, (int)len, 32 * wm + li, brow, acc);
+  // lane: row 32 wn + li of the tile, rank rows 64 group + 32 wm + 8 q + 4 kh + r
+  const unsigned row = 32 * wn + li, kh = lane >> 5, r0 = 64 * group + 32 * wm + 4 * kh;
+  if (kFinal) {
+    const float scale = w.scales != nullptr ? w.scales[id] : 1.0f;
+    const unsigned nk = (w.rank + 31) / 32, kb = 2 * group + wm;
+    if (kb >= nk) return;
+    bf16* o = reinterpret_cast<bf16*>(h) + (((size_t)tile * w.slices + slice) * 4 + (row >> 4)) * nk * 1024 + kb * 1024;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      bf16x4 hi, lo;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float v = r0 + 8 * q + r < rank ? scale * acc[0][0][4 * q + r] : 0.f;
+        hi[r] = f2bf(v);
+        lo[r] = f2bf(v - bf2f(hi[r]));
+      }
+      bf16* at = o + (16 * q + (row & 15)) * 8 + 4 * kh;
+      *reinterpret_cast<bf16x4*>(at) = hi;
+      *reinterpret_cast<bf16x4*>(at + 512) = lo;
+    }
+  } else if (row < count) {
+    float* o = h + (((size_t)part * tokens + first + row) * w.slices + slice) * w.rank;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (r0 + 8 * q < w.rank)
+        *reinterpret_cast<f32x4*>(o + r0 + 8 * q) =
+            f32x4{acc[0][0][4 * q], acc[0][0][4 * q + 1], acc[0][0][4 * q + 2], acc[0][0][4 * q + 3]};
   }
 }
 
 // ---- up: y += (scale h) B^T -----------------------------------------------------
 
-constexpr unsigned kUpCols = 256;        // of a workgroup: 64 a wave
+constexpr unsigned kUpCols = 256;        // of a workgroup: 64 a wave, in two halves
 
 // Workgroup: (tile, 256 columns of a slice).  The product is taken transposed (B's rows
 // first), its row 4 j + r standing for column 8 j + 4 u + r of the pair u = 0, 1, so that
-// a lane holds 8 columns in a row of y: 16-byte reads and writes.
-template <int kTiles>
-__global__ __launch_bounds__(256) void adapter_up_kernel(bf16* __restrict__ y, size_t ldy, Adapters w, Plan p,
-                                                         unsigned tokens, unsigned parts, unsigned chunks,
-                                                         const float* __restrict__ h) {
+// a lane holds 8 columns in a row of y: 16-byte reads and writes.  All of y and B's
+// first 64 of the rank are asked for at once; 16 waves a CU hide the rest.
+template <int kTiles, int kParts>
+__global__ __launch_bounds__(256, kTiles == 1 ? 4 : 3) void adapter_up_kernel(bf16* __restrict__ y, size_t ldy, Adapters w, Plan p,
+                                                            unsigned tokens, unsigned chunks,
+                                                            const float* __restrict__ h) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  bf16x8* hs = reinterpret_cast<bf16x8*>(smem);      // [tile of 16][32 of the index][lane]
+  bf16x8* hs = reinterpret_cast<bf16x8*>(smem);      // [tile of 16][32 of the rank][high, low][lane]
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, li = lane & 15, lg = lane >> 4;
+  const unsigned tile = blockIdx.x / chunks;
   unsigned chunk = blockIdx.x % chunks, slice = 0, first, count, id;
-  if (!plan_tile(p, blockIdx.x / chunks, tokens, w.n, first, count, id)) return;
+  if (!plan_tile(p, tile, tokens, w.n, first, count, id)) return;
+  unsigned row[kTiles];
+#pragma unroll
+  for (int m = 0; m < kTiles; ++m) row[m] = (unsigned)p.rows[first + min((unsigned)(16 * m + li), count - 1)];
   const unsigned rank = adapter_rank(w, (int)id);
   if (rank == 0) return;
   while (slice + 1 < w.slices) {
@@ -229,99 +352,113 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(bf16* __restrict__ y, s
     ++slice;
   }
   const unsigned end = w.begin[slice + 1], c0 = w.begin[slice] + chunk * kUpCols + 64 * wave;
-  // y's values of this lane: row 16 m + li, columns c0 + 32 g + 8 lg .. + 7
-  bf16* yp[kTiles];
-  bf16x8 yv[kTiles][2];
+  const unsigned nk = (rank + 31) / 32;
+  const bf16* bp = w.b + (size_t)id * w.total * w.rank;
+  // half g: columns from c0 + 32 g on; what is behind the slice, or a row that is none,
+  // is read from where there is something
+  bf16x8 yv[2][kTiles], bv[2][2][2];
+  auto load_b = [&](int g, unsigned kb, bf16x8 (&o)[2]) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const unsigned col = min(c0 + 32 * g + 8 * (li >> 2) + 4 * u + (li & 3), end - 1);
+      o[u] = *reinterpret_cast<const bf16x8*>(bp + (size_t)col * w.rank + min(32 * kb + 8 * lg, w.rank - 8));
+    }
+  };
 #pragma unroll
   for (int m = 0; m < kTiles; ++m) {
-    const unsigned at = 16 * m + li;
-    const unsigned row = at < count ? (unsigned)p.rows[first + at] : tokens;
-    yp[m] = row < tokens ? y + row * ldy + c0 + 8 * lg : nullptr;
+    const bf16* yr = y + (row[m] < tokens ? row[m] : 0u) * ldy;
 #pragma unroll
     for (int g = 0; g < 2; ++g)
-      if (yp[m] != nullptr && c0 + 32 * g + 8 * lg < end) yv[m][g] = *reinterpret_cast<const bf16x8*>(yp[m] + 32 * g);
+      yv[g][m] = *reinterpret_cast<const bf16x8*>(yr + min(c0 + 32 * g + 8 * lg, end - 8));
   }
-  // the scaled h as two bf16 values: [high, 0 to r8 | low, r8 to 2 r8 | zeros]
-  const unsigned r8 = (rank + 7) & ~7u, nk = (2 * r8 + 31) / 32;
-  const float scale = w.scales != nullptr ? w.scales[id] : 1.0f;
-  const unsigned eights = 4 * nk;
-  for (unsigned it = tid; it < 16 * kTiles * (eights - r8 / 8); it += 256) {
-    const unsigned row = it % (16 * kTiles), j = it / (16 * kTiles);       // 8 of the rank, or zeros
-    bf16x8 hi = {}, lo = {};
-    if (j < r8 / 8 && row < count) {
-      float s[8] = {};
-      for (unsigned q = 0; q < parts; ++q) {
-        const f32x4* hp = reinterpret_cast<const f32x4*>(
-            h + (((size_t)q * tokens + first + row) * w.slices + slice) * w.rank + 8 * j);
-        const f32x4 u = hp[0], v = hp[1];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[e] += u[e];
-          s[4 + e] += v[e];
+  for (int g = 0; g < 2; ++g) {
+    load_b(g, 0, bv[g][0]);
+    if (nk > 1) load_b(g, 1, bv[g][1]);
+  }
+  if constexpr (kParts == 1) {
+    const unsigned full = (w.rank + 31) / 32;
+    const bf16x8* from = reinterpret_cast<const bf16x8*>(h) + ((size_t)tile * w.slices + slice) * kTiles * full * 128;
+    for (unsigned it = tid; it < kTiles * nk * 128; it += 256) {
+      const unsigned m = it / (nk * 128);
+      hs[it] = from[it + m * (full - nk) * 128];
+    }
+  } else {
+    // the scaled h as two bf16 values
+    const float scale = w.scales != nullptr ? w.scales[id] : 1.0f;
+    for (unsigned it = tid; it < 16 * kTiles * 4 * nk; it += 256) {
+      const unsigned hr = it / (4 * nk), j = it % (4 * nk);       // 8 of the rank
+      bf16x8 hi = {}, lo = {};
+      if (8 * j < rank && hr < count) {
+        f32x4 s[kParts][2];
+#pragma unroll
+        for (int q = 0; q < kParts; ++q) {
+          const f32x4* hp = reinterpret_cast<const f32x4*>(
+              h + (((size_t)q * tokens + first + hr) * w.slices + slice) * w.rank + 8 * j);
+          s[q][0] = hp[0];
+          s[q][1] = hp[1];
+        }
+#pragma unroll
+        for (int q = 1; q < kParts; ++q) {
+          s[0][0] += s[q][0];
+          s[0][1] += s[q][1];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float v = 8 * j + e < rank ? scale * s[0][e >> 2][e & 3] : 0.f;
+          hi[e] = f2bf(v);
+          lo[e] = f2bf(v - bf2f(hi[e]));
         }
       }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float v = 8 * j + e < rank ? scale * s[e] : 0.f;
-        hi[e] = f2bf(v);
-        lo[e] = f2bf(v - bf2f(hi[e]));
-      }
-    }
-    auto put = [&](unsigned at, const bf16x8& v) {
-      hs[((row >> 4) * nk + (at >> 2)) * 64 + 16 * (at & 3) + (row & 15)] = v;
-    };
-    if (j < r8 / 8) {
-      put(j, hi);
-      put(r8 / 8 + j, lo);
-    } else {
-      put(r8 / 8 + j, hi);
+      bf16x8* o = hs + (((hr >> 4) * nk + (j >> 2)) * 2) * 64 + 16 * (j & 3) + (hr & 15);
+      o[0] = hi;
+      o[64] = lo;
     }
   }
   __syncthreads();
   if (c0 >= end) return;
-  f32x4 acc[2][2][kTiles];
 #pragma unroll
-  for (int g = 0; g < 2; ++g)
+  for (int g = 0; g < 2; ++g) {
+    f32x4 acc[2][kTiles];
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int m = 0; m < kTiles; ++m) acc[g][u][m] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const bf16* bp = w.b + (size_t)id * w.total * w.rank;
-  for (unsigned kb = 0; kb < nk; ++kb) {
-    const unsigned kk = 32 * kb + 8 * lg, at = kk < r8 ? kk : kk < 2 * r8 ? kk - r8 : 0u;
-    bf16x8 bv[2][2];
+      for (int m = 0; m < kTiles; ++m) acc[u][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto products = [&](unsigned kb, bf16x8 (&b)[2]) {
+      if (32 * kb + 32 > rank) {           // what stands behind the adapter's rank may be anything
 #pragma unroll
-    for (int g = 0; g < 2; ++g)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const unsigned col = min(c0 + 32 * g + 8 * (li >> 2) + 4 * u + (li & 3), end - 1);
-        bv[g][u] = *reinterpret_cast<const bf16x8*>(bp + (size_t)col * w.rank + at);
-        // what stands behind the adapter's rank, or against the zeros, may be anything
-        if (at + 8 > rank || kk >= 2 * r8) {
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            if (at + e >= rank || kk >= 2 * r8) bv[g][u][e] = (bf16)0.f;
-        }
+            if (32 * kb + 8 * lg + e >= rank) b[u][e] = (bf16)0.f;
       }
 #pragma unroll
-    for (int m = 0; m < kTiles; ++m) {
-      const bf16x8 hv = hs[(m * nk + kb) * 64 + lane];
+      for (int m = 0; m < kTiles; ++m) {
+        const bf16x8 hi = hs[((m * nk + kb) * 2) * 64 + lane], lo = hs[((m * nk + kb) * 2 + 1) * 64 + lane];
 #pragma unroll
-      for (int g = 0; g < 2; ++g)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) acc[g][u][m] = mfma16x16x32(bv[g][u], hv, acc[g][u][m]);
+        for (int u = 0; u < 2; ++u) {
+          acc[u][m] = mfma16x16x32(b[u], lo, acc[u][m]);
+          acc[u][m] = mfma16x16x32(b[u], hi, acc[u][m]);
+        }
+      }
+    };
+    products(0, bv[g][0]);
+    if (nk > 1) products(1, bv[g][1]);
+#pragma unroll 1
+    for (unsigned kb = 2; kb < nk; ++kb) {
+      bf16x8 b[2];
+      load_b(g, kb, b);
+      products(kb, b);
     }
-  }
+    const unsigned col = c0 + 32 * g + 8 * lg;
+    if (col >= end) continue;
 #pragma unroll
-  for (int m = 0; m < kTiles; ++m) {
-    if (yp[m] == nullptr) continue;
-#pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      if (c0 + 32 * g + 8 * lg >= end) continue;
+    for (int m = 0; m < kTiles; ++m) {
+      if ((unsigned)(16 * m + li) >= count || row[m] >= tokens) continue;
       bf16x8 o;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] = f2bf(bf2f(yv[m][g][e]) + acc[g][e >> 2][m][e & 3]);
-      *reinterpret_cast<bf16x8*>(yp[m] + 32 * g) = o;
+      for (int e = 0; e < 8; ++e) o[e] = f2bf(bf2f(yv[g][m][e]) + acc[e >> 2][m][e & 3]);
+      *reinterpret_cast<bf16x8*>(y + row[m] * ldy + col) = o;
     }
   }
 }
@@ -354,10 +491,10 @@ bool adapters_of(const qwen36_adapters* p, Adapters& w) {
   return w.total <= 65536;
 }
 
-// Parts of K: for few tiles so many that 512 workgroups share the adapters' reads.
+// Parts of K: for few tiles so many that 256 workgroups share the adapters' reads.
 unsigned k_parts(const Adapters& w, unsigned tiles) {
   unsigned parts = 1;
-  while (parts < 8 && w.k % (256 * parts) == 0 && (size_t)tiles * w.slices * ((w.rank + 63) / 64) * parts < 512)
+  while (parts < 8 && w.k % (256 * parts) == 0 && (size_t)tiles * w.slices * ((w.rank + 63) / 64) * parts < 256)
     parts *= 2;
   return parts;
 }
@@ -394,7 +531,9 @@ Q36_EXPORT size_t qwen36_adapter_workspace_bytes(const qwen36_adapters* adapters
   Adapters w;
   if (!adapters_of(adapters, w) || !batch_ok(seqs, tokens)) return 0;
   const unsigned most = most_tiles(seqs, tokens, w.n);
-  return (size_t)k_parts(w, most) * tokens * w.slices * w.rank * 4;
+  const unsigned parts = k_parts(w, most);
+  if (parts == 1) return (size_t)most * w.slices * tile_rows(tokens) * ((w.rank + 31) / 32) * 128;
+  return (size_t)parts * tokens * w.slices * w.rank * 4;
 }
 
 Q36_EXPORT int qwen36_adapter_apply(const void* x, size_t x_row_stride, void* y, size_t y_row_stride,
@@ -408,6 +547,18 @@ Q36_EXPORT int qwen36_adapter_apply(const void* x, size_t x_row_stride, void* y,
       plan_bytes < qwen36_adapter_plan_bytes(seqs, tokens, w.n) ||
       workspace_bytes < qwen36_adapter_workspace_bytes(adapters, seqs, tokens))
     return Q36_EINVAL;
+  static std::once_flag once;
+  static hipError_t attr = hipSuccess;
+  std::call_once(once, [] {
+    auto allow = [](const void* f, int bytes) {
+      if (attr == hipSuccess) attr = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    };
+    allow(reinterpret_cast<const void*>(adapter_down_kernel<4, true>), 4 * 64 * kDownPitch * 4);
+    allow(reinterpret_cast<const void*>(adapter_down_kernel<4, false>), 4 * 64 * kDownPitch * 4);
+    allow(reinterpret_cast<const void*>(adapter_down_ring_kernel<true>), DownCfg::Lds);
+    allow(reinterpret_cast<const void*>(adapter_down_ring_kernel<false>), DownCfg::Lds);
+  });
+  if (attr != hipSuccess) return static_cast<int>(attr);
   const unsigned most = most_tiles(seqs, tokens, w.n), parts = k_parts(w, most);
   unsigned chunks = 0;
   for (unsigned s = 0; s < w.slices; ++s) chunks += (w.begin[s + 1] - w.begin[s] + kUpCols - 1) / kUpCols;
@@ -417,15 +568,33 @@ Q36_EXPORT int qwen36_adapter_apply(const void* x, size_t x_row_stride, void* y,
   bf16* yb = static_cast<bf16*>(y);
   float* h = static_cast<float*>(workspace);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 down(most * w.slices * ((w.rank + 63) / 64) * parts), up(most * chunks);
-  const unsigned index = (2 * w.rank + 31) / 32 * 1024;      // bytes of 16 rows of h
-  if (tile_rows(tokens) == 16) {
-    hipLaunchKernelGGL(adapter_down_kernel<1>, down, dim3(256), 0, st, xb, x_row_stride, w, p, tokens, parts, h);
-    hipLaunchKernelGGL(adapter_up_kernel<1>, up, dim3(256), index, st, yb, y_row_stride, w, p, tokens, parts, chunks, h);
+  const dim3 down((most + 7) / 8 * 8 * w.slices * ((w.rank + 63) / 64) * parts), up(most * chunks);
+  const unsigned index = (w.rank + 31) / 32 * 2048;      // bytes of 16 rows of h
+  const unsigned tiles16 = tile_rows(tokens) / 16;
+  // a ring's offsets into x are of 31 bits
+  const bool ring = tiles16 == 4 && w.k / parts % 64 == 0 &&
+                    (((size_t)tokens - 1) * x_row_stride + w.k) * 2 <= (size_t)kGOob;
+  const unsigned lds = ring ? DownCfg::Lds : 4 * 16 * tiles16 * kDownPitch * 4;
+  auto launch = [&](auto down_kernel, auto up_kernel) {
+    hipLaunchKernelGGL(down_kernel, down, dim3(256), lds, st, xb, x_row_stride, w, p, tokens, parts, h);
+    hipLaunchKernelGGL(up_kernel, up, dim3(256), tiles16 * index, st, yb, y_row_stride, w, p, tokens, chunks, h);
+  };
+  if (tiles16 == 1) {
+    if (parts == 1) launch(adapter_down_kernel<1, true>, adapter_up_kernel<1, 1>);
+    else if (parts == 2) launch(adapter_down_kernel<1, false>, adapter_up_kernel<1, 2>);
+    else if (parts == 4) launch(adapter_down_kernel<1, false>, adapter_up_kernel<1, 4>);
+    else launch(adapter_down_kernel<1, false>, adapter_up_kernel<1, 8>);
   } else {
-    hipLaunchKernelGGL(adapter_down_kernel<4>, down, dim3(256), 0, st, xb, x_row_stride, w, p, tokens, parts, h);
-    hipLaunchKernelGGL(adapter_up_kernel<4>, up, dim3(256), 4 * index, st, yb, y_row_stride, w, p, tokens, parts,
-                       chunks, h);
+    auto pair = [&](auto up_kernel) {
+      if (parts == 1 && ring) launch(adapter_down_ring_kernel<true>, up_kernel);
+      else if (parts == 1) launch(adapter_down_kernel<4, true>, up_kernel);
+      else if (ring) launch(adapter_down_ring_kernel<false>, up_kernel);
+      else launch(adapter_down_kernel<4, false>, up_kernel);
+    };
+    if (parts == 1) pair(adapter_up_kernel<4, 1>);
+    else if (parts == 2) pair(adapter_up_kernel<4, 2>);
+    else if (parts == 4) pair(adapter_up_kernel<4, 4>);
+    else pair(adapter_up_kernel<4, 8>);
   }
   return static_cast<int>(hipGetLastError());
 }

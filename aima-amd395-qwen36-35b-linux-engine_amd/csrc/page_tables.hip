@@ -296,20 +296,24 @@ struct Remap {            // table == NULL: nothing to remap
   int max_len;
 };
 
+// 32 KB by 256 threads have 8 loads each in flight; the rest of a row goes 4 KB a step.
 __device__ __forceinline__ void copy16(char* to, const char* from, unsigned bytes) {
-  for (unsigned o = threadIdx.x * 16; o < bytes; o += 256 * 16 * 8) {
+  const unsigned o = threadIdx.x * 16;
+  if (bytes == kPiece) {
     u32x4 x[8];
 #pragma unroll
-    for (unsigned u = 0; u < 8; ++u)
-      if (o + u * 4096 < bytes) x[u] = *reinterpret_cast<const u32x4*>(from + o + u * 4096);
+    for (unsigned u = 0; u < 8; ++u) x[u] = *reinterpret_cast<const u32x4*>(from + o + u * 4096);
 #pragma unroll
-    for (unsigned u = 0; u < 8; ++u)
-      if (o + u * 4096 < bytes) *reinterpret_cast<u32x4*>(to + o + u * 4096) = x[u];
+    for (unsigned u = 0; u < 8; ++u) *reinterpret_cast<u32x4*>(to + o + u * 4096) = x[u];
+    return;
   }
+#pragma unroll 1
+  for (unsigned at = o; at < bytes; at += 4096)
+    *reinterpret_cast<u32x4*>(to + at) = *reinterpret_cast<const u32x4*>(from + at);
 }
 
 // Item: (copy, cache, K or V, piece of 32 KB).  No page is both read and written.
-__global__ __launch_bounds__(256) void pages_copy_kernel(CopyCaches cs, unsigned pieces, Moves m, Remap r) {
+__global__ __launch_bounds__(256, 8) void pages_copy_kernel(CopyCaches cs, unsigned pieces, Moves m, Remap r) {
   if (r.table != nullptr) {
     const unsigned n = *r.held;
     for (unsigned i = blockIdx.x; i < r.rows; i += gridDim.x) {
@@ -357,7 +361,7 @@ struct SlotPools {
   unsigned n;
 };
 
-__global__ __launch_bounds__(256) void slots_fork_kernel(SlotPools s, const int* __restrict__ parent, unsigned slots) {
+__global__ __launch_bounds__(256, 8) void slots_fork_kernel(SlotPools s, const int* __restrict__ parent, unsigned slots) {
   const unsigned per = s.first[s.n];
   const unsigned i = blockIdx.x / per;
   unsigned piece = blockIdx.x % per;

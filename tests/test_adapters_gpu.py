@@ -80,6 +80,21 @@ def test_rows(gpu, proj, n, rank, ranks, lens, ids):
         at += m
 
 
+def test_rows_far_apart(gpu):
+    """Rows of x that reach behind 2^31 bytes, in tiles of 64: other loads than where they
+    do not, the same sums to their rounding."""
+    lens, ids, t = [600, 1, 500], [0, 1, 1], 1101
+    a, b, scales, adapters, g = make(gpu, QKV, 2, 64, [64, 17], 4)
+    x, y = (torch.randn(t, n, generator=g, device=gpu).to(BF16) for n in (2048, 9216))
+    far = torch.empty(t * (1 << 20), dtype=BF16, device=gpu).view(t, 1 << 20)[:, :2048]
+    far.copy_(x)
+    batch = ad.AdapterBatch(vector(R.cu_of(lens), gpu), vector(ids, gpu), t, 2)
+    want, slack = expected(y, x, a, b, scales, [64, 17], QKV[1], lens, ids)
+    for rows in (x, far):
+        got = ad.apply_adapters(y.clone(), rows, adapters, batch).double()
+        assert ((got - want).abs() <= 2.0 ** -8 * (want.abs() + slack) + slack).all()
+
+
 def test_no_ranks_and_no_scales(gpu):
     a, b, _, _, g = make(gpu, ODD, 2, 16, [16, 16], 5)
     x, y = (torch.randn(30, n, generator=g, device=gpu).to(BF16) for n in (128, 344))
