@@ -126,6 +126,8 @@ __global__ __launch_bounds__(kBlock) void pages_extend_kernel(Tables t, const in
   __shared__ int until_lds[kRowsInLds];
   int* until = t.rows <= kRowsInLds ? until_lds : until_ws;
   const unsigned tid = threadIdx.x;
+  int r[kPer];
+  read_counts(t.refs, t.pages, 0, r);      // a pool of one step is read once, and before all else
   unsigned need = 0;
   for (unsigned i0 = 0; i0 < t.rows; i0 += kBlock) {
     const unsigned i = i0 + tid;
@@ -151,9 +153,8 @@ __global__ __launch_bounds__(kBlock) void pages_extend_kernel(Tables t, const in
   __syncthreads();
   // free pages: all there are, or as many as are asked for
   unsigned there = 0;
-  int r[kPer];
   for (unsigned at = 0; at < t.pages && there < need; at += kStep) {
-    read_counts(t.refs, t.pages, at, r);
+    if (at > 0) read_counts(t.refs, t.pages, at, r);
     unsigned n = 0, total;
 #pragma unroll
     for (unsigned u = 0; u < kPer; ++u) n += r[u] <= 0;
@@ -163,20 +164,23 @@ __global__ __launch_bounds__(kBlock) void pages_extend_kernel(Tables t, const in
   // give them out: the k-th free page is the k-th that is asked for
   unsigned base = 0;
   for (unsigned at = 0; at < t.pages && base < need; at += kStep) {
-    read_counts(t.refs, t.pages, at, r);
+    if (t.pages > kStep) read_counts(t.refs, t.pages, at, r);
     unsigned n = 0, total;
 #pragma unroll
     for (unsigned u = 0; u < kPer; ++u) n += r[u] <= 0;
     unsigned k = base + block_scan(n, sums, total) - n;
-    // (the scan's barriers stand between the step's reads and the counts written below)
-#pragma unroll
-    for (unsigned u = 0; u < kPer; ++u) {
-      if (r[u] > 0 || k >= need) continue;
-      unsigned lo = 0, hi = t.rows - 1;          // the first row with until > k
+    // the first row with until > k; for the thread's next pages it is this one or one behind
+    unsigned lo = 0, hi = t.rows - 1;
+    if (n > 0 && k < need)
       while (lo < hi) {
         const unsigned mid = (lo + hi) / 2;
         if ((unsigned)until[mid] > k) hi = mid; else lo = mid + 1;
       }
+    // (the scan's barriers stand between the step's reads and the counts written below)
+#pragma unroll
+    for (unsigned u = 0; u < kPer; ++u) {
+      if (r[u] > 0 || k >= need) continue;
+      while ((unsigned)until[lo] <= k) ++lo;
       if ((unsigned)until[lo] <= there) {
         const unsigned before = lo ? (unsigned)until[lo - 1] : 0u;
         const int page = (int)(at + tid * kPer + u);
@@ -222,6 +226,7 @@ __global__ __launch_bounds__(kBlock) void pages_compact_kernel(const int* refs, 
   const unsigned tid = threadIdx.x;
   int r[kPer];
   unsigned n = 0;
+#pragma unroll 1
   for (unsigned at = 0; at < pages; at += kStep) {
     read_counts(refs, pages, at, r);
     unsigned mine = 0, total;
@@ -232,8 +237,9 @@ __global__ __launch_bounds__(kBlock) void pages_compact_kernel(const int* refs, 
     n += total;
   }
   unsigned moved = 0, holes = 0;
+#pragma unroll 1
   for (unsigned at = 0; at < pages; at += kStep) {
-    read_counts(refs, pages, at, r);
+    if (pages > kStep) read_counts(refs, pages, at, r);
     const unsigned p0 = at + tid * kPer;
     unsigned a = 0, h = 0, total;
 #pragma unroll
