@@ -6,6 +6,7 @@
 //   S <- e^g S;  d = beta (v - k S);  S <- S + k (x) d;  o = q S
 // A sequence begins with its slot's state (zeros where it has none) and leaves its
 // last one there.
+#include "gemm_tile.h"
 #include "ragged.h"
 
 #include <mutex>
@@ -27,7 +28,8 @@ struct DeltaArgs {
 
 // ---------------------------------------------------------------------------
 // Token by token: sequences of up to `limit` tokens.
-// Bound by the states' bytes (4.2 MB a sequence, read and written).  Both
+// Bound by the states' bytes (4.2 MB a sequence, read and written: 53 us for 64
+// sequences of a token, 5.1 TB/s).  Both
 // reductions of a token, S^T k and S^T q, are taken of the state before it:
 // o = e^g S_old^T q + d (k.q), so that a token costs one exchange between waves.
 // One workgroup owns 32 columns of a head: thread (rg, cq) rows rg + 32 i and
@@ -129,41 +131,71 @@ __global__ __launch_bounds__(256) void gdn_ragged_step_kernel(DeltaArgs p, Ragge
 // Chunks of 64 tokens: longer sequences.
 //
 // With G the sum of g from the chunk's first token on, S the state before it:
-//   L = strictly lower part of diag(beta) (k k^T) e^(Gi - Gj),  T = (I + L)^-1 diag(beta)
-//   v' = T (v - diag(e^G) k S)
+//   L = strictly lower part of diag(beta) (k k^T) e^(Gi - Gj),  T = (I + L)^-1
+//   v' = T diag(beta) (v - diag(e^G) k S)
 //   o  = diag(e^G) q S + A v',  A = lower part of (q k^T) e^(Gi - Gj)
 //   S <- e^Glast S + k^T diag(e^(Glast - G)) v'
-// The norms of q and k and the decays are row factors in fp32; products are taken of
-// the raw q and k, which bf16 holds.
+// The norms of q and k and the decays are row factors in fp32; products with S are
+// taken of the raw q and k.
 //
-// Precision: an fp32 operand enters bf16 products as the sum of three bf16 values
-// (24 bits together) wherever the state is computed from it: S, v' and the rows
-// v - .. against exact k, six products of T by those rows (all above 2^-24).  What
-// only reaches the output, which is rounded to bf16, takes two (2^-17): S against q,
-// A and v' against each other.
+// Precision.  S, v', its decayed rows and beta (v - ..) are fp32; into products that the
+// state comes from they enter as the sum of two fp16 values (22 bits), each column scaled
+// by a power of two to its largest value, so that what is lost is 2^-23 of it.  k and q (8
+// bits in bf16) are exact in fp16 once a row is scaled by a power of two to a norm of 8 to
+// 16: values below 2^-20 of their row's norm lose bits, 2^-28 of it at most.  T has two
+// such parts (of 2^8 T: what is lost is 2^-33 at least).  With 0 <= beta <= 2 and g <= 0 a
+// column's v' is at most 129 times the largest row that it comes from, and 2^8 of scale
+// keeps it below fp16's range.  A against v', which only the output comes from, takes two
+// bf16 values of each (2^-17 of a term): decays of any size meet there, and rows that
+// are all decayed keep their bits.
+// (Three bf16 parts throughout, which need no scales, take 182 products a chunk and column
+// tile where this takes 132, and 157 us where the scan takes 134.)
 //
-//  * gdn_ragged_prep_kernel, a workgroup a (chunk, head): T and A, which do not
-//    depend on the state, in fp32, and the row factors: a record of 25,600 bytes.
+// Times below are of 13 prompts of 9,903 rows, 161 chunks, the longest of 24.
+//  * gdn_ragged_prep_kernel, a workgroup a (chunk, key head): T and A of its value heads,
+//    which do not depend on the state, as the scan's operands, and the row factors: a
+//    record of 26,368 bytes a value head.  53 us, of which reading q and k once and writing
+//    the records (193 MB) take 43 at 4.5 TB/s; four workgroups a CU hide most of its steps'
+//    latencies (two, with L and T as whole matrices in LDS, took 81 us).
 //  * gdn_ragged_scan_kernel, a workgroup a (sequence, head or part of its columns),
 //    chunk after chunk.  A wave owns 16 columns of v with all 128 rows of their
 //    state, in registers: the layout of a product's result is that of the next one's
 //    right operand, so that nothing of a column's recurrence leaves its wave, and waves
-//    meet once a chunk, where the next chunk's k, q, T and A are ready in LDS.
+//    meet once a chunk, where the next chunk's k, q, v, T and A are ready in LDS.
+//    134 us: a chunk of 8 waves takes 5.4 us, 3.9 without its fetches, of which each SIMD
+//    issues products for 1.8 and vector instructions for 2, and LDS is read for 2.4.
 // ---------------------------------------------------------------------------
+
+typedef _Float16 f16;
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kC = 64;
 constexpr unsigned kShort = 12;           // longer sequences go by chunks
-constexpr int kPitchR = 136;              // bf16 row pitch of [64][128] tiles: 272 bytes
-constexpr int kPitchF = 68;               // fp32 row pitch of [64][64] matrices
+constexpr int kPitchR = 136;              // 16-bit row pitch of [64][128] tiles: 272 bytes
 
-// A record: T and A as fp32 rows (0 .. 31: 32 columns, 32 .. 63: all 64), then
-// e^G / |k|, e^G / (|q| sqrt(128)), e^(Glast - G) / |k| of each token and e^Glast.
-constexpr unsigned kRecM = 32 * 32 + 32 * 64;
-constexpr unsigned kRecS = 2 * kRecM;
-constexpr unsigned kRecFloats = kRecS + 4 * kC;
-constexpr size_t kRecBytes = kRecFloats * 4;
-
-__device__ __forceinline__ unsigned rec_row(unsigned i) { return i < 32 ? 32 * i : 1024 + 64 * (i - 32); }
+// A record.  T and A as operands: tokens 16 i .. by 32 tokens k, lane 16 g + m of row m the
+// columns 32 k + 4 g .. + 3 and 32 k + 16 + 4 g .. + 3, which is how two tiles of a product's
+// result are the right operand of the next; fragments i + k for i < 2, 2 + 2 (i - 2) + k
+// else.  Then the factors of each token.
+constexpr int kFragA = 12, kFrags = 24;   // 2^8 T: high, low of each fragment; then A so, bf16
+enum {
+  kBeta = 0,
+  kBcy = kC,                // beta e^G / |k'|
+  kRsq = 2 * kC,            // e^G / (|q'| sqrt(128))
+  kRsk = 3 * kC,            // 2^-8 e^(Glast - G) / |k'|
+  kScanFactors = 4 * kC,
+  kKs = 4 * kC,             // k' = ks k, q' = qs q
+  kQs = 5 * kC,
+  kEgl = 6 * kC,            // e^Glast
+  kFactors = 7 * kC
+};
+struct Record {
+  f16x8 frag[kFrags * 64];
+  float f[kFactors];
+};
+static_assert(sizeof(Record) == 26368, "record");
 
 // The long sequences are counted in their order; record a_i / 64 + (long sequences before
 // i) + c is chunk c of sequence i: no two meet, as for tiles of rows (ragged.h).
@@ -232,25 +264,48 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* p, unsig
 __device__ __forceinline__ u32x4 load16(const __amdgpu_buffer_rsrc_t& r, unsigned off) {
   return __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, 0);
 }
+__device__ __forceinline__ f32x4 ld4(const float* p) { return *reinterpret_cast<const f32x4*>(p); }
 
+// e^x from the hardware's 2^x: the rounding of x log2(e), and its low bits, come
+// in to first order (2 units of 2^-24 in all; below 2^-126 zero).
+__device__ __forceinline__ float exp_fast(float x) {
+  const float h = x * kLog2e;
+  const float l = __builtin_fmaf(x, kLog2e, -h) + x * 1.925963033500e-08f;
+  const float e = __builtin_amdgcn_exp2f(h);
+  return __builtin_fmaf(e, l * 0.693147180559945f, e);
+}
+
+template <int kHeads>      // value heads of a key head
 struct PrepLds {
   union {
-    bf16 kr[kC * kPitchR];      // k rows; dead once k k^T is in registers
-    float lm[kC * kPitchF];     // L
+    struct {
+      bf16 k[kC * kPitchR], q[kC * kPitchR];
+    } rows;                                      // dead once k k^T and q k^T are in registers
+    struct {
+      float l[kHeads][10][256], t[kHeads][4][256];      // L and T's diagonal, tiles as at `tile_at`
+    } tiles;
   } u;
-  float tm[kC * kPitchF];       // (I + L)^-1; its upper blocks hold sums on the way
-  float gs[kC], gl[kC];         // G = gs + gl: differences of fast decays keep their bits
-  float bs[kC], kinv[kC], qinv[kC];
+  float gs[kHeads][kC], gl[kHeads][kC];         // G = gs + gl: differences of fast decays keep their bits
+  // e^(Gi - Gj) in tiles of 16 below the diagonal: near[i] far[tile of i][j], by the first
+  // token of i's tile
+  float near[kHeads][kC], far[kHeads][3][48];
+  float bs[kHeads][kC];
+  float kinv[kC], qinv[kC];
 };
 
-// C += A B of 16x16 fp32 blocks of [64][kPitchF] matrices.
-__device__ __forceinline__ f32x4 mm16(const float* a, int ar, int ac, const float* b, int br, int bc, f32x4 acc,
-                                      int li, int lg) {
+// A 16x16 tile of a lower matrix, transposed: column c, row r of it.  Four rows of the 16
+// columns, as a product's left operand reads them, lie in different banks.
+__device__ __forceinline__ int tile_at(int c, int r) { return 16 * c + ((r & 12) ^ (c & 12)) + (r & 3); }
+
+// C += A B: A a tile in LDS (transposed, as it is kept), B a product's result.
+__device__ __forceinline__ f32x4 mm16(const float* a, const f32x4& b, f32x4 acc, int li, int lg) {
+  const f32x4 x = *reinterpret_cast<const f32x4*>(a + tile_at(li, 4 * lg));
 #pragma unroll
-  for (int s = 0; s < 4; ++s)
-    acc = mfma16x16x4f32(a[(ar + li) * kPitchF + ac + 4 * s + lg], b[(br + 4 * s + lg) * kPitchF + bc + li], acc);
+  for (int s = 0; s < 4; ++s) acc = mfma16x16x4f32(x[s], b[s], acc);
   return acc;
 }
+
+__device__ __forceinline__ int frag_of(int i, int k) { return i < 2 ? i : 2 * i - 2 + k; }
 
 // Lower 16x16 tile t (0 .. 9): its row and column of tiles.
 __device__ __forceinline__ int tri_row(int t) { return (t >= 1) + (t >= 3) + (t >= 6); }
@@ -259,19 +314,26 @@ __device__ __forceinline__ int tri_col(int t) {
   return t - r * (r + 1) / 2;
 }
 
-__global__ __launch_bounds__(256, 4) void gdn_ragged_prep_kernel(DeltaArgs p, RaggedBatch b, float* __restrict__ ws) {
+// The power of two that brings a row of inverse norm `inv` to a norm of 8 to 16.
+__device__ __forceinline__ float row_scale(float inv) {
+  const int e = min(max((int)(__float_as_uint(inv) >> 23) - 127, -100), 100);
+  return __uint_as_float((unsigned)(e + 127 + 4) << 23);
+}
+
+template <int kHeads>
+__global__ __launch_bounds__(256, 4) void gdn_ragged_prep_kernel(DeltaArgs p, RaggedBatch b, Record* __restrict__ ws) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  PrepLds& s = *reinterpret_cast<PrepLds*>(smem);
-  // the heads of a key head on one XCD, as in the scan
-  const unsigned slot = blockIdx.x >> 3, rec_i = slot >> 2;
-  const int h = 4 * (blockIdx.x & 7) + (slot & 3);
+  PrepLds<kHeads>& s = *reinterpret_cast<PrepLds<kHeads>*>(smem);
+  // a key head's chunks on the XCD where the scan reads their records
+  constexpr unsigned kEach = 4 / kHeads;       // key heads an XCD
+  const unsigned slot = blockIdx.x >> 3, rec_i = slot / kEach;
+  const int kh = kEach * (blockIdx.x & 7) + slot % kEach, h0 = kh * kHeads;
   RaggedSeq q;
   unsigned chunk;
   if (!find_record(b, rec_i, q, chunk)) return;
-  const int kh = h * (int)p.qk_heads / kGdnHv;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, li = lane & 15, lg = lane >> 4;
   const unsigned tok0 = (unsigned)q.a + chunk * kC, rows = min((unsigned)kC, (unsigned)q.z - tok0);
-  float* rec = ws + ((size_t)rec_i * kGdnHv + h) * kRecFloats;
+  Record* rec = ws + (size_t)rec_i * kGdnHv + h0;
   // rows behind the sequence read as zeros
   const unsigned range = ((rows - 1) * p.qk_stride + kGdnDk) * 2;
   const __amdgpu_buffer_rsrc_t qrs = rows_rsrc(p.q + (size_t)tok0 * p.qk_stride + kh * kGdnDk, range);
@@ -284,26 +346,28 @@ __global__ __launch_bounds__(256, 4) void gdn_ragged_prep_kernel(DeltaArgs p, Ra
     k8[i] = __builtin_bit_cast(bf16x8, load16(krs, off));
     q8[i] = __builtin_bit_cast(bf16x8, load16(qrs, off));
   }
-  if (wave < 2) {
-    const float* from = wave == 0 ? p.g : p.beta;
-    const float v = (unsigned)lane < rows ? from[(size_t)(tok0 + lane) * kGdnHv + h] : 0.f;
-    if (wave == 0) {
+  if ((wave & 1) < kHeads) {      // waves 0, 1: G; 2, 3: beta
+    const int hd = wave & 1;
+    const float* from = wave < 2 ? p.g : p.beta;
+    const float v = (unsigned)lane < rows ? from[(size_t)(tok0 + lane) * kGdnHv + h0 + hd] : 0.f;
+    if (wave < 2) {
       double sum = v;
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
         const double u = __shfl_up(sum, o, 64);
         if (lane >= o) sum += u;
       }
-      s.gs[lane] = (float)sum;
-      s.gl[lane] = (float)(sum - (double)(float)sum);
+      s.gs[hd][lane] = (float)sum;
+      s.gl[hd][lane] = (float)(sum - (double)(float)sum);
     } else {
-      s.bs[lane] = v;
+      s.bs[hd][lane] = v;
     }
   }
   float kss = 0.f, qss = 0.f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    *reinterpret_cast<bf16x8*>(&s.u.kr[r1 * kPitchR + 32 * p1 + 8 * i]) = k8[i];
+    *reinterpret_cast<bf16x8*>(&s.u.rows.k[r1 * kPitchR + 32 * p1 + 8 * i]) = k8[i];
+    *reinterpret_cast<bf16x8*>(&s.u.rows.q[r1 * kPitchR + 32 * p1 + 8 * i]) = q8[i];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float kx = bf2f(k8[i][e]), qx = bf2f(q8[i][e]);
@@ -317,148 +381,279 @@ __global__ __launch_bounds__(256, 4) void gdn_ragged_prep_kernel(DeltaArgs p, Ra
   qss += __shfl_xor(qss, 2, 64);
   if (p1 == 0) {
     s.kinv[r1] = 1.0f / sqrtf(kss + 1e-6f);
-    s.qinv[r1] = kQScale / sqrtf(qss + 1e-6f);
+    s.qinv[r1] = 1.0f / sqrtf(qss + 1e-6f);
   }
   lds_barrier();
-  if (tid < kC) {
-    const float gi = s.gs[tid], eg = expf(gi), left = (s.gs[kC - 1] - gi) + (s.gl[kC - 1] - s.gl[tid]);
-    rec[kRecS + tid] = eg * s.kinv[tid];
-    rec[kRecS + kC + tid] = eg * s.qinv[tid];
-    rec[kRecS + 2 * kC + tid] = s.kinv[tid] * expf(left);
-    rec[kRecS + 3 * kC + tid] = expf(s.gs[kC - 1]);
+  auto decay = [&](int hd, int i, int j) { return (s.gs[hd][i] - s.gs[hd][j]) + (s.gl[hd][i] - s.gl[hd][j]); };
+  if (wave < kHeads) {
+    const int hd = wave, i = lane;
+    const float ki = s.kinv[i], qi = s.qinv[i], ks = row_scale(ki), qs = row_scale(qi);
+    const float eg = expf(s.gs[hd][i]), bt = s.bs[hd][i];
+    const float kn = ki / ks, qn = qi / qs;        // by powers of two
+    Record& r = rec[hd];
+    r.f[kBeta + i] = bt;
+    r.f[kBcy + i] = bt * (eg * kn);
+    r.f[kRsq + i] = eg * (qn * kQScale);
+    r.f[kRsk + i] = kn * expf(decay(hd, kC - 1, i)) * 0.00390625f;
+    r.f[kKs + i] = ks;
+    r.f[kQs + i] = qs;
+    r.f[kEgl + i] = expf(s.gs[hd][kC - 1]);
+    s.near[hd][i] = expf(decay(hd, i, i & ~15));
+  } else {
+    for (int n = tid - 64 * kHeads; n < 96 * kHeads; n += 256 - 64 * kHeads) {
+      const int hd = n / 96, at = n % 96, rt = at < 16 ? 1 : at < 48 ? 2 : 3, j = at - (rt == 1 ? 0 : rt == 2 ? 16 : 48);
+      s.far[hd][rt - 1][j] = expf(decay(hd, 16 * rt, j));
+    }
   }
-  // k k^T and q k^T of the lower tiles, five a wave; q straight from memory
-  f32x4 job[5];
+  // k k^T and q k^T of the lower tiles wave, wave + 4, wave + 8, transposed: lane columns
+  // 4 lg + r of row li
+  f32x4 kk[3], qk[3];
 #pragma unroll
-  for (int jj = 0; jj < 5; ++jj) {
-    const int j = wave + 4 * jj, t = j >= 10 ? j - 10 : j, rt = tri_row(t), ct = tri_col(t);
-    const bf16* brow = s.u.kr + (16 * ct + li) * kPitchR + 8 * lg;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    if (j >= 10) {
+  for (int n = 0; n < 3; ++n) {
+    const int t = wave + 4 * n, rt = tri_row(t), ct = tri_col(t);
+    kk[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    qk[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (t >= 10) continue;
+    const int jrow = (16 * ct + li) * kPitchR + 8 * lg, irow = (16 * rt + li) * kPitchR + 8 * lg;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {     // transposed: row 4 lg + r is column j
-        const u32x4 qf = load16(qrs, ((16 * rt + li) * p.qk_stride + 32 * k + 8 * lg) * 2);
-        acc = mfma16x16x32(ld8(brow + 32 * k), __builtin_bit_cast(bf16x8, qf), acc);
+    for (int k = 0; k < 4; ++k) {
+      const bf16x8 kj = ld8(s.u.rows.k + jrow + 32 * k);
+      kk[n] = mfma16x16x32(kj, ld8(s.u.rows.k + irow + 32 * k), kk[n]);
+      qk[n] = mfma16x16x32(kj, ld8(s.u.rows.q + irow + 32 * k), qk[n]);
+    }
+  }
+  lds_barrier();     // the rows make room for L
+#pragma unroll
+  for (int n = 0; n < 3; ++n) {
+    const int t = wave + 4 * n, rt = tri_row(t), ct = tri_col(t);
+    if (t >= 10) continue;
+    const int i = 16 * rt + li, j0 = 16 * ct + 4 * lg;
+    const f32x4 kj = ld4(s.kinv + j0);
+    const float ki = s.kinv[i], qi = s.qinv[i] * kQScale;
+    const int f = frag_of(rt, ct >> 1), at = 16 * lg + li;
+#pragma unroll
+    for (int hd = 0; hd < kHeads; ++hd) {
+      f32x4 d, l;
+      bf16x4 a, al;
+      if (rt == ct) {      // behind the diagonal anything, chosen against below
+#pragma unroll
+        for (int r = 0; r < 4; ++r) d[r] = exp_fast(decay(hd, i, j0 + r));
+      } else {
+        d = ld4(s.far[hd][rt - 1] + j0) * s.near[hd][i];
       }
-    } else {
-      const bf16* arow = s.u.kr + (16 * rt + li) * kPitchR + 8 * lg;
+      const float bi = s.bs[hd][i];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) acc = mfma16x16x32(ld8(arow + 32 * k), ld8(brow + 32 * k), acc);
-    }
-    job[jj] = acc;
-  }
-  lds_barrier();     // the k rows make room for L
+      for (int r = 0; r < 4; ++r) {
+        l[r] = j0 + r < i ? (((ki * kj[r]) * kk[n][r]) * bi) * d[r] : 0.f;
+        const float av = j0 + r <= i ? ((qi * kj[r]) * qk[n][r]) * d[r] : 0.f;
+        a[r] = f2bf(av);
+        al[r] = f2bf(av - bf2f(a[r]));
+      }
 #pragma unroll
-  for (int jj = 0; jj < 5; ++jj) {
-    const int j = wave + 4 * jj, t = j >= 10 ? j - 10 : j, rt = tri_row(t), ct = tri_col(t);
-    // decays behind the diagonal may overflow: chosen against, not multiplied by zero
-    if (j >= 10) {
-      const int i = 16 * rt + li, j0 = 16 * ct + 4 * lg;
-      const float gi = s.gs[i], hi = s.gl[i], qi = s.qinv[i];
-      const f32x4 gj = *reinterpret_cast<const f32x4*>(s.gs + j0), hj = *reinterpret_cast<const f32x4*>(s.gl + j0);
-      const f32x4 kj = *reinterpret_cast<const f32x4*>(s.kinv + j0);
-      f32x4 a;
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        a[r] = j0 + r <= i ? ((qi * kj[r]) * job[jj][r]) * expf((gi - gj[r]) + (hi - hj[r])) : 0.f;
-      *reinterpret_cast<f32x4*>(rec + kRecM + rec_row(i) + j0) = a;
-    } else {
-      const int c = 16 * ct + li, i0 = 16 * rt + 4 * lg;
-      const float gj = s.gs[c], hj = s.gl[c], kj = s.kinv[c];
-      const f32x4 gi = *reinterpret_cast<const f32x4*>(s.gs + i0), hi = *reinterpret_cast<const f32x4*>(s.gl + i0);
-      const f32x4 ki = *reinterpret_cast<const f32x4*>(s.kinv + i0);
-      const f32x4 bi = *reinterpret_cast<const f32x4*>(s.bs + i0);
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        s.u.lm[(i0 + r) * kPitchF + c] =
-            c < i0 + r ? (((ki[r] * kj) * job[jj][r]) * bi[r]) * expf((gi[r] - gj) + (hi[r] - hj)) : 0.f;
+      for (int r = 0; r < 4; ++r) s.u.tiles.l[hd][t][tile_at(4 * lg + r, li)] = l[r];
+      bf16x4* to = reinterpret_cast<bf16x4*>(rec[hd].frag + (kFragA + 2 * f) * 64 + at) + (ct & 1);
+      to[0] = a;
+      to[128] = al;
     }
   }
-  // upper tiles that the rows of a record hold: (0, 1) and (2, 3)
+  // the upper tiles (0, 1) and (2, 3), which the operands hold too
   if (tid < 128) {
-    const unsigned i = 32 * (tid >> 6) + li, j0 = 32 * (tid >> 6) + 16 + 4 * lg;
-    *reinterpret_cast<f32x4*>(rec + kRecM + rec_row(i) + j0) = f32x4{0.f, 0.f, 0.f, 0.f};
-    *reinterpret_cast<f32x4*>(rec + rec_row(i) + j0) = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int f = frag_of(2 * (tid >> 6), tid >> 6);
+#pragma unroll
+    for (int hd = 0; hd < kHeads; ++hd) {
+      f16x4* to = reinterpret_cast<f16x4*>(rec[hd].frag + (kFragA + 2 * f) * 64 + lane) + 1;
+      to[0] = f16x4{};
+      to[128] = f16x4{};
+    }
   }
   lds_barrier();
-  // (I + L)^-1: diagonal 16x16 blocks by forward substitution, a block a wave, a column a lane
-  if (lane < 16) {
-    const int d = 16 * wave;
+  // (I + L)^-1: diagonal 16x16 blocks by substitution, a block a wave, a column a lane
+  if (lane < 16 * kHeads) {
+    const int hd = lane >> 4;
+    const float* lm = s.u.tiles.l[hd][wave * (wave + 3) / 2];
     float t[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float acc = 0.f;
+    for (int i = 0; i < 16; ++i) t[i] = i == li ? 1.f : 0.f;
 #pragma unroll
-      for (int m = 0; m < i; ++m) acc += s.u.lm[(d + i) * kPitchF + d + m] * t[m];
-      t[i] = i == lane ? 1.f : i > lane ? -acc : 0.f;
-    }
+    for (int m = 0; m < 15; ++m)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s.tm[(d + i) * kPitchF + d + lane] = t[i];
+      for (int i4 = (m + 1) & 12; i4 < 16; i4 += 4) {
+        const f32x4 x = ld4(lm + tile_at(m, i4));
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (i4 + r > m) t[i4 + r] -= x[r] * t[m];
+      }
+#pragma unroll
+    for (int i = 0; i < 16; i += 4)
+      *reinterpret_cast<f32x4*>(s.u.tiles.t[hd][wave] + tile_at(li, i)) = f32x4{t[i], t[i + 1], t[i + 2], t[i + 3]};
   }
   lds_barrier();
-  // the others by distance: T_ij = -T_ii sum_{j <= k < i} L_ik T_kj; the sum lies in block (j, i)
-  for (int d = 1; d < 4; ++d) {
-    const int bj = wave, bi = wave + d;
-    if (bi < 4) {
-      f32x4 x = {0.f, 0.f, 0.f, 0.f};
-      for (int kb = bj; kb < bi; ++kb) x = mm16(s.u.lm, 16 * bi, 16 * kb, s.tm, 16 * kb, 16 * bj, x, li, lg);
+  // Row i of blocks from the diagonal on, T_ij = -(sum_{j < k <= i} T_ik L_kj) T_jj, transposed:
+  // a wave's results are its next products' right operands, and the record's layout.
 #pragma unroll
-      for (int r = 0; r < 4; ++r) s.tm[(16 * bj + 4 * lg + r) * kPitchF + 16 * bi + li] = x[r];
-      // (a wave's own writes to LDS are read back in order)
-      const f32x4 y = mm16(s.tm, 16 * bi, 16 * bi, s.tm, 16 * bj, 16 * bi, f32x4{0.f, 0.f, 0.f, 0.f}, li, lg);
+  for (int hd = 0; hd < kHeads; ++hd) {
+    const int own = hd == 0 ? wave : 3 - wave;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) s.tm[(16 * bi + 4 * lg + r) * kPitchF + 16 * bj + li] = -y[r];
+    for (int i = 0; i < 4; ++i) {
+      if (own != i) continue;
+      f32x4 x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[i][r] = s.u.tiles.t[hd][i][tile_at(4 * lg + r, li)];
+#pragma unroll
+      for (int j = i - 1; j >= 0; --j) {
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = i; k > j; --k) sum = mm16(s.u.tiles.l[hd][k * (k + 1) / 2 + j], x[k], sum, li, lg);
+        x[j] = -mm16(s.u.tiles.t[hd][j], sum, f32x4{0.f, 0.f, 0.f, 0.f}, li, lg);
+      }
+#pragma unroll
+      for (int k = 0; k < (i < 2 ? 1 : 2); ++k) {
+        f16x8 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float v = x[2 * k + (e >> 2)][e & 3] * 256.0f;
+          hi[e] = (f16)v;
+          lo[e] = (f16)(v - (float)hi[e]);
+        }
+        f16x8* to = rec[hd].frag + 2 * frag_of(i, k) * 64 + lane;
+        to[0] = hi;
+        to[64] = lo;
+      }
     }
-    lds_barrier();
-  }
-  for (int idx = tid; idx < 10 * 64; idx += 256) {
-    const int t = idx >> 6, i = 16 * tri_row(t) + ((idx >> 2) & 15), j0 = 16 * tri_col(t) + 4 * (idx & 3);
-    const f32x4 v = *reinterpret_cast<const f32x4*>(s.tm + i * kPitchF + j0);
-    *reinterpret_cast<f32x4*>(rec + rec_row(i) + j0) = v * *reinterpret_cast<const f32x4*>(s.bs + j0);
   }
 }
 
 // ---- scan --------------------------------------------------------------------
 
-// Products of 32 of the reduction index, as LDS holds their left operands: T and A of
-// token tiles (t, u) (tokens 32 t + 8 (m / 4) + 4 u + m % 4 for row m) by 32 tokens k:
-// fragment 0, 1: (0, u) k = 0; 2 .. 5: (1, u) k = 0, 1.
+__device__ __forceinline__ f32x4 mfma_f16(f16x8 a, f16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+#define kFence __builtin_amdgcn_sched_barrier(0)
+#define kPin(x) asm volatile("" : "+v"(x))
+// Products with `n` vector instructions behind each: `a`, then the reads of LDS, then `b`.
+#define kBeside(a, b, n)                                              \
+  do {                                                                \
+    for (int q_ = 0; q_ < (a); ++q_) {                                \
+      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);                \
+      __builtin_amdgcn_sched_group_barrier(0x2, n, 0);                \
+    }                                                                 \
+    __builtin_amdgcn_sched_group_barrier(0x100, 16, 0);               \
+    for (int q_ = 0; q_ < (b); ++q_) {                                \
+      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);                \
+      __builtin_amdgcn_sched_group_barrier(0x2, n, 0);                \
+    }                                                                 \
+    kFence;                                                           \
+  } while (0)
+// s_waitcnt: at most n vector-memory operations outstanding.
+constexpr int kVmcnt(int n) { return (n & 15) | ((n >> 4) << 14) | (7 << 4) | (15 << 8); }
+
+// Rows of k', q' and v in LDS: chunk j (8 values) of a row stands at j ^ row_key, so that
+// sixteen rows of one chunk, and what a transposed read takes of four, lie in different banks.
+__device__ __forceinline__ int row_key(int row) { return (row & 3) << 2 | ((row >> 2) & 3); }
+__device__ __forceinline__ int row_at(int row, int chunk) { return row * kGdnDk + 8 * (chunk ^ row_key(row)); }
+
 struct ScanBuf {
-  bf16 kr[kC * kPitchR], qr[kC * kPitchR];
-  bf16x8 tf[6][3][64], af[6][2][64];
-  float sc[4 * kC];
+  float f[kScanFactors];
+  f16x8 frag[kFrags * 64];
+  f16 kr[kC * kGdnDk], qr[kC * kGdnDk];       // k', q'
+  bf16 vr[kC * kGdnDk];                       // v; then the output, which the fetching waves store
 };
+static_assert(sizeof(ScanBuf) % 256 == 0 && offsetof(ScanBuf, kr) % 256 == 0, "rows begin at bank 0");
+
+// Lane i's 16 bytes at byte `off` of the range to `to` + 16 i, without registers.  (The
+// compiler does not see the load: fetches are waited for where the chunk ends.)
+__device__ __forceinline__ void to_lds(const u32x4& range, unsigned off, void* to) {
+  g_fetch((unsigned)(uintptr_t)(__attribute__((address_space(3))) void*)to, (int)off, range);
+}
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
-// x as kParts bf16 values, each of what the ones before leave.
-template <int kParts>
-__device__ __forceinline__ void split8(const f32x4& a, const f32x4& b, bf16x8 (&o)[kParts]) {
+// Eight values times s as the sum of two fp16 values, by conversions of pairs: the form that
+// multiplies, adds and converts one value (which the pin keeps the compiler from) takes twice
+// a vector instruction's time.
+__device__ __forceinline__ void split8(const f32x4& a, const f32x4& b, float s, f16x8& hi, f16x8& lo) {
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const f32x4& v = e < 4 ? a : b;
+    const f32x2 x = {v[e & 2], v[(e & 2) + 1]};
+    const f16x2 h = __builtin_convertvector(x * s, f16x2);
+    float l0 = __builtin_fmaf(x[0], s, -(float)h[0]), l1 = __builtin_fmaf(x[1], s, -(float)h[1]);
+    kPin(l0);
+    kPin(l1);
+    const f16x2 l = __builtin_convertvector(f32x2{l0, l1}, f16x2);
+    hi[e] = h[0];
+    hi[e + 1] = h[1];
+    lo[e] = l[0];
+    lo[e + 1] = l[1];
+  }
+}
+
+// The same as two bf16 values, without a scale.
+__device__ __forceinline__ void split8(const f32x4& a, const f32x4& b, bf16x8& hi, bf16x8& lo) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const f32x4& v = e < 2 ? a : b;
-    float x0 = v[2 * (e & 1)], x1 = v[2 * (e & 1) + 1];
-#pragma unroll
-    for (int n = 0; n < kParts; ++n) {
-      const bf16x2 y = __builtin_convertvector(f32x2{x0, x1}, bf16x2);
-      o[n][2 * e] = y[0];
-      o[n][2 * e + 1] = y[1];
-      const unsigned u = __builtin_bit_cast(unsigned, y);
-      x0 -= __uint_as_float(u << 16);
-      x1 -= __uint_as_float(u & 0xffff0000u);
-    }
+    const float x0 = v[2 * (e & 1)], x1 = v[2 * (e & 1) + 1];
+    const bf16x2 y = __builtin_convertvector(f32x2{x0, x1}, bf16x2);
+    const unsigned u = __builtin_bit_cast(unsigned, y);
+    const bf16x2 z = __builtin_convertvector(f32x2{x0 - __uint_as_float(u << 16), x1 - __uint_as_float(u & 0xffff0000u)}, bf16x2);
+    hi[2 * e] = y[0];
+    hi[2 * e + 1] = y[1];
+    lo[2 * e] = z[0];
+    lo[2 * e + 1] = z[1];
   }
+}
+
+// A column's largest magnitude: over the lane's values and the four lanes of it.
+struct ColumnMax {
+  float top = 0.f;
+  __device__ __forceinline__ void take(const f32x4& x) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) top = __builtin_fmaxf(top, __builtin_fabsf(x[r]));
+  }
+  __device__ __forceinline__ unsigned bits() const {
+    unsigned m = __float_as_uint(top);
+    const auto a = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+    m = max(a[0], a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+    return max(b[0], b[1]);
+  }
+};
+
+// The power of two that brings the value of bits m into [2^to, 2^(to + 1)), and its inverse.
+template <int kTo>
+__device__ __forceinline__ void scale_of(unsigned m, float& s, float& inv) {
+  const int e = min(max((int)(m >> 23), 27), 253) - kTo;      // biased
+  s = __uint_as_float((unsigned)(254 - e) << 23);
+  inv = __uint_as_float((unsigned)e << 23);
+}
+
+// Eight bf16 values times a power of two in fp16.
+__device__ __forceinline__ f16x8 to_f16(const u32x4& x, float s) {
+  f16x8 o;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const f16x2 y =
+        __builtin_convertvector(f32x2{__uint_as_float(x[e] << 16), __uint_as_float(x[e] & 0xffff0000u)} * s, f16x2);
+    o[2 * e] = y[0];
+    o[2 * e + 1] = y[1];
+  }
+  return o;
 }
 
 // kWaves of the workgroup's 8 waves own 16 columns each; where these are not all, the
 // others only fetch.
 template <int kWaves>
 __global__ __launch_bounds__(512, 1) void gdn_ragged_scan_kernel(DeltaArgs p, RaggedBatch b,
-                                                                 const float* __restrict__ ws, unsigned most) {
+                                                                 const Record* __restrict__ ws, unsigned most) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   ScanBuf* buf = reinterpret_cast<ScanBuf*>(smem);
   constexpr unsigned kGroups = 8 / kWaves;
+  constexpr bool kAll = kWaves == 8;
   const unsigned slot = blockIdx.x >> 3, rest = slot >> 2;
   const int h = 4 * (blockIdx.x & 7) + (slot & 3);
   RaggedSeq s;
@@ -466,211 +661,339 @@ __global__ __launch_bounds__(512, 1) void gdn_ragged_scan_kernel(DeltaArgs p, Ra
   if (!find_long(b, rest / kGroups, most, s, rec0)) return;
   const int kh = h * (int)p.qk_heads / kGdnHv;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, li = lane & 15, lg = lane >> 4;
-  const unsigned len = (unsigned)(s.z - s.a), chunks = (len + kC - 1) / kC;
+  const unsigned len = (unsigned)(s.z - s.a), chunks = (len + kC - 1) / kC, last = chunks - 1;
 
-  // ---- fetching: a chunk ahead in registers, then in the other buffer
-  constexpr int kFirst = kWaves < 8 ? 64 * kWaves : 0, kFetch = 512 - kFirst;
-  constexpr int kRowIts = (1024 + kFetch - 1) / kFetch, kFragIts = (384 + kFetch - 1) / kFetch;
-  const bool fetches = tid >= kFirst;
-  const int ft = tid - kFirst;
-  u32x4 fk[kRowIts], fq[kRowIts];
-  f32x4 fT[kFragIts][2], fA[kFragIts][2], fs;
-  auto fetch = [&](unsigned c) {
+  // ---- fetching a chunk ahead, into the other buffer: v, fragments and factors straight
+  // to LDS; k and q, where they become fp16, by way of registers, two chunks ahead.  And what
+  // the chunk two before left of output there goes out.
+  constexpr int kFirst = kAll ? 0 : kWaves, kFetch = 8 - kFirst;      // waves
+  constexpr int kRowIts = (16 + kFetch - 1) / kFetch, kFragIts = (kFrags + 1 + kFetch - 1) / kFetch;
+  const int fw = __builtin_amdgcn_readfirstlane(wave) - kFirst;
+  __builtin_assume(fw < kFetch);
+  u32x4 fk[kRowIts], fq[kRowIts], out[kRowIts];
+  float sk[kRowIts], sq[kRowIts];
+  auto load_kq = [&](unsigned c) {
     const unsigned t0 = (unsigned)s.a + c * kC, rows = min((unsigned)kC, (unsigned)s.z - t0);
+    const Record* rec = ws + (size_t)(rec0 + c) * kGdnHv + h;
     const unsigned range = ((rows - 1) * p.qk_stride + kGdnDk) * 2;
     const __amdgpu_buffer_rsrc_t qrs = rows_rsrc(p.q + (size_t)t0 * p.qk_stride + kh * kGdnDk, range);
     const __amdgpu_buffer_rsrc_t krs = rows_rsrc(p.k + (size_t)t0 * p.qk_stride + kh * kGdnDk, range);
-    const float* rec = ws + ((size_t)(rec0 + c) * kGdnHv + h) * kRecFloats;
 #pragma unroll
-    for (int n = 0; n < kRowIts; ++n) {
-      const unsigned i = ft + n * kFetch;        // behind row 63: behind the range, zeros
-      const unsigned off = ((i >> 4) * p.qk_stride + 8 * (i & 15)) * 2;
+    for (int n = 0; n < kRowIts; ++n) {        // behind row 63: behind the ranges, zeros
+      const unsigned row = 4 * (fw + n * kFetch) + lg, off = (row * p.qk_stride + 8 * li) * 2;
       fk[n] = load16(krs, off);
       fq[n] = load16(qrs, off);
+      sk[n] = rec->f[kKs + (row & 63)];
+      sq[n] = rec->f[kQs + (row & 63)];
     }
-#pragma unroll
-    for (int n = 0; n < kFragIts; ++n) {
-      const unsigned i = min(ft + n * kFetch, 383), f = i >> 6, l = i & 63, m = l & 15;
-      const unsigned row = (f >= 2 ? 32 : 0) + 8 * (m >> 2) + 4 * (f & 1) + (m & 3);
-      const unsigned at = rec_row(row) + (f >= 4 ? 32 : 0) + 8 * (l >> 4);
-      fT[n][0] = *reinterpret_cast<const f32x4*>(rec + at);
-      fT[n][1] = *reinterpret_cast<const f32x4*>(rec + at + 4);
-      fA[n][0] = *reinterpret_cast<const f32x4*>(rec + kRecM + at);
-      fA[n][1] = *reinterpret_cast<const f32x4*>(rec + kRecM + at + 4);
-    }
-    fs = *reinterpret_cast<const f32x4*>(rec + kRecS + 4 * (ft & 63));
   };
-  auto stage = [&](unsigned c) {
+  auto stage_kq = [&](unsigned c) {
     ScanBuf& o = buf[c & 1];
 #pragma unroll
     for (int n = 0; n < kRowIts; ++n) {
-      const int i = ft + n * kFetch, at = (i >> 4) * kPitchR + 8 * (i & 15);
-      if (i < 1024) {
-        *reinterpret_cast<u32x4*>(o.kr + at) = fk[n];
-        *reinterpret_cast<u32x4*>(o.qr + at) = fq[n];
+      const int i = fw + n * kFetch, at = row_at((4 * i + lg) & 63, li);
+      if (i < 16) {
+        *reinterpret_cast<f16x8*>(o.kr + at) = to_f16(fk[n], sk[n]);
+        *reinterpret_cast<f16x8*>(o.qr + at) = to_f16(fq[n], sq[n]);
       }
     }
-#pragma unroll
-    for (int n = 0; n < kFragIts; ++n) {
-      const int i = ft + n * kFetch;
-      if (i < 384) {
-        bf16x8 t3[3], a2[2];
-        split8<3>(fT[n][0], fT[n][1], t3);
-        split8<2>(fA[n][0], fA[n][1], a2);
-#pragma unroll
-        for (int e = 0; e < 3; ++e) o.tf[i >> 6][e][i & 63] = t3[e];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) o.af[i >> 6][e][i & 63] = a2[e];
-      }
-    }
-    if (ft < 64) *reinterpret_cast<f32x4*>(o.sc + 4 * ft) = fs;
   };
-  const unsigned last = chunks - 1;
-  if (fetches) {
-    fetch(0);
-    stage(0);
-    fetch(min(1u, last));
-  }
-  if (kWaves < 8 && wave >= kWaves) {
-    lds_barrier();
-    for (unsigned c = 0; c < chunks; ++c) {
-      if (c < last) {
-        stage(c + 1);
-        fetch(min(c + 2, last));
-      }
-      lds_barrier();
+  // a lane's 16 bytes of a row of the output are those of v that it fetches next
+  const __amdgpu_buffer_rsrc_t ors =
+      rows_rsrc(p.out + ((size_t)s.a * kGdnHv + h) * kGdnDv, ((len - 1) * kGdnHv + 1) * (unsigned)(kGdnDv * 2));
+  auto read_out = [&](unsigned c) {
+#pragma unroll
+    for (int n = 0; n < kRowIts; ++n)
+      out[n] = *reinterpret_cast<const u32x4*>(buf[c & 1].vr + 4 * min(fw + n * kFetch, 15) * kGdnDk + 8 * lane);
+  };
+  auto store_out = [&](unsigned c) {
+#pragma unroll
+    for (int n = 0; n < kRowIts; ++n) {       // rows behind the sequence fall outside the range and are dropped
+      const int i = fw + n * kFetch, row = 4 * i + lg, chunk = li ^ row_key(row);
+      const bool own = i < 16 && (unsigned)chunk / (2 * kWaves) == rest % kGroups;      // the workgroup's columns
+      const unsigned off = own ? (c * kC + row) * (kGdnHv * kGdnDv * 2) + 16 * chunk : ~15u;
+      __builtin_amdgcn_raw_buffer_store_b128(out[n], ors, (int)off, 0, 0);
     }
+  };
+  auto fetch = [&](unsigned c) {
+    const unsigned t0 = (unsigned)s.a + c * kC, rows = min((unsigned)kC, (unsigned)s.z - t0);
+    ScanBuf& o = buf[c & 1];
+    const u32x4 rrs = g_rsrc(ws + (size_t)(rec0 + c) * kGdnHv + h, sizeof(Record));
+#pragma unroll
+    for (int n = 0; n < kFragIts; ++n) {       // (the factors follow the fragments)
+      const int i = fw + n * kFetch;
+      if (i <= kFrags) to_lds(rrs, 1024 * i + 16 * lane, i < kFrags ? (void*)(o.frag + i * 64) : (void*)o.f);
+    }
+    const u32x4 vrs =
+        g_rsrc(p.v + (size_t)t0 * p.v_stride + h * kGdnDv, ((rows - 1) * p.v_stride + kGdnDv) * 2);
+#pragma unroll
+    for (int n = 0; n < kRowIts; ++n) {        // four rows of v; behind the sequence its last again (beta is 0)
+      const int i = fw + n * kFetch, row = 4 * i + lg;
+      if (i < 16)
+        to_lds(vrs, (min((unsigned)row, rows - 1) * p.v_stride + 8 * (li ^ row_key(row))) * 2, o.vr + 4 * i * kGdnDk);
+    }
+  };
+  if (kAll || wave >= kWaves) {
+    load_kq(0);
+    fetch(0);
+    stage_kq(0);
+    load_kq(min(1u, last));
+    __builtin_amdgcn_s_waitcnt(kVmcnt(0));
+  }
+  if (!kAll && wave >= kWaves) {
+    lds_barrier();
+    for (unsigned c = 0; c < chunks; ++c) {      // beside chunk c
+      if (c >= 1) read_out(c - 1);
+      if (c < last) {
+        stage_kq(c + 1);
+        load_kq(min(c + 2, last));
+        __builtin_amdgcn_s_waitcnt(0xC07F);       // what was read of v's place, before v is fetched there
+        fetch(c + 1);
+      }
+      if (c >= 1) {
+        store_out(c - 1);
+        __builtin_amdgcn_s_waitcnt(kVmcnt(kRowIts));      // all but the stores
+      } else {
+        __builtin_amdgcn_s_waitcnt(kVmcnt(0));
+      }
+      lds_barrier();      // chunk c is done with, c + 1 is there
+    }
+    read_out(last);
+    store_out(last);
     return;
   }
 
   // ---- the wave's columns
-  const int col = 16 * ((int)(rest % kGroups) * kWaves + wave) + li;
-  float* sp = p.states + (size_t)s.slot * p.slot_stride + (size_t)h * kGdnDk * kGdnDv + col;
-  // state[2 k + u][r]: row 32 k + 8 lg + 4 u + r
-  f32x4 state[8];
+  const int col0 = 16 * ((int)(rest % kGroups) * kWaves + wave);
+  float* sp = p.states + (size_t)s.slot * p.slot_stride + ((size_t)h * kGdnDk + 8 * lg) * kGdnDv + col0 + li;
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  auto state_row = [&](int i, int r) { return (32 * (i >> 1) + 4 * (i & 1) + r) * kGdnDv; };
+  f32x4 state[8];      // state[2 k + u][r]: row 32 k + 8 lg + 4 u + r
 #pragma unroll
   for (int i = 0; i < 8; ++i)
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      state[i][r] = s.has ? sp[(32 * (i >> 1) + 8 * lg + 4 * (i & 1) + r) * kGdnDv] : 0.f;
-  unsigned short vn[16];
-  auto fetch_v = [&](unsigned c) {
-    const unsigned t0 = (unsigned)s.a + c * kC, rows = min((unsigned)kC, (unsigned)s.z - t0);
-    const __amdgpu_buffer_rsrc_t vrs =
-        rows_rsrc(p.v + (size_t)t0 * p.v_stride + h * kGdnDv, ((rows - 1) * p.v_stride + kGdnDv) * 2);
+    for (int r = 0; r < 4; ++r) state[i][r] = s.has ? sp[state_row(i, r)] : 0.f;
+
+  // The lane's places in the buffer, in bytes: chunk j ^ 4 n of a row is n << 6 away by XOR,
+  // 16 rows 4096 by addition.
+  const int w2 = 2 * (col0 >> 4);
+  unsigned at_row = 256 * li + 16 * (lg ^ row_key(li));                                          // row li, chunk lg
+  unsigned at_kt = 256 * (4 * lg + (li >> 2)) + 16 * ((li & 3) ^ row_key(4 * lg + (li >> 2)));   // row 4 lg + li / 4
+  unsigned at_v = offsetof(ScanBuf, vr) + 256 * (4 * lg + (li >> 2)) +
+                  16 * ((w2 + ((li & 3) >> 1)) ^ row_key(4 * lg + (li >> 2))) + 8 * (li & 1);
+  unsigned at_o = offsetof(ScanBuf, vr) + 256 * (4 * lg) + 16 * ((w2 + (li >> 3)) ^ row_key(4 * lg)) + 2 * (li & 7);
+  unsigned at_f = 16 * lg, at_frag = offsetof(ScanBuf, frag) + 16 * lane;
+  int step = sizeof(ScanBuf);
+  constexpr unsigned kKr = offsetof(ScanBuf, kr), kQr = offsetof(ScanBuf, qr);
+  f16x8 kf[2][4];
+  auto read_rows = [&](unsigned m, int k, f16x8 (&o)[4]) {
+    const char* from = smem + (at_row ^ (k << 6));
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const unsigned row = 32 * (i >> 3) + 8 * lg + (i & 7);
-      vn[i] = __builtin_amdgcn_raw_buffer_load_b16(vrs, (int)((row * p.v_stride + col) * 2), 0, 0);
-    }
+    for (int i = 0; i < 4; ++i) o[i] = *reinterpret_cast<const f16x8*>(from + m + 4096 * i);
   };
-  fetch_v(0);
-  const __amdgpu_buffer_rsrc_t ors =
-      rows_rsrc(p.out + (size_t)s.a * kGdnHv * kGdnDv, len * (unsigned)(kGdnHv * kGdnDv * 2));
-  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-  const int m4 = 8 * (li >> 2) + (li & 3);       // token (or dim) of operand row li, without 32 t + 4 u
+  auto factors = [&](int which, int i) { return *reinterpret_cast<const f32x4*>(smem + at_f + 4 * which + 64 * i); };
+  // fragments 3 part .. of T or A, in their order: tokens 16 i .. by 32 k ..
+  f16x8 fa[6], fb[6];
+  auto read_frags = [&](int first, int part, f16x8 (&o)[6]) {
+#pragma unroll
+    for (int n = 0; n < 6; ++n) o[n] = *reinterpret_cast<const f16x8*>(smem + at_frag + 1024 * (first + 6 * part + n));
+  };
+  auto frag_i = [](int f) { return f < 2 ? f : 2 + ((f - 2) >> 1); };
+  auto frag_k = [](int f) { return f < 2 ? 0 : f & 1; };
+
+  // The chain of a chunk is S -> k S -> rows -> T rows -> decayed v' -> S.  What does not wait
+  // for it (q S, A v', the output, fetches) stands beside products or vector instructions
+  // that would stand alone, and LDS is read a step ahead; fences and group orders hold the
+  // compiler to that.  What still stands alone runs beside the SIMD's other wave.
+  ColumnMax top;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top.take(state[i]);
+  float egl_next = (ws + (size_t)rec0 * kGdnHv + h)->f[kEgl];
+  __builtin_amdgcn_s_waitcnt(kVmcnt(0));       // here, not in every round of the loop
   lds_barrier();
   for (unsigned c = 0; c < chunks; ++c) {
-    const ScanBuf& x = buf[c & 1];
-    if (kWaves == 8 && c < last) {
-      stage(c + 1);
-      fetch(min(c + 2, last));
+    const float egl = egl_next;
+    f16x8 sh[4], sl[4];
+    f32x4 ks[4], qs[4];
+    float ss, si;
+    read_rows(kKr, 0, kf[0]);
+    if (kAll && c >= 1) read_out(c - 1);
+    scale_of<13>(top.bits(), ss, si);
+    split8(state[0], state[1], ss, sh[0], sl[0]);
+    kFence;
+    egl_next = (ws + (size_t)(rec0 + min(c + 1, last)) * kGdnHv + h)->f[kEgl];
+    if (kAll) {
+      __builtin_amdgcn_s_waitcnt(0xC07F);       // what was read of v's place, before v is fetched there
+      if (c < last) fetch(c + 1);
+      if (c >= 1) store_out(c - 1);
     }
-    // k S and q S: tiles (t, u)
-    bf16x8 sb[4][3];
+    // k' S, S in parts
 #pragma unroll
-    for (int k = 0; k < 4; ++k) split8<3>(state[2 * k], state[2 * k + 1], sb[k]);
-    f32x4 ks[4] = {zero, zero, zero, zero}, qs[4] = {zero, zero, zero, zero};
+    for (int k = 0; k < 4; ++k) {
+      read_rows(k < 3 ? kKr : kQr, (k + 1) & 3, kf[(k + 1) & 1]);
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
+      for (int i = 0; i < 4; ++i) ks[i] = mfma_f16(kf[k & 1][i], sl[k], k == 0 ? zero : ks[i]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int at = (32 * (i >> 1) + m4 + 4 * (i & 1)) * kPitchR + 32 * k + 8 * lg;
-        const bf16x8 kf = ld8(x.kr + at), qf = ld8(x.qr + at);
-#pragma unroll
-        for (int e = 2; e >= 0; --e) ks[i] = mfma16x16x32(kf, sb[k][e], ks[i]);
-#pragma unroll
-        for (int e = 1; e >= 0; --e) qs[i] = mfma16x16x32(qf, sb[k][e], qs[i]);
-      }
-    // rows v - e^G k S
-    f32x4 zr[4];
+      for (int i = 0; i < 4; ++i) ks[i] = mfma_f16(kf[k & 1][i], sh[k], ks[i]);
+      if (k < 3) split8(state[2 * k + 2], state[2 * k + 3], ss, sh[k + 1], sl[k + 1]);
+      kBeside(0, 8, 3);
+    }
+    // q' S, rows beta (v - e^G k S)
+    ColumnMax ztop;
+    i16x4 v4[4];
+    f32x4 bt[4], cy[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const f32x4 cy = *reinterpret_cast<const f32x4*>(x.sc + 32 * (i >> 1) + 8 * lg + 4 * (i & 1));
+      v4[i] = lds_read_tr16(reinterpret_cast<const bf16*>(smem + at_v + 4096 * i));
+      bt[i] = factors(kBeta, i);
+      cy[i] = factors(kBcy, i);
+    }
+    kFence;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (k < 3) read_rows(kQr, k + 1, kf[(k + 1) & 1]);
+      if (k >= 2) read_frags(0, k - 2, k == 2 ? fa : fb);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) qs[i] = mfma_f16(kf[k & 1][i], sl[k], k == 0 ? zero : qs[i]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) qs[i] = mfma_f16(kf[k & 1][i], sh[k], qs[i]);
+      cy[k] *= si;
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        zr[i][r] = bf2f(__builtin_bit_cast(bf16, vn[8 * (i >> 1) + 4 * (i & 1) + r])) - cy[r] * ks[i][r];
+        ks[k][r] = __builtin_fmaf(-cy[k][r], ks[k][r],
+                                  bt[k][r] * __uint_as_float((unsigned)(unsigned short)v4[k][r] << 16));
+      ztop.take(ks[k]);
+      kBeside(0, 8, 3);
     }
-    fetch_v(min(c + 1, last));
-    bf16x8 zb[2][3];
+    float zs, zi;
+    f16x8 xh[2], xl[2];
+    scale_of<7>(ztop.bits(), zs, zi);
 #pragma unroll
-    for (int t = 0; t < 2; ++t) split8<3>(zr[2 * t], zr[2 * t + 1], zb[t]);
-    // v' = T rows
-    f32x4 vp[4] = {zero, zero, zero, zero};
+    for (int k = 0; k < 2; ++k) split8(ks[2 * k], ks[2 * k + 1], zs, xh[k], xl[k]);
+    f32x4 rq[4], rk[4];
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int i = 0; i < 4; ++i) {
+      rq[i] = factors(kRsq, i);
+      rk[i] = factors(kRsk, i);
+    }
+    kFence;
+    // v' = T rows, times 2^8 and the rows' scale: low T by high rows, high by low, high by high
+    auto t_rows = [&](int part, const f16x8 (&m)[6]) {
 #pragma unroll
-      for (int i = 2 * k; i < 4; ++i) {
-        const int f = i < 2 ? i : 2 + 2 * k + (i & 1);
-        const bf16x8 t0 = x.tf[f][0][lane], t1 = x.tf[f][1][lane], t2 = x.tf[f][2][lane];
-        vp[i] = mfma16x16x32(t1, zb[k][1], vp[i]);
-        vp[i] = mfma16x16x32(t2, zb[k][0], vp[i]);
-        vp[i] = mfma16x16x32(t0, zb[k][2], vp[i]);
-        vp[i] = mfma16x16x32(t1, zb[k][0], vp[i]);
-        vp[i] = mfma16x16x32(t0, zb[k][1], vp[i]);
-        vp[i] = mfma16x16x32(t0, zb[k][0], vp[i]);
+      for (int n = 0; n < 3; ++n)
+#pragma unroll
+        for (int j = 0; j < 3; ++j) {
+          const int i = frag_i(3 * part + j), k = frag_k(3 * part + j);
+          ks[i] = mfma_f16(m[2 * j + (n == 0)], n == 1 ? xl[k] : xh[k], n == 0 && k == 0 ? zero : ks[i]);
+        }
+    };
+    t_rows(0, fa);
+    if (kAll) stage_kq(c + 1);       // (behind the last chunk of what was, which nothing reads)
+    kBeside(0, 9, 4);
+    if (kAll) load_kq(min(c + 2, last));
+    t_rows(1, fb);
+    read_frags(kFragA, 0, fa);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) qs[i] *= rq[i] * si;
+    kBeside(0, 9, 4);
+    // decayed v', A v'
+    bf16x8 vh[2], vl[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) split8(ks[2 * k], ks[2 * k + 1], vh[k], vl[k]);
+    read_frags(kFragA, 1, fb);
+    kFence;
+    f32x4 av[4];
+    auto a_rows = [&](int part, const f16x8 (&m)[6]) {
+#pragma unroll
+      for (int n = 0; n < 3; ++n)
+#pragma unroll
+        for (int j = 0; j < 3; ++j) {
+          const int i = frag_i(3 * part + j), k = frag_k(3 * part + j);
+          av[i] = mfma16x16x32(__builtin_bit_cast(bf16x8, m[2 * j + (n == 0)]), n == 1 ? vl[k] : vh[k],
+                               n == 0 && k == 0 ? zero : av[i]);
+        }
+    };
+    f16x8 kt[2][4];
+    auto read_kt = [&](int g) {        // rows 64 (g / 2) .. of S, tokens 32 (g % 2) ..
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = 4 * (g >> 1) + j;
+        const bf16* from =
+            reinterpret_cast<const bf16*>(smem + (at_kt ^ ((i >> 1) << 6)) + kKr + 8 * (i & 1) + 8192 * (g & 1));
+        kt[g & 1][j] = __builtin_bit_cast(f16x8, cat_bf16x8(lds_read_tr16(from), lds_read_tr16(from + 2048)));
       }
-    // o = e^G q S + A v'
-    bf16x8 vb[2][2];
+    };
+    ColumnMax wtop;
+    float wsc, wi;
+    a_rows(0, fa);
 #pragma unroll
-    for (int t = 0; t < 2; ++t) split8<2>(vp[2 * t], vp[2 * t + 1], vb[t]);
+    for (int i = 0; i < 4; ++i) {
+      ks[i] *= rk[i];
+      wtop.take(ks[i]);
+    }
+    scale_of<13>(wtop.bits(), wsc, wi);
+    kBeside(0, 9, 5);
+    read_kt(0);
+    a_rows(1, fb);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      qs[i] *= *reinterpret_cast<const f32x4*>(x.sc + kC + 32 * (i >> 1) + 8 * lg + 4 * (i & 1));
+    for (int k = 0; k < 2; ++k) split8(ks[2 * k], ks[2 * k + 1], wsc, xh[k], xl[k]);
+    wi *= zi;
+    kBeside(0, 9, 6);
+    // S <- e^Glast S + k'^T decayed v'; the output e^G q S + A v', in place of the columns' v
+    const float ai = zi * 0.00390625f;
+    top = ColumnMax{};
+    f32x4 up[2][4];
+    auto update = [&](int i) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+      for (int r = 0; r < 4; ++r) state[i][r] = __builtin_fmaf(up[i >> 2][i & 3][r], wi, egl * state[i][r]);
+      top.take(state[i]);
+    };
 #pragma unroll
-      for (int i = 2 * k; i < 4; ++i) {
-        const int f = i < 2 ? i : 2 + 2 * k + (i & 1);
-        const bf16x8 a0 = x.af[f][0][lane], a1 = x.af[f][1][lane];
-        qs[i] = mfma16x16x32(a1, vb[k][0], qs[i]);
-        qs[i] = mfma16x16x32(a0, vb[k][1], qs[i]);
-        qs[i] = mfma16x16x32(a0, vb[k][0], qs[i]);
+    for (int g = 0; g < 4; ++g) {
+      if (g < 3) read_kt(g + 1);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) up[g >> 1][j] = mfma_f16(kt[g & 1][j], xl[g & 1], (g & 1) == 0 ? zero : up[g >> 1][j]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) up[g >> 1][j] = mfma_f16(kt[g & 1][j], xh[g & 1], up[g >> 1][j]);
+#pragma unroll
+      for (int i = 2 * (g & 1); i < 2 * (g & 1) + 2; ++i) {
+        if (g < 2) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            *reinterpret_cast<bf16*>(smem + (at_o ^ (r << 6)) + 256 * r + 4096 * i) =
+                f2bf(__builtin_fmaf(av[i][r], ai, qs[i][r]));
+        } else {
+          update(i);
+        }
       }
-    // S = e^Glast S + k^T e^(Glast - G) v'
-    bf16x8 wb[2][3];
+      kBeside(0, 8, 3);
+    }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      vp[i] *= *reinterpret_cast<const f32x4*>(x.sc + 2 * kC + 32 * (i >> 1) + 8 * lg + 4 * (i & 1));
-#pragma unroll
-    for (int t = 0; t < 2; ++t) split8<3>(vp[2 * t], vp[2 * t + 1], wb[t]);
-    const float egl = x.sc[3 * kC];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) state[i] *= egl;
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const bf16* ra = x.kr + (32 * t + 8 * lg + (li >> 2)) * kPitchR + 32 * (i >> 1) + 8 * (li & 3) + 4 * (i & 1);
-        const bf16x8 kt = cat_bf16x8(lds_read_tr16(ra), lds_read_tr16(ra + 4 * kPitchR));
-#pragma unroll
-        for (int e = 2; e >= 0; --e) state[i] = mfma16x16x32(kt, wb[t][e], state[i]);
-      }
-    // rows behind the sequence fall outside the range and are dropped
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const unsigned row = c * kC + 32 * (i >> 1) + 8 * lg + 4 * (i & 1) + r;
-        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, f2bf(qs[i][r])), ors,
-                                              (int)(((row * kGdnHv + h) * kGdnDv + col) * 2), 0, 0);
-      }
+    for (int i = 4; i < 8; ++i) update(i);
+    if (kAll) __builtin_amdgcn_s_waitcnt(kVmcnt(0));
     lds_barrier();
+    at_row += step;
+    at_kt += step;
+    at_v += step;
+    at_o += step;
+    at_f += step;
+    at_frag += step;
+    step = -step;
+    kPin(at_row);
+    kPin(at_kt);
+    kPin(at_v);
+    kPin(at_o);
+    kPin(at_f);
+    kPin(at_frag);
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) sp[(32 * (i >> 1) + 8 * lg + 4 * (i & 1) + r) * kGdnDv] = state[i][r];
+    for (int r = 0; r < 4; ++r) sp[state_row(i, r)] = state[i][r];
+  if (kAll) {
+    read_out(last);
+    store_out(last);
+  }
 }
 
 // Sequences that can be long, and records for their chunks.
@@ -693,7 +1016,7 @@ using namespace q36;
 Q36_EXPORT size_t qwen36_gdn_ragged_delta_workspace_bytes(const qwen36_state_batch* batch, unsigned longest) {
   RaggedBatch b;
   if (!ragged_batch_of(batch, b) || !by_chunks(b, longest)) return 0;
-  return (size_t)most_records(b) * kGdnHv * kRecBytes;
+  return (size_t)most_records(b) * kGdnHv * sizeof(Record);
 }
 
 Q36_EXPORT int qwen36_gdn_ragged_delta(const void* q, const void* k, const void* v, unsigned qk_heads,
@@ -722,26 +1045,30 @@ Q36_EXPORT int qwen36_gdn_ragged_delta(const void* q, const void* k, const void*
   static std::once_flag once;
   static hipError_t attr = hipSuccess;
   std::call_once(once, [] {
-    const void* scans[] = {reinterpret_cast<const void*>(gdn_ragged_scan_kernel<1>),
-                           reinterpret_cast<const void*>(gdn_ragged_scan_kernel<2>),
-                           reinterpret_cast<const void*>(gdn_ragged_scan_kernel<4>),
-                           reinterpret_cast<const void*>(gdn_ragged_scan_kernel<8>)};
-    for (const void* f : scans)
-      if (attr == hipSuccess)
-        attr = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)(2 * sizeof(ScanBuf)));
-    if (attr == hipSuccess)
-      attr = hipFuncSetAttribute(reinterpret_cast<const void*>(gdn_ragged_prep_kernel),
-                                 hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(PrepLds));
+    auto allow = [](const void* f, size_t bytes) {
+      if (attr == hipSuccess) attr = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    };
+    allow(reinterpret_cast<const void*>(gdn_ragged_scan_kernel<2>), 2 * sizeof(ScanBuf));
+    allow(reinterpret_cast<const void*>(gdn_ragged_scan_kernel<4>), 2 * sizeof(ScanBuf));
+    allow(reinterpret_cast<const void*>(gdn_ragged_scan_kernel<8>), 2 * sizeof(ScanBuf));
+    allow(reinterpret_cast<const void*>(gdn_ragged_prep_kernel<1>), sizeof(PrepLds<1>));
+    allow(reinterpret_cast<const void*>(gdn_ragged_prep_kernel<2>), sizeof(PrepLds<2>));
   });
   if (attr != hipSuccess) return static_cast<int>(attr);
-  float* ws = static_cast<float*>(workspace);
-  hipLaunchKernelGGL(gdn_ragged_prep_kernel, dim3(most_records(b) * kGdnHv), dim3(256), sizeof(PrepLds), st, p, b, ws);
-  // few sequences: their columns in several workgroups, one a CU
+  Record* ws = static_cast<Record*>(workspace);
+  if (qk_heads == 16)
+    hipLaunchKernelGGL(gdn_ragged_prep_kernel<2>, dim3(most_records(b) * 16), dim3(256), sizeof(PrepLds<2>), st, p, b,
+                       ws);
+  else
+    hipLaunchKernelGGL(gdn_ragged_prep_kernel<1>, dim3(most_records(b) * 32), dim3(256), sizeof(PrepLds<1>), st, p, b,
+                       ws);
+  // Few sequences leave CUs, one a workgroup: their columns in two or four.  A chunk takes
+  // 2.2 us of 2 chains a workgroup, 2.6 of 4 and 4.4 of 8; sequences of 2,000 tokens, all in
+  // all, by 2, 4 and 8 chains: 98, 103, 159 us for one, 110, 114, 170 for two, 227, 159, 203
+  // for four, 353, 289, 261 for six.
   const unsigned n = most_long(b);
   const unsigned lds = 2 * sizeof(ScanBuf);
-  if (n <= 1)
-    hipLaunchKernelGGL(gdn_ragged_scan_kernel<1>, dim3(n * kGdnHv * 8), dim3(512), lds, st, p, b, ws, n);
-  else if (n <= 2)
+  if (n <= 2)
     hipLaunchKernelGGL(gdn_ragged_scan_kernel<2>, dim3(n * kGdnHv * 4), dim3(512), lds, st, p, b, ws, n);
   else if (n <= 4)
     hipLaunchKernelGGL(gdn_ragged_scan_kernel<4>, dim3(n * kGdnHv * 2), dim3(512), lds, st, p, b, ws, n);

@@ -118,8 +118,8 @@ def ragged_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torc
                       has_state: torch.Tensor | None = None, out: torch.Tensor | None = None,
                       longest: int | None = None) -> torch.Tensor:
     """The gated delta rule for a batch: q, k [T, 16 (or 32 repeated), 128], v [T, 32,
-    128] bf16 (q and k are l2-normalised in the kernel), g (log decay), beta [T, 32]
-    fp32, states [slots, 32, 128 (k), 128 (v)] fp32, replaced in place by the sequences'
+    128] bf16 (q and k are l2-normalised in the kernel), g (log decay, at most 0), beta (0
+    to 2) [T, 32] fp32, states [slots, 32, 128 (k), 128 (v)] fp32, replaced in place by the sequences'
     last states.  ``longest``: the most rows that a sequence of the call has, where the
     caller knows it; it only chooses between the forms for few and for many tokens (a
     sequence may have more).  Returns [T, 32, 128] bf16."""
