@@ -106,3 +106,29 @@ def apply_adapters(y: torch.Tensor, x: torch.Tensor, adapters: AdapterSet, batch
     launch(index, "qwen36_adapter_apply", xp, xs, yp, ys, adapters._args, batch._plan.data_ptr(), batch._bytes,
            batch.seqs, t, ws.data_ptr(), nb)
     return y
+
+
+class LayerAdapters:
+    """The adapters of a layer's two projections, either of which may be None:
+    ``into`` for the stacked one that its input goes through (q with its gate | k | v;
+    qkv | z | b | a), ``out`` for its o_proj or out_proj, of as many adapters."""
+
+    def __init__(self, into: AdapterSet | None = None, out: AdapterSet | None = None) -> None:
+        if into is None and out is None or into is not None and out is not None and into.adapters != out.adapters:
+            raise ValueError("a layer has adapters of one or both of its projections, as many of each")
+        self.into, self.out = into, out
+
+    def check(self, into: list[int], out: list[int], k: int, inner: int) -> None:
+        """Refuses adapters of other projections than the layer's."""
+        for name, s, widths, n in (("into", self.into, into, k), ("out", self.out, out, inner)):
+            if s is not None and (s.widths != tuple(widths) or s.k != n):
+                raise ValueError(f"{name} must be adapters of slices of {list(widths)} rows over {n} inputs")
+
+
+def project(x: torch.Tensor, w: torch.Tensor, adapters: AdapterSet | None = None,
+            batch: AdapterBatch | None = None) -> torch.Tensor:
+    """x W^T [T, N] bf16, with what the rows' adapters give if there are any."""
+    from .prefill_gemm import linear
+    from .projections import gemv
+    y = gemv(w, x) if x.shape[0] == 1 else linear(x, w)
+    return y if adapters is None or batch is None else apply_adapters(y, x, adapters, batch)

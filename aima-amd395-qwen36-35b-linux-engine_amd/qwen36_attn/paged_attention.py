@@ -326,12 +326,13 @@ class PagedFullAttentionLayer:
     for a ragged batch: the projections, the append, the attention (over selected
     pages if ``budget`` is given) with the output gate, and o_proj.  ``weights`` as
     there, for all of the model's heads; ``rope``: fp32 (cos, sin) tables that reach the
-    longest sequence.  A sequence longer than they or the page table has no tokens: its
+    longest sequence; ``adapters``: an ``adapters.LayerAdapters`` of q | k | v and o_proj.
+    A sequence longer than they or the page table has no tokens: its
     rows are zeros and its pages stay as they are."""
 
     def __init__(self, weights: dict, cache: PagedKVCache,
                  rope: tuple[torch.Tensor, torch.Tensor], budget: int | None = None,
-                 sink_pages: int = 1, recent_pages: int = 1) -> None:
+                 sink_pages: int = 1, recent_pages: int = 1, adapters=None) -> None:
         if cache.kv_heads != HKV:
             raise ValueError(f"the layer has {HKV} KV heads")
         if budget is not None and cache.bounds is None:
@@ -340,14 +341,18 @@ class PagedFullAttentionLayer:
         self.w, self.cache, self.rope = weights, cache, rope
         self.budget, self.sink_pages, self.recent_pages = budget, sink_pages, recent_pages
         self._qkv = FusedProjection(weights["q_proj"], weights["k_proj"], weights["v_proj"])
+        if adapters is not None:
+            adapters.check(self._qkv.splits, [weights["o_proj"].shape[0]], self._qkv.w.shape[1], weights["o_proj"].shape[1])
+        self._into, self._out = (None, None) if adapters is None else (adapters.into, adapters.out)
 
     def forward(self, inp: torch.Tensor, page_table: torch.Tensor, cu_tokens: torch.Tensor,
-                seq_lens: torch.Tensor) -> torch.Tensor:
-        """inp [T, 2048]: the new rows of the batch's sequences.  Returns [T, 2048]."""
-        from .prefill_gemm import linear
-        from .projections import gemv
-        w, one = self.w, inp.shape[0] == 1
-        q_gate, k, v = self._qkv(inp) if one else self._qkv.split_rows(linear(inp, self._qkv.w))
+                seq_lens: torch.Tensor, adapter_batch=None) -> torch.Tensor:
+        """inp [T, 2048]: the new rows of the batch's sequences.  ``adapter_batch``: the
+        ``adapters.AdapterBatch`` of these rows (None: no request has an adapter).  Returns
+        [T, 2048]."""
+        from .adapters import project
+        w = self.w
+        q_gate, k, v = self._qkv.split_rows(project(inp, self._qkv.w, self._into, adapter_batch))
         where = (page_table, cu_tokens, seq_lens)
         q = paged_append(q_gate, k, v, w["q_norm"], w["k_norm"], self.rope, self.cache, *where)
         positions = self.rope[0].shape[0]
@@ -360,4 +365,4 @@ class PagedFullAttentionLayer:
             pages = select_pages(q, self.cache, *where, self.budget, self.sink_pages,
                                  self.recent_pages)
             attn = sparse_paged_attention(q, self.cache, *where, pages, q_gate=q_gate)
-        return gemv(w["o_proj"], attn) if one else linear(attn, w["o_proj"])
+        return project(attn, w["o_proj"], self._out, adapter_batch)

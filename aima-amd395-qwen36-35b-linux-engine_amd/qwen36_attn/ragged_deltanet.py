@@ -173,9 +173,10 @@ class RaggedLinearAttentionLayer:
     LinearAttentionLayer`` for many sequences: the projections, the convolution and the
     delta rule with their states in ``conv_states`` [slots, 8192, 3] bf16 and
     ``ssm_states`` [slots, 32, 128, 128] fp32, the gated norm and out_proj.
-    ``weights`` as there."""
+    ``weights`` as there; ``adapters``: an ``adapters.LayerAdapters`` of in_proj and
+    out_proj."""
 
-    def __init__(self, weights: dict, conv_states: torch.Tensor, ssm_states: torch.Tensor) -> None:
+    def __init__(self, weights: dict, conv_states: torch.Tensor, ssm_states: torch.Tensor, adapters=None) -> None:
         if _pool(conv_states, "conv_states", torch.bfloat16, (CONV_DIM, 3))[:2] \
                 != _pool(ssm_states, "ssm_states", torch.float32, _STATE)[:2]:
             raise ValueError("conv_states and ssm_states must have the same slots on one device")
@@ -183,16 +184,20 @@ class RaggedLinearAttentionLayer:
         self.w, self.conv_states, self.ssm_states = weights, conv_states, ssm_states
         self._in_proj = FusedProjection(weights["in_proj_qkv"], weights["in_proj_z"], weights["in_proj_b"],
                                         weights["in_proj_a"])
+        if adapters is not None:
+            adapters.check(self._in_proj.splits, [weights["out_proj"].shape[0]], self._in_proj.w.shape[1], VALUE_DIM)
+        self._into, self._out = (None, None) if adapters is None else (adapters.into, adapters.out)
 
     def forward(self, inp: torch.Tensor, cu_tokens: torch.Tensor, slots: torch.Tensor,
-                has_state: torch.Tensor | None = None, longest: int | None = None) -> torch.Tensor:
-        """inp [T, 2048]: the new rows of the batch's sequences.  Returns [T, 2048]; rows
-        of padding hold nothing of use."""
+                has_state: torch.Tensor | None = None, longest: int | None = None,
+                adapter_batch=None) -> torch.Tensor:
+        """inp [T, 2048]: the new rows of the batch's sequences.  ``adapter_batch``: the
+        ``adapters.AdapterBatch`` of these rows (None: no request has an adapter).  Returns
+        [T, 2048]; rows of padding hold nothing of use."""
+        from .adapters import project
         from .gated_deltanet import gated_rmsnorm, gating
-        from .prefill_gemm import linear
-        from .projections import gemv
         w, t = self.w, inp.shape[0]
-        mixed, z, b, a = self._in_proj(inp) if t == 1 else self._in_proj.split_rows(linear(inp, self._in_proj.w))
+        mixed, z, b, a = self._in_proj.split_rows(project(inp, self._in_proj.w, self._into, adapter_batch))
         conv = ragged_conv1d(mixed, w["conv1d"], self.conv_states, cu_tokens, slots, has_state)
         q = conv[:, :KEY_DIM].view(t, HK, DK)
         k = conv[:, KEY_DIM:2 * KEY_DIM].view(t, HK, DK)
@@ -200,4 +205,4 @@ class RaggedLinearAttentionLayer:
         g, beta = gating(a, b, w["A_log"], w["dt_bias"])
         core = ragged_delta_rule(q, k, v, g, beta, self.ssm_states, cu_tokens, slots, has_state, longest=longest)
         gated = gated_rmsnorm(core, z, w["norm"])
-        return gemv(w["out_proj"], gated.view(1, VALUE_DIM)) if t == 1 else linear(gated, w["out_proj"])
+        return project(gated.view(t, VALUE_DIM), w["out_proj"], self._out, adapter_batch)
