@@ -15,9 +15,10 @@ def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-# torch.cuda.current_stream(device).cuda_stream without the Stream object (1.9 us a call)
+# torch.cuda.current_stream(device).cuda_stream without the Stream object (1.9 us a call),
+# torch.cuda.current_device() where a GPU tensor is at hand (0.5 us)
 _raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch.cuda.current_device
+_current_device = torch._C._cuda_getDevice
 
 
 def launch(index: int, name: str, *args) -> None:

@@ -69,11 +69,15 @@ def _caches(caches, refs):
     if not caches or not all(isinstance(c, PagedKVCache) for c in caches):
         raise ValueError("caches must be one or more PagedKVCache")
     page, pages = caches[0].page_tokens, refs.shape[0] if isinstance(refs, torch.Tensor) and refs.dim() else 0
-    if any(c.page_tokens != page or c.num_pages != pages or c.device != refs.device for c in caches):
-        raise ValueError("the caches must have the pages that refs counts, of one size, on its device")
-    if len({c._args.k_pages for c in caches} | {c._args.v_pages for c in caches}) < 2 * len(caches):
+    seen = set()
+    for c in caches:
+        if c.page_tokens != page or c.num_pages != pages or c.device != refs.device:
+            raise ValueError("the caches must have the pages that refs counts, of one size, on its device")
+        seen.add(c._args.k_pages)
+        seen.add(c._args.v_pages)
+    if len(seen) < 2 * len(caches):
         raise ValueError("a cache is listed twice")
-    return (_lib.PagedCacheArgs * len(caches))(*(c._args for c in caches)), page
+    return (_lib.PagedCacheArgs * len(caches))(*[c._args for c in caches]), page
 
 
 def trim(refs: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor, keep: torch.Tensor,

@@ -22,22 +22,22 @@ from ._tensors import launch
 from .full_attention import MAX_TOKENS
 from .gated_deltanet import CONV_DIM, DK, DV, HK, HV, KEY_DIM, VALUE_DIM
 
-_STATE = (HV, DK, DV)
+_STATE, _CONV = ((HV, DK, DV), (DK * DV, DV, 1)), ((CONV_DIM, 3), (3, 1))     # a slot's shape and strides
 
 
-def _pool(t, name: str, dtype, shape: tuple) -> tuple[int, int, int, int]:
-    """Device index, slots, address and slot stride in elements of a [slots, ...] pool."""
+def _pool(t, name: str, dtype, shape: tuple, strides: tuple) -> tuple[int, int, int, int]:
+    """Device index, slots, address and slot stride in elements of a [slots, ...] pool
+    whose slots have ``strides``."""
     if not isinstance(t, torch.Tensor) or t.dtype is not dtype or not t.is_cuda:
         raise ValueError(f"{name} must be a {dtype} GPU tensor")
-    if t.dim() != len(shape) + 1 or t.shape[1:] != shape or t.shape[0] < 1:
+    size, step, at = t.shape, t.stride(), t.data_ptr()
+    if len(size) != len(shape) + 1 or size[1:] != shape or size[0] < 1:
         raise ValueError(f"{name} must be [slots, {', '.join(map(str, shape))}]")
-    n, least = t.shape[0], shape[0]
-    for m in shape[1:]:
-        least *= m
-    stride = t.stride(0) if n > 1 else least
-    if not t[0].is_contiguous() or stride < least or stride * t.element_size() % 16 or t.data_ptr() % 16:
+    n, least = size[0], shape[0] * strides[0]
+    stride = step[0] if n > 1 else least
+    if step[1:] != strides or stride < least or (stride * t.itemsize | at) & 15:
         raise ValueError(f"{name}: a slot must be contiguous, 16-byte aligned and apart from the others")
-    return t.get_device(), n, t.data_ptr(), stride
+    return t.get_device(), n, at, stride
 
 
 def _batch(index: int, tokens: int, n_slots: int, cu_tokens, slots, has_state) -> _lib.StateBatchArgs:
@@ -46,30 +46,35 @@ def _batch(index: int, tokens: int, n_slots: int, cu_tokens, slots, has_state) -
                 or t.dim() != 1 or not t.is_contiguous():
             raise ValueError("cu_tokens [seqs + 1] and slots [seqs] must be contiguous int32 tensors "
                              "on the pool's device")
-    seqs = slots.shape[0]
-    if cu_tokens.shape[0] != seqs + 1 or not 1 <= seqs <= 65536:
+    seqs = len(slots)
+    if len(cu_tokens) != seqs + 1 or not 1 <= seqs <= 65536:
         raise ValueError("a batch is cu_tokens [seqs + 1] and slots [seqs] of 1 to 65536 sequences")
-    if has_state is not None and (not isinstance(has_state, torch.Tensor) or has_state.dtype is not torch.bool
-                                  or has_state.get_device() != index or has_state.shape != (seqs,)
-                                  or not has_state.is_contiguous()):
-        raise ValueError("has_state must be a contiguous bool tensor [seqs] on the pool's device")
+    has = None
+    if has_state is not None:
+        if not isinstance(has_state, torch.Tensor) or has_state.dtype is not torch.bool \
+                or has_state.get_device() != index or has_state.shape != (seqs,) or not has_state.is_contiguous():
+            raise ValueError("has_state must be a contiguous bool tensor [seqs] on the pool's device")
+        has = has_state.data_ptr()
     if not 0 < tokens <= MAX_TOKENS:
         raise ValueError(f"a call has 1 to {MAX_TOKENS} rows")
-    return _lib.StateBatchArgs(cu_tokens.data_ptr(), slots.data_ptr(),
-                               None if has_state is None else has_state.data_ptr(), seqs, tokens, n_slots)
+    return _lib.StateBatchArgs(cu_tokens.data_ptr(), slots.data_ptr(), has, seqs, tokens, n_slots)
 
 
-def _heads(t, name: str, tokens: int, heads: tuple, index: int) -> int:
-    """Token stride of a bf16 [tokens, heads, 128] tensor with contiguous rows."""
+def _heads(t, name: str, tokens: int, heads: tuple, index: int) -> tuple[int, int, int]:
+    """Address, heads and token stride of a bf16 [tokens, heads, 128] tensor with
+    contiguous rows."""
     if not isinstance(t, torch.Tensor) or t.dtype is not torch.bfloat16 or t.get_device() != index:
         raise ValueError(f"{name} must be a bf16 tensor on the pool's device")
-    if t.dim() != 3 or t.shape[0] != tokens or t.shape[1] not in heads or t.shape[2] != DK:
+    size = t.shape
+    if len(size) != 3 or size[0] != tokens or size[1] not in heads or size[2] != DK:
         raise ValueError(f"{name} must be [{tokens}, {' or '.join(map(str, heads))}, 128]")
-    width = t.shape[1] * DK
-    stride = t.stride(0) if tokens > 1 else width
-    if t.stride(2) != 1 or t.stride(1) != DK or not width <= stride <= 1 << 24 or stride % 8 or t.data_ptr() % 16:
+    at, (stride, head, inner) = t.data_ptr(), t.stride()
+    width = size[1] * DK
+    if tokens == 1:
+        stride = width
+    if inner != 1 or head != DK or not width <= stride <= 1 << 24 or stride & 7 or at & 15:
         raise ValueError(f"{name} must have contiguous, 16-byte aligned rows, apart by 2^24 elements at most")
-    return stride
+    return at, size[1], stride
 
 
 def _scalars(t, name: str, tokens: int, index: int) -> int:
@@ -95,20 +100,22 @@ def ragged_conv1d(mixed_qkv: torch.Tensor, weight: torch.Tensor, states: torch.T
     [T, 8192] bf16 (unit inner stride), weight [8192, 4] bf16, states [slots, 8192, 3]
     bf16, replaced in place by each sequence's last three inputs.  Returns SiLU(conv)
     [T, 8192] bf16."""
-    index, n, sp, ss = _pool(states, "states", torch.bfloat16, (CONV_DIM, 3))
+    index, n, sp, ss = _pool(states, "states", torch.bfloat16, *_CONV)
     t = mixed_qkv.shape[0] if isinstance(mixed_qkv, torch.Tensor) and mixed_qkv.dim() == 2 else 0
     if t == 0 or mixed_qkv.dtype is not torch.bfloat16 or mixed_qkv.get_device() != index \
             or mixed_qkv.shape[1] != CONV_DIM:
         raise ValueError("mixed_qkv must be bf16 [T, 8192] on the pool's device")
-    stride = mixed_qkv.stride(0) if t > 1 else CONV_DIM
-    if mixed_qkv.stride(1) != 1 or not CONV_DIM <= stride < 1 << 32 or stride % 8 or mixed_qkv.data_ptr() % 16:
+    at, (stride, inner) = mixed_qkv.data_ptr(), mixed_qkv.stride()
+    if t == 1:
+        stride = CONV_DIM
+    if inner != 1 or not CONV_DIM <= stride < 1 << 32 or stride & 7 or at & 15:
         raise ValueError("mixed_qkv must have unit inner stride and 16-byte aligned rows that do not overlap")
     if not isinstance(weight, torch.Tensor) or weight.dtype is not torch.bfloat16 or weight.get_device() != index \
-            or weight.shape != (CONV_DIM, 4) or not weight.is_contiguous() or weight.data_ptr() % 16:
+            or weight.shape != (CONV_DIM, 4) or not weight.is_contiguous() or weight.data_ptr() & 15:
         raise ValueError("weight must be contiguous bf16 [8192, 4] on the pool's device")
     batch = _batch(index, t, n, cu_tokens, slots, has_state)
     out = _out(out, (t, CONV_DIM), states.device)
-    launch(index, "qwen36_gdn_ragged_conv1d", mixed_qkv.data_ptr(), stride, weight.data_ptr(), sp, ss, batch,
+    launch(index, "qwen36_gdn_ragged_conv1d", at, stride, weight.data_ptr(), sp, ss, batch,
            out.data_ptr())
     return out
 
@@ -123,22 +130,22 @@ def ragged_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torc
     last states.  ``longest``: the most rows that a sequence of the call has, where the
     caller knows it; it only chooses between the forms for few and for many tokens (a
     sequence may have more).  Returns [T, 32, 128] bf16."""
-    index, n, sp, ss = _pool(states, "states", torch.float32, _STATE)
+    index, n, sp, ss = _pool(states, "states", torch.float32, *_STATE)
     t = v.shape[0] if isinstance(v, torch.Tensor) and v.dim() == 3 else 0
-    qs, ks = _heads(q, "q", t, (HK, HV), index), _heads(k, "k", t, (HK, HV), index)
-    if q.shape != k.shape or qs != ks:
+    (qp, heads, qs), (kp, *same) = _heads(q, "q", t, (HK, HV), index), _heads(k, "k", t, (HK, HV), index)
+    if same != [heads, qs]:
         raise ValueError("q and k must share shape and token stride")
-    vs = _heads(v, "v", t, (HV,), index)
+    vp, _, vs = _heads(v, "v", t, (HV,), index)
     gp, bp = _scalars(g, "g", t, index), _scalars(beta, "beta", t, index)
     if longest is not None and longest < 1:
         raise ValueError("longest must be positive")
     batch = _batch(index, t, n, cu_tokens, slots, has_state)
     out = _out(out, (t, HV, DV), states.device)
     most = min(longest or 0, MAX_TOKENS)
-    nb = (_lib._LIB or _lib.load()).qwen36_gdn_ragged_delta_workspace_bytes(batch, most)
+    nb = 0 if t == 1 else (_lib._LIB or _lib.load()).qwen36_gdn_ragged_delta_workspace_bytes(batch, most)
     # allocated per call: calls on several streams, and graphs captured apart, never share one
     ws = torch.empty(nb, dtype=torch.uint8, device=states.device) if nb else None
-    launch(index, "qwen36_gdn_ragged_delta", q.data_ptr(), k.data_ptr(), v.data_ptr(), q.shape[1], qs, vs, gp, bp,
+    launch(index, "qwen36_gdn_ragged_delta", qp, kp, vp, heads, qs, vs, gp, bp,
            sp, ss, batch, most, out.data_ptr(), None if ws is None else ws.data_ptr(), nb)
     return out
 
@@ -152,19 +159,19 @@ def fork_states(pools, parents: torch.Tensor) -> None:
             or parents.dim() != 1 or not parents.is_cuda or not parents.is_contiguous() \
             or not 1 <= parents.shape[0] <= 65536:
         raise ValueError("pools must be one or more tensors and parents a contiguous int32 GPU tensor [slots]")
-    n, args = parents.shape[0], []
+    n, index, args = parents.shape[0], parents.get_device(), []
     for t in pools:
-        if not isinstance(t, torch.Tensor) or t.device != parents.device or t.dim() < 2 or t.shape[0] != n \
+        if not isinstance(t, torch.Tensor) or t.get_device() != index or t.dim() < 2 or t.shape[0] != n \
                 or not t[0].is_contiguous():
             raise ValueError("a pool must be [slots, ...] with contiguous slots on the device of parents")
-        size = t[0].numel() * t.element_size()
-        stride = t.stride(0) * t.element_size() if n > 1 else size
-        if size < 1 or size % 16 or stride % 16 or stride < size or t.data_ptr() % 16:
+        size = t.nbytes // n
+        stride = t.stride(0) * t.itemsize if n > 1 else size
+        if size < 1 or (size | stride | t.data_ptr()) & 15 or stride < size:
             raise ValueError("a pool's slots must be 16-byte aligned, multiples of 16 bytes and apart")
         args.append(_lib.SlotPoolArgs(t.data_ptr(), size, stride))
     if len({a.data for a in args}) < len(args):
         raise ValueError("a pool is listed twice")
-    launch(parents.get_device(), "qwen36_slots_fork", (_lib.SlotPoolArgs * len(args))(*args), len(args), n,
+    launch(index, "qwen36_slots_fork", (_lib.SlotPoolArgs * len(args))(*args), len(args), n,
            parents.data_ptr())
 
 
@@ -177,8 +184,8 @@ class RaggedLinearAttentionLayer:
     out_proj."""
 
     def __init__(self, weights: dict, conv_states: torch.Tensor, ssm_states: torch.Tensor, adapters=None) -> None:
-        if _pool(conv_states, "conv_states", torch.bfloat16, (CONV_DIM, 3))[:2] \
-                != _pool(ssm_states, "ssm_states", torch.float32, _STATE)[:2]:
+        if _pool(conv_states, "conv_states", torch.bfloat16, *_CONV)[:2] \
+                != _pool(ssm_states, "ssm_states", torch.float32, *_STATE)[:2]:
             raise ValueError("conv_states and ssm_states must have the same slots on one device")
         from .projections import FusedProjection
         self.w, self.conv_states, self.ssm_states = weights, conv_states, ssm_states
