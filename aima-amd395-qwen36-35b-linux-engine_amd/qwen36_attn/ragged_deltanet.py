@@ -99,7 +99,7 @@ def ragged_conv1d(mixed_qkv: torch.Tensor, weight: torch.Tensor, states: torch.T
     """``gated_deltanet.causal_conv1d`` for a batch, with its arithmetic: mixed_qkv
     [T, 8192] bf16 (unit inner stride), weight [8192, 4] bf16, states [slots, 8192, 3]
     bf16, replaced in place by each sequence's last three inputs.  Returns SiLU(conv)
-    [T, 8192] bf16."""
+    [T, 8192] bf16; ``out`` overlaps no input."""
     index, n, sp, ss = _pool(states, "states", torch.bfloat16, *_CONV)
     t = mixed_qkv.shape[0] if isinstance(mixed_qkv, torch.Tensor) and mixed_qkv.dim() == 2 else 0
     if t == 0 or mixed_qkv.dtype is not torch.bfloat16 or mixed_qkv.get_device() != index \
@@ -129,7 +129,7 @@ def ragged_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torc
     to 2) [T, 32] fp32, states [slots, 32, 128 (k), 128 (v)] fp32, replaced in place by the sequences'
     last states.  ``longest``: the most rows that a sequence of the call has, where the
     caller knows it; it only chooses between the forms for few and for many tokens (a
-    sequence may have more).  Returns [T, 32, 128] bf16."""
+    sequence may have more).  Returns [T, 32, 128] bf16; ``out`` overlaps no input."""
     index, n, sp, ss = _pool(states, "states", torch.float32, *_STATE)
     t = v.shape[0] if isinstance(v, torch.Tensor) and v.dim() == 3 else 0
     (qp, heads, qs), (kp, *same) = _heads(q, "q", t, (HK, HV), index), _heads(k, "k", t, (HK, HV), index)

@@ -611,7 +611,8 @@ typedef struct {
 /* qwen36_gdn_ragged_conv1d: qwen36_gdn_conv1d for a batch, with its arithmetic:
  * x [tokens, >= 8192 stride], weight [8192, 4], out [tokens, 8192] bf16; states
  * bf16 [num_slots][8192][3], slots slot_stride elements apart, each replaced by its
- * sequence's last three inputs.  Strides multiples of 8, pointers 16-byte aligned. */
+ * sequence's last three inputs.  Strides multiples of 8, pointers 16-byte aligned; out
+ * overlaps no input. */
 int qwen36_gdn_ragged_conv1d(const void* x, unsigned x_row_stride, const void* weight, void* states,
                              size_t slot_stride, const qwen36_state_batch* batch, void* out,
                              void* stream);
@@ -621,7 +622,7 @@ int qwen36_gdn_ragged_conv1d(const void* x, unsigned x_row_stride, const void* w
  * v [tokens, 32, 128] bf16 with token strides (multiples of 8, at most 2^24), g, beta
  * fp32 [tokens, 32], out bf16 [tokens, 32, 128]; states fp32 [num_slots][32][128 k][128 v],
  * slots slot_stride elements (a multiple of 4) apart, replaced by the sequences' last
- * states.  Sequences of 13 and more rows go by chunks, which are made for g <= 0 and
+ * states; out overlaps no input.  Sequences of 13 and more rows go by chunks, which are made for g <= 0 and
  * 0 <= beta <= 2 (outside, their values may leave fp16's range).  longest: 0, or the most
  * rows that a sequence has as the host knows it; it only chooses the launches, a sequence
  * may have more.  Pointers 16-byte aligned (g and

@@ -216,3 +216,73 @@ def test_on_another_stream(gpu):
         got = rd.ragged_delta_rule(q, k, v, g, beta, other, *where)
     s.synchronize()
     assert torch.equal(got, want) and torch.equal(other, states)
+
+
+@pytest.mark.parametrize("lens,qk_heads", [([200, 330, 257, 70, 500, 12, 13], 16), ([449, 13, 64, 320, 1, 193], 32)])
+def test_delta_of_many_chunks(gpu, lens, qk_heads):
+    n = len(lens)
+    slots, has = [(3 * i + 1) % n if n % 3 else (5 * i + 1) % n for i in range(n)], [i % 3 != 1 for i in range(n)]
+    q, k, v, g, beta, gen = core(gpu, sum(lens), 31, 0.5, qk_heads)
+    states = torch.randn(n, 32, 128, 128, generator=gen, device=gpu)
+    before = states.clone()
+    out = torch.full((sum(lens), 32, 128), 7.0, dtype=BF16, device=gpu)
+    rd.ragged_delta_rule(q, k, v, g, beta, states, *batch(lens, slots, has, gpu), out=out, longest=max(lens))
+    want, after = R.delta(q, k, v, g, beta, before, R.cu_of(lens), slots, has)
+    check_delta(out, states, want, after, [])
+
+
+def test_delta_without_decay_and_with_reflections(gpu):
+    """g = 0 and beta = 2, the ends of what the gates give: every token reflects the state."""
+    lens, slots, has = [300, 70, 5], [2, 0, 1], [True, False, True]
+    q, k, v, g, beta, gen = core(gpu, sum(lens), 17)
+    states = torch.randn(3, 32, 128, 128, generator=gen, device=gpu)
+    before = states.clone()
+    out = torch.full((sum(lens), 32, 128), 7.0, dtype=BF16, device=gpu)
+    rd.ragged_delta_rule(q, k, v, torch.zeros_like(g), torch.full_like(beta, 2.0), states, *batch(lens, slots, has, gpu), out=out)
+    want, after = R.delta(q, k, v, torch.zeros_like(g), torch.full_like(beta, 2.0), before, R.cu_of(lens), slots, has)
+    check_delta(out, states, want, after, [])
+
+
+def test_states_far_apart(gpu):
+    """Slots behind 2^31 elements and 2^32 bytes of their pools."""
+    lens, slots, has = [3, 80], [2, 1], [True, True]
+    q, k, v, g, beta, gen = core(gpu, sum(lens), 23)
+    at, size = 2 ** 30 + 128, 32 * 128 * 128
+    states = torch.empty(2 * at + size, device=gpu).as_strided((3, 32, 128, 128), (at, 128 * 128, 128, 1))
+    near = torch.randn(3, 32, 128, 128, generator=gen, device=gpu)
+    states[1:] = near[1:]
+    where = batch(lens, slots, has, gpu)
+    got = rd.ragged_delta_rule(q, k, v, g, beta, states, *where)
+    assert torch.equal(got, rd.ragged_delta_rule(q, k, v, g, beta, near, *where)) and torch.equal(states[1:], near[1:])
+    rd.fork_states([states], torch.tensor([2, -1, -1], dtype=torch.int32, device=gpu))
+    assert torch.equal(states[0], near[2])
+    del states
+    x = torch.randn(sum(lens), 8192, generator=gen, device=gpu).to(BF16)
+    w = torch.randn(8192, 4, generator=gen, device=gpu).to(BF16)
+    conv = torch.empty(2 * at + 8192 * 3, dtype=BF16, device=gpu).as_strided((3, 8192, 3), (at, 3, 1))
+    close = torch.randn(3, 8192, 3, generator=gen, device=gpu).to(BF16)
+    conv[1:] = close[1:]
+    got = rd.ragged_conv1d(x, w, conv, *where)
+    assert torch.equal(got, rd.ragged_conv1d(x, w, close, *where)) and torch.equal(conv[1:], close[1:])
+
+
+def test_two_calls_at_once(gpu):
+    """Calls on two streams, their workspaces their own."""
+    lens, slots, has = [700, 90, 400, 13, 64], [1, 0, 3, 2, 4], [True] * 5
+    q, k, v, g, beta, gen = core(gpu, sum(lens), 29)
+    first = torch.randn(5, 32, 128, 128, generator=gen, device=gpu)
+    where = batch(lens, slots, has, gpu)
+    ins = [(q, k, v, g, beta), (k, q, v, 0.5 * g, 1 - beta)]
+    want = []
+    for x in ins:
+        states = first.clone()
+        want += [rd.ragged_delta_rule(*x, states, *where), states]
+    pools = [first.clone() for _ in range(6)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for n in range(6):
+        with torch.cuda.stream(streams[n % 2]):
+            got.append(rd.ragged_delta_rule(*ins[n % 2], pools[n], *where))
+    torch.cuda.synchronize()
+    for n in range(6):
+        assert torch.equal(got[n], want[2 * (n % 2)]) and torch.equal(pools[n], want[2 * (n % 2) + 1])
