@@ -118,8 +118,11 @@ __global__ __launch_bounds__(1024) void adapter_plan_kernel(const int* __restric
 // overlap can make places behind the call's rows).
 __device__ __forceinline__ bool plan_tile(const Plan& p, unsigned i, unsigned tokens, unsigned n, unsigned& first,
                                           unsigned& count, unsigned& id) {
-  if (i >= (unsigned)p.tiles[0]) return false;
-  const int4 t = *reinterpret_cast<const int4*>(p.tiles + 4 * (1 + i));
+  // both at once; what is asked for behind the plan's places (its rows follow) is none of them
+  const int tiles = p.tiles[0];
+  const unsigned most = (unsigned)(p.rows - p.tiles) / 4 - 1;
+  const int4 t = *reinterpret_cast<const int4*>(p.tiles + 4 * min(1 + i, most));
+  if (i >= (unsigned)tiles) return false;
   first = (unsigned)t.x;
   count = (unsigned)t.y;
   id = (unsigned)t.z;
