@@ -35,11 +35,17 @@ struct DeltaArgs {
 // One workgroup owns 32 columns of a head: thread (rg, cq) rows rg + 32 i and
 // columns 4 cq .. +3, a row of the 32 columns being one 128-byte line.
 // ---------------------------------------------------------------------------
-__global__ __launch_bounds__(256) void gdn_ragged_step_kernel(DeltaArgs p, RaggedBatch b, unsigned limit) {
-  __shared__ f32x4 red[2][4][2][8];    // [parity][wave][k | q][column quad]
-  __shared__ float dots[2][4][4];      // [parity][wave][k.k, q.q, k.q]
-  const unsigned seq = blockIdx.x >> 7;
-  const int h = (blockIdx.x >> 2) & 31, cg = blockIdx.x & 3;
+struct StepLds {
+  f32x4 red[2][4][2][8];    // [parity][wave][k | q][column quad]
+  float dots[2][4][4];      // [parity][wave][k.k, q.q, k.q]
+};
+
+__device__ __forceinline__ void step_rows(const DeltaArgs& p, const RaggedBatch& b, unsigned block, unsigned limit,
+                                          StepLds& lds) {
+  auto& red = lds.red;
+  auto& dots = lds.dots;
+  const unsigned seq = block >> 7;
+  const int h = (block >> 2) & 31, cg = block & 3;
   const RaggedSeq s = ragged_seq(b, seq);
   const unsigned len = (unsigned)(s.z - s.a);
   if (s.slot < 0 || len == 0 || len > limit) return;
@@ -127,6 +133,11 @@ __global__ __launch_bounds__(256) void gdn_ragged_step_kernel(DeltaArgs p, Ragge
   for (int i = 0; i < 4; ++i) __builtin_nontemporal_store(st[i], reinterpret_cast<f32x4*>(sp + 32 * i * kGdnDv));
 }
 
+__global__ __launch_bounds__(256) void gdn_ragged_step_kernel(DeltaArgs p, RaggedBatch b) {
+  __shared__ StepLds lds;
+  step_rows(p, b, blockIdx.x, ~0u, lds);
+}
+
 // ---------------------------------------------------------------------------
 // Chunks of 64 tokens: longer sequences.
 //
@@ -154,9 +165,10 @@ __global__ __launch_bounds__(256) void gdn_ragged_step_kernel(DeltaArgs p, Ragge
 // Times below are of 13 prompts of 9,903 rows, 161 chunks, the longest of 24.
 //  * gdn_ragged_prep_kernel, a workgroup a (chunk, key head): T and A of its value heads,
 //    which do not depend on the state, as the scan's operands, and the row factors: a
-//    record of 26,368 bytes a value head.  53 us, of which reading q and k once and writing
-//    the records (193 MB) take 43 at 4.5 TB/s; four workgroups a CU hide most of its steps'
-//    latencies (two, with L and T as whole matrices in LDS, took 81 us).
+//    record of 26,368 bytes a value head.  54 us, of which reading q and k once and writing
+//    the records (217 MB) take 48 at 4.5 TB/s; four workgroups a CU hide most of its steps'
+//    latencies (two, with L and T as whole matrices in LDS, took 81 us).  The short sequences'
+//    workgroups are behind them (a launch of their own takes 4.8 us even where there are none).
 //  * gdn_ragged_scan_kernel, a workgroup a (sequence, head or part of its columns),
 //    chunk after chunk.  A wave owns 16 columns of v with all 128 rows of their
 //    state, in registers: the layout of a product's result is that of the next one's
@@ -172,7 +184,11 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kC = 64;
-constexpr unsigned kShort = 12;           // longer sequences go by chunks
+// Longer sequences go by chunks.  Token by token and by chunks, us: one sequence of 8 tokens
+// 12.4 and 14.9, of 12 17.1 and 14.9; 16 sequences of 8 39 and 36, 64 of 8 132 and 112, of 12
+// 190 and 112.  A call of up to 12 rows goes token by token whatever its lengths, without a
+// workspace (2 us more for one sequence of 12).
+constexpr unsigned kShort = 7, kFewRows = 12;
 constexpr int kPitchR = 136;              // 16-bit row pitch of [64][128] tiles: 272 bytes
 
 // A record.  T and A as operands: tokens 16 i .. by 32 tokens k, lane 16 g + m of row m the
@@ -321,8 +337,13 @@ __device__ __forceinline__ float row_scale(float inv) {
 }
 
 template <int kHeads>
-__global__ __launch_bounds__(256, 4) void gdn_ragged_prep_kernel(DeltaArgs p, RaggedBatch b, Record* __restrict__ ws) {
+__global__ __launch_bounds__(256, 4) void gdn_ragged_prep_kernel(DeltaArgs p, RaggedBatch b, Record* __restrict__ ws,
+                                                               unsigned blocks) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
+  if (blockIdx.x >= blocks) {      // the batch's short sequences
+    step_rows(p, b, blockIdx.x - blocks, kShort, *reinterpret_cast<StepLds*>(smem));
+    return;
+  }
   PrepLds<kHeads>& s = *reinterpret_cast<PrepLds<kHeads>*>(smem);
   // a key head's chunks on the XCD where the scan reads their records
   constexpr unsigned kEach = 4 / kHeads;       // key heads an XCD
@@ -1005,7 +1026,7 @@ unsigned most_records(const RaggedBatch& b) { return b.tokens / kC + most_long(b
 // Chunks are not needed where the host knows that no sequence is long (one that is all
 // the same goes token by token).
 bool by_chunks(const RaggedBatch& b, unsigned longest) {
-  return most_long(b) > 0 && (longest == 0 || longest > kShort);
+  return b.tokens > kFewRows && (longest == 0 || longest > kShort);
 }
 
 }  // namespace
@@ -1040,8 +1061,10 @@ Q36_EXPORT int qwen36_gdn_ragged_delta(const void* q, const void* k, const void*
                        static_cast<bf16*>(out), slot_stride, qk_heads, qk_token_stride, v_token_stride};
   hipStream_t st = static_cast<hipStream_t>(stream);
   const bool chunks = by_chunks(b, longest);
-  hipLaunchKernelGGL(gdn_ragged_step_kernel, dim3(b.seqs * 128), dim3(256), 0, st, p, b, chunks ? kShort : ~0u);
-  if (!chunks) return static_cast<int>(hipGetLastError());
+  if (!chunks) {
+    hipLaunchKernelGGL(gdn_ragged_step_kernel, dim3(b.seqs * 128), dim3(256), 0, st, p, b);
+    return static_cast<int>(hipGetLastError());
+  }
   static std::once_flag once;
   static hipError_t attr = hipSuccess;
   std::call_once(once, [] {
@@ -1056,12 +1079,12 @@ Q36_EXPORT int qwen36_gdn_ragged_delta(const void* q, const void* k, const void*
   });
   if (attr != hipSuccess) return static_cast<int>(attr);
   Record* ws = static_cast<Record*>(workspace);
+  const unsigned blocks = most_records(b) * (qk_heads == 16 ? 16 : 32);
+  const dim3 grid(blocks + b.seqs * 128);
   if (qk_heads == 16)
-    hipLaunchKernelGGL(gdn_ragged_prep_kernel<2>, dim3(most_records(b) * 16), dim3(256), sizeof(PrepLds<2>), st, p, b,
-                       ws);
+    hipLaunchKernelGGL(gdn_ragged_prep_kernel<2>, grid, dim3(256), sizeof(PrepLds<2>), st, p, b, ws, blocks);
   else
-    hipLaunchKernelGGL(gdn_ragged_prep_kernel<1>, dim3(most_records(b) * 32), dim3(256), sizeof(PrepLds<1>), st, p, b,
-                       ws);
+    hipLaunchKernelGGL(gdn_ragged_prep_kernel<1>, grid, dim3(256), sizeof(PrepLds<1>), st, p, b, ws, blocks);
   // Few sequences leave CUs, one a workgroup: their columns in two or four.  A chunk takes
   // 2.2 us of 2 chains a workgroup, 2.6 of 4 and 4.4 of 8; sequences of 2,000 tokens, all in
   // all, by 2, 4 and 8 chains: 98, 103, 159 us for one, 110, 114, 170 for two, 227, 159, 203
