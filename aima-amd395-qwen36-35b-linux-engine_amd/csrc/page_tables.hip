@@ -14,9 +14,9 @@
 //
 // trim and fork are a workgroup a row (a chain of three dependent loads); extend and
 // compact do their bookkeeping in one workgroup, which scans 16,384 counts a step,
-// and a second launch copies the pages.  Copies are bound by their bytes; the
-// bookkeeping by latency (one step holds any pool of a few thousand pages; 400K
-// pages take 25 of them, once for all layers).
+// and a second launch copies the pages.  Copies are bound by their bytes (6 layers'
+// compaction of 461 MB: 97 us, 4.8 TB/s); the bookkeeping by latency (5 to 12 us a step,
+// which holds any pool of a few thousand pages; 400K pages take 25, once for all layers).
 #include "paged_common.h"
 
 namespace q36 {
