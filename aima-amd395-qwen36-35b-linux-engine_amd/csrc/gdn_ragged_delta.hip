@@ -666,15 +666,15 @@ __device__ __forceinline__ f16x8 to_f16(const u32x4& x, float s) {
   return o;
 }
 
-// kWaves of the workgroup's 8 waves own 16 columns each; where these are not all, the
-// others only fetch.
+// The workgroup's first kWaves waves own 16 columns each, the others only fetch.
+constexpr int scan_waves(int chains) { return chains == 8 ? 12 : 8; }
+
 template <int kWaves>
-__global__ __launch_bounds__(512, 1) void gdn_ragged_scan_kernel(DeltaArgs p, RaggedBatch b,
+__global__ __launch_bounds__(64 * scan_waves(kWaves), 1) void gdn_ragged_scan_kernel(DeltaArgs p, RaggedBatch b,
                                                                  const Record* __restrict__ ws, unsigned most) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   ScanBuf* buf = reinterpret_cast<ScanBuf*>(smem);
   constexpr unsigned kGroups = 8 / kWaves;
-  constexpr bool kAll = kWaves == 8;
   const unsigned slot = blockIdx.x >> 3, rest = slot >> 2;
   const int h = 4 * (blockIdx.x & 7) + (slot & 3);
   RaggedSeq s;
@@ -687,81 +687,79 @@ __global__ __launch_bounds__(512, 1) void gdn_ragged_scan_kernel(DeltaArgs p, Ra
   // ---- fetching a chunk ahead, into the other buffer: v, fragments and factors straight
   // to LDS; k and q, where they become fp16, by way of registers, two chunks ahead.  And what
   // the chunk two before left of output there goes out.
-  constexpr int kFirst = kAll ? 0 : kWaves, kFetch = 8 - kFirst;      // waves
-  constexpr int kRowIts = (16 + kFetch - 1) / kFetch, kFragIts = (kFrags + 1 + kFetch - 1) / kFetch;
-  const int fw = __builtin_amdgcn_readfirstlane(wave) - kFirst;
-  __builtin_assume(fw < kFetch);
-  u32x4 fk[kRowIts], fq[kRowIts], out[kRowIts];
-  float sk[kRowIts], sq[kRowIts];
-  auto load_kq = [&](unsigned c) {
-    const unsigned t0 = (unsigned)s.a + c * kC, rows = min((unsigned)kC, (unsigned)s.z - t0);
-    const Record* rec = ws + (size_t)(rec0 + c) * kGdnHv + h;
-    const unsigned range = ((rows - 1) * p.qk_stride + kGdnDk) * 2;
-    const __amdgpu_buffer_rsrc_t qrs = rows_rsrc(p.q + (size_t)t0 * p.qk_stride + kh * kGdnDk, range);
-    const __amdgpu_buffer_rsrc_t krs = rows_rsrc(p.k + (size_t)t0 * p.qk_stride + kh * kGdnDk, range);
+  if (wave >= kWaves) {
+    constexpr int kFetch = scan_waves(kWaves) - kWaves;      // waves
+    constexpr int kRowIts = (16 + kFetch - 1) / kFetch, kFragIts = (kFrags + 1 + kFetch - 1) / kFetch;
+    const int fw = __builtin_amdgcn_readfirstlane(wave) - kWaves;
+    __builtin_assume(fw < kFetch);
+    u32x4 fk[kRowIts], fq[kRowIts], out[kRowIts];
+    float sk[kRowIts], sq[kRowIts];
+    auto load_kq = [&](unsigned c) {
+      const unsigned t0 = (unsigned)s.a + c * kC, rows = min((unsigned)kC, (unsigned)s.z - t0);
+      const Record* rec = ws + (size_t)(rec0 + c) * kGdnHv + h;
+      const unsigned range = ((rows - 1) * p.qk_stride + kGdnDk) * 2;
+      const __amdgpu_buffer_rsrc_t qrs = rows_rsrc(p.q + (size_t)t0 * p.qk_stride + kh * kGdnDk, range);
+      const __amdgpu_buffer_rsrc_t krs = rows_rsrc(p.k + (size_t)t0 * p.qk_stride + kh * kGdnDk, range);
 #pragma unroll
-    for (int n = 0; n < kRowIts; ++n) {        // behind row 63: behind the ranges, zeros
-      const unsigned row = 4 * (fw + n * kFetch) + lg, off = (row * p.qk_stride + 8 * li) * 2;
-      fk[n] = load16(krs, off);
-      fq[n] = load16(qrs, off);
-      sk[n] = rec->f[kKs + (row & 63)];
-      sq[n] = rec->f[kQs + (row & 63)];
-    }
-  };
-  auto stage_kq = [&](unsigned c) {
-    ScanBuf& o = buf[c & 1];
-#pragma unroll
-    for (int n = 0; n < kRowIts; ++n) {
-      const int i = fw + n * kFetch, at = row_at((4 * i + lg) & 63, li);
-      if (i < 16) {
-        *reinterpret_cast<f16x8*>(o.kr + at) = to_f16(fk[n], sk[n]);
-        *reinterpret_cast<f16x8*>(o.qr + at) = to_f16(fq[n], sq[n]);
+      for (int n = 0; n < kRowIts; ++n) {        // behind row 63: behind the ranges, zeros
+        const unsigned row = 4 * (fw + n * kFetch) + lg, off = (row * p.qk_stride + 8 * li) * 2;
+        fk[n] = load16(krs, off);
+        fq[n] = load16(qrs, off);
+        sk[n] = rec->f[kKs + (row & 63)];
+        sq[n] = rec->f[kQs + (row & 63)];
       }
-    }
-  };
-  // a lane's 16 bytes of a row of the output are those of v that it fetches next
-  const __amdgpu_buffer_rsrc_t ors =
-      rows_rsrc(p.out + ((size_t)s.a * kGdnHv + h) * kGdnDv, ((len - 1) * kGdnHv + 1) * (unsigned)(kGdnDv * 2));
-  auto read_out = [&](unsigned c) {
+    };
+    auto stage_kq = [&](unsigned c) {
+      ScanBuf& o = buf[c & 1];
 #pragma unroll
-    for (int n = 0; n < kRowIts; ++n)
-      out[n] = *reinterpret_cast<const u32x4*>(buf[c & 1].vr + 4 * min(fw + n * kFetch, 15) * kGdnDk + 8 * lane);
-  };
-  auto store_out = [&](unsigned c) {
+      for (int n = 0; n < kRowIts; ++n) {
+        const int i = fw + n * kFetch, at = row_at((4 * i + lg) & 63, li);
+        if (i < 16) {
+          *reinterpret_cast<f16x8*>(o.kr + at) = to_f16(fk[n], sk[n]);
+          *reinterpret_cast<f16x8*>(o.qr + at) = to_f16(fq[n], sq[n]);
+        }
+      }
+    };
+    // a lane's 16 bytes of a row of the output are those of v that it fetches next
+    const __amdgpu_buffer_rsrc_t ors =
+        rows_rsrc(p.out + ((size_t)s.a * kGdnHv + h) * kGdnDv, ((len - 1) * kGdnHv + 1) * (unsigned)(kGdnDv * 2));
+    auto read_out = [&](unsigned c) {
 #pragma unroll
-    for (int n = 0; n < kRowIts; ++n) {       // rows behind the sequence fall outside the range and are dropped
-      const int i = fw + n * kFetch, row = 4 * i + lg, chunk = li ^ row_key(row);
-      const bool own = i < 16 && (unsigned)chunk / (2 * kWaves) == rest % kGroups;      // the workgroup's columns
-      const unsigned off = own ? (c * kC + row) * (kGdnHv * kGdnDv * 2) + 16 * chunk : ~15u;
-      __builtin_amdgcn_raw_buffer_store_b128(out[n], ors, (int)off, 0, 0);
-    }
-  };
-  auto fetch = [&](unsigned c) {
-    const unsigned t0 = (unsigned)s.a + c * kC, rows = min((unsigned)kC, (unsigned)s.z - t0);
-    ScanBuf& o = buf[c & 1];
-    const u32x4 rrs = g_rsrc(ws + (size_t)(rec0 + c) * kGdnHv + h, sizeof(Record));
+      for (int n = 0; n < kRowIts; ++n)
+        out[n] = *reinterpret_cast<const u32x4*>(buf[c & 1].vr + 4 * min(fw + n * kFetch, 15) * kGdnDk + 8 * lane);
+    };
+    auto store_out = [&](unsigned c) {
 #pragma unroll
-    for (int n = 0; n < kFragIts; ++n) {       // (the factors follow the fragments)
-      const int i = fw + n * kFetch;
-      if (i <= kFrags) to_lds(rrs, 1024 * i + 16 * lane, i < kFrags ? (void*)(o.frag + i * 64) : (void*)o.f);
-    }
-    const u32x4 vrs =
-        g_rsrc(p.v + (size_t)t0 * p.v_stride + h * kGdnDv, ((rows - 1) * p.v_stride + kGdnDv) * 2);
+      for (int n = 0; n < kRowIts; ++n) {       // rows behind the sequence fall outside the range and are dropped
+        const int i = fw + n * kFetch, row = 4 * i + lg, chunk = li ^ row_key(row);
+        const bool own = i < 16 && (unsigned)chunk / (2 * kWaves) == rest % kGroups;      // the workgroup's columns
+        const unsigned off = own ? (c * kC + row) * (kGdnHv * kGdnDv * 2) + 16 * chunk : ~15u;
+        __builtin_amdgcn_raw_buffer_store_b128(out[n], ors, (int)off, 0, 0);
+      }
+    };
+    auto fetch = [&](unsigned c) {
+      const unsigned t0 = (unsigned)s.a + c * kC, rows = min((unsigned)kC, (unsigned)s.z - t0);
+      ScanBuf& o = buf[c & 1];
+      const u32x4 rrs = g_rsrc(ws + (size_t)(rec0 + c) * kGdnHv + h, sizeof(Record));
 #pragma unroll
-    for (int n = 0; n < kRowIts; ++n) {        // four rows of v; behind the sequence its last again (beta is 0)
-      const int i = fw + n * kFetch, row = 4 * i + lg;
-      if (i < 16)
-        to_lds(vrs, (min((unsigned)row, rows - 1) * p.v_stride + 8 * (li ^ row_key(row))) * 2, o.vr + 4 * i * kGdnDk);
-    }
-  };
-  if (kAll || wave >= kWaves) {
+      for (int n = 0; n < kFragIts; ++n) {       // (the factors follow the fragments)
+        const int i = fw + n * kFetch;
+        if (i <= kFrags) to_lds(rrs, 1024 * i + 16 * lane, i < kFrags ? (void*)(o.frag + i * 64) : (void*)o.f);
+      }
+      const u32x4 vrs =
+          g_rsrc(p.v + (size_t)t0 * p.v_stride + h * kGdnDv, ((rows - 1) * p.v_stride + kGdnDv) * 2);
+#pragma unroll
+      for (int n = 0; n < kRowIts; ++n) {        // four rows of v; behind the sequence its last again (beta is 0)
+        const int i = fw + n * kFetch, row = 4 * i + lg;
+        if (i < 16)
+          to_lds(vrs, (min((unsigned)row, rows - 1) * p.v_stride + 8 * (li ^ row_key(row))) * 2, o.vr + 4 * i * kGdnDk);
+      }
+    };
     load_kq(0);
     fetch(0);
     stage_kq(0);
     load_kq(min(1u, last));
     __builtin_amdgcn_s_waitcnt(kVmcnt(0));
-  }
-  if (!kAll && wave >= kWaves) {
     lds_barrier();
     for (unsigned c = 0; c < chunks; ++c) {      // beside chunk c
       if (c >= 1) read_out(c - 1);
@@ -813,11 +811,11 @@ __global__ __launch_bounds__(512, 1) void gdn_ragged_scan_kernel(DeltaArgs p, Ra
     for (int i = 0; i < 4; ++i) o[i] = *reinterpret_cast<const f16x8*>(from + m + 4096 * i);
   };
   auto factors = [&](int which, int i) { return *reinterpret_cast<const f32x4*>(smem + at_f + 4 * which + 64 * i); };
-  // fragments 3 part .. of T or A, in their order: tokens 16 i .. by 32 k ..
-  f16x8 fa[6], fb[6];
-  auto read_frags = [&](int first, int part, f16x8 (&o)[6]) {
+  // fragments 2 part, 2 part + 1 of T or A, in their order: tokens 16 i .. by 32 k ..
+  f16x8 fa[4], fb[4];
+  auto read_frags = [&](int first, int part, f16x8 (&o)[4]) {
 #pragma unroll
-    for (int n = 0; n < 6; ++n) o[n] = *reinterpret_cast<const f16x8*>(smem + at_frag + 1024 * (first + 6 * part + n));
+    for (int n = 0; n < 4; ++n) o[n] = *reinterpret_cast<const f16x8*>(smem + at_frag + 1024 * (first + 4 * part + n));
   };
   auto frag_i = [](int f) { return f < 2 ? f : 2 + ((f - 2) >> 1); };
   auto frag_k = [](int f) { return f < 2 ? 0 : f & 1; };
@@ -838,16 +836,10 @@ __global__ __launch_bounds__(512, 1) void gdn_ragged_scan_kernel(DeltaArgs p, Ra
     f32x4 ks[4], qs[4];
     float ss, si;
     read_rows(kKr, 0, kf[0]);
-    if (kAll && c >= 1) read_out(c - 1);
     scale_of<13>(top.bits(), ss, si);
     split8(state[0], state[1], ss, sh[0], sl[0]);
     kFence;
     egl_next = (ws + (size_t)(rec0 + min(c + 1, last)) * kGdnHv + h)->f[kEgl];
-    if (kAll) {
-      __builtin_amdgcn_s_waitcnt(0xC07F);       // what was read of v's place, before v is fetched there
-      if (c < last) fetch(c + 1);
-      if (c >= 1) store_out(c - 1);
-    }
     // k' S, S in parts
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -863,16 +855,19 @@ __global__ __launch_bounds__(512, 1) void gdn_ragged_scan_kernel(DeltaArgs p, Ra
     ColumnMax ztop;
     i16x4 v4[4];
     f32x4 bt[4], cy[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    auto read_in = [&](int i) {
       v4[i] = lds_read_tr16(reinterpret_cast<const bf16*>(smem + at_v + 4096 * i));
       bt[i] = factors(kBeta, i);
       cy[i] = factors(kBcy, i);
-    }
+    };
+    read_in(0);
     kFence;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      if (k < 3) read_rows(kQr, k + 1, kf[(k + 1) & 1]);
+      if (k < 3) {
+        read_rows(kQr, k + 1, kf[(k + 1) & 1]);
+        read_in(k + 1);
+      }
       if (k >= 2) read_frags(0, k - 2, k == 2 ? fa : fb);
 #pragma unroll
       for (int i = 0; i < 4; ++i) qs[i] = mfma_f16(kf[k & 1][i], sl[k], k == 0 ? zero : qs[i]);
@@ -893,43 +888,44 @@ __global__ __launch_bounds__(512, 1) void gdn_ragged_scan_kernel(DeltaArgs p, Ra
     for (int k = 0; k < 2; ++k) split8(ks[2 * k], ks[2 * k + 1], zs, xh[k], xl[k]);
     f32x4 rq[4], rk[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      rq[i] = factors(kRsq, i);
-      rk[i] = factors(kRsk, i);
-    }
+    for (int i = 0; i < 4; ++i) rq[i] = factors(kRsq, i);
     kFence;
     // v' = T rows, times 2^8 and the rows' scale: low T by high rows, high by low, high by high
-    auto t_rows = [&](int part, const f16x8 (&m)[6]) {
+    auto t_rows = [&](int part, const f16x8 (&m)[4]) {
 #pragma unroll
       for (int n = 0; n < 3; ++n)
 #pragma unroll
-        for (int j = 0; j < 3; ++j) {
-          const int i = frag_i(3 * part + j), k = frag_k(3 * part + j);
+        for (int j = 0; j < 2; ++j) {
+          const int i = frag_i(2 * part + j), k = frag_k(2 * part + j);
           ks[i] = mfma_f16(m[2 * j + (n == 0)], n == 1 ? xl[k] : xh[k], n == 0 && k == 0 ? zero : ks[i]);
         }
     };
     t_rows(0, fa);
-    if (kAll) stage_kq(c + 1);       // (behind the last chunk of what was, which nothing reads)
-    kBeside(0, 9, 4);
-    if (kAll) load_kq(min(c + 2, last));
+    kBeside(0, 6, 0);
     t_rows(1, fb);
-    read_frags(kFragA, 0, fa);
+    read_frags(0, 2, fa);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) qs[i] *= rq[i] * si;
-    kBeside(0, 9, 4);
+    for (int i = 0; i < 2; ++i) qs[i] *= rq[i] * si;
+    kBeside(0, 6, 3);
+    t_rows(2, fa);
+    read_frags(kFragA, 0, fb);
+#pragma unroll
+    for (int i = 2; i < 4; ++i) qs[i] *= rq[i] * si;
+    kBeside(0, 6, 3);
     // decayed v', A v'
     bf16x8 vh[2], vl[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) split8(ks[2 * k], ks[2 * k + 1], vh[k], vl[k]);
-    read_frags(kFragA, 1, fb);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) rk[i] = factors(kRsk, i);
     kFence;
     f32x4 av[4];
-    auto a_rows = [&](int part, const f16x8 (&m)[6]) {
+    auto a_rows = [&](int part, const f16x8 (&m)[4]) {
 #pragma unroll
       for (int n = 0; n < 3; ++n)
 #pragma unroll
-        for (int j = 0; j < 3; ++j) {
-          const int i = frag_i(3 * part + j), k = frag_k(3 * part + j);
+        for (int j = 0; j < 2; ++j) {
+          const int i = frag_i(2 * part + j), k = frag_k(2 * part + j);
           av[i] = mfma16x16x32(__builtin_bit_cast(bf16x8, m[2 * j + (n == 0)]), n == 1 ? vl[k] : vh[k],
                                n == 0 && k == 0 ? zero : av[i]);
         }
@@ -946,20 +942,24 @@ __global__ __launch_bounds__(512, 1) void gdn_ragged_scan_kernel(DeltaArgs p, Ra
     };
     ColumnMax wtop;
     float wsc, wi;
-    a_rows(0, fa);
+    a_rows(0, fb);
+    read_frags(kFragA, 1, fa);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       ks[i] *= rk[i];
       wtop.take(ks[i]);
     }
+    kBeside(0, 6, 4);
+    a_rows(1, fa);
+    read_frags(kFragA, 2, fb);
     scale_of<13>(wtop.bits(), wsc, wi);
-    kBeside(0, 9, 5);
-    read_kt(0);
-    a_rows(1, fb);
-#pragma unroll
-    for (int k = 0; k < 2; ++k) split8(ks[2 * k], ks[2 * k + 1], wsc, xh[k], xl[k]);
+    split8(ks[0], ks[1], wsc, xh[0], xl[0]);
     wi *= zi;
-    kBeside(0, 9, 6);
+    kBeside(0, 6, 6);
+    a_rows(2, fb);
+    read_kt(0);
+    split8(ks[2], ks[3], wsc, xh[1], xl[1]);
+    kBeside(0, 6, 4);
     // S <- e^Glast S + k'^T decayed v'; the output e^G q S + A v', in place of the columns' v
     const float ai = zi * 0.00390625f;
     top = ColumnMax{};
@@ -991,7 +991,6 @@ __global__ __launch_bounds__(512, 1) void gdn_ragged_scan_kernel(DeltaArgs p, Ra
     }
 #pragma unroll
     for (int i = 4; i < 8; ++i) update(i);
-    if (kAll) __builtin_amdgcn_s_waitcnt(kVmcnt(0));
     lds_barrier();
     at_row += step;
     at_kt += step;
@@ -1011,10 +1010,6 @@ __global__ __launch_bounds__(512, 1) void gdn_ragged_scan_kernel(DeltaArgs p, Ra
   for (int i = 0; i < 8; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r) sp[state_row(i, r)] = state[i][r];
-  if (kAll) {
-    read_out(last);
-    store_out(last);
-  }
 }
 
 // Sequences that can be long, and records for their chunks.
@@ -1096,6 +1091,6 @@ Q36_EXPORT int qwen36_gdn_ragged_delta(const void* q, const void* k, const void*
   else if (n <= 4)
     hipLaunchKernelGGL(gdn_ragged_scan_kernel<4>, dim3(n * kGdnHv * 2), dim3(512), lds, st, p, b, ws, n);
   else
-    hipLaunchKernelGGL(gdn_ragged_scan_kernel<8>, dim3(n * kGdnHv), dim3(512), lds, st, p, b, ws, n);
+    hipLaunchKernelGGL(gdn_ragged_scan_kernel<8>, dim3(n * kGdnHv), dim3(64 * scan_waves(8)), lds, st, p, b, ws, n);
   return static_cast<int>(hipGetLastError());
 }
