@@ -160,7 +160,7 @@ __global__ __launch_bounds__(256) void gdn_ragged_step_kernel(DeltaArgs p, Ragge
 // bf16 values of each (2^-17 of a term): decays of any size meet there, and rows that
 // are all decayed keep their bits.
 // (Three bf16 parts throughout, which need no scales, take 182 products a chunk and column
-// tile where this takes 132, and 157 us where the scan takes 134.)
+// tile where this takes 132: 157 us where the scan then took 134.)
 //
 // Times below are of 13 prompts of 9,903 rows, 161 chunks, the longest of 24.
 //  * gdn_ragged_prep_kernel, a workgroup a (chunk, key head): T and A of its value heads,
@@ -174,8 +174,9 @@ __global__ __launch_bounds__(256) void gdn_ragged_step_kernel(DeltaArgs p, Ragge
 //    state, in registers: the layout of a product's result is that of the next one's
 //    right operand, so that nothing of a column's recurrence leaves its wave, and waves
 //    meet once a chunk, where the next chunk's k, q, v, T and A are ready in LDS.
-//    134 us: a chunk of 8 waves takes 5.4 us, 3.9 without its fetches, of which each SIMD
-//    issues products for 1.8 and vector instructions for 2, and LDS is read for 2.4.
+//    117 us: a chunk takes 4.7 us, 4.3 without its fetches, in which each SIMD issues
+//    products for 1.8 and vector instructions for 1.9 and LDS is read for 2.4.  (131 with the
+//    fetches in the eight waves that own columns; 4 such waves of 32 columns each 128.)
 // ---------------------------------------------------------------------------
 
 typedef _Float16 f16;
@@ -1081,9 +1082,9 @@ Q36_EXPORT int qwen36_gdn_ragged_delta(const void* q, const void* k, const void*
   else
     hipLaunchKernelGGL(gdn_ragged_prep_kernel<1>, grid, dim3(256), sizeof(PrepLds<1>), st, p, b, ws, blocks);
   // Few sequences leave CUs, one a workgroup: their columns in two or four.  A chunk takes
-  // 2.2 us of 2 chains a workgroup, 2.6 of 4 and 4.4 of 8; sequences of 2,000 tokens, all in
-  // all, by 2, 4 and 8 chains: 98, 103, 159 us for one, 110, 114, 170 for two, 227, 159, 203
-  // for four, 353, 289, 261 for six.
+  // 2.2 us of 2 chains a workgroup, 2.6 of 4 and 4 of 8 where few CUs are at work; sequences of
+  // 2,000 tokens, all in all, by 2 and 4 chains 98 and 103 us for one, by 4 and 8 108 and 147
+  // for two, 156 and 181 for four, 245 and 210 for five, 343 and 297 for eight.
   const unsigned n = most_long(b);
   const unsigned lds = 2 * sizeof(ScanBuf);
   if (n <= 2)
