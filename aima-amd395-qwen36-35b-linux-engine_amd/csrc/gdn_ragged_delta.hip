@@ -573,8 +573,12 @@ __device__ __forceinline__ f32x4 mfma_f16(f16x8 a, f16x8 b, f32x4 c) {
 constexpr int kVmcnt(int n) { return (n & 15) | ((n >> 4) << 14) | (7 << 4) | (15 << 8); }
 
 // Rows of k', q' and v in LDS: chunk j (8 values) of a row stands at j ^ row_key, so that
-// sixteen rows of one chunk, and what a transposed read takes of four, lie in different banks.
-__device__ __forceinline__ int row_key(int row) { return (row & 3) << 2 | ((row >> 2) & 3); }
+// what one cycle takes of a 16-byte read (lanes 0-3, 12-15, 20-27 and so on: eight rows of one
+// chunk, the eight others of the next) lies in different banks.
+__device__ __forceinline__ int row_key(int row) {
+  const int x = (row >> 2) & 3;
+  return (row & 3) << 2 | ((x ^ x >> 1) & 1) << 1 | x >> 1;
+}
 __device__ __forceinline__ int row_at(int row, int chunk) { return row * kGdnDk + 8 * (chunk ^ row_key(row)); }
 
 struct ScanBuf {
