@@ -324,13 +324,6 @@ __device__ __forceinline__ f32x4 mm16(const float* a, const f32x4& b, f32x4 acc,
 
 __device__ __forceinline__ int frag_of(int i, int k) { return i < 2 ? i : 2 * i - 2 + k; }
 
-// Lower 16x16 tile t (0 .. 9): its row and column of tiles.
-__device__ __forceinline__ int tri_row(int t) { return (t >= 1) + (t >= 3) + (t >= 6); }
-__device__ __forceinline__ int tri_col(int t) {
-  const int r = tri_row(t);
-  return t - r * (r + 1) / 2;
-}
-
 // The power of two that brings a row of inverse norm `inv` to a norm of 8 to 16.
 __device__ __forceinline__ float row_scale(float inv) {
   const int e = min(max((int)(__float_as_uint(inv) >> 23) - 127, -100), 100);
@@ -427,65 +420,64 @@ __global__ __launch_bounds__(256, 4) void gdn_ragged_prep_kernel(DeltaArgs p, Ra
       s.far[hd][rt - 1][j] = expf(decay(hd, 16 * rt, j));
     }
   }
-  // k k^T and q k^T of the lower tiles wave, wave + 4, wave + 8, transposed: lane columns
-  // 4 lg + r of row li
-  f32x4 kk[3], qk[3];
+  // k k^T and q k^T by fragments of A (two tiles of a row of tiles, the second not behind the
+  // diagonal), transposed: lane columns 4 lg + r of row li.  Waves 0, 1 take fragments 2 wave
+  // and the next, 2 and 3 fragments 4 and 5: 3, 3, 2 and 2 tiles.
+  const int f0 = wave < 2 ? 2 * wave : wave + 2, n_frags = wave < 2 ? 2 : 1;
+  auto frag_row = [](int f) { return f < 2 ? f : f < 4 ? 2 : 3; };
+  auto frag_col = [](int f) { return f < 2 ? 0 : f & 1; };
+  f32x4 kk[2][2], qk[2][2];
 #pragma unroll
-  for (int n = 0; n < 3; ++n) {
-    const int t = wave + 4 * n, rt = tri_row(t), ct = tri_col(t);
-    kk[n] = f32x4{0.f, 0.f, 0.f, 0.f};
-    qk[n] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (t >= 10) continue;
-    const int jrow = (16 * ct + li) * kPitchR + 8 * lg, irow = (16 * rt + li) * kPitchR + 8 * lg;
+  for (int n = 0; n < 2; ++n)
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const bf16x8 kj = ld8(s.u.rows.k + jrow + 32 * k);
-      kk[n] = mfma16x16x32(kj, ld8(s.u.rows.k + irow + 32 * k), kk[n]);
-      qk[n] = mfma16x16x32(kj, ld8(s.u.rows.q + irow + 32 * k), qk[n]);
+    for (int u = 0; u < 2; ++u) {
+      const int rt = frag_row(f0 + n), ct = 2 * frag_col(f0 + n) + u;
+      kk[n][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+      qk[n][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (n >= n_frags || ct > rt) continue;
+      const int jrow = (16 * ct + li) * kPitchR + 8 * lg, irow = (16 * rt + li) * kPitchR + 8 * lg;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const bf16x8 kj = ld8(s.u.rows.k + jrow + 32 * k);
+        kk[n][u] = mfma16x16x32(kj, ld8(s.u.rows.k + irow + 32 * k), kk[n][u]);
+        qk[n][u] = mfma16x16x32(kj, ld8(s.u.rows.q + irow + 32 * k), qk[n][u]);
+      }
     }
-  }
   lds_barrier();     // the rows make room for L
 #pragma unroll
-  for (int n = 0; n < 3; ++n) {
-    const int t = wave + 4 * n, rt = tri_row(t), ct = tri_col(t);
-    if (t >= 10) continue;
-    const int i = 16 * rt + li, j0 = 16 * ct + 4 * lg;
-    const f32x4 kj = ld4(s.kinv + j0);
+  for (int n = 0; n < 2; ++n) {
+    if (n >= n_frags) continue;
+    const int rt = frag_row(f0 + n), i = 16 * rt + li;
     const float ki = s.kinv[i], qi = s.qinv[i] * kQScale;
-    const int f = frag_of(rt, ct >> 1), at = 16 * lg + li;
 #pragma unroll
     for (int hd = 0; hd < kHeads; ++hd) {
-      f32x4 d, l;
-      bf16x4 a, al;
-      if (rt == ct) {      // behind the diagonal anything, chosen against below
-#pragma unroll
-        for (int r = 0; r < 4; ++r) d[r] = exp_fast(decay(hd, i, j0 + r));
-      } else {
-        d = ld4(s.far[hd][rt - 1] + j0) * s.near[hd][i];
-      }
+      bf16x8 hi = {}, lo = {};
       const float bi = s.bs[hd][i];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        l[r] = j0 + r < i ? (((ki * kj[r]) * kk[n][r]) * bi) * d[r] : 0.f;
-        const float av = j0 + r <= i ? ((qi * kj[r]) * qk[n][r]) * d[r] : 0.f;
-        a[r] = f2bf(av);
-        al[r] = f2bf(av - bf2f(a[r]));
+      for (int u = 0; u < 2; ++u) {
+        const int ct = 2 * frag_col(f0 + n) + u, j0 = 16 * ct + 4 * lg;
+        if (ct > rt) continue;
+        const f32x4 kj = ld4(s.kinv + j0);
+        f32x4 d;
+        if (rt == ct) {      // behind the diagonal anything, chosen against below
+#pragma unroll
+          for (int r = 0; r < 4; ++r) d[r] = exp_fast(decay(hd, i, j0 + r));
+        } else {
+          d = ld4(s.far[hd][rt - 1] + j0) * s.near[hd][i];
+        }
+        float* lt = s.u.tiles.l[hd][rt * (rt + 1) / 2 + ct];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          lt[tile_at(4 * lg + r, li)] = j0 + r < i ? (((ki * kj[r]) * kk[n][u][r]) * bi) * d[r] : 0.f;
+          const float av = j0 + r <= i ? ((qi * kj[r]) * qk[n][u][r]) * d[r] : 0.f;
+          const bf16 ah = f2bf(av);
+          hi[4 * u + r] = ah;
+          lo[4 * u + r] = f2bf(av - bf2f(ah));
+        }
       }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) s.u.tiles.l[hd][t][tile_at(4 * lg + r, li)] = l[r];
-      bf16x4* to = reinterpret_cast<bf16x4*>(rec[hd].frag + (kFragA + 2 * f) * 64 + at) + (ct & 1);
-      to[0] = a;
-      to[128] = al;
-    }
-  }
-  // the upper tiles (0, 1) and (2, 3), which the operands hold too
-  if (tid < 128) {
-    const int f = frag_of(2 * (tid >> 6), tid >> 6);
-#pragma unroll
-    for (int hd = 0; hd < kHeads; ++hd) {
-      f16x4* to = reinterpret_cast<f16x4*>(rec[hd].frag + (kFragA + 2 * f) * 64 + lane) + 1;
-      to[0] = f16x4{};
-      to[128] = f16x4{};
+      f16x8* to = rec[hd].frag + (kFragA + 2 * (f0 + n)) * 64 + lane;
+      to[0] = __builtin_bit_cast(f16x8, hi);
+      to[64] = __builtin_bit_cast(f16x8, lo);
     }
   }
   lds_barrier();
