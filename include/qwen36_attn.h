@@ -626,8 +626,9 @@ int qwen36_gdn_ragged_conv1d(const void* x, unsigned x_row_stride, const void* w
  * 0 <= beta <= 2 (outside, their values may leave fp16's range).  longest: 0, or the most
  * rows that a sequence has as the host knows it; it only chooses the launches, a sequence
  * may have more.  Pointers 16-byte aligned (g and
- * beta 4); workspace of qwen36_gdn_ragged_delta_workspace_bytes(...) bytes (0: none);
- * calls that overlap on one workspace race. */
+ * beta 4); workspace of qwen36_gdn_ragged_delta_workspace_bytes(...) bytes (0: none;
+ * else 824 KiB for every 64 rows and every sequence that may have 8 and more, at most an
+ * eighth of the rows); calls that overlap on one workspace race. */
 size_t qwen36_gdn_ragged_delta_workspace_bytes(const qwen36_state_batch* batch, unsigned longest);
 int qwen36_gdn_ragged_delta(const void* q, const void* k, const void* v, unsigned qk_heads,
                             unsigned qk_token_stride, unsigned v_token_stride, const void* g,

@@ -286,3 +286,60 @@ def test_two_calls_at_once(gpu):
     torch.cuda.synchronize()
     for n in range(6):
         assert torch.equal(got[n], want[2 * (n % 2)]) and torch.equal(pools[n], want[2 * (n % 2) + 1])
+
+
+def test_delta_of_hundreds_of_sequences(gpu):
+    """More sequences than a wave has lanes, of all kinds, some of them padding."""
+    n = 150
+    lens = [(7 * i) % 23 if i % 31 else 70 + i for i in range(n)]
+    slots, has = [(11 * i + 3) % n if i % 9 != 4 else -1 for i in range(n)], [i % 4 > 0 for i in range(n)]
+    q, k, v, g, beta, gen = core(gpu, sum(lens), 37)
+    states = torch.randn(n, 32, 128, 128, generator=gen, device=gpu) * 0.3
+    before = states.clone()
+    out = torch.full((sum(lens), 32, 128), 7.0, dtype=BF16, device=gpu)
+    rd.ragged_delta_rule(q, k, v, g, beta, states, *batch(lens, slots, has, gpu), out=out)
+    want, after = R.delta(q, k, v, g, beta, before, R.cu_of(lens), slots, has)
+    used = {s for s, m in zip(slots, lens) if m}
+    check_delta(out, states, want, after, [i for i in range(n) if i not in used])
+
+
+def test_as_many_sequences_as_a_call_has(gpu):
+    """65,536 rows of a sequence each, all but a few of them padding."""
+    n, real = 65536, {0: 2, 63: 0, 64: 5, 40000: 1, 65535: 3}
+    q, k, v, g, beta, gen = core(gpu, n, 41)
+    x = torch.randn(n, 8192, generator=gen, device=gpu).to(BF16)
+    w = torch.randn(8192, 4, generator=gen, device=gpu).to(BF16)
+    slots = torch.full((n,), -1, dtype=torch.int32, device=gpu)
+    for i, s in real.items():
+        slots[i] = s
+    cu = torch.arange(n + 1, dtype=torch.int32, device=gpu)
+    states, conv = torch.randn(6, 32, 128, 128, generator=gen, device=gpu), torch.randn(6, 8192, 3, generator=gen, device=gpu).to(BF16)
+    few, few_conv, at = states.clone(), conv.clone(), torch.tensor(list(real), device=gpu)
+    where = batch([1] * len(real), list(real.values()), [True] * len(real), gpu)
+    got = rd.ragged_delta_rule(q, k, v, g, beta, states, cu, slots, longest=1)
+    want = rd.ragged_delta_rule(q[at], k[at], v[at], g[at], beta[at], few, *where, longest=1)
+    assert torch.equal(got[at], want) and torch.equal(states, few)
+    got, want = rd.ragged_conv1d(x, w, conv, cu, slots), rd.ragged_conv1d(x[at], w, few_conv, *where)
+    assert torch.equal(got[at], want) and torch.equal(conv, few_conv)
+
+
+@pytest.mark.parametrize("cu,slots", [([5, -3, 1 << 30, 7, 40], [0, 1, 7, -5]), ([0, 90, 30, 90, 200], [2, 3, 0, 1 << 30]),
+                                      ([-(1 << 31), (1 << 31) - 1, 0, 64, 1], [1, -(1 << 31), 2, 0])])
+def test_offsets_that_make_no_sense(gpu, cu, slots):
+    """They are cut to the call's rows: nothing around its tensors changes."""
+    t, n = 90, 4
+    q, k, v, g, beta, gen = core(gpu, t, 43)
+    out, pool = torch.full((t + 64, 32, 128), 7.0, dtype=BF16, device=gpu), torch.full((n + 2, 32, 128, 128), 0.5, device=gpu)
+    rows, conv = torch.full((t + 64, 8192), 7.0, dtype=BF16, device=gpu), torch.full((n + 2, 8192, 3), 0.5, dtype=BF16, device=gpu)
+    x = torch.randn(t, 8192, generator=gen, device=gpu).to(BF16)
+    w = torch.randn(8192, 4, generator=gen, device=gpu).to(BF16)
+    cu, sl = torch.tensor(cu, device=gpu).to(torch.int32), torch.tensor(slots, device=gpu).to(torch.int32)
+    named = [s for s in slots if 0 <= s < n]
+    for longest in (None, 1):
+        rd.ragged_delta_rule(q, k, v, g, beta, pool[1:n + 1], cu, sl, out=out[32:t + 32], longest=longest)
+        rd.ragged_conv1d(x, w, conv[1:n + 1], cu, sl, out=rows[32:t + 32])
+        for y in (out, rows):
+            assert (y[:32] == 7.0).all() and (y[t + 32:] == 7.0).all()
+        for p in (pool, conv):
+            for s in set(range(-1, n + 1)) - set(named):
+                assert (p[s + 1] == 0.5).all(), s
