@@ -174,10 +174,10 @@ __global__ __launch_bounds__(256) void gdn_ragged_step_kernel(DeltaArgs p, Ragge
 //    state, in registers: the layout of a product's result is that of the next one's
 //    right operand, so that nothing of a column's recurrence leaves its wave, and waves
 //    meet once a chunk, where the next chunk's k, q, v, T and A are ready in LDS.
-//    117 us: a chunk takes 4.7 us, 4.3 without its fetches, in which each SIMD issues
-//    products for 1.8 and vector instructions for 1.9 and LDS is read for 1.7: what is left is
-//    the chain's latency.  (131 with the fetches in the eight waves that own columns; 4 such
-//    waves of 32 columns each 128.)
+//    117 us: a chunk takes 4.7 us, 4.3 without its fetches.  Products hold a SIMD's vector
+//    instructions up for half of their 16 cycles: 132 x 8 and 656 x 4 cycles of two waves are
+//    3.1 us; LDS is read for 1.7.  What is left is the chain's latency.  (131 us with the
+//    fetches in the eight waves that own columns; 4 such waves of 32 columns each 128.)
 // ---------------------------------------------------------------------------
 
 typedef _Float16 f16;
