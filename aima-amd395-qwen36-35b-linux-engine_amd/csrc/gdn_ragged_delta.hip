@@ -4,7 +4,7 @@
 // [128 v] in fp32:
 //   q, k <- x / sqrt(sum x^2 + 1e-6), q *= 1/sqrt(128)
 //   S <- e^g S;  d = beta (v - k S);  S <- S + k (x) d;  o = q S
-// A sequence begins with its slot's state (zeros where it has none) and leaves its
+// (or q and k as given, q /= sqrt(128); or S kept as [128 v] [128 k]).  A sequence begins with its slot's state (zeros where it has none) and leaves its
 // last one there.
 #include "gemm_tile.h"
 #include "ragged.h"
@@ -24,6 +24,8 @@ struct DeltaArgs {
   bf16* out;
   size_t slot_stride;
   unsigned qk_heads, qk_stride, v_stride;
+  bool normalized;         // q and k are used as given
+  int row_step, col_step;  // elements between rows (of k) and columns (of v) of a state
 };
 
 // ---------------------------------------------------------------------------
@@ -53,12 +55,18 @@ __device__ __forceinline__ void step_rows(const DeltaArgs& p, const RaggedBatch&
   const int rg = tid >> 3, cq = tid & 7;
   const int col = 32 * cg + 4 * cq;
   const int kh = h * (int)p.qk_heads / kGdnHv;
-  float* sp = p.states + (size_t)s.slot * p.slot_stride + ((size_t)h * kGdnDk + rg) * kGdnDv + col;
+  float* sp = p.states + (size_t)s.slot * p.slot_stride + (size_t)h * kGdnDk * kGdnDv + rg * p.row_step + col * p.col_step;
   f32x4 st[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    st[i] = s.has ? __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(sp + 32 * i * kGdnDv))
-                  : f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < 4; ++i) {
+    st[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (s.has && p.col_step == 1) {
+      st[i] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(sp + 32 * i * kGdnDv));
+    } else if (s.has) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) st[i][e] = sp[32 * i + e * kGdnDk];
+    }
+  }
   for (int t = s.a; t < s.z; ++t) {
     const bf16* qp = p.q + (size_t)t * p.qk_stride + kh * kGdnDk + rg;
     const bf16* kp = p.k + (size_t)t * p.qk_stride + kh * kGdnDk + rg;
@@ -112,7 +120,8 @@ __device__ __forceinline__ void step_rows(const DeltaArgs& p, const RaggedBatch&
       nq += dots[par][w][1];
       nkq += dots[par][w][2];
     }
-    const float kinv = 1.0f / sqrtf(nk + 1e-6f), qn = kQScale / sqrtf(nq + 1e-6f);
+    const float kinv = p.normalized ? 1.0f : 1.0f / sqrtf(nk + 1e-6f);
+    const float qn = p.normalized ? kQScale : kQScale / sqrtf(nq + 1e-6f);
     const float eg = expf(gt), dot = nkq * kinv * qn;
     f32x4 d, o;
 #pragma unroll
@@ -130,7 +139,14 @@ __device__ __forceinline__ void step_rows(const DeltaArgs& p, const RaggedBatch&
     }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) __builtin_nontemporal_store(st[i], reinterpret_cast<f32x4*>(sp + 32 * i * kGdnDv));
+  for (int i = 0; i < 4; ++i) {
+    if (p.col_step == 1) {
+      __builtin_nontemporal_store(st[i], reinterpret_cast<f32x4*>(sp + 32 * i * kGdnDv));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sp[32 * i + e * kGdnDk] = st[i][e];
+    }
+  }
 }
 
 __global__ __launch_bounds__(256) void gdn_ragged_step_kernel(DeltaArgs p, RaggedBatch b) {
@@ -308,7 +324,8 @@ struct PrepLds {
   // token of i's tile
   float near[kHeads][kC], far[kHeads][3][48];
   float bs[kHeads][kC];
-  float kinv[kC], qinv[kC];
+  float kinv[kC], qinv[kC];             // 1 where rows are taken as given
+  float kscale[kC], qscale[kC];
 };
 
 // A 16x16 tile of a lower matrix, transposed: column c, row r of it.  Four rows of the 16
@@ -396,14 +413,17 @@ __global__ __launch_bounds__(256, 4) void gdn_ragged_prep_kernel(DeltaArgs p, Ra
   qss += __shfl_xor(qss, 1, 64);
   qss += __shfl_xor(qss, 2, 64);
   if (p1 == 0) {
-    s.kinv[r1] = 1.0f / sqrtf(kss + 1e-6f);
-    s.qinv[r1] = 1.0f / sqrtf(qss + 1e-6f);
+    const float ki = 1.0f / sqrtf(kss + 1e-6f), qi = 1.0f / sqrtf(qss + 1e-6f);
+    s.kscale[r1] = row_scale(ki);
+    s.qscale[r1] = row_scale(qi);
+    s.kinv[r1] = p.normalized ? 1.0f : ki;
+    s.qinv[r1] = p.normalized ? 1.0f : qi;
   }
   lds_barrier();
   auto decay = [&](int hd, int i, int j) { return (s.gs[hd][i] - s.gs[hd][j]) + (s.gl[hd][i] - s.gl[hd][j]); };
   if (wave < kHeads) {
     const int hd = wave, i = lane;
-    const float ki = s.kinv[i], qi = s.qinv[i], ks = row_scale(ki), qs = row_scale(qi);
+    const float ki = s.kinv[i], qi = s.qinv[i], ks = s.kscale[i], qs = s.qscale[i];
     const float eg = expf(s.gs[hd][i]), bt = s.bs[hd][i];
     const float kn = ki / ks, qn = qi / qs;        // by powers of two
     Record& r = rec[hd];
@@ -782,9 +802,10 @@ __global__ __launch_bounds__(64 * scan_waves(kWaves), 1) void gdn_ragged_scan_ke
 
   // ---- the wave's columns
   const int col0 = 16 * ((int)(rest % kGroups) * kWaves + wave);
-  float* sp = p.states + (size_t)s.slot * p.slot_stride + ((size_t)h * kGdnDk + 8 * lg) * kGdnDv + col0 + li;
+  float* sp = p.states + (size_t)s.slot * p.slot_stride + (size_t)h * kGdnDk * kGdnDv + 8 * lg * p.row_step +
+              (col0 + li) * p.col_step;
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-  auto state_row = [&](int i, int r) { return (32 * (i >> 1) + 4 * (i & 1) + r) * kGdnDv; };
+  auto state_row = [&](int i, int r) { return (32 * (i >> 1) + 4 * (i & 1) + r) * p.row_step; };
   f32x4 state[8];      // state[2 k + u][r]: row 32 k + 8 lg + 4 u + r
 #pragma unroll
   for (int i = 0; i < 8; ++i)
@@ -1033,25 +1054,28 @@ Q36_EXPORT size_t qwen36_gdn_ragged_delta_workspace_bytes(const qwen36_state_bat
   return (size_t)most_records(b) * kGdnHv * sizeof(Record);
 }
 
-Q36_EXPORT int qwen36_gdn_ragged_delta(const void* q, const void* k, const void* v, unsigned qk_heads,
-                                       unsigned qk_token_stride, unsigned v_token_stride, const void* g,
-                                       const void* beta, void* states, size_t slot_stride,
-                                       const qwen36_state_batch* batch, unsigned longest, void* out,
-                                       void* workspace, size_t workspace_bytes, void* stream) {
+Q36_EXPORT int qwen36_gdn_ragged_delta_ex(const void* q, const void* k, const void* v, unsigned qk_heads,
+                                          unsigned qk_token_stride, unsigned v_token_stride, const void* g,
+                                          const void* beta, void* states, size_t slot_stride,
+                                          const qwen36_state_batch* batch, unsigned longest, unsigned flags,
+                                          void* out, void* workspace, size_t workspace_bytes, void* stream) {
   RaggedBatch b;
   if (q == nullptr || k == nullptr || v == nullptr || g == nullptr || beta == nullptr || states == nullptr ||
       out == nullptr || !ragged_batch_of(batch, b) || (qk_heads != 16u && qk_heads != 32u) ||
       qk_token_stride < qk_heads * kGdnDk || qk_token_stride % 8 != 0 || qk_token_stride > kMaxStride ||
       v_token_stride > kMaxStride || v_token_stride < (unsigned)(kGdnHv * kGdnDv) || v_token_stride % 8 != 0 ||
       slot_stride < (size_t)kGdnHv * kGdnDk * kGdnDv || slot_stride % 4 != 0 || !aligned16(q) ||
-      !aligned16(k) || !aligned16(v) || !aligned16(states) || !aligned16(out))
+      !aligned16(k) || !aligned16(v) || !aligned16(states) || !aligned16(out) ||
+      (flags & ~(QWEN36_GDN_QK_NORMALIZED | QWEN36_GDN_STATE_VK)) != 0)
     return Q36_EINVAL;
+  const bool vk = (flags & QWEN36_GDN_STATE_VK) != 0;
   const size_t need = qwen36_gdn_ragged_delta_workspace_bytes(batch, longest);
   if (need > 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < need)) return Q36_EINVAL;
   const DeltaArgs p = {static_cast<const bf16*>(q),  static_cast<const bf16*>(k),
                        static_cast<const bf16*>(v),  static_cast<const float*>(g),
                        static_cast<const float*>(beta), static_cast<float*>(states),
-                       static_cast<bf16*>(out), slot_stride, qk_heads, qk_token_stride, v_token_stride};
+                       static_cast<bf16*>(out), slot_stride, qk_heads, qk_token_stride, v_token_stride,
+                       (flags & QWEN36_GDN_QK_NORMALIZED) != 0, vk ? 1 : kGdnDv, vk ? kGdnDk : 1};
   hipStream_t st = static_cast<hipStream_t>(stream);
   const bool chunks = by_chunks(b, longest);
   if (!chunks) {
@@ -1091,4 +1115,13 @@ Q36_EXPORT int qwen36_gdn_ragged_delta(const void* q, const void* k, const void*
   else
     hipLaunchKernelGGL(gdn_ragged_scan_kernel<8>, dim3(n * kGdnHv), dim3(64 * scan_waves(8)), lds, st, p, b, ws, n);
   return static_cast<int>(hipGetLastError());
+}
+
+Q36_EXPORT int qwen36_gdn_ragged_delta(const void* q, const void* k, const void* v, unsigned qk_heads,
+                                       unsigned qk_token_stride, unsigned v_token_stride, const void* g,
+                                       const void* beta, void* states, size_t slot_stride,
+                                       const qwen36_state_batch* batch, unsigned longest, void* out,
+                                       void* workspace, size_t workspace_bytes, void* stream) {
+  return qwen36_gdn_ragged_delta_ex(q, k, v, qk_heads, qk_token_stride, v_token_stride, g, beta, states, slot_stride,
+                                    batch, longest, 0, out, workspace, workspace_bytes, stream);
 }

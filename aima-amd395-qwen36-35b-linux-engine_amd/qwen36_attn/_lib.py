@@ -151,6 +151,8 @@ SIGNATURES: dict[str, tuple] = {
     "qwen36_gdn_ragged_delta_workspace_bytes": (_sz, [_psbatch, _u32]),
     "qwen36_gdn_ragged_delta": (_i32, [_vp, _vp, _vp, _u32, _u32, _u32, _vp, _vp, _vp, _sz,
                                        _psbatch, _u32, _vp, _vp, _sz, _vp]),
+    "qwen36_gdn_ragged_delta_ex": (_i32, [_vp, _vp, _vp, _u32, _u32, _u32, _vp, _vp, _vp, _sz,
+                                          _psbatch, _u32, _u32, _vp, _vp, _sz, _vp]),
     "qwen36_slots_fork": (_i32, [_pslots, _u32, _u32, _vp, _vp]),
     # page tables
     "qwen36_pages_trim": (_i32, [_ptables, _vp, _vp]),

@@ -162,17 +162,27 @@ def vllm_chunk_gated_delta_rule(q, k, v, g, beta, scale: float | None = None,
     q and k as given; True normalises them in the kernel.  Returns (o [1, T,
     32, 128] bf16, final_state [1, 32, 128, 128] fp32 in the same [v, k]
     orientation, or None unless ``output_final_state``).  Chunk 64, scale
-    1/sqrt(128) (vLLM's default; other scales are rejected), batch 1 without
-    varlen packing, as the reference uses it."""
-    if cu_seqlens is not None:
-        raise NotImplementedError("cu_seqlens (varlen batches) is not provided: the engine "
-                                  "runs batch 1")
+    1/sqrt(128) (vLLM's default; other scales are rejected), batch 1, as the
+    reference uses it; ``cu_seqlens`` [N + 1]: N sequences packed along T, with
+    states [N, 32, 128, 128] (``ragged_deltanet.ragged_delta_rule``)."""
     if head_first:
         raise ValueError("head_first layout is not supported (vLLM deprecated it)")
     if scale is not None and abs(scale - DK ** -0.5) > 1e-12:
         raise ValueError("the HIP kernel applies scale 1/sqrt(128)")
     qq, kk, vv, t, hq = _qkv_views(q, k, v)
     g, beta = _gb(g, beta, t)
+    if cu_seqlens is not None:
+        from .ragged_deltanet import ragged_delta_rule
+        n, dev = cu_seqlens.shape[0] - 1, qq.device
+        if initial_state is None:
+            states, has = torch.zeros(n, HV, DV, DK, device=dev), torch.zeros(n, dtype=torch.bool, device=dev)
+        else:
+            require(initial_state, "initial_state", torch.float32, shape=(n, HV, DV, DK))
+            states, has = initial_state.clone(), None
+        out = ragged_delta_rule(qq, kk, vv, g, beta, states, cu_seqlens.to(torch.int32),
+                                torch.arange(n, dtype=torch.int32, device=dev), has,
+                                flags=STATE_VK | (0 if use_qk_l2norm_in_kernel else QK_NORMALIZED))
+        return out[None], (states if output_final_state else None)
     s_in = None
     if initial_state is not None:
         s_in = initial_state.reshape(HV, DV, DK)

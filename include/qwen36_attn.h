@@ -636,6 +636,15 @@ int qwen36_gdn_ragged_delta(const void* q, const void* k, const void* v, unsigne
                             const qwen36_state_batch* batch, unsigned longest, void* out,
                             void* workspace, size_t workspace_bytes, void* stream);
 
+/* qwen36_gdn_ragged_delta_ex: the same with qwen36_gdn_chunk_prefill_ex's flags:
+ * QWEN36_GDN_QK_NORMALIZED (q and k are used as given; the chunks are made for keys of
+ * norm 1 at most) and QWEN36_GDN_STATE_VK (states are [128 v][128 k]); 0: none. */
+int qwen36_gdn_ragged_delta_ex(const void* q, const void* k, const void* v, unsigned qk_heads,
+                               unsigned qk_token_stride, unsigned v_token_stride, const void* g,
+                               const void* beta, void* states, size_t slot_stride,
+                               const qwen36_state_batch* batch, unsigned longest, unsigned flags,
+                               void* out, void* workspace, size_t workspace_bytes, void* stream);
+
 /* qwen36_slots_fork: slot i of every pool becomes a copy of its slot parent[i] (int32
  * [slots] in device memory; -1: it stays; a child of a slot that is a child of the same
  * call stays too).  Slots are slot_bytes (a multiple of 16, at most 2^30) at multiples

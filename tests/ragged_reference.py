@@ -27,7 +27,7 @@ def normed(x):
     return x / (x.square().sum(-1, keepdim=True) + 1e-6).sqrt()
 
 
-def delta(q, k, v, g, beta, states, cu, slots, has):
+def delta(q, k, v, g, beta, states, cu, slots, has, norm=normed):
     """The delta rule's rows (NaN where a row has no sequence) and the states after."""
     states = states.double()
     out = torch.full(v.shape, float("nan"), dtype=torch.float64, device=v.device)
@@ -37,8 +37,8 @@ def delta(q, k, v, g, beta, states, cu, slots, has):
         if a == z or not 0 <= slot < states.shape[0]:
             continue
         s = states[slot] if has[i] else torch.zeros_like(states[slot])
-        qn = normed(q[a:z]).repeat_interleave(rep, 1) * 128 ** -0.5
-        kn = normed(k[a:z]).repeat_interleave(rep, 1)
+        qn = norm(q[a:z]).repeat_interleave(rep, 1) * 128 ** -0.5
+        kn = norm(k[a:z]).repeat_interleave(rep, 1)
         for t in range(z - a):
             s = s * g[a + t].double().exp()[:, None, None]
             d = (v[a + t].double() - (s * kn[t][:, :, None]).sum(1)) * beta[a + t].double()[:, None]

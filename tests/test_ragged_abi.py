@@ -69,3 +69,9 @@ def test_python_refuses_cpu_tensors():
         rd.ragged_conv1d(x, x.new_zeros(8192, 4), x.new_zeros(2, 8192, 3), i, i[:1])
     with pytest.raises(ValueError):
         rd.ragged_delta_rule(x, x, x, x, x, torch.zeros(2, 32, 128, 128), i, i[:1])
+
+
+@pytest.mark.parametrize("flags,status", [(4, 1), (8, 1), (1 << 31, 1)])
+def test_delta_flags(lib, flags, status):  # noqa: F811
+    args = delta_args(batch(tokens=90))
+    assert lib.qwen36_gdn_ragged_delta_ex(*args[:12], flags, *args[12:]) == status

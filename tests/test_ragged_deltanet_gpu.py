@@ -343,3 +343,44 @@ def test_offsets_that_make_no_sense(gpu, cu, slots):
         for p in (pool, conv):
             for s in set(range(-1, n + 1)) - set(named):
                 assert (p[s + 1] == 0.5).all(), s
+
+
+@pytest.mark.parametrize("flags", [gd.QK_NORMALIZED, gd.STATE_VK, gd.QK_NORMALIZED | gd.STATE_VK])
+@pytest.mark.parametrize("lens", [[5, 1, 0, 7, 2], [130, 1, 64, 9, 7], [300]])
+def test_delta_flags(gpu, lens, flags):
+    """q and k as given (of norm 1, rounded to bf16), states by columns."""
+    n = len(lens)
+    slots, has = [(2 * i + 1) % n for i in range(n)], [i % 2 == 0 for i in range(n)]
+    q, k, v, g, beta, gen = core(gpu, sum(lens), 47)
+    as_given, by_columns = bool(flags & gd.QK_NORMALIZED), bool(flags & gd.STATE_VK)
+    if as_given:
+        q, k = R.normed(q).to(BF16), R.normed(k).to(BF16)
+    states = torch.randn(n, 32, 128, 128, generator=gen, device=gpu)
+    before = states.mT if by_columns else states.clone()
+    before = before.contiguous()
+    out = torch.full((sum(lens), 32, 128), 7.0, dtype=BF16, device=gpu)
+    rd.ragged_delta_rule(q, k, v, g, beta, states, *batch(lens, slots, has, gpu), out=out, flags=flags)
+    want, after = R.delta(q, k, v, g, beta, before, R.cu_of(lens), slots, has, *([torch.Tensor.double] if as_given else []))
+    check_delta(out, (states.mT if by_columns else states).contiguous(), want, after, [s for s, m in zip(slots, lens) if not m])
+
+
+@pytest.mark.parametrize("norm_in_kernel", [True, False])
+@pytest.mark.parametrize("initial", [True, False])
+def test_vllm_chunk_rule_over_packed_sequences(gpu, norm_in_kernel, initial):
+    lens = [70, 1, 200, 9]
+    q, k, v, g, beta, gen = core(gpu, sum(lens), 53)
+    if not norm_in_kernel:
+        q, k = R.normed(q).to(BF16), R.normed(k).to(BF16)
+    first = torch.randn(4, 32, 128, 128, generator=gen, device=gpu) if initial else None
+    kept = None if first is None else first.clone()
+    cu = torch.tensor(R.cu_of(lens), device=gpu)
+    out, last = gd.vllm_chunk_gated_delta_rule(q[None], k[None], v[None], g[None], beta[None], initial_state=first,
+                                               output_final_state=True, cu_seqlens=cu, use_qk_l2norm_in_kernel=norm_in_kernel)
+    before = torch.zeros(4, 32, 128, 128, device=gpu) if first is None else first.mT.contiguous()
+    want, after = R.delta(q, k, v, g, beta, before, R.cu_of(lens), range(4), [initial] * 4,
+                          *([] if norm_in_kernel else [torch.Tensor.double]))
+    assert out.shape == (1, sum(lens), 32, 128) and (first is None or torch.equal(first, kept))
+    check_delta(out[0], last.mT.contiguous(), want, after, [])
+    none = gd.vllm_chunk_gated_delta_rule(q[None], k[None], v[None], g[None], beta[None], initial_state=first,
+                                          cu_seqlens=cu, use_qk_l2norm_in_kernel=norm_in_kernel)
+    assert none[1] is None and torch.equal(none[0], out)
