@@ -568,15 +568,11 @@ __device__ __forceinline__ f32x4 mfma_f16(f16x8 a, f16x8 b, f32x4 c) {
 
 #define kFence __builtin_amdgcn_sched_barrier(0)
 #define kPin(x) asm volatile("" : "+v"(x))
-// Products with `n` vector instructions behind each: `a`, then the reads of LDS, then `b`.
-#define kBeside(a, b, n)                                              \
+// The reads of LDS, then `m` products with `n` vector instructions behind each.
+#define kBeside(m, n)                                                 \
   do {                                                                \
-    for (int q_ = 0; q_ < (a); ++q_) {                                \
-      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);                \
-      __builtin_amdgcn_sched_group_barrier(0x2, n, 0);                \
-    }                                                                 \
     __builtin_amdgcn_sched_group_barrier(0x100, 16, 0);               \
-    for (int q_ = 0; q_ < (b); ++q_) {                                \
+    for (int q_ = 0; q_ < (m); ++q_) {                                \
       __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);                \
       __builtin_amdgcn_sched_group_barrier(0x2, n, 0);                \
     }                                                                 \
@@ -688,8 +684,8 @@ __device__ __forceinline__ f16x8 to_f16(const u32x4& x, float s) {
 constexpr int scan_waves(int chains) { return chains == 8 ? 12 : 8; }
 
 template <int kWaves>
-__global__ __launch_bounds__(64 * scan_waves(kWaves), 1) void gdn_ragged_scan_kernel(DeltaArgs p, RaggedBatch b,
-                                                                 const Record* __restrict__ ws, unsigned most) {
+__global__ __launch_bounds__(64 * scan_waves(kWaves), 1) void gdn_ragged_scan_kernel(
+    DeltaArgs p, RaggedBatch b, const Record* __restrict__ ws, unsigned most) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   ScanBuf* buf = reinterpret_cast<ScanBuf*>(smem);
   constexpr unsigned kGroups = 8 / kWaves;
@@ -840,7 +836,7 @@ __global__ __launch_bounds__(64 * scan_waves(kWaves), 1) void gdn_ragged_scan_ke
   auto frag_k = [](int f) { return f < 2 ? 0 : f & 1; };
 
   // The chain of a chunk is S -> k S -> rows -> T rows -> decayed v' -> S.  What does not wait
-  // for it (q S, A v', the output, fetches) stands beside products or vector instructions
+  // for it (q S, A v', the output) stands beside products or vector instructions
   // that would stand alone, and LDS is read a step ahead; fences and group orders hold the
   // compiler to that.  What still stands alone runs beside the SIMD's other wave.
   ColumnMax top;
@@ -868,7 +864,7 @@ __global__ __launch_bounds__(64 * scan_waves(kWaves), 1) void gdn_ragged_scan_ke
 #pragma unroll
       for (int i = 0; i < 4; ++i) ks[i] = mfma_f16(kf[k & 1][i], sh[k], ks[i]);
       if (k < 3) split8(state[2 * k + 2], state[2 * k + 3], ss, sh[k + 1], sl[k + 1]);
-      kBeside(0, 8, 3);
+      kBeside(8, 3);
     }
     // q' S, rows beta (v - e^G k S)
     ColumnMax ztop;
@@ -898,7 +894,7 @@ __global__ __launch_bounds__(64 * scan_waves(kWaves), 1) void gdn_ragged_scan_ke
         ks[k][r] = __builtin_fmaf(-cy[k][r], ks[k][r],
                                   bt[k][r] * __uint_as_float((unsigned)(unsigned short)v4[k][r] << 16));
       ztop.take(ks[k]);
-      kBeside(0, 8, 3);
+      kBeside(8, 3);
     }
     float zs, zi;
     f16x8 xh[2], xl[2];
@@ -920,17 +916,17 @@ __global__ __launch_bounds__(64 * scan_waves(kWaves), 1) void gdn_ragged_scan_ke
         }
     };
     t_rows(0, fa);
-    kBeside(0, 6, 0);
+    kBeside(6, 0);
     t_rows(1, fb);
     read_frags(0, 2, fa);
 #pragma unroll
     for (int i = 0; i < 2; ++i) qs[i] *= rq[i] * si;
-    kBeside(0, 6, 3);
+    kBeside(6, 3);
     t_rows(2, fa);
     read_frags(kFragA, 0, fb);
 #pragma unroll
     for (int i = 2; i < 4; ++i) qs[i] *= rq[i] * si;
-    kBeside(0, 6, 3);
+    kBeside(6, 3);
     // decayed v', A v'
     bf16x8 vh[2], vl[2];
 #pragma unroll
@@ -968,17 +964,17 @@ __global__ __launch_bounds__(64 * scan_waves(kWaves), 1) void gdn_ragged_scan_ke
       ks[i] *= rk[i];
       wtop.take(ks[i]);
     }
-    kBeside(0, 6, 4);
+    kBeside(6, 4);
     a_rows(1, fa);
     read_frags(kFragA, 2, fb);
     scale_of<13>(wtop.bits(), wsc, wi);
     split8(ks[0], ks[1], wsc, xh[0], xl[0]);
     wi *= zi;
-    kBeside(0, 6, 6);
+    kBeside(6, 6);
     a_rows(2, fb);
     read_kt(0);
     split8(ks[2], ks[3], wsc, xh[1], xl[1]);
-    kBeside(0, 6, 4);
+    kBeside(6, 4);
     // S <- e^Glast S + k'^T decayed v'; the output e^G q S + A v', in place of the columns' v
     const float ai = zi * 0.00390625f;
     top = ColumnMax{};
@@ -1006,7 +1002,7 @@ __global__ __launch_bounds__(64 * scan_waves(kWaves), 1) void gdn_ragged_scan_ke
           update(i);
         }
       }
-      kBeside(0, 8, 3);
+      kBeside(8, 3);
     }
 #pragma unroll
     for (int i = 4; i < 8; ++i) update(i);
