@@ -208,6 +208,9 @@ constexpr int kC = 64;
 // workspace (2 us more for one sequence of 12).
 constexpr unsigned kShort = 7, kFewRows = 12;
 constexpr int kPitchR = 136;              // 16-bit row pitch of [64][128] tiles: 272 bytes
+// g below this is taken as this: e^g is zero in fp32 either way (below -104), and sums of 64
+// stay finite and small enough for what comes after to keep its bits.
+constexpr float kGateMin = -128.0f;
 
 // A record.  T and A as operands: tokens 16 i .. by 32 tokens k, lane 16 g + m of row m the
 // columns 32 k + 4 g .. + 3 and 32 k + 16 + 4 g .. + 3, which is how two tiles of a product's
@@ -384,7 +387,7 @@ __global__ __launch_bounds__(256, 4) void gdn_ragged_prep_kernel(DeltaArgs p, Ra
     const float* from = wave < 2 ? p.g : p.beta;
     const float v = (unsigned)lane < rows ? from[(size_t)(tok0 + lane) * kGdnHv + h0 + hd] : 0.f;
     if (wave < 2) {
-      double sum = v;
+      double sum = v < kGateMin ? kGateMin : v;
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
         const double u = __shfl_up(sum, o, 64);

@@ -125,13 +125,14 @@ def ragged_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torc
                       has_state: torch.Tensor | None = None, out: torch.Tensor | None = None,
                       longest: int | None = None, flags: int = 0) -> torch.Tensor:
     """The gated delta rule for a batch: q, k [T, 16 (or 32 repeated), 128], v [T, 32,
-    128] bf16 (q and k are l2-normalised in the kernel), g (log decay, at most 0), beta (0
-    to 2) [T, 32] fp32, states [slots, 32, 128 (k), 128 (v)] fp32, replaced in place by the sequences'
-    last states.  ``longest``: the most rows that a sequence of the call has, where the
-    caller knows it; it only chooses between the forms for few and for many tokens (a
-    sequence may have more).  ``flags``: ``gated_deltanet.QK_NORMALIZED`` (q and k, of norm
-    1 at most, are used as given) and ``STATE_VK`` (states are [slots, 32, 128 (v), 128
-    (k)]).  Returns [T, 32, 128] bf16; ``out`` overlaps no input.  A call of more than 12
+    128] bf16 (q and k are l2-normalised in the kernel), g (log decay, at most 0, -inf
+    among them), beta (0 to 2) [T, 32] fp32, states [slots, 32, 128 (k), 128 (v)] fp32,
+    replaced in place by the sequences' last states.  ``longest``: the most rows that a
+    sequence of the call has, where the caller knows it; it only chooses between the forms
+    for few and for many tokens (a sequence may have more).  ``flags``:
+    ``gated_deltanet.QK_NORMALIZED`` (q and k, of norm 1 at most, are used as given) and
+    ``STATE_VK`` (states are [slots, 32, 128 (v), 128 (k)]).  Returns [T, 32, 128] bf16;
+    ``out`` overlaps no input.  A call of more than 12
     rows takes 824 KiB of workspace for every 64 rows and every sequence that may have 8 and
     more of them (none where ``longest`` is less)."""
     index, n, sp, ss = _pool(states, "states", torch.float32, *_STATE)

@@ -622,10 +622,10 @@ int qwen36_gdn_ragged_conv1d(const void* x, unsigned x_row_stride, const void* w
  * v [tokens, 32, 128] bf16 with token strides (multiples of 8, at most 2^24), g, beta
  * fp32 [tokens, 32], out bf16 [tokens, 32, 128]; states fp32 [num_slots][32][128 k][128 v],
  * slots slot_stride elements (a multiple of 4) apart, replaced by the sequences' last
- * states; out overlaps no input.  Sequences of 8 and more rows go by chunks, which are made for g <= 0 and
- * 0 <= beta <= 2 (outside, their values may leave fp16's range).  longest: 0, or the most
- * rows that a sequence has as the host knows it; it only chooses the launches, a sequence
- * may have more.  Pointers 16-byte aligned (g and
+ * states; out overlaps no input.  Sequences of 8 and more rows go by chunks, which are made
+ * for g <= 0, -inf (the state is forgotten) among them, and 0 <= beta <= 2 (outside, their
+ * values may leave fp16's range).  longest: 0, or the most rows that a sequence has as the
+ * host knows it; it only chooses the launches, a sequence may have more.  Pointers 16-byte aligned (g and
  * beta 4); workspace of qwen36_gdn_ragged_delta_workspace_bytes(...) bytes (0: none;
  * else 824 KiB for every 64 rows and every sequence that may have 8 and more, at most an
  * eighth of the rows); calls that overlap on one workspace race. */
