@@ -410,8 +410,9 @@ __global__ __launch_bounds__(256, 8) void pages_copy_kernel(CopyCaches cs, unsig
   if (r.table != nullptr) {
     const unsigned n = *r.held;
     for (unsigned i = blockIdx.x; i < r.rows; i += gridDim.x) {
+      // a row of no valid length keeps its entries, whose pages are counted still
       const int len = r.lens[i];
-      const int have = len >= 0 && len <= r.max_len ? pages_of(len, r.page) : 0;
+      const int have = len >= 0 && len <= r.max_len ? pages_of(len, r.page) : (int)r.width;
       for (unsigned c = threadIdx.x; c < r.width; c += 256) {
         int p = (int)c < have ? r.table[i * r.stride + c] : -1;
         if ((unsigned)p >= n && (unsigned)p < r.pages) p = r.map[p];

@@ -122,7 +122,9 @@ def compact(refs: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor
     """Moves the held pages together: with n of them, those at n or behind go, in every
     one of ``caches``, to the free pages before n, in ascending order.  Returns the counts
     and the table after it (``refs_out`` and ``table_out``, which may be ``refs`` and
-    ``page_table`` themselves); entries behind a row's length come out as -1."""
+    ``page_table`` themselves); entries behind a row's length come out as -1.  A row whose
+    length is negative or above what its table holds keeps all of its entries, which name
+    its pages where they are then."""
     args, page = _caches(caches, refs)
     index, t = _args(refs, page_table, seq_lens, page)
     if refs_out is None:

@@ -702,8 +702,9 @@ int qwen36_pages_extend(const qwen36_page_tables* tables, const void* add, void*
 /* qwen36_pages_compact: with n pages held, those at n or behind go, in every cache, to
  * the free pages before n, in ascending order; refs_out [num_pages] and table_out (rows
  * table_out_stride apart) are the counts and the table after it, entries behind a row's
- * length -1; they may be refs and the table themselves.  Workspace of
- * qwen36_pages_compact_workspace_bytes(...) bytes, 16-byte aligned. */
+ * length -1; a row whose length is negative or above what the table holds keeps all of its
+ * entries, which name its pages where they are then.  Both may be refs and the table
+ * themselves.  Workspace of qwen36_pages_compact_workspace_bytes(...) bytes, 16-byte aligned. */
 size_t qwen36_pages_compact_workspace_bytes(const qwen36_page_tables* tables);
 int qwen36_pages_compact(const qwen36_page_tables* tables, void* refs_out, void* table_out,
                          size_t table_out_stride, const qwen36_paged_cache* caches,
