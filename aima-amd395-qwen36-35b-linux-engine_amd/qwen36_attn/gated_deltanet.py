@@ -175,7 +175,8 @@ def vllm_chunk_gated_delta_rule(q, k, v, g, beta, scale: float | None = None,
         from .ragged_deltanet import ragged_delta_rule
         n, dev = cu_seqlens.shape[0] - 1, qq.device
         if initial_state is None:
-            states, has = torch.zeros(n, HV, DV, DK, device=dev), torch.zeros(n, dtype=torch.bool, device=dev)
+            states = torch.zeros(n, HV, DV, DK, dtype=torch.float32, device=dev)
+            has = torch.zeros(n, dtype=torch.bool, device=dev)
         else:
             require(initial_state, "initial_state", torch.float32, shape=(n, HV, DV, DK))
             states, has = initial_state.clone(), None
