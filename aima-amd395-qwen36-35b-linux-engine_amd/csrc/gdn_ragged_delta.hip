@@ -167,14 +167,16 @@ __global__ __launch_bounds__(256) void gdn_ragged_step_kernel(DeltaArgs p, Ragge
 //
 // Precision.  S, v', its decayed rows and beta (v - ..) are fp32; into products that the
 // state comes from they enter as the sum of two fp16 values (22 bits), each column scaled
-// by a power of two to its largest value, so that what is lost is 2^-23 of it.  k and q (8
-// bits in bf16) are exact in fp16 once a row is scaled by a power of two to a norm of 8 to
-// 16: values below 2^-20 of their row's norm lose bits, 2^-28 of it at most.  T has two
-// such parts (of 2^8 T: what is lost is 2^-33 at least).  With 0 <= beta <= 2 and g <= 0 a
-// column's v' is at most 129 times the largest row that it comes from, and 2^8 of scale
-// keeps it below fp16's range.  A against v', which only the output comes from, takes two
-// bf16 values of each (2^-17 of a term): decays of any size meet there, and rows that
-// are all decayed keep their bits.
+// by a power of two that brings its largest to 2^13 .. 2^14: what is lost of a value is
+// 2^-22 of it or, for small ones beside large, 2^-38 of the column's largest (half of
+// fp16's least step).  Sums are fp32, so that only the operands have to stay within fp16.  k
+// and q (8 bits in bf16) are exact in fp16 once a row is scaled by a power of two to a norm
+// of 8 to 16: values below 2^-20 of their row's norm lose bits, 2^-28 of it at most.  T has
+// two such parts, of 2^8 T (with 0 <= beta <= 2 and g <= 0 its values are at most 2:
+// T_ij is -beta_i k_i (reflections, which lengthen nothing) k_j): what is lost is 2^-22 of a
+// value or 2^-33.  Low by low parts are left out (2^-22 of a term).  A against v', which
+// only the output comes from, takes two bf16 values of each (2^-17 of a term): decays of
+// any size meet there, and rows that are all decayed keep their bits.
 // (Three bf16 parts throughout, which need no scales, take 182 products a chunk and column
 // tile where this takes 132: 157 us where the scan then took 134.)
 //
@@ -662,10 +664,9 @@ struct ColumnMax {
   }
 };
 
-// The power of two that brings the value of bits m into [2^to, 2^(to + 1)), and its inverse.
-template <int kTo>
+// The power of two that brings the value of bits m into [2^13, 2^14), and its inverse.
 __device__ __forceinline__ void scale_of(unsigned m, float& s, float& inv) {
-  const int e = min(max((int)(m >> 23), 27), 253) - kTo;      // biased
+  const int e = min(max((int)(m >> 23), 27), 253) - 13;      // biased
   s = __uint_as_float((unsigned)(254 - e) << 23);
   inv = __uint_as_float((unsigned)e << 23);
 }
@@ -854,7 +855,7 @@ __global__ __launch_bounds__(64 * scan_waves(kWaves), 1) void gdn_ragged_scan_ke
     f32x4 ks[4], qs[4];
     float ss, si;
     read_rows(kKr, 0, kf[0]);
-    scale_of<13>(top.bits(), ss, si);
+    scale_of(top.bits(), ss, si);
     split8(state[0], state[1], ss, sh[0], sl[0]);
     kFence;
     egl_next = (ws + (size_t)(rec0 + min(c + 1, last)) * kGdnHv + h)->f[kEgl];
@@ -901,7 +902,7 @@ __global__ __launch_bounds__(64 * scan_waves(kWaves), 1) void gdn_ragged_scan_ke
     }
     float zs, zi;
     f16x8 xh[2], xl[2];
-    scale_of<7>(ztop.bits(), zs, zi);
+    scale_of(ztop.bits(), zs, zi);
 #pragma unroll
     for (int k = 0; k < 2; ++k) split8(ks[2 * k], ks[2 * k + 1], zs, xh[k], xl[k]);
     f32x4 rq[4], rk[4];
@@ -970,7 +971,7 @@ __global__ __launch_bounds__(64 * scan_waves(kWaves), 1) void gdn_ragged_scan_ke
     kBeside(6, 4);
     a_rows(1, fa);
     read_frags(kFragA, 2, fb);
-    scale_of<13>(wtop.bits(), wsc, wi);
+    scale_of(wtop.bits(), wsc, wi);
     split8(ks[0], ks[1], wsc, xh[0], xl[0]);
     wi *= zi;
     kBeside(6, 6);
