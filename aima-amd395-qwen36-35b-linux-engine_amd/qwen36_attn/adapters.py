@@ -4,8 +4,9 @@ No counterpart in the reference.  The projections of a ragged batch are shared
 products (``projections.FusedProjection``, ``prefill_gemm.linear``); a request with
 an adapter of its own gets ``scale * (x A^T) B^T`` added to its rows, for every slice
 of the stacked weights (q | k | v ...) with matrices of its own.  Requests choose
-their adapter by a number on the GPU, read when the launch runs, so that captured
-calls follow it.  All arithmetic runs in ``libqwen36_attn.so``.
+their adapter by a number on the GPU, which the launch that makes an
+``AdapterBatch`` reads: a captured step follows new numbers where the batch is
+made within the capture.  All arithmetic runs in ``libqwen36_attn.so``.
 """
 from __future__ import annotations
 
@@ -58,7 +59,9 @@ class AdapterBatch:
     """The rows of a ragged batch by adapter: made once for all projections of a step.
     ``cu_tokens`` int32 [seqs + 1]: row offsets of the call's ``tokens`` rows (cut to them);
     ``adapter_ids`` int32 [seqs]: each sequence's adapter; one outside [0, ``adapters``)
-    means none."""
+    means none.  Both are read by a launch on the current stream, here and not again: a
+    batch stays what it was when they change, in a graph that was captured over it too.
+    Made within a capture, it is made anew by every replay."""
 
     def __init__(self, cu_tokens: torch.Tensor, adapter_ids: torch.Tensor, tokens: int, adapters: int) -> None:
         for t in (cu_tokens, adapter_ids):

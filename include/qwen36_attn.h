@@ -734,9 +734,11 @@ typedef struct {
 /* qwen36_adapter_plan: the rows of a batch by adapter, for any number of
  * qwen36_adapter_apply calls with the same seqs, tokens and adapters: sequence i, rows
  * [cu_tokens[i], cu_tokens[i+1]) cut to the call's rows, has adapter adapter_ids[i]
- * (int32; one outside [0, adapters): none).  plan: qwen36_adapter_plan_bytes(...) bytes,
- * 16-byte aligned.  Nothing in device memory can make a launch read or write out of
- * bounds; rows of sequences that overlap are any of theirs or left as they were. */
+ * (int32; one outside [0, adapters): none).  Both are read when this launch runs, and by no
+ * other: qwen36_adapter_apply goes by the plan, also where they have changed since.  plan:
+ * qwen36_adapter_plan_bytes(...) bytes, 16-byte aligned.  Nothing in device memory can make
+ * a launch read or write out of bounds; rows of sequences that overlap are any of theirs or
+ * left as they were. */
 size_t qwen36_adapter_plan_bytes(unsigned seqs, unsigned tokens, unsigned adapters);
 int qwen36_adapter_plan(const void* cu_tokens, const void* adapter_ids, unsigned seqs, unsigned tokens,
                         unsigned adapters, void* plan, size_t plan_bytes, void* stream);
