@@ -15,6 +15,9 @@ A turn of a server: ``trim`` the rows that end (or whose drafts were refused),
 ``fork`` rows whose prompt is shared, ``extend`` the rows that get tokens, then
 ``paged_append`` and the attention over the rows of the batch.  A page that several
 rows hold is never written: ``extend`` gives a row that would write one a copy of it.
+A row that it could not serve has its old length and pages, so that tokens of it in the
+turn's batch would be written over its last ones, in pages that others may hold: such a
+row has no tokens there (``cu_tokens``) until it is served.
 """
 from __future__ import annotations
 
@@ -92,8 +95,10 @@ def fork(refs: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor, p
          page_tokens: int) -> None:
     """Row i becomes a fork of row ``parents[i]`` (-1: it stays): its tokens and pages,
     each of which gains a count.  A row that is not empty stays, and so does a child of
-    a row that is a child of the same call.  ``ragged_deltanet.fork_states`` does the
-    same for states in slots."""
+    a row that is a child of the same call.  ``ragged_deltanet.fork_states`` copies the
+    states in slots by such numbers, but slots have no lengths: where a row stays because
+    it is not empty, or its parent is, its slot is copied over all the same.  One vector
+    serves both if it names no such row."""
     index, t = _args(refs, page_table, seq_lens, page_tokens)
     launch(index, "qwen36_pages_fork", t, _vector(parents, "parents", index, t.rows))
 

@@ -132,9 +132,11 @@ def ragged_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torc
     for few and for many tokens (a sequence may have more).  ``flags``:
     ``gated_deltanet.QK_NORMALIZED`` (q and k, of norm 1 at most, are used as given) and
     ``STATE_VK`` (states are [slots, 32, 128 (v), 128 (k)]).  Returns [T, 32, 128] bf16;
-    ``out`` overlaps no input.  A call of more than 12
+    ``out`` overlaps no input.  A value that is not finite may reach any row of its chunk of
+    64, those before it too, where a sequence has 8 and more rows.  A call of more than 12
     rows takes 824 KiB of workspace for every 64 rows and every sequence that may have 8 and
-    more of them (none where ``longest`` is less)."""
+    more of them, an eighth of the rows at most (none where ``longest`` is less: a decode
+    step of many sequences says 1)."""
     index, n, sp, ss = _pool(states, "states", torch.float32, *_STATE)
     t = v.shape[0] if isinstance(v, torch.Tensor) and v.dim() == 3 else 0
     (qp, heads, qs), (kp, *same) = _heads(q, "q", t, (HK, HV), index), _heads(k, "k", t, (HK, HV), index)
@@ -158,7 +160,8 @@ def ragged_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torc
 def fork_states(pools, parents: torch.Tensor) -> None:
     """Slot i of every pool (the layers' [slots, ...] conv and recurrent states) becomes a
     copy of its slot ``parents[i]`` (int32 [slots], -1: it stays; a child of a slot that
-    is a child of the same call stays too): what ``page_tables.fork`` is for pages."""
+    is a child of the same call stays too): what ``page_tables.fork`` is for pages, but
+    for rows that are not empty, which stay there and are copied over here."""
     pools = list(pools)
     if not pools or not isinstance(parents, torch.Tensor) or parents.dtype is not torch.int32 \
             or parents.dim() != 1 or not parents.is_cuda or not parents.is_contiguous() \

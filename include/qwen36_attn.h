@@ -624,9 +624,10 @@ int qwen36_gdn_ragged_conv1d(const void* x, unsigned x_row_stride, const void* w
  * slots slot_stride elements (a multiple of 4) apart, replaced by the sequences' last
  * states; out overlaps no input.  Sequences of 8 and more rows go by chunks, which are made
  * for g <= 0, -inf (the state is forgotten) among them, and 0 <= beta <= 2 (outside, their
- * values may leave fp16's range).  longest: 0, or the most rows that a sequence has as the
- * host knows it; it only chooses the launches, a sequence may have more.  Pointers 16-byte aligned (g and
- * beta 4); workspace of qwen36_gdn_ragged_delta_workspace_bytes(...) bytes (0: none;
+ * values may leave fp16's range); there a value that is not finite may reach any row of its
+ * chunk of 64, those before it too.  longest: 0, or the most rows that a sequence has as the
+ * host knows it; it only chooses the launches, a sequence may have more.  Pointers 16-byte
+ * aligned (g and beta 4); workspace of qwen36_gdn_ragged_delta_workspace_bytes(...) bytes (0: none;
  * else 824 KiB for every 64 rows and every sequence that may have 8 and more, at most an
  * eighth of the rows); calls that overlap on one workspace race. */
 size_t qwen36_gdn_ragged_delta_workspace_bytes(const qwen36_state_batch* batch, unsigned longest);
@@ -647,8 +648,10 @@ int qwen36_gdn_ragged_delta_ex(const void* q, const void* k, const void* v, unsi
 
 /* qwen36_slots_fork: slot i of every pool becomes a copy of its slot parent[i] (int32
  * [slots] in device memory; -1: it stays; a child of a slot that is a child of the same
- * call stays too).  Slots are slot_bytes (a multiple of 16, at most 2^30) at multiples
- * of slot_stride_bytes (one of 16); data 16-byte aligned; at most 1024 pools. */
+ * call stays too).  Slots have no lengths: what qwen36_pages_fork leaves because a row is
+ * not empty, or its parent is, is copied here.  Slots are slot_bytes (a multiple of 16, at
+ * most 2^30) at multiples of slot_stride_bytes (one of 16); data 16-byte aligned; at most
+ * 1024 pools. */
 typedef struct {
   void* data;
   size_t slot_bytes;
@@ -689,7 +692,9 @@ int qwen36_pages_fork(const qwen36_page_tables* tables, const void* parent, void
 /* qwen36_pages_extend: row i grows by add[i] tokens (int32; none if not positive): the
  * lowest free pages go to the rows in their order, to each all that it needs or nothing
  * (once the pool cannot serve a row, it serves no later one that needs pages; a row that
- * asks for more than its table holds needs none and gets nothing).  A row whose last page
+ * asks for more than its table holds needs none and gets nothing).  A row that gets nothing
+ * keeps its length and pages: tokens of it in the batch that follows would be written over
+ * its last ones, in pages that others may hold, so it has none there.  A row whose last page
  * is not full and has other holders gets a copy of it in every cache (pages, scales,
  * bounds).  granted int32 [rows]: 0 where the row could not grow, else 1.  The caches
  * have num_pages pages of page_tokens; at most 1024; workspace of
