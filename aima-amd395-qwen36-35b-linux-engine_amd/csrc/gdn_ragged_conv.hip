@@ -8,10 +8,10 @@
 // to bf16.
 //
 // Bound by its bytes (32 KB a row) for prompts (9,903 rows 73 us, 4.4 TB/s) and by the
-// chain offsets -> slot -> state -> store for single tokens (64 sequences 7 us).  A thread takes 8 channels (16-byte loads) of
-// a tile of 4 rows counted from the sequence's first row, so that only a
-// sequence's first tile reads its slot, and that tile alone writes it: the state
-// is read before it is written by the same thread, whatever the order of tiles.
+// chain offsets -> slot -> state -> store for single tokens (64 sequences 7 us).  A thread
+// takes 8 channels (16-byte loads) of a tile of 4 rows counted from the sequence's first
+// row, so that only a sequence's first tile reads its slot, and that tile alone writes it:
+// the state is read before it is written by the same thread, whatever the order of tiles.
 #include "ragged.h"
 
 namespace q36 {

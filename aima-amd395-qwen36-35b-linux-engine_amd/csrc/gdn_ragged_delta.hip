@@ -4,8 +4,8 @@
 // [128 v] in fp32:
 //   q, k <- x / sqrt(sum x^2 + 1e-6), q *= 1/sqrt(128)
 //   S <- e^g S;  d = beta (v - k S);  S <- S + k (x) d;  o = q S
-// (or q and k as given, q /= sqrt(128); or S kept as [128 v] [128 k]).  A sequence begins with its slot's state (zeros where it has none) and leaves its
-// last one there.
+// (or q and k as given, q /= sqrt(128); or S kept as [128 v] [128 k]).  A sequence begins
+// with its slot's state (zeros where it has none) and leaves its last one there.
 #include "gemm_tile.h"
 #include "ragged.h"
 
@@ -31,9 +31,10 @@ struct DeltaArgs {
 // ---------------------------------------------------------------------------
 // Token by token: sequences of up to `limit` tokens.
 // Bound by the states' bytes (4.2 MB a sequence, read and written: 53 us for 64
-// sequences of a token, 5.1 TB/s).  Both
-// reductions of a token, S^T k and S^T q, are taken of the state before it:
-// o = e^g S_old^T q + d (k.q), so that a token costs one exchange between waves.
+// sequences of a token, 5.1 TB/s; 81 where states are by columns, whose rows are loads of 4
+// bytes).  Both reductions of a token, S^T k and S^T q, are taken of the state before it:
+// o = e^g S_old^T q + d (k.q), so that a token costs one exchange between waves (64
+// sequences of 2 tokens 63 us, of 4 90, of 7 131).
 // One workgroup owns 32 columns of a head: thread (rg, cq) rows rg + 32 i and
 // columns 4 cq .. +3, a row of the 32 columns being one 128-byte line.
 // ---------------------------------------------------------------------------
@@ -183,7 +184,7 @@ __global__ __launch_bounds__(256) void gdn_ragged_step_kernel(DeltaArgs p, Ragge
 // Times below are of 13 prompts of 9,903 rows, 161 chunks, the longest of 24.
 //  * gdn_ragged_prep_kernel, a workgroup a (chunk, key head): T and A of its value heads,
 //    which do not depend on the state, as the scan's operands, and the row factors: a
-//    record of 26,368 bytes a value head.  54 us, of which reading q and k once and writing
+//    record of 26,368 bytes a value head.  53 us, of which reading q and k once and writing
 //    the records (217 MB) take 48 at 4.5 TB/s; four workgroups a CU hide most of its steps'
 //    latencies (two, with L and T as whole matrices in LDS, took 81 us).  The short sequences'
 //    workgroups are behind them (a launch of their own takes 4.8 us even where there are none).
@@ -204,10 +205,11 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kC = 64;
-// Longer sequences go by chunks.  Token by token and by chunks, us: one sequence of 8 tokens
-// 12.4 and 14.9, of 12 17.1 and 14.9; 16 sequences of 8 39 and 36, 64 of 8 132 and 112, of 12
-// 190 and 112.  A call of up to 12 rows goes token by token whatever its lengths, without a
-// workspace (2 us more for one sequence of 12).
+// Longer sequences go by chunks.  Token by token and by chunks, us, over three inputs and
+// their states in turn: one sequence of 8 tokens 12.7 and 15.1, of 12 17.7 and 15.2; 16
+// sequences of 8 48 and 40, of 12 63 and 39; 64 of 7 131 and 142, of 8 152 and 136, of 12 212
+// and 139.  A call of up to 12 rows goes token by token whatever its lengths, without a
+// workspace (2.5 us more for one sequence of 12).
 constexpr unsigned kShort = 7, kFewRows = 12;
 constexpr int kPitchR = 136;              // 16-bit row pitch of [64][128] tiles: 272 bytes
 // g below this is taken as this: e^g is zero in fp32 either way (below -104), and sums of 64
@@ -1102,10 +1104,13 @@ Q36_EXPORT int qwen36_gdn_ragged_delta_ex(const void* q, const void* k, const vo
     hipLaunchKernelGGL(gdn_ragged_prep_kernel<2>, grid, dim3(256), sizeof(PrepLds<2>), st, p, b, ws, blocks);
   else
     hipLaunchKernelGGL(gdn_ragged_prep_kernel<1>, grid, dim3(256), sizeof(PrepLds<1>), st, p, b, ws, blocks);
-  // Few sequences leave CUs, one a workgroup: their columns in two or four.  A chunk takes
-  // 2.2 us of 2 chains a workgroup, 2.6 of 4 and 4 of 8 where few CUs are at work; sequences of
-  // 2,000 tokens, all in all, by 2 and 4 chains 98 and 103 us for one, by 4 and 8 108 and 147
-  // for two, 156 and 181 for four, 245 and 210 for five, 343 and 297 for eight.
+  // Few sequences leave CUs, one a workgroup: their columns in two or four.  Sequences of
+  // 2,000 tokens, all in all, by 2, 4 and 8 chains a workgroup, us: one 90, 93 and 134; two 98,
+  // 104 and 144; three 183, 123 and 160; four 198, 145 and 173; five 282, 236 and 185; eight
+  // 394, 290 and 245.  Two of 4,096: 193, 215 and 282.
+  // n is how many sequences may be long, as the host knows no more.  A prompt beside many
+  // single tokens goes by 8 chains: 2,000 beside 40 take 159 us (116 by 2 chains), 8,192 beside
+  // 63 541 (364).
   const unsigned n = most_long(b);
   const unsigned lds = 2 * sizeof(ScanBuf);
   if (n <= 2)

@@ -164,7 +164,8 @@ def vllm_chunk_gated_delta_rule(q, k, v, g, beta, scale: float | None = None,
     orientation, or None unless ``output_final_state``).  Chunk 64, scale
     1/sqrt(128) (vLLM's default; other scales are rejected), batch 1, as the
     reference uses it; ``cu_seqlens`` [N + 1]: N sequences packed along T, with
-    states [N, 32, 128, 128] (``ragged_deltanet.ragged_delta_rule``)."""
+    states [N, 32, 128, 128] (``ragged_deltanet.ragged_delta_rule``, which takes g
+    of -inf; without ``cu_seqlens`` g is finite, as the sums it makes are subtracted)."""
     if head_first:
         raise ValueError("head_first layout is not supported (vLLM deprecated it)")
     if scale is not None and abs(scale - DK ** -0.5) > 1e-12:

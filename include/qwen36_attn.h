@@ -217,7 +217,7 @@ int qwen36_output_gate(const void* attn, int attn_is_f32, const void* q_gate,
  * qwen36_gdn_chunk_prefill: replaces torch_chunk_gated_delta_rule
  *   (:5167-5240, chunk 64) / the FLA chunk pipeline launched by
  *   native_linear_prefill.hip.cpp:474-836.  Same tensors as the recurrent
- *   step; state_in may be NULL (zeros).  Workspace of at least
+ *   step, g finite; state_in may be NULL (zeros).  Workspace of at least
  *   qwen36_gdn_chunk_prefill_workspace_bytes(tokens) bytes.  q, k and v
  *   16-byte aligned (their rows are read as 16-byte vectors).
  * qwen36_gdn_chunk_prefill_ex: the same with flags, for vLLM's
